@@ -21,13 +21,20 @@ from .block_fht import (
     signs_for,
     suspend_block_fht_weight_cache,
 )
+from .attention import attention, attention_packed
 from .batched import block_fht_grouped_input_linear, block_fht_headwise_linear
+from .gelu8 import Checkpoint8, gelu_checkpoint8, gelu_linear_checkpoint8
 from .mix import FixedFHTMix, fixed_fht_mix
+from .norm import LayerNorm, layer_norm
 
 __all__ = [
     "BlockFHT",
     "BlockFHTLinear",
+    "Checkpoint8",
     "FixedFHTMix",
+    "LayerNorm",
+    "attention",
+    "attention_packed",
     "block_fht_grad_latent",
     "block_fht_grouped_input_linear",
     "block_fht_headwise_linear",
@@ -36,6 +43,9 @@ __all__ = [
     "fixed_fht_mix",
     "flush_block_fht_weight_cache",
     "forward_fused_grouped",
+    "gelu_checkpoint8",
+    "gelu_linear_checkpoint8",
+    "layer_norm",
     "lowbias32",
     "next_power_of_two",
     "prepare_block_fht_weight_cache",

@@ -131,6 +131,9 @@ def _bind(lib) -> None:
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args
+    from . import layer_ops  # its structures name this module's types
+
+    layer_ops.bind(lib)
 
 
 def lib():

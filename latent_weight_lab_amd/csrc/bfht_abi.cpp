@@ -14,18 +14,24 @@
 #include <vector>
 
 #include "bfht_launch.h"
+#include "layer_launch.h"
 
 namespace {
 
 thread_local std::string g_last_error;
 
-int fail(int code, const char* fmt, ...) {
+int vfail(int code, const char* fmt, va_list ap) {
   char buf[512];
+  vsnprintf(buf, sizeof buf, fmt, ap);
+  g_last_error = buf;
+  return code;
+}
+
+int fail(int code, const char* fmt, ...) {
   va_list ap;
   va_start(ap, fmt);
-  vsnprintf(buf, sizeof buf, fmt, ap);
+  vfail(code, fmt, ap);
   va_end(ap);
-  g_last_error = buf;
   return code;
 }
 
@@ -384,6 +390,20 @@ int check_weight_jobs(const lwl_bfht_weight_job* jobs, int64_t count, bool fwd, 
 }
 
 }  // namespace
+
+// The same for the layer operators' entries (layer_abi.cpp).
+namespace lwl {
+int status_fail(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vfail(code, fmt, ap);
+  va_end(ap);
+  return code;
+}
+int status_ok() { return ok(); }
+int status_hip(hipError_t e, const char* what) { return hip_status(e, what); }
+int status_workspace(size_t need, const void* ws, size_t have) { return check_workspace(need, ws, have); }
+}  // namespace lwl
 
 extern "C" {
 

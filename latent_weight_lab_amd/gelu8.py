@@ -1,0 +1,95 @@
+"""GELU that keeps its input in 8 bits for the backward pass.
+
+A generated linear stores no weight; what a training step then holds is activations.  The MLP's
+hidden ones are the largest: in a 16-bit type GELU's input and its output (the next linear's input,
+needed for that weight's gradient) take 4 bytes an element.  ``gelu_checkpoint8`` keeps the input as
+8-bit codes with a float32 scale for 128 features (1.03 bytes), ``gelu_linear_checkpoint8`` lets the next
+linear's gradient take its input from the same codes, so that the activation is not kept at all.
+"""
+from __future__ import annotations
+
+import torch
+from torch import nn
+from torch.autograd.function import once_differentiable
+
+from . import layer_ops
+
+
+class Checkpoint8:
+    """What is kept of GELU's input z: int8 ``codes``, float32 ``scales`` for groups of 128 features;
+    they stand for ``codes * scale``."""
+
+    def __init__(self, codes, scales, shape, dtype, approximate):
+        self.codes, self.scales = codes, scales
+        self.shape, self.dtype, self.approximate = tuple(shape), dtype, approximate
+
+    def values(self) -> torch.Tensor:
+        """What the codes stand for, in float32 and the input's shape."""
+        features = self.shape[-1]
+        scale = self.scales.repeat_interleave(layer_ops.GELU8_GROUP, dim=1)[:, :features]
+        return (self.codes[:, :features].float() * scale).reshape(self.shape)
+
+    def activation(self) -> torch.Tensor:
+        """GELU of what the codes stand for, in the input's type and shape."""
+        return layer_ops.gelu8_activation(self.codes, self.scales, self.shape, self.dtype, self.approximate)
+
+    def nbytes(self) -> int:
+        return self.codes.numel() + 4 * self.scales.numel()
+
+
+class _Gelu8Fn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, bias, approximate, holder):
+        out, codes, scales = layer_ops.gelu8_forward(x, bias, approximate, True)
+        holder.append(Checkpoint8(codes, scales, x.shape, x.dtype, approximate))
+        ctx.save_for_backward(codes, scales)
+        ctx.meta = (x.dtype, approximate)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        codes, scales = ctx.saved_tensors
+        gx, gb = layer_ops.gelu8_backward(codes, scales, grad_out, *ctx.meta, ctx.needs_input_grad[1])
+        return gx, gb, None, None
+
+
+def gelu_checkpoint8(x: torch.Tensor, bias: torch.Tensor | None = None, approximate: str = "none",
+                     return_checkpoint: bool = False):
+    """``gelu(x + bias)`` over any leading dimensions; ``approximate`` as ``torch.nn.functional.gelu``'s.
+
+    The forward value is exact (float32, rounded once); the backward pass takes the derivative at
+    the 8-bit checkpoint of ``x + bias``.  With ``return_checkpoint`` returns ``(activation,
+    Checkpoint8)``.  Where no gradient is recorded and no checkpoint asked for, nothing is kept."""
+    recorded = torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad))
+    if recorded:
+        holder: list[Checkpoint8] = []
+        out = _Gelu8Fn.apply(x, bias, approximate, holder)
+        return (out, holder[0]) if return_checkpoint else out
+    out, codes, scales = layer_ops.gelu8_forward(x, bias, approximate, return_checkpoint)
+    return (out, Checkpoint8(codes, scales, x.shape, x.dtype, approximate)) if return_checkpoint else out
+
+
+def gelu_linear_checkpoint8(x: torch.Tensor, linear: nn.Module, bias: torch.Tensor | None = None,
+                            approximate: str = "none") -> torch.Tensor:
+    """``linear(gelu(x + bias))`` that keeps 1.03 bytes of each hidden element.
+
+    What ``linear`` (a ``BlockFHTLinear``, cached or not, or any other module) saves of its input for the
+    backward pass is replaced by the checkpoint and computed again from it there; the weight's (or
+    latent's) gradient is then that of the checkpoint's activation."""
+    if not torch.is_grad_enabled():
+        return linear(gelu_checkpoint8(x, bias, approximate))
+    y, checkpoint = gelu_checkpoint8(x, bias, approximate, return_checkpoint=True)
+    span = (y.data_ptr(), y.numel(), y.dtype)
+
+    def pack(t):
+        # the activation itself or a dense view of all of it (flattened rows)
+        if t.is_cuda and (t.data_ptr(), t.numel(), t.dtype) == span and t.is_contiguous() and t.numel():
+            return tuple(t.shape)
+        return t
+
+    def unpack(kept):
+        return checkpoint.activation().view(kept) if isinstance(kept, tuple) else kept
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+        return linear(y)
