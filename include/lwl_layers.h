@@ -30,20 +30,13 @@ extern "C" {
  * (float32 [2][rows]: mu, then s) is what the backward needs and may be NULL.  out and sum may not
  * overlap the inputs.
  */
-typedef struct lwl_layer_norm_args {
-  int32_t dtype, weight_dtype;
-  int64_t rows, features;
-  double eps;
-  const void *x, *residual, *weight, *bias;
-  void *out, *sum;
-  float* stats;
-} lwl_layer_norm_args;
+int lwl_layer_norm_check(int dtype, int weight_dtype, int64_t rows, int64_t features, double eps); /* host only */
+int lwl_layer_norm_forward(const void* x, const void* residual, const void* weight, const void* bias, int dtype,
+                           int weight_dtype, int64_t rows, int64_t features, double eps, void* out, void* sum,
+                           float* stats, void* stream);
 
-int lwl_layer_norm_check(const lwl_layer_norm_args* args); /* host only; does not look at pointers */
-int lwl_layer_norm_forward(const lwl_layer_norm_args* args, void* stream);
-
-/* Backward: args->x is h (x, or the stored sum), args->weight and args->stats as in the forward; the
- * other pointers of args are not read.  With n = (h - mu) s, a = grad_out * weight:
+/* Backward: h is what was normed (x, or the stored sum), stats as the forward left it.  With
+ * n = (h - mu) s, a = grad_out * weight:
  *
  *   grad_x = s (a - mean(a) - n mean(a n)) + grad_sum     (of x, and of residual: the same)
  *   grad_weight = sum over rows of grad_out * n,  grad_bias = sum over rows of grad_out
@@ -52,7 +45,8 @@ int lwl_layer_norm_forward(const lwl_layer_norm_args* args, void* stream);
  * over rows run in a fixed order.
  */
 size_t lwl_layer_norm_backward_workspace_size(int64_t rows, int64_t features);
-int lwl_layer_norm_backward(const lwl_layer_norm_args* args, const void* grad_out, const void* grad_sum,
+int lwl_layer_norm_backward(const void* h, const void* weight, const float* stats, const void* grad_out,
+                            const void* grad_sum, int dtype, int weight_dtype, int64_t rows, int64_t features,
                             void* grad_x, void* grad_weight, void* grad_bias, void* workspace,
                             size_t workspace_bytes, void* stream);
 
@@ -61,27 +55,23 @@ int lwl_layer_norm_backward(const lwl_layer_norm_args* args, const void* grad_ou
  * tanh_form its tanh approximation.  Kept of z: for each row and each group of
  * LWL_GELU8_GROUP consecutive features one float32 scale s = max|z| / 127 and int8 codes
  * c = rint(z / s), standing for c * s.  codes: rows of lwl_gelu8_pitch(features) bytes, 8-byte aligned;
- * scales: float32 rows of ceil(features / LWL_GELU8_GROUP).  codes == NULL (then scales is not read)
- * keeps nothing.  A group of values below 2^-100 stands for zeros; one with an infinity or a NaN
- * stands for NaN.
+ * scales: float32 rows of ceil(features / LWL_GELU8_GROUP).  In the forward codes == NULL (then scales is
+ * not read) keeps nothing.  A group of values below 2^-100 stands for zeros; one with an infinity or a
+ * NaN stands for NaN.
  */
 #define LWL_GELU8_GROUP 128
-typedef struct lwl_gelu8_args {
-  int32_t dtype, tanh_form;
-  int64_t rows, features;
-  int8_t* codes;
-  float* scales;
-} lwl_gelu8_args;
-
 int64_t lwl_gelu8_pitch(int64_t features);
-int lwl_gelu8_check(const lwl_gelu8_args* args); /* host only; does not look at pointers */
-int lwl_gelu8_forward(const lwl_gelu8_args* args, const void* x, const void* bias, void* out, void* stream);
+int lwl_gelu8_check(int dtype, int64_t rows, int64_t features); /* host only */
+int lwl_gelu8_forward(const void* x, const void* bias, int dtype, int tanh_form, int64_t rows, int64_t features,
+                      void* out, int8_t* codes, float* scales, void* stream);
 /* out = gelu(c * s): the activation again, from the checkpoint. */
-int lwl_gelu8_activation(const lwl_gelu8_args* args, void* out, void* stream);
+int lwl_gelu8_activation(const int8_t* codes, const float* scales, int dtype, int tanh_form, int64_t rows,
+                         int64_t features, void* out, void* stream);
 /* grad_x = grad_out * gelu'(c * s); grad_bias (may be NULL): its sum over rows, in a fixed order. */
 size_t lwl_gelu8_backward_workspace_size(int64_t rows, int64_t features);
-int lwl_gelu8_backward(const lwl_gelu8_args* args, const void* grad_out, void* grad_x, void* grad_bias,
-                       void* workspace, size_t workspace_bytes, void* stream);
+int lwl_gelu8_backward(const int8_t* codes, const float* scales, const void* grad_out, int dtype, int tanh_form,
+                       int64_t rows, int64_t features, void* grad_x, void* grad_bias, void* workspace,
+                       size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------- attention
  * For each sequence b and query head h, whose key head is h / (heads / kv_heads):

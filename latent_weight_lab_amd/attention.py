@@ -9,7 +9,6 @@ gradients do not depend on the order in which workgroups run.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native as N
 from . import layer_ops
@@ -24,7 +23,7 @@ class _AttentionFn(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @layer_ops.once
     def backward(ctx, grad_out):
         q, k, v, out, lse, lengths = ctx.saved_tensors
         causal, scale, offset = ctx.meta
@@ -77,7 +76,7 @@ class _PackedFn(torch.autograd.Function):
         return out.transpose(1, 2).reshape(*qkv.shape[:2], -1)
 
     @staticmethod
-    @once_differentiable
+    @layer_ops.once
     def backward(ctx, grad_out):
         qkv, out, lse, lengths = ctx.saved_tensors
         heads, kv_heads, causal, scale, offset = ctx.meta

@@ -24,7 +24,7 @@ namespace lwl {
 namespace {
 
 constexpr int kBlock = 128;  // keys (queries) of a workgroup: 32 for each of four waves
-constexpr int kTile = 64;    // queries (keys) of a tile
+constexpr int kTile = kTileRows;  // queries (keys) of a tile
 
 // In dV's product the probabilities are 2^kLift times too large (exact, and taken back at the end): dV sums
 // a key's probabilities over the queries, all of which may be small, and small ones are subnormal in
@@ -34,40 +34,8 @@ constexpr float kLift = 14.0f, kLower = 0x1p-14f;
 template <class T, int DP>
 struct BwdTile {
   static constexpr int S = DP + 16 / (int)sizeof(T);  // LDS row: 16-byte reads of 16 rows on distinct banks
-  static constexpr int CPR = DP / 8;
-  static constexpr int PER = kTile * CPR / 256;
 };
 
-// Rows row0 .. + 63 of base that ok() allows, else zeros.
-template <class T, int DP, class Ok>
-__device__ __forceinline__ void fetch_rows(Raw8<T>* r, const T* base, int64_t stride, int64_t row0, int dim, Ok ok) {
-  using Tile = BwdTile<T, DP>;
-#pragma unroll
-  for (int i = 0; i < Tile::PER; ++i) {
-    const int c = threadIdx.x + i * 256, row = c / Tile::CPR, col = (c % Tile::CPR) * 8;
-    load_raw8(r[i], base + (row0 + row) * stride + col, ok(row0 + row) ? dim - col : 0);
-  }
-}
-template <class T, int DP>
-__device__ __forceinline__ void stage_rows(T* lds, const Raw8<T>* r) {
-  using Tile = BwdTile<T, DP>;
-#pragma unroll
-  for (int i = 0; i < Tile::PER; ++i) {
-    const int c = threadIdx.x + i * 256;
-    lds_put(lds + (c / Tile::CPR) * Tile::S + (c % Tile::CPR) * 8, r[i]);
-  }
-}
-template <class T, int DP>
-__device__ __forceinline__ void load_operand(Frag<T> (&f)[DP / 16], const T* row, int dim, bool ok) {
-  const int half = (threadIdx.x & 63) >> 5;
-#pragma unroll
-  for (int kk = 0; kk < DP / 16; ++kk) {
-    const int col = kk * 16 + half * 8;
-    Raw8<T> r;
-    load_raw8(r, row + col, ok ? dim - col : 0);
-    f[kk] = frag_of(r);
-  }
-}
 // A result whose columns are rows of a tensor: lane's row, values 8 r4 + 4 half .. + 3 of each 32.
 template <class T, int DP>
 __device__ __forceinline__ void store_rows(T* row, const f32x16 (&v)[DP / 32], float scale, int dim) {
@@ -83,101 +51,146 @@ __device__ __forceinline__ void store_rows(T* row, const f32x16 (&v)[DP / 32], f
     }
 }
 
-// work: [rows] log2 units of lse, [rows] D
-template <class T>
+// work: [rows] lse in units of log2, [rows] D.  LANES lanes of eight values a row.
+template <class T, int LANES>
 __global__ __launch_bounds__(256) void attention_bwd_rows(const AttnArgs a) {
-  const int lane = threadIdx.x & 15;
-  const int64_t rows = a.batch * a.heads * a.queries;
-  const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-  const bool live = row < rows;
-  const int64_t rr = live ? row : 0;
-  const int64_t b = rr / (a.heads * a.queries), h = rr / a.queries % a.heads, q = rr % a.queries;
+  constexpr uint32_t PER = 256 / LANES;  // rows of a workgroup, all of one head
+  const int lane = threadIdx.x & (LANES - 1);
+  const uint32_t queries = (uint32_t)a.queries, heads = (uint32_t)a.heads, blocks = (queries + PER - 1) / PER;
+  const uint32_t bh = blockIdx.x / blocks, q = (blockIdx.x - bh * blocks) * PER + threadIdx.x / LANES;
+  const int64_t b = uniform((int)(bh / heads)), h = uniform((int)(bh % heads));
+  const int64_t rows = a.batch * a.heads * a.queries, row = (int64_t)bh * queries + q;
+  const Allowed allow = allowed_keys(a, b);
+  const bool live = q < queries;
   const int col = lane * 8, n = live ? (int)a.dim - col : 0;
   float o[8], g[8], s = 0.0f;
-  load8(o, (const T*)a.out + b * a.os[0] + h * a.os[1] + q * a.os[2] + col, n);
-  load8(g, (const T*)a.dout + b * a.dos[0] + h * a.dos[1] + q * a.dos[2] + col, n);
+  load8(o, (const T*)a.out + b * a.os[0] + h * a.os[1] + (int64_t)q * a.os[2] + col, n);
+  load8(g, (const T*)a.dout + b * a.dos[0] + h * a.dos[1] + (int64_t)q * a.dos[2] + col, n);
 #pragma unroll
   for (int i = 0; i < 8; ++i) s += o[i] * g[i];
-  s = lanes_sum<16>(s);
+  s = lanes_sum<LANES>(s);
   if (!live || lane != 0) return;
-  const bool none = key_end(allowed_keys(a, b), q) == 0;
+  const bool none = key_end(allow, (int)q) == 0;
   a.work[row] = none ? INFINITY : a.lse[row] * kLog2E;
   a.work[rows + row] = none ? 0.0f : s;
 }
 
-template <class T, int DP>
-__global__ __launch_bounds__(256) void attention_bwd_keys(const AttnArgs a) {
+template <class T, int DP, bool FAST>
+__global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void attention_bwd_keys(const AttnArgs a) {
   using Tile = BwdTile<T, DP>;
   constexpr int KK = DP / 16, DT = DP / 32;
-  __shared__ __attribute__((aligned(16))) T lds_q[kTile * Tile::S];
-  __shared__ __attribute__((aligned(16))) T lds_g[kTile * Tile::S];
-  __shared__ __attribute__((aligned(16))) float lds_stat[2][kTile];
-  const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
-  const int64_t kvb = a.batch * a.kv_heads, group = a.heads / a.kv_heads;
-  const int64_t bk = (int64_t)blockIdx.x % kvb, b = bk / a.kv_heads, hk = bk % a.kv_heads;
-  const int64_t k0 = (int64_t)blockIdx.x / kvb * kBlock;  // causal: the first keys have the most queries
+  __shared__ __attribute__((aligned(16))) T lds_q[2][kTile * Tile::S];
+  __shared__ __attribute__((aligned(16))) T lds_g[2][kTile * Tile::S];
+  __shared__ __attribute__((aligned(16))) float lds_stat[2][2][kTile];
+  const int lane = threadIdx.x & 63, half = lane >> 5, wave = uniform((int)threadIdx.x >> 6);
+  const uint32_t kvh = (uint32_t)a.kv_heads, kvb = (uint32_t)a.batch * kvh, group = (uint32_t)a.heads / kvh;
+  const uint32_t id = work_order(blockIdx.x, gridDim.x, (uint32_t)a.cus), bk = id % kvb;
+  const int64_t b = uniform((int)(bk / kvh)), hk = uniform((int)(bk % kvh));
+  const int k0 = uniform((int)(id / kvb)) * kBlock;  // causal: the first keys have the most queries
   const int dim = (int)a.dim;
   const Allowed allow = allowed_keys(a, b);
-  const int seen = key_end(allow, a.queries - 1);  // keys that some query sees
-  const int64_t key = k0 + wave * 32 + (lane & 31);
+  const int queries = (int)a.queries;
+  const int seen = key_end(allow, queries - 1);  // keys that some query sees
+  const int wk0 = k0 + wave * 32, key = wk0 + (lane & 31);
   Frag<T> kf[KK], vf[KK];
-  load_operand<T, DP>(kf, (const T*)a.k + b * a.ks[0] + hk * a.ks[1] + key * a.ks[2], dim, key < seen);
-  load_operand<T, DP>(vf, (const T*)a.v + b * a.vs[0] + hk * a.vs[1] + key * a.vs[2], dim, key < seen);
+  load_operand<T, DP>(kf, (const T*)a.k + b * a.ks[0] + hk * a.ks[1] + (int64_t)key * a.ks[2], dim, key < seen);
+  load_operand<T, DP>(vf, (const T*)a.v + b * a.vs[0] + hk * a.vs[1] + (int64_t)key * a.vs[2], dim, key < seen);
   f32x16 dk[DT] = {}, dv[DT] = {};
-  const float c = a.scale * kLog2E;
-  // queries before k0 - off see none of the block's keys
-  const int64_t first = k0 >= seen ? a.queries : std::max<int64_t>(0, k0 - allow.off) / kTile * kTile;
+  // The products start from what is to be subtracted: S - lse / c, with c = scale log2(e), and dP - D.
+  const float c = a.scale * kLog2E, inv_c = 1.0f / c;
+  // queries before k0 - off see none of the block's keys (so none that sees nothing is ever read), those
+  // before wk0 - off none of the wave's
+  const int first = k0 >= seen ? queries : std::max(0, k0 - allow.off);
+  const int wave_first = wk0 >= seen ? queries : wk0 - allow.off;
   const int64_t rows = a.batch * a.heads * a.queries;
-  auto ok = [&](int64_t q) { return q < a.queries && key_end(allow, q) > 0; };
-  for (int64_t g = 0; g < group; ++g) {
-    const int64_t h = hk * group + g;
-    const T* qp = (const T*)a.q + b * a.qs[0] + h * a.qs[1];
-    const T* gp = (const T*)a.dout + b * a.dos[0] + h * a.dos[1];
-    const float* stat = a.work + (b * a.heads + h) * a.queries;
-    Raw8<T> qr[Tile::PER], gr[Tile::PER];
-    float sr = 0.0f;
-    auto fetch = [&](int64_t q0) {
-      fetch_rows<T, DP>(qr, qp, a.qs[2], q0, dim, ok);
-      fetch_rows<T, DP>(gr, gp, a.dos[2], q0, dim, ok);
-      if (threadIdx.x < 2 * kTile) {
-        const int64_t q = q0 + (threadIdx.x & (kTile - 1));
-        const bool is_d = threadIdx.x >= kTile;
-        sr = q < a.queries ? stat[(is_d ? rows : 0) + q] : (is_d ? 0.0f : INFINITY);
-        sr = is_d ? sr * kLower : sr - kLift;
-      }
-    };
-    if (first < a.queries) fetch(first);
-    for (int64_t q0 = first; q0 < a.queries; q0 += kTile) {
-      __syncthreads();  // the previous tile has been read
-      stage_rows<T, DP>(lds_q, qr);
-      stage_rows<T, DP>(lds_g, gr);
-      if (threadIdx.x < 2 * kTile) lds_stat[threadIdx.x / kTile][threadIdx.x & (kTile - 1)] = sr;
-      __syncthreads();
-      if (q0 + kTile < a.queries) fetch(q0 + kTile);
-      const bool masked = key_end(allow, q0) < k0 + kBlock;  // some pair of the tile is not allowed
-#pragma unroll
+  const T* qp = (const T*)a.q + b * a.qs[0] + hk * group * a.qs[1];
+  const T* gp = (const T*)a.dout + b * a.dos[0] + hk * group * a.dos[1];
+  const float* stat = a.work + (b * a.heads + hk * group) * a.queries;
+  TileLoader<T, DP, FAST> qt, gt;
+  qt.init(qp, a.qs[2], dim);
+  gt.init(gp, a.dos[2], dim);
+  float sr = 0.0f;
+  // tiles of the first head, then of the next one of the group: one sequence of loads
+  uint32_t g = 0;
+  int q0 = first;
+  auto fetch = [&](uint32_t fg, int fq) {
+    qt.base = qp + fg * a.qs[1];
+    gt.base = gp + fg * a.dos[1];
+    qt.fetch(fq, queries);
+    gt.fetch(fq, queries);
+    if (threadIdx.x < 2 * kTile) {
+      const int q = fq + (threadIdx.x & (kTile - 1));
+      const bool is_d = threadIdx.x >= kTile;
+      sr = q < queries ? stat[(int64_t)fg * queries + (is_d ? rows : 0) + q] : (is_d ? 0.0f : INFINITY);
+      sr = is_d ? -sr : (kLift - sr) * inv_c;
+    }
+  };
+  auto put = [&](int buf) {
+    qt.template put<Tile::S>(lds_q[buf]);
+    gt.template put<Tile::S>(lds_g[buf]);
+    if (threadIdx.x < 2 * kTile) lds_stat[buf][threadIdx.x / kTile][threadIdx.x & (kTile - 1)] = sr;
+  };
+  int buf = 0;
+  if (first < queries) {
+    fetch(0, first);
+    put(0);
+  }
+  while (g < group && q0 < queries) {
+    __syncthreads();  // this tile is there, the one before has been read
+    const bool last = q0 + kTile >= queries;
+    const uint32_t next_g = last ? g + 1 : g;
+    const int next_q = last ? first : q0 + kTile;
+    if (next_g < group) fetch(next_g, next_q);
+    if (q0 + kTile > wave_first) {
+      const bool masked = key_end(allow, q0) < wk0 + 32;  // some pair of the tile is not allowed
+#pragma unroll 1
       for (int t = 0; t < 2; ++t) {
-        f32x16 s = {}, dp = {};
+        const int at = t * 32;
+        const T* lq = lds_q[buf] + at * Tile::S;
+        const T* lg = lds_g[buf] + at * Tile::S;
+        f32x16 s, dp;
+        {
+          Frag<T> qf[KK], gf[KK];
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-          const int at = (t * 32 + (lane & 31)) * Tile::S + kk * 16 + half * 8;
-          s = mma32(lds_frag(lds_q + at), kf[kk], s);
-          dp = mma32(lds_frag(lds_g + at), vf[kk], dp);
-        }
+          for (int r4 = 0; r4 < 4; ++r4) {
+            const f32x4 l = *(const f32x4*)&lds_stat[buf][0][at + r4 * 8 + half * 4];
+            const f32x4 d = *(const f32x4*)&lds_stat[buf][1][at + r4 * 8 + half * 4];
 #pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4) {
-          const f32x4 l = *(const f32x4*)&lds_stat[0][t * 32 + r4 * 8 + half * 4];
-          const f32x4 d = *(const f32x4*)&lds_stat[1][t * 32 + r4 * 8 + half * 4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int i = r4 * 4 + r;
-            s[i] = exp2_hw(fmaf(s[i], c, -l[r]));
-            dp[i] = s[i] * fmaf(dp[i], kLower, -d[r]);
+            for (int r = 0; r < 4; ++r) {
+              s[r4 * 4 + r] = l[r];
+              dp[r4 * 4 + r] = d[r];
+            }
           }
+#pragma unroll
+          for (int kk = 0; kk < KK; ++kk) {
+            qf[kk] = lds_frag(lq + (lane & 31) * Tile::S + kk * 16 + half * 8);
+            gf[kk] = lds_frag(lg + (lane & 31) * Tile::S + kk * 16 + half * 8);
+          }
+          fence_schedule<T>();
+#pragma unroll
+          for (int kk = 0; kk < KK; ++kk) {
+            s = mma32(qf[kk], kf[kk], s);
+            dp = mma32(gf[kk], vf[kk], dp);
+          }
+        }
+        Frag<T> gc[2][DT], qc[2][DT];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            const int row = u * 16 + half * 4;
+            gc[u][d] = lds_column_frag(lg, Tile::S, row, row + 8, d * 32 + (lane & 16));
+            qc[u][d] = lds_column_frag(lq, Tile::S, row, row + 8, d * 32 + (lane & 16));
+          }
+        fence_schedule<T>();
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[r] = exp2_hw(s[r] * c);
+          dp[r] = s[r] * (dp[r] * kLower);
         }
         if (masked) {
           // key < key_end(q), that is q >= key - off
-          const int64_t from = key < allow.len ? key - allow.off - q0 - t * 32 - half * 4 : kTile;
+          const int from = key < allow.len ? key - allow.off - q0 - at - half * 4 : kTile;
 #pragma unroll
           for (int r = 0; r < 16; ++r)
             if ((r >> 2) * 8 + (r & 3) < from) s[r] = dp[r] = 0.0f;
@@ -190,113 +203,157 @@ __global__ __launch_bounds__(256) void attention_bwd_keys(const AttnArgs a) {
             p[r] = (T)s[u * 8 + r];
             ds[r] = (T)dp[u * 8 + r];
           }
-          const int row = t * 32 + u * 16 + half * 4;
 #pragma unroll
           for (int d = 0; d < DT; ++d) {
-            dv[d] = mma32(lds_column_frag(lds_g, Tile::S, row, row + 8, d * 32 + (lane & 16)), p, dv[d]);
-            dk[d] = mma32(lds_column_frag(lds_q, Tile::S, row, row + 8, d * 32 + (lane & 16)), ds, dk[d]);
+            dv[d] = mma32(gc[u][d], p, dv[d]);
+            dk[d] = mma32(qc[u][d], ds, dk[d]);
           }
         }
       }
     }
+    if (next_g < group) put(buf ^ 1);
+    buf ^= 1;
+    g = next_g;
+    q0 = next_q;
   }
-  if (key >= a.keys) return;
-  store_rows<T, DP>((T*)a.dk + b * a.dks[0] + hk * a.dks[1] + key * a.dks[2], dk, a.scale, dim);
-  store_rows<T, DP>((T*)a.dv + b * a.dvs[0] + hk * a.dvs[1] + key * a.dvs[2], dv, kLower, dim);
+  if (key >= (int)a.keys) return;
+  store_rows<T, DP>((T*)a.dk + b * a.dks[0] + hk * a.dks[1] + (int64_t)key * a.dks[2], dk, a.scale, dim);
+  store_rows<T, DP>((T*)a.dv + b * a.dvs[0] + hk * a.dvs[1] + (int64_t)key * a.dvs[2], dv, kLower, dim);
 }
 
-template <class T, int DP>
-__global__ __launch_bounds__(256) void attention_bwd_queries(const AttnArgs a) {
+template <class T, int DP, bool FAST>
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_bwd_queries(const AttnArgs a) {
   using Tile = BwdTile<T, DP>;
   constexpr int KK = DP / 16, DT = DP / 32;
-  __shared__ __attribute__((aligned(16))) T lds_k[kTile * Tile::S];
-  __shared__ __attribute__((aligned(16))) T lds_v[kTile * Tile::S];
-  const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
-  const int64_t kvb = a.batch * a.kv_heads, group = a.heads / a.kv_heads, nbh = kvb * group;
-  const int64_t bh = (int64_t)blockIdx.x % nbh, id = (int64_t)blockIdx.x / nbh;
-  const int64_t qblocks = (a.queries + kBlock - 1) / kBlock;
-  const int64_t q0 = (qblocks - 1 - id) * kBlock;
-  const int64_t b = (bh % kvb) / a.kv_heads, hk = (bh % kvb) % a.kv_heads, h = hk * group + bh / kvb;
+  __shared__ __attribute__((aligned(16))) T lds_k[2][kTile * Tile::S];
+  __shared__ __attribute__((aligned(16))) T lds_v[2][kTile * Tile::S];
+  const int lane = threadIdx.x & 63, half = lane >> 5, wave = uniform((int)threadIdx.x >> 6);
+  const uint32_t kvh = (uint32_t)a.kv_heads, kvb = (uint32_t)a.batch * kvh, group = (uint32_t)a.heads / kvh;
+  const uint32_t id = work_order(blockIdx.x, gridDim.x, (uint32_t)a.cus);
+  const uint32_t nbh = kvb * group, bh = id % nbh, kv = bh % kvb;
+  const uint32_t qblocks = (uint32_t)((a.queries + kBlock - 1) / kBlock);
+  const int q0 = uniform((int)(qblocks - 1 - id / nbh)) * kBlock;
+  const int64_t b = uniform((int)(kv / kvh)), hk = uniform((int)(kv % kvh)), h = hk * group + uniform((int)(bh / kvb));
   const int dim = (int)a.dim;
   const Allowed allow = allowed_keys(a, b);
-  const int64_t q = q0 + wave * 32 + (lane & 31);
-  const int q_end = q < a.queries ? key_end(allow, q) : 0;
-  const int end = key_end(allow, std::min<int64_t>(q0 + kBlock, a.queries) - 1);
-  const int64_t wq0 = q0 + wave * 32;
-  const int free_end = wq0 < a.queries ? key_end(allow, wq0) : 0;
+  const int queries = (int)a.queries, wq0 = q0 + wave * 32, q = wq0 + (lane & 31);
+  const int q_end = q < queries ? key_end(allow, q) : 0;
+  const int end = key_end(allow, std::min(q0 + kBlock, queries) - 1);
+  const int free_end = wq0 < queries ? key_end(allow, wq0) : 0;
+  const int wave_end = wq0 < queries ? key_end(allow, std::min(wq0 + 32, queries) - 1) : 0;
   const T* kp = (const T*)a.k + b * a.ks[0] + hk * a.ks[1];
   const T* vp = (const T*)a.v + b * a.vs[0] + hk * a.vs[1];
+  TileLoader<T, DP, FAST> kt, vt;
+  kt.init(kp, a.ks[2], dim);
+  vt.init(vp, a.vs[2], dim);
+  if (end > 0) {
+    kt.fetch(0, end);
+    vt.fetch(0, end);
+  }
   Frag<T> qf[KK], gf[KK];
-  load_operand<T, DP>(qf, (const T*)a.q + b * a.qs[0] + h * a.qs[1] + q * a.qs[2], dim, q_end > 0);
-  load_operand<T, DP>(gf, (const T*)a.dout + b * a.dos[0] + h * a.dos[1] + q * a.dos[2], dim, q_end > 0);
+  load_operand<T, DP>(qf, (const T*)a.q + b * a.qs[0] + h * a.qs[1] + (int64_t)q * a.qs[2], dim, q_end > 0);
+  load_operand<T, DP>(gf, (const T*)a.dout + b * a.dos[0] + h * a.dos[1] + (int64_t)q * a.dos[2], dim, q_end > 0);
   const int64_t rows = a.batch * a.heads * a.queries, row = (b * a.heads + h) * a.queries + q;
-  const float lse = q < a.queries ? a.work[row] : INFINITY, delta = q < a.queries ? a.work[rows + row] : 0.0f;
+  const float lse = q < queries ? a.work[row] : INFINITY, delta = q < queries ? a.work[rows + row] : 0.0f;
   f32x16 dq[DT] = {};
   const float c = a.scale * kLog2E;
-  auto ok = [&](int64_t j) { return j < end; };
-  Raw8<T> kr[Tile::PER], vr[Tile::PER];
-  auto fetch = [&](int j0) {
-    fetch_rows<T, DP>(kr, kp, a.ks[2], j0, dim, ok);
-    fetch_rows<T, DP>(vr, vp, a.vs[2], j0, dim, ok);
-  };
-  if (end > 0) fetch(0);
-  for (int j0 = 0; j0 < end; j0 += kTile) {
-    __syncthreads();
-    stage_rows<T, DP>(lds_k, kr);
-    stage_rows<T, DP>(lds_v, vr);
-    __syncthreads();
-    if (j0 + kTile < end) fetch(j0 + kTile);
+  if (end > 0) {
+    kt.template put<Tile::S>(lds_k[0]);
+    vt.template put<Tile::S>(lds_v[0]);
+  }
+  int buf = 0;
+  for (int j0 = 0; j0 < end; j0 += kTile, buf ^= 1) {
+    __syncthreads();  // this tile is there, the one before has been read
+    const bool more = j0 + kTile < end;
+    if (more) {
+      kt.fetch(j0 + kTile, end);
+      vt.fetch(j0 + kTile, end);
+    }
+    if (j0 < wave_end) {
+#pragma unroll 1
+      for (int t = 0; t < 2; ++t) {
+        const T* lk = lds_k[buf] + t * 32 * Tile::S;
+        const T* lv = lds_v[buf] + t * 32 * Tile::S;
+        f32x16 s = {}, dp = {};
+        {
+          Frag<T> kf[KK], vf[KK];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      f32x16 s = {}, dp = {};
+          for (int kk = 0; kk < KK; ++kk) {
+            kf[kk] = lds_frag(lk + (lane & 31) * Tile::S + kk * 16 + half * 8);
+            vf[kk] = lds_frag(lv + (lane & 31) * Tile::S + kk * 16 + half * 8);
+          }
+          fence_schedule<T>();
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk) {
-        const int at = (t * 32 + (lane & 31)) * Tile::S + kk * 16 + half * 8;
-        s = mma32(lds_frag(lds_k + at), qf[kk], s);
-        dp = mma32(lds_frag(lds_v + at), gf[kk], dp);
-      }
+          for (int kk = 0; kk < KK; ++kk) {
+            s = mma32(kf[kk], qf[kk], s);
+            dp = mma32(vf[kk], gf[kk], dp);
+          }
+        }
+        Frag<T> kc[2][DT];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = exp2_hw(fmaf(s[r], c, -lse)) * (dp[r] - delta);
-      if (j0 + kTile > free_end) {
-        const int lim = q_end - j0 - t * 32 - half * 4;
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if ((r >> 2) * 8 + (r & 3) >= lim) s[r] = 0.0f;
-      }
+          for (int d = 0; d < DT; ++d)
+            kc[u][d] = lds_column_frag(lk, Tile::S, u * 16 + half * 4, u * 16 + half * 4 + 8, d * 32 + (lane & 16));
+        fence_schedule<T>();
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        Frag<T> ds;
+        for (int r = 0; r < 16; ++r) s[r] = exp2_hw(fmaf(s[r], c, -lse)) * (dp[r] - delta);
+        if (j0 + kTile > free_end) {
+          const int lim = q_end - j0 - t * 32 - half * 4;
 #pragma unroll
-        for (int r = 0; r < 8; ++r) ds[r] = (T)s[u * 8 + r];
-        const int krow = t * 32 + u * 16 + half * 4;
+          for (int r = 0; r < 16; ++r)
+            if ((r >> 2) * 8 + (r & 3) >= lim) s[r] = 0.0f;
+        }
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
-          dq[d] = mma32(lds_column_frag(lds_k, Tile::S, krow, krow + 8, d * 32 + (lane & 16)), ds, dq[d]);
+        for (int u = 0; u < 2; ++u) {
+          Frag<T> ds;
+#pragma unroll
+          for (int r = 0; r < 8; ++r) ds[r] = (T)s[u * 8 + r];
+#pragma unroll
+          for (int d = 0; d < DT; ++d) dq[d] = mma32(kc[u][d], ds, dq[d]);
+        }
       }
     }
+    if (more) {
+      kt.template put<Tile::S>(lds_k[buf ^ 1]);
+      vt.template put<Tile::S>(lds_v[buf ^ 1]);
+    }
   }
-  if (q >= a.queries) return;
-  store_rows<T, DP>((T*)a.dq + b * a.dqs[0] + h * a.dqs[1] + q * a.dqs[2], dq, a.scale, dim);
+  if (q >= queries) return;
+  store_rows<T, DP>((T*)a.dq + b * a.dqs[0] + h * a.dqs[1] + (int64_t)q * a.dqs[2], dq, a.scale, dim);
+}
+
+template <class T, int DP, bool FAST>
+hipError_t launch(const AttnArgs& a, hipStream_t s) {
+  const int64_t kgrid = a.batch * a.kv_heads * ((a.keys + kBlock - 1) / kBlock);
+  const int64_t qgrid = a.batch * a.heads * ((a.queries + kBlock - 1) / kBlock);
+  if (kgrid > 0) {
+    hipLaunchKernelGGL((attention_bwd_keys<T, DP, FAST>), dim3((unsigned)kgrid), dim3(256), 0, s, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  if (qgrid > 0)
+    hipLaunchKernelGGL((attention_bwd_queries<T, DP, FAST>), dim3((unsigned)qgrid), dim3(256), 0, s, a);
+  return hipGetLastError();
 }
 
 template <class T, int DP>
 hipError_t run(const AttnArgs& a, hipStream_t s) {
-  const int64_t kgrid = a.batch * a.kv_heads * ((a.keys + kBlock - 1) / kBlock);
-  const int64_t qgrid = a.batch * a.heads * ((a.queries + kBlock - 1) / kBlock);
-  if (kgrid > 0) {
-    hipLaunchKernelGGL((attention_bwd_keys<T, DP>), dim3((unsigned)kgrid), dim3(256), 0, s, a);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-  }
-  if (qgrid > 0) hipLaunchKernelGGL((attention_bwd_queries<T, DP>), dim3((unsigned)qgrid), dim3(256), 0, s, a);
-  return hipGetLastError();
+  const bool fast = a.dim % 8 == 0 && fast_rows(a.q, a.qs, sizeof(T)) && fast_rows(a.k, a.ks, sizeof(T)) &&
+                    fast_rows(a.v, a.vs, sizeof(T)) && fast_rows(a.dout, a.dos, sizeof(T));
+  return fast ? launch<T, DP, true>(a, s) : launch<T, DP, false>(a, s);
 }
 
 template <class T>
 hipError_t run_dim(const AttnArgs& a, hipStream_t s) {
-  const int64_t rows = a.batch * a.heads * a.queries;
-  if (rows > 0) {
-    hipLaunchKernelGGL((attention_bwd_rows<T>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, s, a);
+  const int64_t bh = a.batch * a.heads;
+  if (bh > 0 && a.queries > 0) {
+    if (a.dim <= 32)
+      hipLaunchKernelGGL((attention_bwd_rows<T, 4>), dim3((unsigned)(bh * ((a.queries + 63) / 64))), dim3(256), 0, s, a);
+    else if (a.dim <= 64)
+      hipLaunchKernelGGL((attention_bwd_rows<T, 8>), dim3((unsigned)(bh * ((a.queries + 31) / 32))), dim3(256), 0, s, a);
+    else
+      hipLaunchKernelGGL((attention_bwd_rows<T, 16>), dim3((unsigned)(bh * ((a.queries + 15) / 16))), dim3(256), 0, s, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
@@ -314,6 +371,7 @@ hipError_t run_dim(const AttnArgs& a, hipStream_t s) {
 int64_t attention_bwd_work(const AttnArgs& a) { return 2 * a.batch * a.heads * a.queries; }
 
 hipError_t launch_attention_bwd(AttnArgs a, hipStream_t s) {
+  a.cus = (int)device_cus();
   switch (a.dtype) {
     case kF32: return run_dim<float>(a, s);
     case kF16: return run_dim<f16>(a, s);

@@ -93,33 +93,159 @@ __device__ __forceinline__ Frag<T> lds_column_frag(const T* tile, int stride, in
   return f;
 }
 
+// Tiles of 64 rows that a workgroup of 256 threads brings from memory through registers into LDS: fetch()
+// starts the loads, put() stores what came.  Rows from `end` on and columns past the head size are zeros.
+//
+// FAST: head size, strides and addresses are multiples of 16 bytes and a tile spans less than 2 GiB.  A
+// thread's byte offsets within a tile are then the same for every tile, the tile's address is scalar,
+// and the buffer's range check makes the zeros: no vector arithmetic for a tile.  Otherwise
+// load_raw8 with 64-bit addresses for every row.
+constexpr int kTileRows = 64;
+template <class T, int DP, bool FAST>
+struct TileLoader {
+  static constexpr int CPR = DP / 8;                    // chunks of eight values a row
+  static constexpr int PER = kTileRows * CPR / 256;     // chunks a thread brings
+  const T* base;
+  int64_t stride;
+  int dim;
+  uint32_t offset[PER];
+  Raw8<T> r[PER];
+
+  __device__ __forceinline__ void init(const T* b, int64_t s, int d) {
+    base = b;
+    stride = s;
+    dim = d;
+    if constexpr (FAST) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int c = threadIdx.x + i * 256, row = c / CPR, col = (c % CPR) * 8;
+        offset[i] = col < dim ? (uint32_t)(row * (int)stride + col) * (uint32_t)sizeof(T) : 0x80000000u;
+      }
+    }
+  }
+  // row0 and end are the same in all lanes
+  __device__ __forceinline__ void fetch(int row0, int end) {
+    if constexpr (FAST) {
+      const int left = end - row0 < kTileRows ? end - row0 : kTileRows;
+      const uint32_t bytes = left > 0 ? (uint32_t)((left - 1) * (int)stride + dim) * (uint32_t)sizeof(T) : 0u;
+      const auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base + (int64_t)row0 * stride), (short)0,
+                                                        (int)bytes, 0x00020000);
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+#pragma unroll
+        for (int j = 0; j < Raw8<T>::N; ++j)
+          r[i].q[j] = __builtin_amdgcn_raw_buffer_load_b128(rs, (int)offset[i] + 16 * j, 0, 0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int c = threadIdx.x + i * 256, row = c / CPR, col = (c % CPR) * 8;
+        load_raw8(r[i], base + (int64_t)(row0 + row) * stride + col, row0 + row < end ? dim - col : 0);
+      }
+    }
+  }
+  template <int STRIDE>
+  __device__ __forceinline__ void put(T* lds) const {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int c = threadIdx.x + i * 256;
+      lds_put(lds + (c / CPR) * STRIDE + (c % CPR) * 8, r[i]);
+    }
+  }
+};
+// Whether a tensor's rows meet FAST's terms (the head size is checked beside it).
+inline bool fast_rows(const void* p, const int64_t (&stride)[3], int64_t size) {
+  const int64_t unit = 16 / size;
+  return (uintptr_t)p % 16 == 0 && stride[0] % unit == 0 && stride[1] % unit == 0 && stride[2] % unit == 0 &&
+         stride[2] * size * kTileRows < ((int64_t)1 << 31);
+}
+
+// A row of a tensor as operands: lane l holds chunks of eight values, 8 (l / 32) + 16 kk (32-wide products).
+template <class T, int DP>
+__device__ __forceinline__ void load_operand(Frag<T> (&f)[DP / 16], const T* row, int dim, bool ok) {
+  const int half = (threadIdx.x & 63) >> 5;
+#pragma unroll
+  for (int kk = 0; kk < DP / 16; ++kk) {
+    const int col = kk * 16 + half * 8;
+    Raw8<T> r;
+    load_raw8(r, row + col, ok ? dim - col : 0);
+    f[kk] = frag_of(r);
+  }
+}
+
+// The larger of the two; a NaN stays a NaN (one instruction for three operands).
+__device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+// Nothing is moved across this point by the instruction scheduler: loads from LDS issued before it are
+// under way together, where the scheduler would issue each just before its use to save registers.
+template <class T>
+__device__ __forceinline__ void fence_schedule() {
+  // a float32 operand feeds eight instructions of 64 cycles: its load needs no such lead
+  if constexpr (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
+}
+
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float log2_hw(float x) { return __builtin_amdgcn_logf(x); }
 constexpr float kLog2E = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-// The other half's value: lane l gets lane l ^ 32's.
-__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
+__device__ __forceinline__ float max_nan(float a, float b);
 
-// Which keys a sequence's queries may see: j < len, and with causal j <= i + off.
+// The other half's value: lane l gets lane l ^ 32's.
+__device__ __forceinline__ float other_half(float v) {
+  const uint32_t u = __float_as_uint(v);
+  // the first result has the lower half's value in both halves, the second the upper half's
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+}
+// Over both halves, without choosing.
+__device__ __forceinline__ float max_halves(float v) {
+  const uint32_t u = __float_as_uint(v);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return max_nan(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// A value that is the same in all lanes of the wave, as a scalar: branches on it are then scalar branches and
+// addresses from it scalar addresses.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+  return (int64_t)(((uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32) | (uint32_t)uniform((int)v));
+}
+
+// The work of workgroup `block` when works are numbered heaviest first.  Every other `cus` of them (one for
+// each compute unit) are taken in reverse, so that where several workgroups share a compute unit from
+// the start, the one that got the heaviest first gets the lightest next.  In units of eight, so that a
+// work stays with its die (workgroups go to the eight dies in turn, and heads vary fastest).
+__device__ __forceinline__ uint32_t work_order(uint32_t block, uint32_t blocks, uint32_t cus) {
+  const uint32_t round = block / cus, first = round * cus;
+  if (!(round & 1) || first + cus > blocks || cus % 8) return block;
+  const uint32_t r = block - first;
+  return first + (cus / 8 - 1 - r / 8) * 8 + r % 8;
+}
+
+// Which keys a sequence's queries may see: j < len, and with causal j <= i + off.  Token numbers are 32 bits
+// (the C entry refuses more than 2^30), so that comparisons of wave-uniform ones are scalar.
+constexpr int kFar = (1 << 30) - 1;  // i + kFar + 1 does not overflow and is past every key
 struct Allowed {
-  int len;      // keys of this sequence
-  int64_t off;  // keys - 1 when not causal
+  int len;  // keys of this sequence
+  int off;
 };
+// For the sequence b that a whole wave works on.
 __device__ __forceinline__ Allowed allowed_keys(const AttnArgs& a, int64_t b) {
   Allowed w;
-  int64_t len = a.keys;
+  const int keys = (int)a.keys;
+  int len = keys;
   if (a.lengths) {
-    const int64_t l = a.lengths[b];
-    len = l < 0 ? 0 : l < a.keys ? l : a.keys;  // a length past the tensor would read past it
+    const int l = uniform(a.lengths[b]);
+    len = l < 0 ? 0 : l < keys ? l : keys;  // a length past the tensor would read past it
   }
-  w.len = (int)len;
-  w.off = !a.causal ? a.keys : a.bottom_right ? len - a.queries : a.causal_offset;
+  w.len = len;
+  const int given = a.causal_offset > kFar ? kFar : (int)a.causal_offset;
+  w.off = !a.causal ? kFar : a.bottom_right ? len - (int)a.queries : given;
   return w;
 }
 // First key that query i may not see.
-__device__ __forceinline__ int key_end(const Allowed& w, int64_t i) {
-  const int64_t e = i + w.off + 1;
-  return e < 0 ? 0 : e < w.len ? (int)e : w.len;
+__device__ __forceinline__ int key_end(const Allowed& w, int i) {
+  const int e = i + w.off + 1;
+  return e < 0 ? 0 : e < w.len ? e : w.len;
 }
 
 }  // namespace lwl

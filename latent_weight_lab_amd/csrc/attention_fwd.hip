@@ -31,7 +31,7 @@ namespace lwl {
 namespace {
 
 constexpr float kLift = 6.0f, kSlack = 8.0f;
-constexpr int kKeys = 64;   // keys of a tile
+constexpr int kKeys = kTileRows;  // keys of a tile
 constexpr int kWaveRows = 32;
 constexpr int kWaves = 4;
 constexpr int kRows = kWaves * kWaveRows;
@@ -44,145 +44,134 @@ template <class T, int DP>
 struct RowsTile {
   static constexpr int KS = DP + 16 / (int)sizeof(T);
   static constexpr int VS = sizeof(T) == 2 ? DP + ((DP / 32) % 2 ? 0 : 32) : DP + 8;
-  static constexpr int CPR = DP / 8;                     // chunks of eight a row
-  static constexpr int PER = kKeys * CPR / 256;          // chunks a thread brings of a tile
 };
 
-template <class T, int DP>
-__device__ __forceinline__ void fetch_tile(Raw8<T>* r, const T* base, int64_t stride, int j0,
-                                           int end, int dim) {
-  using Tile = RowsTile<T, DP>;
-#pragma unroll
-  for (int i = 0; i < Tile::PER; ++i) {
-    const int c = threadIdx.x + i * 256, row = c / Tile::CPR, col = (c % Tile::CPR) * 8;
-    // keys past the end are zeros: nothing past a sequence's length is multiplied in
-    load_raw8(r[i], base + (int64_t)(j0 + row) * stride + col, j0 + row < end ? dim - col : 0);
-  }
-}
-template <class T, int DP, int STRIDE>
-__device__ __forceinline__ void stage_tile(T* lds, const Raw8<T>* r) {
-  using Tile = RowsTile<T, DP>;
-#pragma unroll
-  for (int i = 0; i < Tile::PER; ++i) {
-    const int c = threadIdx.x + i * 256;
-    lds_put(lds + (c / Tile::CPR) * STRIDE + (c % Tile::CPR) * 8, r[i]);
-  }
-}
-
-template <class T, int DP>
-__global__ __launch_bounds__(256) void attention_rows(const AttnArgs a) {
+template <class T, int DP, bool FAST>
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_rows(const AttnArgs a) {
   using Tile = RowsTile<T, DP>;
   constexpr int KK = DP / 16, DT = DP / 32;
-  __shared__ __attribute__((aligned(16))) T lds_k[kKeys * Tile::KS];
-  __shared__ __attribute__((aligned(16))) T lds_v[kKeys * Tile::VS];
-  const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
+  __shared__ __attribute__((aligned(16))) T lds_k[2][kKeys * Tile::KS];
+  __shared__ __attribute__((aligned(16))) T lds_v[2][kKeys * Tile::VS];
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int wave = uniform((int)threadIdx.x >> 6);
   // Heads vary fastest, those that share a key head a multiple of the key heads apart; queries with
   // the most keys first (causal: the last ones).
-  const int64_t kvb = a.batch * a.kv_heads, group = a.heads / a.kv_heads, nbh = kvb * group;
-  int64_t id = blockIdx.x;
-  const int64_t bh = id % nbh;
-  id /= nbh;
-  const int split = (int)(id % a.splits);
-  id /= a.splits;
-  const int64_t qblocks = (a.queries + kRows - 1) / kRows;
-  const int64_t q0 = (qblocks - 1 - id) * kRows;
-  const int64_t b = (bh % kvb) / a.kv_heads, hk = (bh % kvb) % a.kv_heads, h = hk * group + bh / kvb;
+  const uint32_t kvh = (uint32_t)a.kv_heads, kvb = (uint32_t)a.batch * kvh, group = (uint32_t)a.heads / kvh;
+  const uint32_t nbh = kvb * group, splits = (uint32_t)a.splits, id = work_order(blockIdx.x, gridDim.x, (uint32_t)a.cus);
+  const uint32_t bh = (uint32_t)uniform((int)(id % nbh)), rest = id / nbh;
+  const int split = uniform((int)(rest % splits));
+  const uint32_t qblocks = (uint32_t)((a.queries + kRows - 1) / kRows);
+  const int q0 = uniform((int)(qblocks - 1 - rest / splits)) * kRows;
+  const uint32_t kv = bh % kvb;
+  const int64_t b = uniform((int)(kv / kvh)), hk = uniform((int)(kv % kvh)), h = hk * group + uniform((int)(bh / kvb));
   const int dim = (int)a.dim;
   const Allowed allow = allowed_keys(a, b);
-  const int64_t q = q0 + wave * kWaveRows + (lane & 31);
-  const int q_end = q < a.queries ? key_end(allow, q) : 0;  // this lane's query sees keys below
-  const int64_t last = std::min<int64_t>(q0 + kRows, a.queries) - 1;
-  const int begin = (int)std::min<int64_t>((int64_t)split * a.split_len, allow.len);
-  const int end = (int)std::min<int64_t>(key_end(allow, last), (int64_t)begin + a.split_len);
-  // keys below which every query of the wave sees: no mask
-  const int64_t wq0 = q0 + wave * kWaveRows;
-  const int free_end = wq0 < a.queries ? key_end(allow, wq0) : 0;
+  const int queries = (int)a.queries, wq0 = q0 + wave * kWaveRows, q = wq0 + (lane & 31);
+  const int q_end = q < queries ? key_end(allow, q) : 0;  // this lane's query sees keys below
+  const int begin = std::min(split * (int)a.split_len, allow.len);
+  const int end = std::min(key_end(allow, std::min(q0 + kRows, queries) - 1), begin + (int)a.split_len);
+  // keys below free_end are seen by every query of the wave, keys from wave_end on by none
+  const int free_end = wq0 < queries ? std::min(key_end(allow, wq0), end) : 0;
+  const int wave_end = wq0 < queries ? std::min(key_end(allow, std::min(wq0 + kWaveRows, queries) - 1), end) : 0;
 
   const T* qp = (const T*)a.q + b * a.qs[0] + h * a.qs[1];
   const T* kp = (const T*)a.k + b * a.ks[0] + hk * a.ks[1];
   const T* vp = (const T*)a.v + b * a.vs[0] + hk * a.vs[1];
   Frag<T> qf[KK];
-#pragma unroll
-  for (int kk = 0; kk < KK; ++kk) {
-    const int col = kk * 16 + half * 8;
-    Raw8<T> r;
-    load_raw8(r, qp + q * a.qs[2] + col, q < a.queries ? dim - col : 0);
-    qf[kk] = frag_of(r);
-  }
+  load_operand<T, DP>(qf, qp + (int64_t)q * a.qs[2], dim, q < queries);
   f32x16 o[DT] = {};
   float top = -FLT_MAX, sum = 0.0f;  // subtracted, in units of log2; sum of this lane's half of the keys
   const float c = a.scale * kLog2E;
 
-  Raw8<T> kr[Tile::PER], vr[Tile::PER];
+  // one tile's products in LDS while the next one's loads are under way, a barrier a tile
+  TileLoader<T, DP, FAST> kt, vt;
+  kt.init(kp, a.ks[2], dim);
+  vt.init(vp, a.vs[2], dim);
   if (begin < end) {
-    fetch_tile<T, DP>(kr, kp, a.ks[2], begin, end, dim);
-    fetch_tile<T, DP>(vr, vp, a.vs[2], begin, end, dim);
+    kt.fetch(begin, end);
+    vt.fetch(begin, end);
+    kt.template put<Tile::KS>(lds_k[0]);
+    vt.template put<Tile::VS>(lds_v[0]);
   }
-  for (int j0 = begin; j0 < end; j0 += kKeys) {
-    __syncthreads();  // the previous tile has been read
-    stage_tile<T, DP, Tile::KS>(lds_k, kr);
-    stage_tile<T, DP, Tile::VS>(lds_v, vr);
-    __syncthreads();
-    if (j0 + kKeys < end) {
-      fetch_tile<T, DP>(kr, kp, a.ks[2], j0 + kKeys, end, dim);
-      fetch_tile<T, DP>(vr, vp, a.vs[2], j0 + kKeys, end, dim);
+  int buf = 0;
+  for (int j0 = begin; j0 < end; j0 += kKeys, buf ^= 1) {
+    __syncthreads();  // this tile is there, the one before has been read
+    const bool more = j0 + kKeys < end;
+    if (more) {
+      kt.fetch(j0 + kKeys, end);
+      vt.fetch(j0 + kKeys, end);
     }
-    f32x16 s[2] = {};
+    if (j0 < wave_end) {
+      const T* lk = lds_k[buf] + (lane & 31) * Tile::KS + half * 8;
+      const T* lv = lds_v[buf];
+      f32x16 s[2] = {};
+      {
+        Frag<T> kf[2][KK];
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+        for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk)
-        s[t] = mma32(lds_frag(lds_k + (t * 32 + (lane & 31)) * Tile::KS + kk * 16 + half * 8), qf[kk], s[t]);
-    if (j0 + kKeys > free_end || j0 + kKeys > end) {
-      const int lim = std::min(q_end, end) - j0 - half * 4;
+          for (int t = 0; t < 2; ++t) kf[t][kk] = lds_frag(lk + t * 32 * Tile::KS + kk * 16);
+        fence_schedule<T>();
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) s[t] = mma32(kf[t][kk], qf[kk], s[t]);
+      }
+      Frag<T> vf[4][DT];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+          vf[u][d] = lds_column_frag(lv, Tile::VS, u * 16 + half * 4, u * 16 + half * 4 + 8, d * 32 + (lane & 16));
+      fence_schedule<T>();
+      if (j0 + kKeys > free_end) {
+        const int lim = std::min(q_end, end) - j0 - half * 4;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[t][r] = t * 32 + (r >> 2) * 8 + (r & 3) < lim ? s[t][r] : -INFINITY;
+      }
+      float most = s[0][0];
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (t * 32 + (r >> 2) * 8 + (r & 3) >= lim) s[t][r] = -INFINITY;
-    }
-    float most = s[0][0];
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) most = fmaxf(most, s[t][r]);
-    most = fmaxf(most, other_half(most)) * c;
-    if (__any(most > top + (kLift + kSlack))) {
-      const float next = fmaxf(top, most - kLift), shrink = exp2_hw(top - next);
-      top = next;
-      sum *= shrink;
-#pragma unroll
-      for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[d][r] *= shrink;
-    }
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[t][r] = exp2_hw(fmaf(s[t][r], c, -top));
-        sum += s[t][r];
-      }
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        Frag<T> p;
-#pragma unroll
-        for (int r = 0; r < 8; ++r) p[r] = (T)s[t][u * 8 + r];
-        const int row = t * 32 + u * 16 + half * 4;
+        for (int r = 0; r < 16; ++r) most = max_nan(most, s[t][r]);
+      most = max_halves(most) * c;
+      if (__any(most > top + (kLift + kSlack))) {
+        const float next = fmaxf(top, most - kLift), shrink = exp2_hw(top - next);
+        top = next;
+        sum *= shrink;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
-          o[d] = mma32(lds_column_frag(lds_v, Tile::VS, row, row + 8, d * 32 + (lane & 16)), p, o[d]);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[d][r] *= shrink;
       }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        Frag<T> p;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const float e = exp2_hw(fmaf(s[u >> 1][(u & 1) * 8 + r], c, -top));
+          sum += e;
+          p[r] = (T)e;
+        }
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[d] = mma32(vf[u][d], p, o[d]);
+      }
+    }
+    if (more) {
+      kt.template put<Tile::KS>(lds_k[buf ^ 1]);
+      vt.template put<Tile::VS>(lds_v[buf ^ 1]);
     }
   }
   sum += other_half(sum);
-  if (q >= a.queries) return;
+  if (q >= queries) return;
   const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
   const float lse = sum > 0.0f ? top + log2_hw(sum) : (sum == 0.0f ? -INFINITY : sum);
   const int64_t rows = a.batch * a.heads * a.queries, row = (b * a.heads + h) * a.queries + q;
   if (a.splits > 1) {
-    float* part = a.work + (int64_t)split * rows * dim + row * dim;
-    if (half == 0) a.work[(int64_t)a.splits * rows * dim + split * rows + row] = lse;
+    float* part = a.work + (row * a.splits + split) * dim;
+    if (half == 0) a.work[rows * a.splits * dim + row * a.splits + split] = lse;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -193,7 +182,7 @@ __global__ __launch_bounds__(256) void attention_rows(const AttnArgs a) {
     return;
   }
   if (a.lse && half == 0) a.lse[row] = lse * kLn2;
-  T* op = (T*)a.out + b * a.os[0] + h * a.os[1] + q * a.os[2];
+  T* op = (T*)a.out + b * a.os[0] + h * a.os[1] + (int64_t)q * a.os[2];
 #pragma unroll
   for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -220,23 +209,21 @@ __global__ __launch_bounds__(256) void attention_token(const AttnArgs a) {
   constexpr int kWaveBytes = kTileBytes > kJoinBytes ? kTileBytes : kJoinBytes;
   __shared__ __attribute__((aligned(16))) unsigned char lds[kWaves * kWaveBytes];
   __shared__ float lds_stat[kWaves][2][kTokenRows];
-  const int lane = threadIdx.x & 63, quad = lane >> 4, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, quad = lane >> 4, wave = uniform((int)threadIdx.x >> 6);
   T* lds_v = reinterpret_cast<T*>(lds + wave * kWaveBytes);
-  const int64_t group = a.heads / a.kv_heads;
-  int64_t id = blockIdx.x;
-  const int64_t hk = id % a.kv_heads;
-  id /= a.kv_heads;
-  const int64_t b = id % a.batch;
-  const int split = (int)(id / a.batch);
-  const int dim = (int)a.dim, queries = (int)a.queries, rows_here = (int)group * queries;
+  const uint32_t kvh = (uint32_t)a.kv_heads, batch = (uint32_t)a.batch;
+  const int group = uniform((int)((uint32_t)a.heads / kvh));
+  const int64_t hk = uniform((int)(blockIdx.x % kvh)), b = uniform((int)(blockIdx.x / kvh % batch));
+  const int split = uniform((int)(blockIdx.x / kvh / batch));
+  const int dim = (int)a.dim, queries = (int)a.queries, rows_here = group * queries;
   const Allowed allow = allowed_keys(a, b);
   const int row = lane & 15;  // this lane's column of the products: query row % queries of head row / queries
   const bool live = row < rows_here;
   const int g = live ? row / queries : 0, qi = live ? row % queries : 0;
   const int64_t h = hk * group + g;
   const int q_end = live ? key_end(allow, qi) : 0;
-  const int begin = (int)std::min<int64_t>((int64_t)split * a.split_len, allow.len);
-  const int end = (int)std::min<int64_t>(key_end(allow, queries - 1), (int64_t)begin + a.split_len);
+  const int begin = std::min(split * (int)a.split_len, allow.len);
+  const int end = std::min(key_end(allow, queries - 1), begin + (int)a.split_len);
   const T* kp = (const T*)a.k + b * a.ks[0] + hk * a.ks[1];
   const T* vp = (const T*)a.v + b * a.vs[0] + hk * a.vs[1];
   const T* qp = (const T*)a.q + b * a.qs[0] + h * a.qs[1] + qi * a.qs[2];
@@ -346,8 +333,8 @@ __global__ __launch_bounds__(256) void attention_token(const AttnArgs a) {
     const int64_t hh = hk * group + rr / queries, qq = rr % queries, out_row = (b * a.heads + hh) * queries + qq;
     if (col >= dim) continue;
     if (a.splits > 1) {
-      a.work[(int64_t)split * rows * dim + out_row * dim + col] = v;
-      if (col == 0) a.work[(int64_t)a.splits * rows * dim + split * rows + out_row] = lse;
+      a.work[(out_row * a.splits + split) * dim + col] = v;
+      if (col == 0) a.work[rows * a.splits * dim + out_row * a.splits + split] = lse;
     } else {
       ((T*)a.out)[b * a.os[0] + hh * a.os[1] + qq * a.os[2] + col] = (T)v;
       if (a.lse && col == 0) a.lse[out_row] = lse * kLn2;
@@ -355,37 +342,48 @@ __global__ __launch_bounds__(256) void attention_token(const AttnArgs a) {
   }
 }
 
-// The ranges' outputs weighed by their sums: a wave for each row.
+// The ranges' outputs weighed by their sums: a workgroup for each row.  32 lanes of four columns each, eight
+// groups of lanes that take every eighth range, joined through LDS in the groups' order.
 template <class T>
 __global__ __launch_bounds__(256) void attention_join(const AttnArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t rows = a.batch * a.heads * a.queries;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= rows) return;
+  __shared__ float lds_m[4], lds_t[4], lds_v[8][kAttnMaxDim];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = threadIdx.x >> 5, col = (threadIdx.x & 31) * 4;
+  const int64_t rows = a.batch * a.heads * a.queries, row = blockIdx.x;
   const int dim = (int)a.dim, splits = a.splits;
-  const float* lses = a.work + (int64_t)splits * rows * dim + row;
-  float m = -FLT_MAX;
-  for (int s = lane; s < splits; s += 64) m = fmaxf(m, lses[s * rows]);
+  const float* lses = a.work + rows * splits * dim + row * splits;
+  float m = -FLT_MAX, total = 0.0f;
+  for (int s = threadIdx.x; s < splits; s += 256) m = max_nan(m, lses[s]);
 #pragma unroll
-  for (int k = 32; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor(m, k, 64));
-  float total = 0.0f, v[2] = {0.0f, 0.0f};
-  for (int s = 0; s < splits; ++s) {
-    const float l = lses[s * rows];
-    if (l == -INFINITY) continue;
-    const float w = exp2_hw(l - m);
-    total += w;
-    const float* part = a.work + (int64_t)s * rows * dim + row * dim;
+  for (int k = 32; k > 0; k >>= 1) m = max_nan(m, __shfl_xor(m, k, 64));
+  if (lane == 0) lds_m[wave] = m;
+  __syncthreads();
+  m = max_nan(max_nan(lds_m[0], lds_m[1]), max_nan(lds_m[2], lds_m[3]));
+  for (int s = threadIdx.x; s < splits; s += 256) total += exp2_hw(lses[s] - m);
+  total = lanes_sum<64>(total);
+  if (lane == 0) lds_t[wave] = total;
+  float v[4] = {};
+  const float* part = a.work + row * splits * dim;
+#pragma unroll 4
+  for (int s = group; s < splits; s += 8) {
+    const float w = exp2_hw(lses[s] - m);
+    if (lses[s] == -INFINITY) continue;  // holds nothing
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (lane + 64 * i < dim) v[i] += w * part[lane + 64 * i];
+    for (int i = 0; i < 4; ++i)
+      if (col + i < dim) v[i] += w * part[(int64_t)s * dim + col + i];
   }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) lds_v[group][col + i] = v[i];
+  __syncthreads();
+  total = (lds_t[0] + lds_t[1]) + (lds_t[2] + lds_t[3]);
   const int64_t b = row / (a.heads * a.queries), h = row / a.queries % a.heads, q = row % a.queries;
   const float inv = total > 0.0f ? 1.0f / total : (total == 0.0f ? 0.0f : total);
-  T* op = (T*)a.out + b * a.os[0] + h * a.os[1] + q * a.os[2];
+  if ((int)threadIdx.x < dim) {
+    float o = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-    if (lane + 64 * i < dim) op[lane + 64 * i] = (T)(v[i] * inv);
-  if (a.lse && lane == 0)
+    for (int g = 0; g < 8; ++g) o += lds_v[g][threadIdx.x];
+    ((T*)a.out)[b * a.os[0] + h * a.os[1] + q * a.os[2] + threadIdx.x] = (T)(o * inv);
+  }
+  if (a.lse && threadIdx.x == 0)
     a.lse[row] = total > 0.0f ? (m + log2_hw(total)) * kLn2 : (total == 0.0f ? -INFINITY : total);
 }
 
@@ -408,13 +406,16 @@ hipError_t run(const AttnArgs& a, hipStream_t s) {
     const int64_t grid = a.batch * a.kv_heads * a.splits;
     hipLaunchKernelGGL((attention_token<T, DP>), dim3((unsigned)grid), dim3(256), 0, s, a);
   } else {
-    const int64_t grid = a.batch * a.heads * a.splits * ((a.queries + kRows - 1) / kRows);
-    hipLaunchKernelGGL((attention_rows<T, DP>), dim3((unsigned)grid), dim3(256), 0, s, a);
+    const dim3 grid((unsigned)(a.batch * a.heads * a.splits * ((a.queries + kRows - 1) / kRows)));
+    if (a.dim % 8 == 0 && fast_rows(a.k, a.ks, sizeof(T)) && fast_rows(a.v, a.vs, sizeof(T)))
+      hipLaunchKernelGGL((attention_rows<T, DP, true>), grid, dim3(256), 0, s, a);
+    else
+      hipLaunchKernelGGL((attention_rows<T, DP, false>), grid, dim3(256), 0, s, a);
   }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.splits == 1) return e;
   const int64_t rows = a.batch * a.heads * a.queries;
-  hipLaunchKernelGGL((attention_join<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((attention_join<T>), dim3((unsigned)rows), dim3(256), 0, s, a);
   return hipGetLastError();
 }
 
@@ -439,6 +440,7 @@ int64_t attention_fwd_work(const AttnArgs& args) {
 
 hipError_t launch_attention_fwd(AttnArgs a, hipStream_t s) {
   plan_splits(a);
+  a.cus = (int)device_cus();
   switch (a.dtype) {
     case kF32: return run_dim<float>(a, s);
     case kF16: return run_dim<f16>(a, s);

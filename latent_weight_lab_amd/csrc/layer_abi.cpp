@@ -21,72 +21,55 @@ size_t align_up(size_t v) { return (v + kAlign - 1) / kAlign * kAlign; }
 
 bool valid_dtype(int d) { return d == LWL_DTYPE_F32 || d == LWL_DTYPE_F16 || d == LWL_DTYPE_BF16; }
 
+constexpr int64_t kMostFeatures = (int64_t)1 << 24;
 // rows x features elements that fit 2^47 (pointers) with room for a workgroup's rounding up
 bool fits(int64_t rows, int64_t features) { return rows <= ((int64_t)1 << 46) / features; }
 
-int check_norm(const lwl_layer_norm_args* a) {
-  if (!a) return status_fail(LWL_ERR_INVALID, "layer norm: args must be non-null");
-  if (!valid_dtype(a->dtype) || !valid_dtype(a->weight_dtype))
+int check_norm(int dtype, int weight_dtype, int64_t rows, int64_t features, double eps) {
+  if (!valid_dtype(dtype) || !valid_dtype(weight_dtype))
     return status_fail(LWL_ERR_UNSUPPORTED, "layer norm supports float32, float16 and bfloat16");
-  if (a->weight_dtype != a->dtype && a->weight_dtype != LWL_DTYPE_F32)
+  if (weight_dtype != dtype && weight_dtype != LWL_DTYPE_F32)
     return status_fail(LWL_ERR_UNSUPPORTED, "layer norm's weight must be float32 or of the input's type");
-  if (a->rows < 0) return status_fail(LWL_ERR_INVALID, "layer norm: rows must be non-negative");
-  if (a->features <= 0) return status_fail(LWL_ERR_INVALID, "layer norm: features must be positive");
-  if (a->features > ((int64_t)1 << 24) || !fits(a->rows, a->features))
-    return status_fail(LWL_ERR_UNSUPPORTED, "layer norm: %lld rows of %lld features are too many",
-                       (long long)a->rows, (long long)a->features);
-  if (!(a->eps >= 0.0) || !std::isfinite(a->eps))
+  if (rows < 0) return status_fail(LWL_ERR_INVALID, "layer norm: rows must be non-negative");
+  if (features <= 0) return status_fail(LWL_ERR_INVALID, "layer norm: features must be positive");
+  if (features > kMostFeatures || !fits(rows, features))
+    return status_fail(LWL_ERR_UNSUPPORTED, "layer norm: %lld rows of %lld features are too many", (long long)rows,
+                       (long long)features);
+  if (!(eps >= 0.0) || !std::isfinite(eps))
     return status_fail(LWL_ERR_INVALID, "layer norm: eps must be finite and non-negative");
   return LWL_OK;
 }
 
-lwl::NormArgs norm_args(const lwl_layer_norm_args* a) {
-  lwl::NormArgs n{};
-  n.dtype = a->dtype;
-  n.weight_dtype = a->weight_dtype;
-  n.rows = a->rows;
-  n.features = a->features;
-  n.x = a->x;
-  n.residual = a->residual;
-  n.weight = a->weight;
-  n.bias = a->bias;
-  n.out = a->out;
-  n.sum = a->sum;
-  n.stats = a->stats;
-  n.eps = (float)a->eps;
-  return n;
-}
-
-int check_gelu8(const lwl_gelu8_args* a) {
-  if (!a) return status_fail(LWL_ERR_INVALID, "GELU checkpoint: args must be non-null");
-  if (!valid_dtype(a->dtype))
+int check_gelu8(int dtype, int64_t rows, int64_t features) {
+  if (!valid_dtype(dtype))
     return status_fail(LWL_ERR_UNSUPPORTED, "GELU checkpoint supports float32, float16 and bfloat16 (dtype code %d)",
-                       a->dtype);
-  if (a->rows < 0) return status_fail(LWL_ERR_INVALID, "GELU checkpoint: rows must be non-negative");
-  if (a->features <= 0) return status_fail(LWL_ERR_INVALID, "GELU checkpoint: features must be positive");
-  if (a->features > ((int64_t)1 << 24) || !fits(a->rows, a->features))
+                       dtype);
+  if (rows < 0) return status_fail(LWL_ERR_INVALID, "GELU checkpoint: rows must be non-negative");
+  if (features <= 0) return status_fail(LWL_ERR_INVALID, "GELU checkpoint: features must be positive");
+  if (features > kMostFeatures || !fits(rows, features))
     return status_fail(LWL_ERR_UNSUPPORTED, "GELU checkpoint: %lld rows of %lld features are too many",
-                       (long long)a->rows, (long long)a->features);
+                       (long long)rows, (long long)features);
   return LWL_OK;
 }
 
-lwl::Gelu8Args gelu8_args(const lwl_gelu8_args* a) {
-  lwl::Gelu8Args g{};
-  g.dtype = a->dtype;
-  g.tanh_form = a->tanh_form != 0;
-  g.rows = a->rows;
-  g.features = a->features;
-  g.codes = a->codes;
-  g.scales = a->scales;
-  return g;
-}
-
-int check_kept(const lwl_gelu8_args* a) {
-  if (a->rows == 0) return LWL_OK;
-  if (!a->codes || !a->scales)
+int check_kept(const int8_t* codes, const float* scales, int64_t rows) {
+  if (rows == 0) return LWL_OK;
+  if (!codes || !scales)
     return status_fail(LWL_ERR_INVALID, "GELU checkpoint: codes and scales must be non-null");
-  if ((uintptr_t)a->codes % 8) return status_fail(LWL_ERR_INVALID, "GELU checkpoint: codes must be 8-byte aligned");
+  if ((uintptr_t)codes % 8) return status_fail(LWL_ERR_INVALID, "GELU checkpoint: codes must be 8-byte aligned");
   return LWL_OK;
+}
+
+lwl::Gelu8Args gelu8_args(int dtype, int tanh_form, int64_t rows, int64_t features, const int8_t* codes,
+                          const float* scales) {
+  lwl::Gelu8Args g{};
+  g.dtype = dtype;
+  g.tanh_form = tanh_form != 0;
+  g.rows = rows;
+  g.features = features;
+  g.codes = const_cast<int8_t*>(codes);
+  g.scales = const_cast<float*>(scales);
+  return g;
 }
 
 int check_attention(const lwl_attention_args* a) {
@@ -109,8 +92,8 @@ int check_attention(const lwl_attention_args* a) {
   const int64_t kTokens = (int64_t)1 << 30, kCount = (int64_t)1 << 31;
   if (a->keys > kTokens || a->queries > kTokens || a->heads > kTokens || a->batch > kTokens)
     return status_fail(LWL_ERR_UNSUPPORTED, "attention: more than 2^30 tokens, heads or sequences");
-  const int64_t bh = a->batch * a->heads, blocks = (std::max(a->queries, a->keys) + 127) / 128;
-  if (bh >= kCount || bh * blocks >= kCount || bh * std::max<int64_t>(a->queries, 1) >= ((int64_t)1 << 34))
+  const int64_t bh = a->batch * a->heads, blocks = (std::max(a->queries, a->keys) + 15) / 16;
+  if (bh >= kCount || bh * blocks >= kCount)
     return status_fail(LWL_ERR_UNSUPPORTED, "attention: too many heads, sequences and tokens in one call");
   if (a->causal && !a->bottom_right && (a->causal_offset > kTokens || a->causal_offset < -kTokens))
     return status_fail(LWL_ERR_UNSUPPORTED, "attention: causal offset beyond 2^30");
@@ -157,20 +140,33 @@ lwl::AttnArgs attention_args(const lwl_attention_args* a) {
 
 extern "C" {
 
-int lwl_layer_norm_check(const lwl_layer_norm_args* args) {
-  const int rc = check_norm(args);
+int lwl_layer_norm_check(int dtype, int weight_dtype, int64_t rows, int64_t features, double eps) {
+  const int rc = check_norm(dtype, weight_dtype, rows, features, eps);
   return rc ? rc : status_ok();
 }
 
-int lwl_layer_norm_forward(const lwl_layer_norm_args* args, void* stream) {
-  const int rc = check_norm(args);
+int lwl_layer_norm_forward(const void* x, const void* residual, const void* weight, const void* bias, int dtype,
+                           int weight_dtype, int64_t rows, int64_t features, double eps, void* out, void* sum,
+                           float* stats, void* stream) {
+  const int rc = check_norm(dtype, weight_dtype, rows, features, eps);
   if (rc) return rc;
-  if (args->rows == 0) return status_ok();
-  if (!args->x || !args->weight || !args->out)
-    return status_fail(LWL_ERR_INVALID, "layer norm: x, weight and out must be non-null");
-  if (!args->residual != !args->sum)
-    return status_fail(LWL_ERR_INVALID, "layer norm: residual and sum go together");
-  return status_hip(lwl::launch_norm_fwd(norm_args(args), (hipStream_t)stream), "lwl_layer_norm_forward");
+  if (rows == 0) return status_ok();
+  if (!x || !weight || !out) return status_fail(LWL_ERR_INVALID, "layer norm: x, weight and out must be non-null");
+  if (!residual != !sum) return status_fail(LWL_ERR_INVALID, "layer norm: residual and sum go together");
+  lwl::NormArgs n{};
+  n.dtype = dtype;
+  n.weight_dtype = weight_dtype;
+  n.rows = rows;
+  n.features = features;
+  n.x = x;
+  n.residual = residual;
+  n.weight = weight;
+  n.bias = bias;
+  n.out = out;
+  n.sum = sum;
+  n.stats = stats;
+  n.eps = (float)eps;
+  return status_hip(lwl::launch_norm_fwd(n, (hipStream_t)stream), "lwl_layer_norm_forward");
 }
 
 size_t lwl_layer_norm_backward_workspace_size(int64_t rows, int64_t features) {
@@ -178,20 +174,27 @@ size_t lwl_layer_norm_backward_workspace_size(int64_t rows, int64_t features) {
   return align_up((size_t)lwl::norm_bwd_partial_rows(rows, features) * 2 * (size_t)features * sizeof(float));
 }
 
-int lwl_layer_norm_backward(const lwl_layer_norm_args* args, const void* grad_out, const void* grad_sum,
+int lwl_layer_norm_backward(const void* h, const void* weight, const float* stats, const void* grad_out,
+                            const void* grad_sum, int dtype, int weight_dtype, int64_t rows, int64_t features,
                             void* grad_x, void* grad_weight, void* grad_bias, void* workspace,
                             size_t workspace_bytes, void* stream) {
-  int rc = check_norm(args);
+  int rc = check_norm(dtype, weight_dtype, rows, features, 0.0);
   if (rc) return rc;
-  if (args->rows > 0 && (!args->x || !args->weight || !args->stats || !grad_out))
-    return status_fail(LWL_ERR_INVALID, "layer norm backward: x, weight, stats and grad_out must be non-null");
+  if (rows > 0 && (!h || !weight || !stats || !grad_out))
+    return status_fail(LWL_ERR_INVALID, "layer norm backward: h, weight, stats and grad_out must be non-null");
   if (!grad_x && !grad_weight && !grad_bias) return status_ok();
   if (grad_weight || grad_bias) {
-    rc = status_workspace(lwl_layer_norm_backward_workspace_size(args->rows, args->features), workspace,
-                          workspace_bytes);
+    rc = status_workspace(lwl_layer_norm_backward_workspace_size(rows, features), workspace, workspace_bytes);
     if (rc) return rc;
   }
-  lwl::NormArgs n = norm_args(args);
+  lwl::NormArgs n{};
+  n.dtype = dtype;
+  n.weight_dtype = weight_dtype;
+  n.rows = rows;
+  n.features = features;
+  n.x = h;
+  n.weight = weight;
+  n.stats = const_cast<float*>(stats);
   n.grad_out = grad_out;
   n.grad_sum = grad_sum;
   n.grad_x = grad_x;
@@ -203,30 +206,32 @@ int lwl_layer_norm_backward(const lwl_layer_norm_args* args, const void* grad_ou
 
 int64_t lwl_gelu8_pitch(int64_t features) { return lwl::gelu8_pitch(features); }
 
-int lwl_gelu8_check(const lwl_gelu8_args* args) {
-  const int rc = check_gelu8(args);
+int lwl_gelu8_check(int dtype, int64_t rows, int64_t features) {
+  const int rc = check_gelu8(dtype, rows, features);
   return rc ? rc : status_ok();
 }
 
-int lwl_gelu8_forward(const lwl_gelu8_args* args, const void* x, const void* bias, void* out, void* stream) {
-  int rc = check_gelu8(args);
+int lwl_gelu8_forward(const void* x, const void* bias, int dtype, int tanh_form, int64_t rows, int64_t features,
+                      void* out, int8_t* codes, float* scales, void* stream) {
+  int rc = check_gelu8(dtype, rows, features);
   if (rc) return rc;
-  if (args->rows == 0) return status_ok();
+  if (rows == 0) return status_ok();
   if (!x || !out) return status_fail(LWL_ERR_INVALID, "GELU checkpoint: x and out must be non-null");
-  if (args->codes && (rc = check_kept(args))) return rc;
-  lwl::Gelu8Args g = gelu8_args(args);
+  if (codes && (rc = check_kept(codes, scales, rows))) return rc;
+  lwl::Gelu8Args g = gelu8_args(dtype, tanh_form, rows, features, codes, scales);
   g.x = x;
   g.bias = bias;
   g.out = out;
   return status_hip(lwl::launch_gelu8_fwd(g, (hipStream_t)stream), "lwl_gelu8_forward");
 }
 
-int lwl_gelu8_activation(const lwl_gelu8_args* args, void* out, void* stream) {
-  int rc = check_gelu8(args);
-  if (rc || (rc = check_kept(args))) return rc;
-  if (args->rows == 0) return status_ok();
+int lwl_gelu8_activation(const int8_t* codes, const float* scales, int dtype, int tanh_form, int64_t rows,
+                         int64_t features, void* out, void* stream) {
+  int rc = check_gelu8(dtype, rows, features);
+  if (rc || (rc = check_kept(codes, scales, rows))) return rc;
+  if (rows == 0) return status_ok();
   if (!out) return status_fail(LWL_ERR_INVALID, "GELU checkpoint: out must be non-null");
-  lwl::Gelu8Args g = gelu8_args(args);
+  lwl::Gelu8Args g = gelu8_args(dtype, tanh_form, rows, features, codes, scales);
   g.out = out;
   return status_hip(lwl::launch_gelu8_activation(g, (hipStream_t)stream), "lwl_gelu8_activation");
 }
@@ -236,17 +241,18 @@ size_t lwl_gelu8_backward_workspace_size(int64_t rows, int64_t features) {
   return align_up((size_t)lwl::gelu8_bwd_partial_rows(rows, features) * (size_t)features * sizeof(float));
 }
 
-int lwl_gelu8_backward(const lwl_gelu8_args* args, const void* grad_out, void* grad_x, void* grad_bias,
-                       void* workspace, size_t workspace_bytes, void* stream) {
-  int rc = check_gelu8(args);
-  if (rc || (rc = check_kept(args))) return rc;
-  if (args->rows > 0 && (!grad_out || !grad_x))
+int lwl_gelu8_backward(const int8_t* codes, const float* scales, const void* grad_out, int dtype, int tanh_form,
+                       int64_t rows, int64_t features, void* grad_x, void* grad_bias, void* workspace,
+                       size_t workspace_bytes, void* stream) {
+  int rc = check_gelu8(dtype, rows, features);
+  if (rc || (rc = check_kept(codes, scales, rows))) return rc;
+  if (rows > 0 && (!grad_out || !grad_x))
     return status_fail(LWL_ERR_INVALID, "GELU checkpoint backward: grad_out and grad_x must be non-null");
   if (grad_bias) {
-    rc = status_workspace(lwl_gelu8_backward_workspace_size(args->rows, args->features), workspace, workspace_bytes);
+    rc = status_workspace(lwl_gelu8_backward_workspace_size(rows, features), workspace, workspace_bytes);
     if (rc) return rc;
   }
-  lwl::Gelu8Args g = gelu8_args(args);
+  lwl::Gelu8Args g = gelu8_args(dtype, tanh_form, rows, features, codes, scales);
   g.grad_out = grad_out;
   g.out = grad_x;
   g.grad_bias = grad_bias;

@@ -75,6 +75,7 @@ struct AttnArgs {
   // filled in by the launchers
   int splits;         // ranges of keys that different workgroups take (forward)
   int64_t split_len;  // keys of a range
+  int cus;            // compute units
 };
 // float32 values in the workspace
 int64_t attention_fwd_work(const AttnArgs& a);

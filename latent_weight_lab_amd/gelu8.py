@@ -10,7 +10,6 @@ from __future__ import annotations
 
 import torch
 from torch import nn
-from torch.autograd.function import once_differentiable
 
 from . import layer_ops
 
@@ -47,7 +46,7 @@ class _Gelu8Fn(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @layer_ops.once
     def backward(ctx, grad_out):
         codes, scales = ctx.saved_tensors
         gx, gb = layer_ops.gelu8_backward(codes, scales, grad_out, *ctx.meta, ctx.needs_input_grad[1])

@@ -4,32 +4,24 @@ layer norm, GELU with an 8-bit checkpoint, attention.
 As in ``ops``: each function checks its arguments, allocates outputs and scratch through torch's
 caching allocator and launches on the current stream of the tensors' device; nothing computes on
 the CPU, and nothing here records gradients.
+
+These calls are short on the GPU (a layer norm's training step of 8192 x 768 is 36 us of kernels), and in a
+training step autograd runs the backward on a thread of its own, where every Python operation costs
+two to three times what it does in a loop.  So they keep to few operations: the current stream and device
+are read without building torch objects, arguments go to the library as plain values, and the library's
+own checks are the only ones of what it checks.
 """
 from __future__ import annotations
 
 import ctypes
 import math
+import struct
 
 import torch
 
 from . import _native as N
 
 GELU8_GROUP = 128
-
-
-class LayerNormArgs(ctypes.Structure):
-    """``lwl_layer_norm_args``."""
-    _fields_ = [("dtype", ctypes.c_int32), ("weight_dtype", ctypes.c_int32), ("rows", ctypes.c_int64),
-                ("features", ctypes.c_int64), ("eps", ctypes.c_double), ("x", ctypes.c_void_p),
-                ("residual", ctypes.c_void_p), ("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p),
-                ("out", ctypes.c_void_p), ("sum", ctypes.c_void_p), ("stats", ctypes.c_void_p)]
-
-
-class Gelu8Args(ctypes.Structure):
-    """``lwl_gelu8_args``."""
-    _fields_ = [("dtype", ctypes.c_int32), ("tanh_form", ctypes.c_int32), ("rows", ctypes.c_int64),
-                ("features", ctypes.c_int64), ("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p)]
-
 
 _Strides = ctypes.c_int64 * 3
 
@@ -48,26 +40,30 @@ class AttentionArgs(ctypes.Structure):
                 ("grad_k_stride", _Strides), ("grad_v_stride", _Strides)]
 
 
+# The same, packed in one call: 4 int32, 7 int64, a double, 6 pointers, 12 strides, 4 pointers, 12 strides.
+_ATTENTION = struct.Struct("@4i7qd6Q12q4Q12q")
+assert _ATTENTION.size == ctypes.sizeof(AttentionArgs)
+
+
 def bind(lib) -> None:
     """Signatures of ``lwl_layers.h`` on the loaded library."""
-    i64, i32, sz, vp = ctypes.c_int64, ctypes.c_int, ctypes.c_size_t, ctypes.c_void_p
-    normp, gelup, attnp = (ctypes.POINTER(t) for t in (LayerNormArgs, Gelu8Args, AttentionArgs))
+    i64, i32, sz, vp, dbl = ctypes.c_int64, ctypes.c_int, ctypes.c_size_t, ctypes.c_void_p, ctypes.c_double
     sigs = {
-        "lwl_layer_norm_check": (i32, [normp]),
-        "lwl_layer_norm_forward": (i32, [normp, vp]),
+        "lwl_layer_norm_check": (i32, [i32, i32, i64, i64, dbl]),
+        "lwl_layer_norm_forward": (i32, [vp, vp, vp, vp, i32, i32, i64, i64, dbl, vp, vp, vp, vp]),
         "lwl_layer_norm_backward_workspace_size": (sz, [i64, i64]),
-        "lwl_layer_norm_backward": (i32, [normp, vp, vp, vp, vp, vp, vp, sz, vp]),
+        "lwl_layer_norm_backward": (i32, [vp, vp, vp, vp, vp, i32, i32, i64, i64, vp, vp, vp, vp, sz, vp]),
         "lwl_gelu8_pitch": (i64, [i64]),
-        "lwl_gelu8_check": (i32, [gelup]),
-        "lwl_gelu8_forward": (i32, [gelup, vp, vp, vp, vp]),
-        "lwl_gelu8_activation": (i32, [gelup, vp, vp]),
+        "lwl_gelu8_check": (i32, [i32, i64, i64]),
+        "lwl_gelu8_forward": (i32, [vp, vp, i32, i32, i64, i64, vp, vp, vp, vp]),
+        "lwl_gelu8_activation": (i32, [vp, vp, i32, i32, i64, i64, vp, vp]),
         "lwl_gelu8_backward_workspace_size": (sz, [i64, i64]),
-        "lwl_gelu8_backward": (i32, [gelup, vp, vp, vp, vp, sz, vp]),
-        "lwl_attention_check": (i32, [attnp]),
-        "lwl_attention_forward_workspace_size": (sz, [attnp]),
-        "lwl_attention_forward": (i32, [attnp, vp, sz, vp]),
-        "lwl_attention_backward_workspace_size": (sz, [attnp]),
-        "lwl_attention_backward": (i32, [attnp, vp, sz, vp]),
+        "lwl_gelu8_backward": (i32, [vp, vp, vp, i32, i32, i64, i64, vp, vp, vp, sz, vp]),
+        "lwl_attention_check": (i32, [vp]),
+        "lwl_attention_forward_workspace_size": (sz, [vp]),
+        "lwl_attention_forward": (i32, [vp, vp, sz, vp]),
+        "lwl_attention_backward_workspace_size": (sz, [vp]),
+        "lwl_attention_backward": (i32, [vp, vp, sz, vp]),
     }
     for name, (res, args) in sigs.items():
         fn = getattr(lib, name)
@@ -75,74 +71,101 @@ def bind(lib) -> None:
         fn.argtypes = args
 
 
-def _ptr(t: torch.Tensor | None) -> int | None:
-    return None if t is None else t.data_ptr()
+_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
+def _device_index(*tensors) -> int:
+    """The GPU that all tensors (None: skipped) are on."""
+    index = -1
+    for t in tensors:
+        if t is None:
+            continue
+        i = t.get_device()
+        if i < 0 or (index >= 0 and i != index):
+            N.require_cuda(*[t for t in tensors if t is not None])  # raises
+        index = i
+    return index
+
+
+def _launch(index: int, fn, *args) -> None:
+    """``fn(*args, stream)`` on the tensors' device and its current stream."""
+    if index == _device():
+        N.check(fn(*args, _stream(index)))
+    else:
+        with torch.cuda.device(index):
+            N.check(fn(*args, _stream(index)))
+
+
+def _ptr(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _scratch(nbytes: int, like: torch.Tensor) -> torch.Tensor | None:
+    return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
+
+
+def _dense(t: torch.Tensor) -> torch.Tensor:
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _vector(name: str, t: torch.Tensor, n: int, dtype: torch.dtype) -> torch.Tensor:
+    if t.shape != (n,) or t.dtype != dtype:
+        raise N.BlockFHTArgumentError(f"{name} must be {n} values of {dtype}, got {tuple(t.shape)} of {t.dtype}")
+    return _dense(t)
+
+
+def _rows(what: str, x: torch.Tensor) -> tuple[int, int]:
+    features = x.shape[-1] if x.dim() else 0
+    if features == 0:
+        raise N.BlockFHTArgumentError(f"{what} needs at least one feature, got {tuple(x.shape)}")
+    return x.numel() // features, features
 
 
 # ---------------------------------------------------------------- layer norm
-def _check_vector(name: str, t: torch.Tensor, n: int, dtype: torch.dtype) -> torch.Tensor:
-    if t.dim() != 1 or t.numel() != n or t.dtype != dtype:
-        raise N.BlockFHTArgumentError(f"{name} must be {n} values of {dtype}, got {tuple(t.shape)} of {t.dtype}")
-    return t.contiguous()
-
-
-def _norm_args(x: torch.Tensor, weight: torch.Tensor, eps: float, rows: int) -> LayerNormArgs:
-    a = LayerNormArgs()
-    a.dtype, a.weight_dtype = N.dtype_code(x.dtype), N.dtype_code(weight.dtype)
-    a.rows, a.features, a.eps = rows, int(x.shape[-1]), float(eps)
-    return a
-
-
 def layer_norm_forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, eps: float,
                        residual: torch.Tensor | None, keep_stats: bool):
     """``(out, sum, stats)`` over the last dimension of x; ``sum`` is None without a residual, ``stats``
     (float32 ``[2, rows]``: means, reciprocal deviations) unless ``keep_stats``."""
-    if x.dim() < 1 or x.shape[-1] == 0:
-        raise N.BlockFHTArgumentError("layer norm needs at least one feature")
-    dev = N.require_cuda(x, weight, *[t for t in (bias, residual) if t is not None])
-    features = int(x.shape[-1])
-    a = _norm_args(x, weight, eps, x.numel() // features)
-    L = N.lib()
-    N.check(L.lwl_layer_norm_check(ctypes.byref(a)))
-    weight = _check_vector("layer norm's weight", weight, features, weight.dtype)
+    index = _device_index(x, weight, bias, residual)
+    rows, features = _rows("layer norm", x)
+    weight = _vector("layer norm's weight", weight, features, weight.dtype)
     if bias is not None:
-        bias = _check_vector("layer norm's bias", bias, features, weight.dtype)
+        bias = _vector("layer norm's bias", bias, features, weight.dtype)
     if residual is not None:
         if residual.shape != x.shape or residual.dtype != x.dtype:
             raise N.BlockFHTArgumentError(
                 f"residual must be {tuple(x.shape)} of {x.dtype}, got {tuple(residual.shape)} of {residual.dtype}")
-        residual = residual.contiguous()
-    x = x.contiguous()
+        residual = _dense(residual)
+    code, weight_code = N.dtype_code(x.dtype), N.dtype_code(weight.dtype)
+    x = _dense(x)
     out = torch.empty_like(x)
     total = torch.empty_like(x) if residual is not None else None
-    stats = torch.empty(2, a.rows, dtype=torch.float32, device=dev) if keep_stats else None
-    a.x, a.residual, a.weight, a.bias = _ptr(x), _ptr(residual), _ptr(weight), _ptr(bias)
-    a.out, a.sum, a.stats = _ptr(out), _ptr(total), _ptr(stats)
-    with torch.cuda.device(dev):
-        N.check(L.lwl_layer_norm_forward(ctypes.byref(a), N.stream_ptr(dev)))
+    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if keep_stats else None
+    _launch(index, N.lib().lwl_layer_norm_forward, x.data_ptr(), _ptr(residual), weight.data_ptr(), _ptr(bias), code,
+            weight_code, rows, features, eps, out.data_ptr(), _ptr(total), _ptr(stats))
     return out, total, stats
 
 
-def layer_norm_backward(h: torch.Tensor, weight: torch.Tensor, stats: torch.Tensor, eps: float, grad_out: torch.Tensor,
+def layer_norm_backward(h: torch.Tensor, weight: torch.Tensor, stats: torch.Tensor, grad_out: torch.Tensor,
                         grad_sum: torch.Tensor | None, need_x: bool, need_weight: bool, need_bias: bool):
-    """``(grad_x, grad_weight, grad_bias)``, None for what is not needed; ``h`` is what was normed."""
-    dev = N.require_cuda(h, weight, stats, grad_out)
-    features = int(h.shape[-1])
-    a = _norm_args(h, weight, eps, h.numel() // features)
+    """``(grad_x, grad_weight, grad_bias)``, None for what is not needed; ``h`` is what was normed (contiguous)."""
+    index = _device_index(h, weight, stats, grad_out, grad_sum)
+    rows, features = _rows("layer norm", h)
+    dtype = h.dtype
+    weight = _dense(weight)
+    grad_out = _dense(grad_out if grad_out.dtype == dtype else grad_out.to(dtype))
+    if grad_sum is not None:
+        grad_sum = _dense(grad_sum if grad_sum.dtype == dtype else grad_sum.to(dtype))
     L = N.lib()
-    N.check(L.lwl_layer_norm_check(ctypes.byref(a)))
-    grad_out = grad_out.to(h.dtype).contiguous()
-    grad_sum = None if grad_sum is None else grad_sum.to(h.dtype).contiguous()
     gx = torch.empty_like(h) if need_x else None
-    gw = torch.empty(features, dtype=weight.dtype, device=dev) if need_weight else None
-    gb = torch.empty(features, dtype=weight.dtype, device=dev) if need_bias else None
-    a.x, a.weight, a.stats = _ptr(h), _ptr(weight), _ptr(stats)
-    with torch.cuda.device(dev):
-        need = L.lwl_layer_norm_backward_workspace_size(a.rows, a.features) if need_weight or need_bias else 0
-        ws_ptr, ws_size, ws = N.workspace(need, dev)
-        N.check(L.lwl_layer_norm_backward(ctypes.byref(a), _ptr(grad_out), _ptr(grad_sum), _ptr(gx), _ptr(gw),
-                                          _ptr(gb), ws_ptr, ws_size, N.stream_ptr(dev)))
-    del ws
+    gw = torch.empty_like(weight) if need_weight else None
+    gb = torch.empty_like(weight) if need_bias else None
+    need = L.lwl_layer_norm_backward_workspace_size(rows, features) if need_weight or need_bias else 0
+    ws = _scratch(need, h)
+    _launch(index, L.lwl_layer_norm_backward, h.data_ptr(), weight.data_ptr(), stats.data_ptr(), grad_out.data_ptr(),
+            _ptr(grad_sum), N.dtype_code(dtype), N.dtype_code(weight.dtype), rows, features, _ptr(gx), _ptr(gw), _ptr(gb),
+            _ptr(ws), need)
     return gx, gw, gb
 
 
@@ -150,142 +173,134 @@ def layer_norm_backward(h: torch.Tensor, weight: torch.Tensor, stats: torch.Tens
 _FORMS = {"none": 0, "tanh": 1}
 
 
-def _gelu8_args(dtype: torch.dtype, rows: int, features: int, approximate: str) -> Gelu8Args:
+def _form(approximate: str) -> int:
     if approximate not in _FORMS:
         raise N.BlockFHTArgumentError(f"approximate must be 'none' or 'tanh', got {approximate!r}")
-    a = Gelu8Args()
-    a.dtype, a.tanh_form, a.rows, a.features = N.dtype_code(dtype), _FORMS[approximate], rows, features
-    return a
+    return _FORMS[approximate]
 
 
 def gelu8_forward(x: torch.Tensor, bias: torch.Tensor | None, approximate: str, keep: bool):
     """``(gelu(x + bias), codes, scales)`` over the last dimension of x; codes (int8 ``[rows, pitch]``) and
     scales (float32 ``[rows, groups]``) are None unless ``keep``."""
-    if x.dim() < 1 or x.shape[-1] == 0:
-        raise N.BlockFHTArgumentError("GELU checkpoint needs at least one feature")
-    dev = N.require_cuda(x, *[t for t in (bias,) if t is not None])
-    features = int(x.shape[-1])
-    rows = x.numel() // features
-    a = _gelu8_args(x.dtype, rows, features, approximate)
-    L = N.lib()
-    N.check(L.lwl_gelu8_check(ctypes.byref(a)))
+    index = _device_index(x, bias)
+    rows, features = _rows("GELU checkpoint", x)
+    code, form = N.dtype_code(x.dtype), _form(approximate)
     if bias is not None:
-        bias = _check_vector("GELU's bias", bias, features, x.dtype)
-    x = x.contiguous()
+        bias = _vector("GELU's bias", bias, features, x.dtype)
+    x = _dense(x)
     out = torch.empty_like(x)
     codes = scales = None
     if keep:
-        codes = torch.empty(rows, (features + 7) // 8 * 8, dtype=torch.int8, device=dev)
-        scales = torch.empty(rows, -(-features // GELU8_GROUP), dtype=torch.float32, device=dev)
-        a.codes, a.scales = _ptr(codes), _ptr(scales)
-    with torch.cuda.device(dev):
-        N.check(L.lwl_gelu8_forward(ctypes.byref(a), _ptr(x), _ptr(bias), _ptr(out), N.stream_ptr(dev)))
+        codes = torch.empty((rows, (features + 7) // 8 * 8), dtype=torch.int8, device=x.device)
+        scales = torch.empty((rows, -(-features // GELU8_GROUP)), dtype=torch.float32, device=x.device)
+    _launch(index, N.lib().lwl_gelu8_forward, x.data_ptr(), _ptr(bias), code, form, rows, features, out.data_ptr(),
+            _ptr(codes), _ptr(scales))
     return out, codes, scales
 
 
 def gelu8_activation(codes: torch.Tensor, scales: torch.Tensor, shape: tuple[int, ...], dtype: torch.dtype,
                      approximate: str) -> torch.Tensor:
     """``gelu`` of what the checkpoint stands for, in ``shape`` and ``dtype``."""
-    dev = N.require_cuda(codes, scales)
-    out = torch.empty(shape, dtype=dtype, device=dev)
-    a = _gelu8_args(dtype, codes.shape[0], int(shape[-1]), approximate)
-    a.codes, a.scales = _ptr(codes), _ptr(scales)
-    with torch.cuda.device(dev):
-        N.check(N.lib().lwl_gelu8_activation(ctypes.byref(a), _ptr(out), N.stream_ptr(dev)))
+    index = _device_index(codes, scales)
+    out = torch.empty(shape, dtype=dtype, device=codes.device)
+    _launch(index, N.lib().lwl_gelu8_activation, codes.data_ptr(), scales.data_ptr(), N.dtype_code(dtype),
+            _form(approximate), codes.shape[0], shape[-1], out.data_ptr())
     return out
 
 
 def gelu8_backward(codes: torch.Tensor, scales: torch.Tensor, grad_out: torch.Tensor, dtype: torch.dtype,
                    approximate: str, need_bias: bool):
     """``(grad_x, grad_bias)``; ``grad_out`` has the activation's shape."""
-    dev = N.require_cuda(codes, scales, grad_out)
-    grad_out = grad_out.to(dtype).contiguous()
-    features = int(grad_out.shape[-1])
-    a = _gelu8_args(dtype, codes.shape[0], features, approximate)
-    a.codes, a.scales = _ptr(codes), _ptr(scales)
-    gx = torch.empty_like(grad_out)
-    gb = torch.empty(features, dtype=dtype, device=dev) if need_bias else None
+    index = _device_index(codes, scales, grad_out)
+    grad_out = _dense(grad_out if grad_out.dtype == dtype else grad_out.to(dtype))
+    rows, features = codes.shape[0], grad_out.shape[-1]
     L = N.lib()
-    with torch.cuda.device(dev):
-        need = L.lwl_gelu8_backward_workspace_size(a.rows, a.features) if need_bias else 0
-        ws_ptr, ws_size, ws = N.workspace(need, dev)
-        N.check(L.lwl_gelu8_backward(ctypes.byref(a), _ptr(grad_out), _ptr(gx), _ptr(gb), ws_ptr, ws_size,
-                                     N.stream_ptr(dev)))
-    del ws
+    gx = torch.empty_like(grad_out)
+    gb = torch.empty(features, dtype=dtype, device=gx.device) if need_bias else None
+    need = L.lwl_gelu8_backward_workspace_size(rows, features) if need_bias else 0
+    ws = _scratch(need, gx)
+    _launch(index, L.lwl_gelu8_backward, codes.data_ptr(), scales.data_ptr(), grad_out.data_ptr(), N.dtype_code(dtype),
+            _form(approximate), rows, features, gx.data_ptr(), _ptr(gb), _ptr(ws), need)
     return gx, gb
 
 
 # ---------------------------------------------------------------- attention
 ATTENTION_MAX_DIM = 128
+_NO_GRADS = (0,) * 16
 
 
 def _dense_dim(t: torch.Tensor) -> torch.Tensor:
     # the kernels take any strides but that of a head's values, which lie one after the other
-    return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-def _strides(t: torch.Tensor) -> _Strides:
-    return _Strides(t.stride(0), t.stride(1), t.stride(2))
-
-
-def _attention_args(q, k, v, causal, scale, key_lengths, causal_offset) -> tuple[AttentionArgs, list]:
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if t.dim() != 4:
-            raise N.BlockFHTArgumentError(f"attention: {name} must be [batch, heads, tokens, head size], got {tuple(t.shape)}")
-    if k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
+def _attention_head(q, k, v, causal, scale, key_lengths, causal_offset):
+    """The first fields of the arguments, up to the scale, and the lengths as int32."""
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        raise N.BlockFHTArgumentError(f"attention: q, k and v must be [batch, heads, tokens, head size], got "
+                                      f"{tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
+    batch, heads, queries, dim = q.shape
+    if k.shape != v.shape or k.shape[0] != batch or k.shape[3] != dim:
         raise N.BlockFHTArgumentError(f"attention: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not match")
     if not q.dtype == k.dtype == v.dtype:
         raise N.BlockFHTArgumentError(f"attention: q, k and v must have one type, got {q.dtype}, {k.dtype} and {v.dtype}")
-    a = AttentionArgs()
-    a.dtype, a.causal = N.dtype_code(q.dtype), int(bool(causal))
-    a.bottom_right, a.causal_offset = int(causal_offset is None), int(causal_offset or 0)
-    a.batch, a.heads, a.queries, a.dim = q.shape
-    a.kv_heads, a.keys = int(k.shape[1]), int(k.shape[2])
-    a.scale = 1.0 / math.sqrt(max(1, a.dim)) if scale is None else float(scale)
-    N.check(N.lib().lwl_attention_check(ctypes.byref(a)))
-    keep = [_dense_dim(t.detach()) for t in (q, k, v)]
-    a.q, a.k, a.v = (_ptr(t) for t in keep)
-    a.q_stride, a.k_stride, a.v_stride = (_strides(t) for t in keep)
     if key_lengths is not None:
-        if key_lengths.dim() != 1 or key_lengths.numel() != a.batch or key_lengths.is_floating_point():
-            raise N.BlockFHTArgumentError(f"attention: key_lengths must be {a.batch} integers, got {tuple(key_lengths.shape)}"
-                                          f" of {key_lengths.dtype}")
-        lengths = key_lengths.to(torch.int32).contiguous()
-        a.key_lengths = _ptr(lengths)
-        keep.append(lengths)
-    return a, keep
+        if key_lengths.shape != (batch,) or key_lengths.is_floating_point():
+            raise N.BlockFHTArgumentError(f"attention: key_lengths must be {batch} integers, got "
+                                          f"{tuple(key_lengths.shape)} of {key_lengths.dtype}")
+        key_lengths = _dense(key_lengths.to(torch.int32))
+    offset = 0 if causal_offset is None else int(causal_offset)
+    if not -(1 << 62) < offset < 1 << 62:
+        raise N.BlockFHTArgumentError(f"attention: causal_offset {offset} is too large")
+    head = (N.dtype_code(q.dtype), bool(causal), causal_offset is None, 0, offset, batch, heads, k.shape[1], queries,
+            k.shape[2], dim, 1.0 / math.sqrt(dim) if scale is None and dim else float(scale or 0.0))
+    return head, key_lengths
 
 
 def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool, scale: float | None,
-                      key_lengths: torch.Tensor | None, causal_offset: int | None, keep_lse: bool,
-                      out: torch.Tensor | None = None):
+                      key_lengths: torch.Tensor | None, causal_offset: int | None, keep_lse: bool):
     """``(out, lse)`` for ``[batch, heads, tokens, head size]`` tensors; ``out`` lies in memory token by token
     (all heads of a token together); ``lse`` (float32 ``[batch, heads, queries]``) is None unless ``keep_lse``."""
-    dev = N.require_cuda(q, k, v, *[t for t in (key_lengths,) if t is not None])
-    a, keep = _attention_args(q, k, v, causal, scale, key_lengths, causal_offset)
-    if out is None:
-        out = torch.empty(a.batch, a.queries, a.heads, a.dim, dtype=q.dtype, device=dev).transpose(1, 2)
-    lse = torch.empty(a.batch, a.heads, a.queries, dtype=torch.float32, device=dev) if keep_lse else None
-    a.out, a.lse, a.out_stride = _ptr(out), _ptr(lse), _strides(out)
+    index = _device_index(q, k, v, key_lengths)
+    head, lengths = _attention_head(q, k, v, causal, scale, key_lengths, causal_offset)
+    batch, heads, queries, dim = q.shape
+    q, k, v = _dense_dim(q), _dense_dim(k), _dense_dim(v)
+    dev = q.device
+    out = torch.empty((batch, queries, heads, dim), dtype=q.dtype, device=dev).transpose(1, 2)
+    lse = torch.empty((batch, heads, queries), dtype=torch.float32, device=dev) if keep_lse else None
     L = N.lib()
-    with torch.cuda.device(dev):
-        ws_ptr, ws_size, ws = N.workspace(L.lwl_attention_forward_workspace_size(ctypes.byref(a)), dev)
-        N.check(L.lwl_attention_forward(ctypes.byref(a), ws_ptr, ws_size, N.stream_ptr(dev)))
-    del ws, keep
+    args = _ATTENTION.pack(*head, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(lengths),
+                           *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], *_NO_GRADS)
+    need = L.lwl_attention_forward_workspace_size(args)
+    ws = _scratch(need, q)
+    _launch(index, L.lwl_attention_forward, args, _ptr(ws), need)
     return out, lse
 
 
-def attention_backward(q, k, v, out, lse, grad_out, causal, scale, key_lengths, causal_offset, grads):
+def attention_backward(q, k, v, out, lse, grad_out, causal, scale, key_lengths, causal_offset, grads) -> None:
     """Fills ``grads``, the three gradients like q, k and v (any strides, a head's values dense)."""
-    dev = N.require_cuda(q, k, v, out, lse, grad_out)
-    a, keep = _attention_args(q, k, v, causal, scale, key_lengths, causal_offset)
-    grad_out = _dense_dim(grad_out.to(q.dtype))
-    a.out, a.lse, a.grad_out = _ptr(out), _ptr(lse), _ptr(grad_out)
-    a.out_stride, a.grad_out_stride = _strides(out), _strides(grad_out)
-    a.grad_q, a.grad_k, a.grad_v = (_ptr(t) for t in grads)
-    a.grad_q_stride, a.grad_k_stride, a.grad_v_stride = (_strides(t) for t in grads)
+    index = _device_index(q, k, v, out, lse, grad_out, key_lengths)
+    head, lengths = _attention_head(q, k, v, causal, scale, key_lengths, causal_offset)
+    q, k, v = _dense_dim(q), _dense_dim(k), _dense_dim(v)
+    grad_out = _dense_dim(grad_out if grad_out.dtype == q.dtype else grad_out.to(q.dtype))
+    gq, gk, gv = grads
     L = N.lib()
-    with torch.cuda.device(dev):
-        ws_ptr, ws_size, ws = N.workspace(L.lwl_attention_backward_workspace_size(ctypes.byref(a)), dev)
-        N.check(L.lwl_attention_backward(ctypes.byref(a), ws_ptr, ws_size, N.stream_ptr(dev)))
-    del ws, keep
+    args = _ATTENTION.pack(*head, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _ptr(lengths),
+                           *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], grad_out.data_ptr(),
+                           gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), *grad_out.stride()[:3], *gq.stride()[:3],
+                           *gk.stride()[:3], *gv.stride()[:3])
+    need = L.lwl_attention_backward_workspace_size(args)
+    ws = _scratch(need, q)
+    _launch(index, L.lwl_attention_backward, args, _ptr(ws), need)
+
+
+def once(backward):
+    """A custom function's backward that cannot be differentiated itself.  What torch's
+    ``once_differentiable`` guards against can only come about where the backward records a graph
+    (``create_graph=True``); elsewhere its cost is spared."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    def call(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return call

@@ -8,7 +8,6 @@ from __future__ import annotations
 
 import torch
 from torch import nn
-from torch.autograd.function import once_differentiable
 
 from . import layer_ops
 
@@ -19,18 +18,17 @@ class _LayerNormFn(torch.autograd.Function):
         out, total, stats = layer_ops.layer_norm_forward(x, weight, bias, eps, residual, True)
         h = total if total is not None else x.contiguous()
         ctx.save_for_backward(h, weight, stats)
-        ctx.eps = eps
         ctx.set_materialize_grads(False)
         return (out, total) if total is not None else out
 
     @staticmethod
-    @once_differentiable
+    @layer_ops.once
     def backward(ctx, grad_out, grad_sum=None):
         h, weight, stats = ctx.saved_tensors
         need = ctx.needs_input_grad
         if grad_out is None:  # only the sum was used
             return (grad_sum if need[0] else None), (grad_sum if need[1] else None), None, None, None
-        gx, gw, gb = layer_ops.layer_norm_backward(h, weight, stats, ctx.eps, grad_out, grad_sum, need[0] or need[1],
+        gx, gw, gb = layer_ops.layer_norm_backward(h, weight, stats, grad_out, grad_sum, need[0] or need[1],
                                                    need[2], need[3])
         return (gx if need[0] else None), (gx if need[1] else None), gw, gb, None
 

@@ -18,8 +18,7 @@ ROOT = Path(__file__).resolve().parents[1]
 
 
 def test_structures_match_the_header(tmp_path):
-    fields = {"lwl_layer_norm_args": layer_ops.LayerNormArgs, "lwl_gelu8_args": layer_ops.Gelu8Args,
-              "lwl_attention_args": layer_ops.AttentionArgs}
+    fields = {"lwl_attention_args": layer_ops.AttentionArgs}
     lines = []
     for name, t in fields.items():
         lines.append(f'printf("%zu\\n", sizeof({name}));')
@@ -42,44 +41,38 @@ def test_header_names_are_exported_and_bound():
         assert getattr(N.lib(), n).argtypes is not None
 
 
-def norm_args(**kw):
-    a = layer_ops.LayerNormArgs()
-    a.dtype, a.weight_dtype, a.rows, a.features, a.eps = 2, 0, 4, 768, 1e-5
-    for k, v in kw.items():
-        setattr(a, k, v)
-    return a
-
-
 @pytest.mark.parametrize("kw,rc", [({}, 0), ({"rows": 0}, 0), ({"rows": -1}, -1), ({"features": 0}, -1), ({"dtype": 3}, -2),
                                    ({"weight_dtype": 1}, -2), ({"eps": -1.0}, -1), ({"eps": float("inf")}, -1),
                                    ({"rows": 1 << 50}, -2), ({"features": 1 << 25}, -2)])
 def test_norm_refusals(kw, rc):
     L = N.lib()
-    a = norm_args(**kw)
-    assert L.lwl_layer_norm_check(ctypes.byref(a)) == rc
+    a = {"dtype": 2, "weight_dtype": 0, "rows": 4, "features": 768, "eps": 1e-5, **kw}
+    assert L.lwl_layer_norm_check(*a.values()) == rc
     if rc:
         assert L.lwl_last_error()
-        assert L.lwl_layer_norm_forward(ctypes.byref(a), None) == rc
+        assert L.lwl_layer_norm_forward(None, None, None, None, *a.values(), None, None, None, None) == rc
 
 
 def test_null_pointers_and_workspaces_are_refused():
+    # pointers of 256 are never dereferenced
     L = N.lib()
-    a = norm_args()
-    assert L.lwl_layer_norm_forward(ctypes.byref(a), None) == -1
-    a.x = a.weight = a.out = a.sum = 256  # a sum without a residual; never dereferenced
-    assert L.lwl_layer_norm_forward(ctypes.byref(a), None) == -1
-    assert L.lwl_layer_norm_backward(ctypes.byref(a), 256, None, 256, 256, None, None, 0, None) == -1  # no stats
-    a.stats = 256
-    a.rows = 100
+    shape = (2, 0, 100, 768)
+    assert L.lwl_layer_norm_forward(None, None, None, None, *shape, 1e-5, None, None, None, None) == -1
+    # a sum without a residual
+    assert L.lwl_layer_norm_forward(256, None, 256, None, *shape, 1e-5, 256, 256, None, None) == -1
+    # no stats
+    assert L.lwl_layer_norm_backward(256, 256, None, 256, None, *shape, 256, 256, None, None, 0, None) == -1
     assert L.lwl_layer_norm_backward_workspace_size(100, 768) > 0
-    assert L.lwl_layer_norm_backward(ctypes.byref(a), 256, None, 256, 256, None, None, 0, None) == -3
-    assert L.lwl_layer_norm_check(None) == -1 and L.lwl_gelu8_check(None) == -1 and L.lwl_attention_check(None) == -1
-    g = layer_ops.Gelu8Args(2, 0, 5, 300, None, None)
-    assert L.lwl_gelu8_forward(ctypes.byref(g), None, None, None, None) == -1
-    assert L.lwl_gelu8_activation(ctypes.byref(g), 256, None) == -1
-    g.codes, g.scales = 257, 256
-    assert L.lwl_gelu8_forward(ctypes.byref(g), 256, None, 256, None) == -1  # codes off the 8-byte grid
+    assert L.lwl_layer_norm_backward(256, 256, 256, 256, None, *shape, 256, 256, None, None, 0, None) == -3
+    assert L.lwl_gelu8_check(2, 5, 0) == -1 and L.lwl_gelu8_check(9, 5, 300) == -2 and L.lwl_gelu8_check(2, -1, 300) == -1
+    assert L.lwl_gelu8_check(2, 5, 300) == 0 and L.lwl_gelu8_check(2, 1 << 50, 300) == -2
+    assert L.lwl_gelu8_forward(None, None, 2, 0, 5, 300, None, None, None, None) == -1
+    assert L.lwl_gelu8_activation(None, None, 2, 0, 5, 300, 256, None) == -1
+    # codes off the 8-byte grid
+    assert L.lwl_gelu8_forward(256, None, 2, 0, 5, 300, 256, 257, 256, None) == -1
+    assert L.lwl_gelu8_backward(256, 256, None, 2, 0, 5, 300, None, None, None, 0, None) == -1
     assert L.lwl_gelu8_pitch(1) == 8 and L.lwl_gelu8_pitch(3072) == 3072
+    assert L.lwl_attention_check(None) == -1
     t = attn_args()
     assert L.lwl_attention_forward(ctypes.byref(t), None, 0, None) == -1
     assert L.lwl_attention_backward(ctypes.byref(t), None, 0, None) == -1
