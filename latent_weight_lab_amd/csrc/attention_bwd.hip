@@ -36,21 +36,6 @@ struct BwdTile {
   static constexpr int S = DP + 16 / (int)sizeof(T);  // LDS row: 16-byte reads of 16 rows on distinct banks
 };
 
-// A result whose columns are rows of a tensor: lane's row, values 8 r4 + 4 half .. + 3 of each 32.
-template <class T, int DP>
-__device__ __forceinline__ void store_rows(T* row, const f32x16 (&v)[DP / 32], float scale, int dim) {
-  const int half = (threadIdx.x & 63) >> 5;
-#pragma unroll
-  for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-    for (int r4 = 0; r4 < 4; ++r4) {
-      const int col = d * 32 + r4 * 8 + half * 4;
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (col + r < dim) row[col + r] = (T)(v[d][r4 * 4 + r] * scale);
-    }
-}
-
 // work: [rows] lse in units of log2, [rows] D.  LANES lanes of eight values a row.
 template <class T, int LANES>
 __global__ __launch_bounds__(256) void attention_bwd_rows(const AttnArgs a) {
@@ -93,8 +78,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void atten
   const int seen = key_end(allow, queries - 1);  // keys that some query sees
   const int wk0 = k0 + wave * 32, key = wk0 + (lane & 31);
   Frag<T> kf[KK], vf[KK];
-  load_operand<T, DP>(kf, (const T*)a.k + b * a.ks[0] + hk * a.ks[1] + (int64_t)key * a.ks[2], dim, key < seen);
-  load_operand<T, DP>(vf, (const T*)a.v + b * a.vs[0] + hk * a.vs[1] + (int64_t)key * a.vs[2], dim, key < seen);
+  load_operand<T, DP, FAST>(kf, (const T*)a.k + b * a.ks[0] + hk * a.ks[1] + (int64_t)key * a.ks[2], dim, key < seen);
+  load_operand<T, DP, FAST>(vf, (const T*)a.v + b * a.vs[0] + hk * a.vs[1] + (int64_t)key * a.vs[2], dim, key < seen);
   f32x16 dk[DT] = {}, dv[DT] = {};
   // The products start from what is to be subtracted: S - lse / c, with c = scale log2(e), and dP - D.
   const float c = a.scale * kLog2E, inv_c = 1.0f / c;
@@ -217,8 +202,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void atten
     q0 = next_q;
   }
   if (key >= (int)a.keys) return;
-  store_rows<T, DP>((T*)a.dk + b * a.dks[0] + hk * a.dks[1] + (int64_t)key * a.dks[2], dk, a.scale, dim);
-  store_rows<T, DP>((T*)a.dv + b * a.dvs[0] + hk * a.dvs[1] + (int64_t)key * a.dvs[2], dv, kLower, dim);
+  store_result<T, DP, FAST>((T*)a.dk + b * a.dks[0] + hk * a.dks[1] + (int64_t)key * a.dks[2], dk, a.scale, dim);
+  store_result<T, DP, FAST>((T*)a.dv + b * a.dvs[0] + hk * a.dvs[1] + (int64_t)key * a.dvs[2], dv, kLower, dim);
 }
 
 template <class T, int DP, bool FAST>
@@ -251,8 +236,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_bwd_que
     vt.fetch(0, end);
   }
   Frag<T> qf[KK], gf[KK];
-  load_operand<T, DP>(qf, (const T*)a.q + b * a.qs[0] + h * a.qs[1] + (int64_t)q * a.qs[2], dim, q_end > 0);
-  load_operand<T, DP>(gf, (const T*)a.dout + b * a.dos[0] + h * a.dos[1] + (int64_t)q * a.dos[2], dim, q_end > 0);
+  load_operand<T, DP, FAST>(qf, (const T*)a.q + b * a.qs[0] + h * a.qs[1] + (int64_t)q * a.qs[2], dim, q_end > 0);
+  load_operand<T, DP, FAST>(gf, (const T*)a.dout + b * a.dos[0] + h * a.dos[1] + (int64_t)q * a.dos[2], dim, q_end > 0);
   const int64_t rows = a.batch * a.heads * a.queries, row = (b * a.heads + h) * a.queries + q;
   const float lse = q < queries ? a.work[row] : INFINITY, delta = q < queries ? a.work[rows + row] : 0.0f;
   f32x16 dq[DT] = {};
@@ -320,7 +305,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_bwd_que
     }
   }
   if (q >= queries) return;
-  store_rows<T, DP>((T*)a.dq + b * a.dqs[0] + h * a.dqs[1] + (int64_t)q * a.dqs[2], dq, a.scale, dim);
+  store_result<T, DP, FAST>((T*)a.dq + b * a.dqs[0] + h * a.dqs[1] + (int64_t)q * a.dqs[2], dq, a.scale, dim);
 }
 
 template <class T, int DP, bool FAST>

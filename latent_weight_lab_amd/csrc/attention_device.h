@@ -160,16 +160,39 @@ inline bool fast_rows(const void* p, const int64_t (&stride)[3], int64_t size) {
 }
 
 // A row of a tensor as operands: lane l holds chunks of eight values, 8 (l / 32) + 16 kk (32-wide products).
-template <class T, int DP>
+// WHOLE: the head size is a multiple of eight.
+template <class T, int DP, bool WHOLE>
 __device__ __forceinline__ void load_operand(Frag<T> (&f)[DP / 16], const T* row, int dim, bool ok) {
   const int half = (threadIdx.x & 63) >> 5;
 #pragma unroll
   for (int kk = 0; kk < DP / 16; ++kk) {
     const int col = kk * 16 + half * 8;
     Raw8<T> r;
-    load_raw8(r, row + col, ok ? dim - col : 0);
+    if constexpr (WHOLE) load_whole8(r, row + col, ok && col < dim);
+    else load_raw8(r, row + col, ok ? dim - col : 0);
     f[kk] = frag_of(r);
   }
+}
+// A result whose columns are rows of a tensor: the lane's row, values 8 r4 + 4 (l / 32) .. + 3 of each 32.
+template <class T, int DP, bool WHOLE>
+__device__ __forceinline__ void store_result(T* row, const f32x16 (&v)[DP / 32], float scale, int dim) {
+  const int half = (threadIdx.x & 63) >> 5;
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int r4 = 0; r4 < 4; ++r4) {
+      const int col = d * 32 + r4 * 8 + half * 4;
+      const float x0 = v[d][r4 * 4] * scale, x1 = v[d][r4 * 4 + 1] * scale, x2 = v[d][r4 * 4 + 2] * scale,
+                  x3 = v[d][r4 * 4 + 3] * scale;
+      if (WHOLE || col + 4 <= dim) {
+        if (col < dim) store4(row + col, x0, x1, x2, x3);
+      } else {
+        const float x[4] = {x0, x1, x2, x3};
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (col + r < dim) row[col + r] = (T)x[r];
+      }
+    }
 }
 
 // The larger of the two; a NaN stays a NaN (one instruction for three operands).

@@ -78,7 +78,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_rows(co
   const T* kp = (const T*)a.k + b * a.ks[0] + hk * a.ks[1];
   const T* vp = (const T*)a.v + b * a.vs[0] + hk * a.vs[1];
   Frag<T> qf[KK];
-  load_operand<T, DP>(qf, qp + (int64_t)q * a.qs[2], dim, q < queries);
+  load_operand<T, DP, FAST>(qf, qp + (int64_t)q * a.qs[2], dim, q < queries);
   f32x16 o[DT] = {};
   float top = -FLT_MAX, sum = 0.0f;  // subtracted, in units of log2; sum of this lane's half of the keys
   const float c = a.scale * kLog2E;
@@ -170,35 +170,19 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_rows(co
   const float lse = sum > 0.0f ? top + log2_hw(sum) : (sum == 0.0f ? -INFINITY : sum);
   const int64_t rows = a.batch * a.heads * a.queries, row = (b * a.heads + h) * a.queries + q;
   if (a.splits > 1) {
-    float* part = a.work + (row * a.splits + split) * dim;
     if (half == 0) a.work[rows * a.splits * dim + row * a.splits + split] = lse;
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int col = d * 32 + (r >> 2) * 8 + half * 4 + (r & 3);
-        if (col < dim) part[col] = o[d][r] * inv;
-      }
+    store_result<float, DP, FAST>(a.work + (row * a.splits + split) * dim, o, inv, dim);
     return;
   }
   if (a.lse && half == 0) a.lse[row] = lse * kLn2;
-  T* op = (T*)a.out + b * a.os[0] + h * a.os[1] + (int64_t)q * a.os[2];
-#pragma unroll
-  for (int d = 0; d < DT; ++d)
-#pragma unroll
-    for (int r4 = 0; r4 < 4; ++r4) {
-      const int col = d * 32 + r4 * 8 + half * 4;
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (col + r < dim) op[col + r] = (T)(o[d][r4 * 4 + r] * inv);
-    }
+  store_result<T, DP, FAST>((T*)a.out + b * a.os[0] + h * a.os[1] + (int64_t)q * a.os[2], o, inv, dim);
 }
 
 // ---------------------------------------------------------------- few queries
 constexpr int kTokenRows = 16;  // queries times heads that share a key head
 constexpr int kStep = 32;       // keys of a wave's step
 
-template <class T, int DP>
+template <class T, int DP, bool WHOLE>
 __global__ __launch_bounds__(256) void attention_token(const AttnArgs a) {
   constexpr int KK = DP / 32, DT = DP / 16, CPR = DP / 8, PER = kStep * CPR / 64;
   // values' rows: 16-bit 8 dwords more than a multiple of 16 (a transposing read's eight rows of 32
@@ -227,12 +211,16 @@ __global__ __launch_bounds__(256) void attention_token(const AttnArgs a) {
   const T* kp = (const T*)a.k + b * a.ks[0] + hk * a.ks[1];
   const T* vp = (const T*)a.v + b * a.vs[0] + hk * a.vs[1];
   const T* qp = (const T*)a.q + b * a.qs[0] + h * a.qs[1] + qi * a.qs[2];
+  auto load8_or = [](Raw8<T>& r, const T* p, bool ok, int left) {  // zeros where not ok
+    if constexpr (WHOLE) load_whole8(r, p, ok && left > 0);
+    else load_raw8(r, p, ok ? left : 0);
+  };
   Frag<T> qf[KK];
 #pragma unroll
   for (int kk = 0; kk < KK; ++kk) {
     const int col = kk * 32 + quad * 8;
     Raw8<T> r;
-    load_raw8(r, qp + col, live ? dim - col : 0);
+    load8_or(r, qp + col, live, dim - col);
     qf[kk] = frag_of(r);
   }
   Raw8<T> kr[2][KK], vr[PER];
@@ -242,12 +230,12 @@ __global__ __launch_bounds__(256) void attention_token(const AttnArgs a) {
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
         const int j = j0 + t * 16 + row, col = kk * 32 + quad * 8;
-        load_raw8(kr[t][kk], kp + (int64_t)j * a.ks[2] + col, j < end ? dim - col : 0);
+        load8_or(kr[t][kk], kp + (int64_t)j * a.ks[2] + col, j < end, dim - col);
       }
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int cc = lane + i * 64, j = j0 + cc / CPR, col = (cc % CPR) * 8;
-      load_raw8(vr[i], vp + (int64_t)j * a.vs[2] + col, j < end ? dim - col : 0);
+      load8_or(vr[i], vp + (int64_t)j * a.vs[2] + col, j < end, dim - col);
     }
   };
   f32x4 o[DT] = {};
@@ -342,60 +330,86 @@ __global__ __launch_bounds__(256) void attention_token(const AttnArgs a) {
   }
 }
 
-// The ranges' outputs weighed by their sums: a workgroup for each row.  32 lanes of four columns each, eight
-// groups of lanes that take every eighth range, joined through LDS in the groups' order.
-template <class T>
+// The ranges' outputs weighed by their sums.  32 lanes of four columns each hold a row; GROUPS groups of lanes
+// share a row's ranges, taking every GROUPS-th, and join through LDS in the groups' order: eight (one row a
+// workgroup) where there are many ranges, one (eight rows) where there are few.
+constexpr int kMaxSplits = 512;
+template <class T, int GROUPS>
 __global__ __launch_bounds__(256) void attention_join(const AttnArgs a) {
-  __shared__ float lds_m[4], lds_t[4], lds_v[8][kAttnMaxDim];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = threadIdx.x >> 5, col = (threadIdx.x & 31) * 4;
-  const int64_t rows = a.batch * a.heads * a.queries, row = blockIdx.x;
+  constexpr int ROWS = 8 / GROUPS, WIDTH = 32 * GROUPS;  // rows of a workgroup, threads of a row
+  __shared__ float lds_w[ROWS][kMaxSplits / ROWS], lds_v[ROWS][GROUPS][kAttnMaxDim], lds_t[2][8];
+  const int r = threadIdx.x / WIDTH, t = threadIdx.x % WIDTH, group = t >> 5, col = (t & 31) * 4;
+  const uint32_t rows = (uint32_t)(a.batch * a.heads * a.queries), row = blockIdx.x * ROWS + r;
   const int dim = (int)a.dim, splits = a.splits;
-  const float* lses = a.work + rows * splits * dim + row * splits;
+  const bool live = row < rows;
+  const int64_t first = (int64_t)(live ? row : 0) * splits;
+  const float* lses = a.work + (int64_t)rows * splits * dim + first;
   float m = -FLT_MAX, total = 0.0f;
-  for (int s = threadIdx.x; s < splits; s += 256) m = max_nan(m, lses[s]);
+  for (int s = t; s < splits; s += WIDTH) m = max_nan(m, lses[s]);
 #pragma unroll
-  for (int k = 32; k > 0; k >>= 1) m = max_nan(m, __shfl_xor(m, k, 64));
-  if (lane == 0) lds_m[wave] = m;
+  for (int k = 16; k > 0; k >>= 1) m = max_nan(m, __shfl_xor(m, k, 64));
+  if constexpr (GROUPS > 1) {
+    if ((t & 31) == 0) lds_t[0][group] = m;
+    __syncthreads();
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) m = max_nan(m, lds_t[0][g]);
+  }
+  for (int s = t; s < splits; s += WIDTH) {
+    const float w = exp2_hw(lses[s] - m);  // 0 for a range that holds nothing
+    lds_w[r][s] = w;
+    total += w;
+  }
+  total = lanes_sum<32>(total);
+  if ((t & 31) == 0) lds_t[1][threadIdx.x >> 5] = total;
   __syncthreads();
-  m = max_nan(max_nan(lds_m[0], lds_m[1]), max_nan(lds_m[2], lds_m[3]));
-  for (int s = threadIdx.x; s < splits; s += 256) total += exp2_hw(lses[s] - m);
-  total = lanes_sum<64>(total);
-  if (lane == 0) lds_t[wave] = total;
   float v[4] = {};
-  const float* part = a.work + row * splits * dim;
-#pragma unroll 4
-  for (int s = group; s < splits; s += 8) {
-    const float w = exp2_hw(lses[s] - m);
-    if (lses[s] == -INFINITY) continue;  // holds nothing
+  const float* part = a.work + first * dim;
+#pragma unroll 8
+  for (int s = group; s < splits; s += GROUPS) {
+    const float w = lds_w[r][s];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (col + i < dim) v[i] += w * part[(int64_t)s * dim + col + i];
+    for (int i = 0; i < 4; ++i) {
+      const float x = col + i < dim ? part[(int64_t)s * dim + col + i] : 0.0f;  // written, zeros where nothing is held
+      v[i] += w * x;
+    }
   }
+  if constexpr (GROUPS > 1) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) lds_v[group][col + i] = v[i];
-  __syncthreads();
-  total = (lds_t[0] + lds_t[1]) + (lds_t[2] + lds_t[3]);
-  const int64_t b = row / (a.heads * a.queries), h = row / a.queries % a.heads, q = row % a.queries;
+    for (int i = 0; i < 4; ++i) lds_v[r][group][col + i] = v[i];
+    __syncthreads();
+    total = 0.0f;
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) total += lds_t[1][g];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] = 0.0f;
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) v[i] += lds_v[r][g][col + i];
+    }
+  }
+  if (!live || group != 0) return;
+  const uint32_t queries = (uint32_t)a.queries, heads = (uint32_t)a.heads, bh = row / queries, q = row - bh * queries;
+  const int64_t b = bh / heads, h = bh % heads;
   const float inv = total > 0.0f ? 1.0f / total : (total == 0.0f ? 0.0f : total);
-  if ((int)threadIdx.x < dim) {
-    float o = 0.0f;
+  T* op = (T*)a.out + b * a.os[0] + h * a.os[1] + (int64_t)q * a.os[2];
 #pragma unroll
-    for (int g = 0; g < 8; ++g) o += lds_v[g][threadIdx.x];
-    ((T*)a.out)[b * a.os[0] + h * a.os[1] + q * a.os[2] + threadIdx.x] = (T)(o * inv);
-  }
-  if (a.lse && threadIdx.x == 0)
+  for (int i = 0; i < 4; ++i)
+    if (col + i < dim) op[col + i] = (T)(v[i] * inv);
+  if (a.lse && t == 0)
     a.lse[row] = total > 0.0f ? (m + log2_hw(total)) * kLn2 : (total == 0.0f ? -INFINITY : total);
 }
 
 bool by_token(const AttnArgs& a) { return a.heads / a.kv_heads * a.queries <= kTokenRows; }
 
-// Ranges of keys: enough that the workgroups fill the chip, none shorter than 256 keys.
+// Ranges of keys.  Single tokens: as many as make two workgroups for each compute unit, none shorter than
+// 256 keys.  Otherwise, where there is not half a workgroup for each compute unit, as many as make one,
+// none shorter than 512 keys: more costs the join more than the shorter walk gains.
 void plan_splits(AttnArgs& a) {
   const bool token = by_token(a);
   const int64_t wgs = token ? a.batch * a.kv_heads : a.batch * a.heads * ((a.queries + kRows - 1) / kRows);
-  const int64_t want = (token ? 4 : 1) * device_cus();
-  int64_t splits = wgs > 0 ? (want + wgs - 1) / wgs : 1;
-  splits = std::max<int64_t>(1, std::min(splits, a.keys / 256));
+  const int64_t want = (token ? 2 : 1) * device_cus();
+  int64_t splits = wgs > 0 ? want / wgs : 1;
+  splits = std::max<int64_t>(1, std::min({splits, a.keys / (token ? 256 : 512), (int64_t)kMaxSplits}));
   a.split_len = splits > 1 ? ((a.keys + splits - 1) / splits + kKeys - 1) / kKeys * kKeys : std::max<int64_t>(a.keys, 1);
   a.splits = splits > 1 ? (int)((a.keys + a.split_len - 1) / a.split_len) : 1;
 }
@@ -404,7 +418,8 @@ template <class T, int DP>
 hipError_t run(const AttnArgs& a, hipStream_t s) {
   if (by_token(a)) {
     const int64_t grid = a.batch * a.kv_heads * a.splits;
-    hipLaunchKernelGGL((attention_token<T, DP>), dim3((unsigned)grid), dim3(256), 0, s, a);
+    if (a.dim % 8 == 0) hipLaunchKernelGGL((attention_token<T, DP, true>), dim3((unsigned)grid), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((attention_token<T, DP, false>), dim3((unsigned)grid), dim3(256), 0, s, a);
   } else {
     const dim3 grid((unsigned)(a.batch * a.heads * a.splits * ((a.queries + kRows - 1) / kRows)));
     if (a.dim % 8 == 0 && fast_rows(a.k, a.ks, sizeof(T)) && fast_rows(a.v, a.vs, sizeof(T)))
@@ -415,7 +430,8 @@ hipError_t run(const AttnArgs& a, hipStream_t s) {
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.splits == 1) return e;
   const int64_t rows = a.batch * a.heads * a.queries;
-  hipLaunchKernelGGL((attention_join<T>), dim3((unsigned)rows), dim3(256), 0, s, a);
+  if (a.splits > 16) hipLaunchKernelGGL((attention_join<T, 8>), dim3((unsigned)rows), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((attention_join<T, 1>), dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s, a);
   return hipGetLastError();
 }
 

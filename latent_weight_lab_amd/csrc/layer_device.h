@@ -17,7 +17,7 @@ struct Vec8 {
   typedef T type __attribute__((ext_vector_type(8)));
 };
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
-typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
 
 template <class T>
 struct Raw8 {
@@ -43,6 +43,31 @@ __device__ __forceinline__ void load_raw8(Raw8<T>& v, const T* p, int64_t n) {
       }
     }
     __builtin_memcpy(&v, &e, sizeof(v));
+  }
+}
+// The same where n is known to be 8 or none.
+template <class T>
+__device__ __forceinline__ void load_whole8(Raw8<T>& v, const T* p, bool ok) {
+#pragma unroll
+  for (int i = 0; i < Raw8<T>::N; ++i) v.q[i] = u32x4_any{0, 0, 0, 0};
+  if (ok) {
+#pragma unroll
+    for (int i = 0; i < Raw8<T>::N; ++i) v.q[i] = reinterpret_cast<const u32x4_any*>(p)[i];
+  }
+}
+// v[0 .. 4) as one store.
+template <class T>
+__device__ __forceinline__ void store4(T* p, float v0, float v1, float v2, float v3) {
+  typedef T vec __attribute__((ext_vector_type(4)));
+  const vec e = {(T)v0, (T)v1, (T)v2, (T)v3};
+  if constexpr (sizeof(T) == 2) {
+    u32x2_any w;
+    __builtin_memcpy(&w, &e, sizeof(w));
+    *reinterpret_cast<u32x2_any*>(p) = w;
+  } else {
+    u32x4_any w;
+    __builtin_memcpy(&w, &e, sizeof(w));
+    *reinterpret_cast<u32x4_any*>(p) = w;
   }
 }
 template <class T>
