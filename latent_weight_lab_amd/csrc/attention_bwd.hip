@@ -14,9 +14,9 @@
 // column a query (bwd_queries: S^T = K Q^T) dS^T is the operand of dQ^T = K^T dS^T.  The other operand of
 // these is a column of the tile in LDS (the transposing read).
 //
-// attention_bwd_rows prepares for each query lse in units of log2 (+infinity for a query without
-// keys, whose probabilities are then zero) and D.
+// bwd_queries runs first and leaves each query's D in the workspace for bwd_keys.
 #include <algorithm>
+#include <cmath>
 
 #include "attention_device.h"
 
@@ -31,34 +31,21 @@ constexpr int kTile = kTileRows;  // queries (keys) of a tile
 // float16 and flushed by the exponential in float32.
 constexpr float kLift = 14.0f, kLower = 0x1p-14f;
 
+// Head sizes up to 64 leave registers for two waves a SIMD, which overlap; larger ones of a 16-bit type run
+// one, whose two halves of a tile the scheduler may interleave.
+template <class T, int DP>
+constexpr int kUnroll = sizeof(T) == 2 && DP > 64 ? 2 : 1;
+
 template <class T, int DP>
 struct BwdTile {
   static constexpr int S = DP + 16 / (int)sizeof(T);  // LDS row: 16-byte reads of 16 rows on distinct banks
 };
 
-// work: [rows] lse in units of log2, [rows] D.  LANES lanes of eight values a row.
-template <class T, int LANES>
-__global__ __launch_bounds__(256) void attention_bwd_rows(const AttnArgs a) {
-  constexpr uint32_t PER = 256 / LANES;  // rows of a workgroup, all of one head
-  const int lane = threadIdx.x & (LANES - 1);
-  const uint32_t queries = (uint32_t)a.queries, heads = (uint32_t)a.heads, blocks = (queries + PER - 1) / PER;
-  const uint32_t bh = blockIdx.x / blocks, q = (blockIdx.x - bh * blocks) * PER + threadIdx.x / LANES;
-  const int64_t b = uniform((int)(bh / heads)), h = uniform((int)(bh % heads));
-  const int64_t rows = a.batch * a.heads * a.queries, row = (int64_t)bh * queries + q;
-  const Allowed allow = allowed_keys(a, b);
-  const bool live = q < queries;
-  const int col = lane * 8, n = live ? (int)a.dim - col : 0;
-  float o[8], g[8], s = 0.0f;
-  load8(o, (const T*)a.out + b * a.os[0] + h * a.os[1] + (int64_t)q * a.os[2] + col, n);
-  load8(g, (const T*)a.dout + b * a.dos[0] + h * a.dos[1] + (int64_t)q * a.dos[2] + col, n);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) s += o[i] * g[i];
-  s = lanes_sum<LANES>(s);
-  if (!live || lane != 0) return;
-  const bool none = key_end(allow, (int)q) == 0;
-  a.work[row] = none ? INFINITY : a.lse[row] * kLog2E;
-  a.work[rows + row] = none ? 0.0f : s;
+// The workspace: D of every query, then (256-byte aligned) the key gradients' partial sums.
+__host__ __device__ inline int64_t delta_floats(const AttnArgs& a) {
+  return (a.batch * a.heads * a.queries + 63) / 64 * 64;
 }
+__device__ __forceinline__ float* partials(const AttnArgs& a) { return a.work + delta_floats(a); }
 
 template <class T, int DP, bool FAST>
 __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void attention_bwd_keys(const AttnArgs a) {
@@ -69,9 +56,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void atten
   __shared__ __attribute__((aligned(16))) float lds_stat[2][2][kTile];
   const int lane = threadIdx.x & 63, half = lane >> 5, wave = uniform((int)threadIdx.x >> 6);
   const uint32_t kvh = (uint32_t)a.kv_heads, kvb = (uint32_t)a.batch * kvh, group = (uint32_t)a.heads / kvh;
-  const uint32_t id = work_order(blockIdx.x, gridDim.x, (uint32_t)a.cus), bk = id % kvb;
+  const uint32_t id = work_order(blockIdx.x, gridDim.x, (uint32_t)a.cus), bk = id % kvb, splits = (uint32_t)a.splits;
   const int64_t b = uniform((int)(bk / kvh)), hk = uniform((int)(bk % kvh));
-  const int k0 = uniform((int)(id / kvb)) * kBlock;  // causal: the first keys have the most queries
+  const int split = uniform((int)(id / kvb % splits));
+  const int k0 = uniform((int)(id / kvb / splits)) * kBlock;  // causal: the first keys have the most queries
   const int dim = (int)a.dim;
   const Allowed allow = allowed_keys(a, b);
   const int queries = (int)a.queries;
@@ -87,17 +75,18 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void atten
   // before wk0 - off none of the wave's
   const int first = k0 >= seen ? queries : std::max(0, k0 - allow.off);
   const int wave_first = wk0 >= seen ? queries : wk0 - allow.off;
-  const int64_t rows = a.batch * a.heads * a.queries;
   const T* qp = (const T*)a.q + b * a.qs[0] + hk * group * a.qs[1];
   const T* gp = (const T*)a.dout + b * a.dos[0] + hk * group * a.dos[1];
-  const float* stat = a.work + (b * a.heads + hk * group) * a.queries;
+  const int64_t head0 = (b * a.heads + hk * group) * a.queries;
   TileLoader<T, DP, FAST> qt, gt;
   qt.init(qp, a.qs[2], dim);
   gt.init(gp, a.dos[2], dim);
   float sr = 0.0f;
-  // tiles of the first head, then of the next one of the group: one sequence of loads
-  uint32_t g = 0;
-  int q0 = first;
+  // Tiles of the first head, then of the next one of the group: one sequence, of which this workgroup
+  // takes the tiles begin .. end.
+  const int per_head = (queries - first + kTile - 1) / kTile, tiles = per_head * (int)group;
+  const int share = (tiles + (int)splits - 1) / (int)splits;
+  const int begin = std::min(split * share, tiles), end = std::min(begin + share, tiles);
   auto fetch = [&](uint32_t fg, int fq) {
     qt.base = qp + fg * a.qs[1];
     gt.base = gp + fg * a.dos[1];
@@ -106,8 +95,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void atten
     if (threadIdx.x < 2 * kTile) {
       const int q = fq + (threadIdx.x & (kTile - 1));
       const bool is_d = threadIdx.x >= kTile;
-      sr = q < queries ? stat[(int64_t)fg * queries + (is_d ? rows : 0) + q] : (is_d ? 0.0f : INFINITY);
-      sr = is_d ? -sr : (kLift - sr) * inv_c;
+      const float* stat = (is_d ? a.work : a.lse) + head0 + (int64_t)fg * queries;
+      sr = q < queries ? stat[q] : (is_d ? 0.0f : INFINITY);  // past the last: no probabilities
+      sr = is_d ? -sr : (kLift - sr * kLog2E) * inv_c;
     }
   };
   auto put = [&](int buf) {
@@ -116,19 +106,21 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void atten
     if (threadIdx.x < 2 * kTile) lds_stat[buf][threadIdx.x / kTile][threadIdx.x & (kTile - 1)] = sr;
   };
   int buf = 0;
-  if (first < queries) {
-    fetch(0, first);
+  uint32_t g = begin < end ? (uint32_t)uniform(begin / per_head) : 0;
+  int q0 = begin < end ? first + (begin - (int)g * per_head) * kTile : 0;
+  if (begin < end) {
+    fetch(g, q0);
     put(0);
   }
-  while (g < group && q0 < queries) {
+  for (int i = begin; i < end; ++i) {
     __syncthreads();  // this tile is there, the one before has been read
-    const bool last = q0 + kTile >= queries;
+    const bool last = q0 + kTile >= queries, more = i + 1 < end;
     const uint32_t next_g = last ? g + 1 : g;
     const int next_q = last ? first : q0 + kTile;
-    if (next_g < group) fetch(next_g, next_q);
+    if (more) fetch(next_g, next_q);
     if (q0 + kTile > wave_first) {
       const bool masked = key_end(allow, q0) < wk0 + 32;  // some pair of the tile is not allowed
-#pragma unroll 1
+#pragma unroll kUnroll<T, DP>
       for (int t = 0; t < 2; ++t) {
         const int at = t * 32;
         const T* lq = lds_q[buf] + at * Tile::S;
@@ -151,7 +143,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void atten
             qf[kk] = lds_frag(lq + (lane & 31) * Tile::S + kk * 16 + half * 8);
             gf[kk] = lds_frag(lg + (lane & 31) * Tile::S + kk * 16 + half * 8);
           }
-          fence_schedule<T>();
+          fence_schedule<T, DP>();
 #pragma unroll
           for (int kk = 0; kk < KK; ++kk) {
             s = mma32(qf[kk], kf[kk], s);
@@ -167,7 +159,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void atten
             gc[u][d] = lds_column_frag(lg, Tile::S, row, row + 8, d * 32 + (lane & 16));
             qc[u][d] = lds_column_frag(lq, Tile::S, row, row + 8, d * 32 + (lane & 16));
           }
-        fence_schedule<T>();
+        fence_schedule<T, DP>();
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           s[r] = exp2_hw(s[r] * c);
@@ -196,12 +188,19 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void atten
         }
       }
     }
-    if (next_g < group) put(buf ^ 1);
+    if (more) put(buf ^ 1);
     buf ^= 1;
     g = next_g;
     q0 = next_q;
   }
   if (key >= (int)a.keys) return;
+  if (splits > 1) {  // summed by attention_bwd_join
+    const int64_t kv_rows = a.batch * a.kv_heads * a.keys, row = (b * a.kv_heads + hk) * a.keys + key;
+    float* part = partials(a) + (split * kv_rows + row) * 2 * dim;
+    store_result<float, DP, FAST>(part, dk, a.scale, dim);
+    store_result<float, DP, FAST>(part + dim, dv, kLower, dim);
+    return;
+  }
   store_result<T, DP, FAST>((T*)a.dk + b * a.dks[0] + hk * a.dks[1] + (int64_t)key * a.dks[2], dk, a.scale, dim);
   store_result<T, DP, FAST>((T*)a.dv + b * a.dvs[0] + hk * a.dvs[1] + (int64_t)key * a.dvs[2], dv, kLower, dim);
 }
@@ -238,8 +237,20 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_bwd_que
   Frag<T> qf[KK], gf[KK];
   load_operand<T, DP, FAST>(qf, (const T*)a.q + b * a.qs[0] + h * a.qs[1] + (int64_t)q * a.qs[2], dim, q_end > 0);
   load_operand<T, DP, FAST>(gf, (const T*)a.dout + b * a.dos[0] + h * a.dos[1] + (int64_t)q * a.dos[2], dim, q_end > 0);
-  const int64_t rows = a.batch * a.heads * a.queries, row = (b * a.heads + h) * a.queries + q;
-  const float lse = q < queries ? a.work[row] : INFINITY, delta = q < queries ? a.work[rows + row] : 0.0f;
+  const int64_t row = (b * a.heads + h) * a.queries + q;
+  // a query without keys has no probabilities: exp2(-infinity)
+  const float lse = q_end > 0 ? a.lse[row] * kLog2E : INFINITY;
+  float delta = 0.0f;
+  {
+    Frag<T> of[KK];
+    load_operand<T, DP, FAST>(of, (const T*)a.out + b * a.os[0] + h * a.os[1] + (int64_t)q * a.os[2], dim, q_end > 0);
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+      for (int r = 0; r < 8; ++r) delta += (float)of[kk][r] * (float)gf[kk][r];
+    delta += other_half(delta);
+    if (half == 0 && q < queries) a.work[row] = delta;
+  }
   f32x16 dq[DT] = {};
   const float c = a.scale * kLog2E;
   if (end > 0) {
@@ -263,14 +274,19 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_bwd_que
         {
           Frag<T> kf[KK], vf[KK];
 #pragma unroll
-          for (int kk = 0; kk < KK; ++kk) {
-            kf[kk] = lds_frag(lk + (lane & 31) * Tile::S + kk * 16 + half * 8);
-            vf[kk] = lds_frag(lv + (lane & 31) * Tile::S + kk * 16 + half * 8);
+          for (int kk = 0; kk < KK; ++kk) kf[kk] = lds_frag(lk + (lane & 31) * Tile::S + kk * 16 + half * 8);
+          // beyond 64 the two products one after the other, which holds half as many operands at a time
+          if constexpr (DP > 64) {
+            fence_schedule<T>();
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) s = mma32(kf[kk], qf[kk], s);
           }
+#pragma unroll
+          for (int kk = 0; kk < KK; ++kk) vf[kk] = lds_frag(lv + (lane & 31) * Tile::S + kk * 16 + half * 8);
           fence_schedule<T>();
 #pragma unroll
           for (int kk = 0; kk < KK; ++kk) {
-            s = mma32(kf[kk], qf[kk], s);
+            if constexpr (DP <= 64) s = mma32(kf[kk], qf[kk], s);
             dp = mma32(vf[kk], gf[kk], dp);
           }
         }
@@ -308,17 +324,47 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_bwd_que
   store_result<T, DP, FAST>((T*)a.dq + b * a.dqs[0] + h * a.dqs[1] + (int64_t)q * a.dqs[2], dq, a.scale, dim);
 }
 
+// dK and dV of a key from the ranges' partial sums, in the ranges' order: 32 lanes of eight values for the two
+// rows of a key, dK's then dV's.
+template <class T>
+__global__ __launch_bounds__(256) void attention_bwd_join(const AttnArgs a) {
+  const int lane = threadIdx.x & 31, dim = (int)a.dim, col = (lane & 15) * 8;
+  const uint32_t keys = (uint32_t)a.keys, kvh = (uint32_t)a.kv_heads, blocks = (keys + 7) / 8;
+  const uint32_t bk = blockIdx.x / blocks, key = (blockIdx.x - bk * blocks) * 8 + (threadIdx.x >> 5);
+  if (key >= keys || col >= dim) return;
+  const bool is_v = lane >= 16;
+  const int64_t kv_rows = a.batch * a.kv_heads * a.keys, row = (int64_t)bk * keys + key, b = bk / kvh, hk = bk % kvh;
+  const float* part = partials(a) + row * 2 * dim + (is_v ? dim : 0) + col;
+  float sum[8] = {};
+#pragma unroll 4
+  for (int s = 0; s < a.splits; ++s) {
+    float v[8];
+    load8(v, part + s * kv_rows * 2 * dim, dim - col);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum[i] += v[i];
+  }
+  T* dst = is_v ? (T*)a.dv + b * a.dvs[0] + hk * a.dvs[1] + (int64_t)key * a.dvs[2]
+                : (T*)a.dk + b * a.dks[0] + hk * a.dks[1] + (int64_t)key * a.dks[2];
+  store8(dst + col, sum, dim - col);
+}
+
 template <class T, int DP, bool FAST>
 hipError_t launch(const AttnArgs& a, hipStream_t s) {
   const int64_t kgrid = a.batch * a.kv_heads * ((a.keys + kBlock - 1) / kBlock);
   const int64_t qgrid = a.batch * a.heads * ((a.queries + kBlock - 1) / kBlock);
-  if (kgrid > 0) {
-    hipLaunchKernelGGL((attention_bwd_keys<T, DP, FAST>), dim3((unsigned)kgrid), dim3(256), 0, s, a);
+  if (qgrid > 0) {
+    hipLaunchKernelGGL((attention_bwd_queries<T, DP, FAST>), dim3((unsigned)qgrid), dim3(256), 0, s, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  if (qgrid > 0)
-    hipLaunchKernelGGL((attention_bwd_queries<T, DP, FAST>), dim3((unsigned)qgrid), dim3(256), 0, s, a);
+  if (kgrid > 0) {
+    hipLaunchKernelGGL((attention_bwd_keys<T, DP, FAST>), dim3((unsigned)(kgrid * a.splits)), dim3(256), 0, s, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    if (a.splits > 1)
+      hipLaunchKernelGGL((attention_bwd_join<T>), dim3((unsigned)(a.batch * a.kv_heads * ((a.keys + 7) / 8))), dim3(256),
+                         0, s, a);
+  }
   return hipGetLastError();
 }
 
@@ -331,17 +377,6 @@ hipError_t run(const AttnArgs& a, hipStream_t s) {
 
 template <class T>
 hipError_t run_dim(const AttnArgs& a, hipStream_t s) {
-  const int64_t bh = a.batch * a.heads;
-  if (bh > 0 && a.queries > 0) {
-    if (a.dim <= 32)
-      hipLaunchKernelGGL((attention_bwd_rows<T, 4>), dim3((unsigned)(bh * ((a.queries + 63) / 64))), dim3(256), 0, s, a);
-    else if (a.dim <= 64)
-      hipLaunchKernelGGL((attention_bwd_rows<T, 8>), dim3((unsigned)(bh * ((a.queries + 31) / 32))), dim3(256), 0, s, a);
-    else
-      hipLaunchKernelGGL((attention_bwd_rows<T, 16>), dim3((unsigned)(bh * ((a.queries + 15) / 16))), dim3(256), 0, s, a);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-  }
   switch ((a.dim + 31) / 32) {
     case 1: return run<T, 32>(a, s);
     case 2: return run<T, 64>(a, s);
@@ -353,9 +388,41 @@ hipError_t run_dim(const AttnArgs& a, hipStream_t s) {
 
 }  // namespace
 
-int64_t attention_bwd_work(const AttnArgs& a) { return 2 * a.batch * a.heads * a.queries; }
+// Ranges of a key block's queries (all query heads that share the key head in one sequence): what an estimate
+// of the time makes shortest, in us, as in the forward pass: the longest walk alone, or all work spread over
+// the compute units, in whole rounds where the works are equal; and with several ranges the join.
+// Measured on MI355X, a tile of 64 queries: bfloat16 of head size 64 1.2 us when a compute unit has two
+// workgroups and 1.6 alone, of size 128 2.8 us (one fits); float32 of size 64 8.5 us.
+static void plan_bwd_splits(AttnArgs& a) {
+  const double unit = (double)((a.dim + 31) / 32 * 32) / 64, cus = (double)device_cus();
+  const double spread = (a.dtype == kF32 ? 8.5 : a.dim <= 64 ? 1.2 : 1.4) * unit;
+  const double alone = (a.dtype == kF32 ? 8.5 : a.dim <= 64 ? 1.6 : 1.4) * unit;
+  const int64_t tiles = a.heads / a.kv_heads * ((a.queries + kTile - 1) / kTile);
+  const double wgs = (double)(a.batch * a.kv_heads) * (double)((a.keys + kBlock - 1) / kBlock);
+  const bool halves = a.causal && a.keys * 2 > a.queries;
+  const double bytes = 16.0 * (double)(a.batch * a.kv_heads) * (double)a.keys * (double)a.dim;
+  double best = 0.0;
+  a.splits = 1;
+  for (int64_t n = 1; n <= std::min<int64_t>(tiles / 4 + 1, 256); n = n < 4 ? n + 1 : n + n / 4) {
+    const double walk = (double)((tiles + n - 1) / n);
+    const double slots = a.dtype != kF32 && a.dim <= 64 ? 2 * cus : cus, rounds = std::ceil(wgs * (double)n / slots);
+    const double all = halves ? 0.55 * wgs * (double)tiles / cus * spread : rounds * walk * spread * slots / cus;
+    const double t = std::max(walk * alone, all) + (n > 1 ? 4.0 + (double)n * bytes / 4.5e6 : 0.0);
+    if (n == 1 || t < best) {
+      best = t;
+      a.splits = (int)n;
+    }
+  }
+}
+
+int64_t attention_bwd_work(const AttnArgs& args) {
+  AttnArgs a = args;
+  plan_bwd_splits(a);
+  return delta_floats(a) + (a.splits > 1 ? (int64_t)a.splits * 2 * a.batch * a.kv_heads * a.keys * a.dim : 0);
+}
 
 hipError_t launch_attention_bwd(AttnArgs a, hipStream_t s) {
+  plan_bwd_splits(a);
   a.cus = (int)device_cus();
   switch (a.dtype) {
     case kF32: return run_dim<float>(a, s);

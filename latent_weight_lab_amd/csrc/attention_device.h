@@ -200,10 +200,10 @@ __device__ __forceinline__ float max_nan(float a, float b) { return __builtin_el
 
 // Nothing is moved across this point by the instruction scheduler: loads from LDS issued before it are
 // under way together, where the scheduler would issue each just before its use to save registers.
-template <class T>
+// Not for float32, where an operand feeds eight instructions of 64 cycles and its load needs no such lead.
+template <class T, int DP = 64>
 __device__ __forceinline__ void fence_schedule() {
-  // a float32 operand feeds eight instructions of 64 cycles: its load needs no such lead
-  if constexpr (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
+  if constexpr (sizeof(T) == 2 && DP <= 64) __builtin_amdgcn_sched_barrier(0);
 }
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }

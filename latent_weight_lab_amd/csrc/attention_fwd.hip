@@ -402,14 +402,35 @@ __global__ __launch_bounds__(256) void attention_join(const AttnArgs a) {
 bool by_token(const AttnArgs& a) { return a.heads / a.kv_heads * a.queries <= kTokenRows; }
 
 // Ranges of keys.  Single tokens: as many as make two workgroups for each compute unit, none shorter than
-// 256 keys.  Otherwise, where there is not half a workgroup for each compute unit, as many as make one,
-// none shorter than 512 keys: more costs the join more than the shorter walk gains.
+// 256 keys.  Otherwise what an estimate of the time makes shortest, in us: the larger of a workgroup's
+// own walk (kAlone a tile) and all work spread over the compute units (kSpread a tile), and with more
+// than one range the join.  The rates are measured on MI355X: bfloat16 of head size 64, 0.7 us a tile
+// when a compute unit has three workgroups and 1.2 us alone; float32 3.8 us either way (matrix cores).
 void plan_splits(AttnArgs& a) {
-  const bool token = by_token(a);
-  const int64_t wgs = token ? a.batch * a.kv_heads : a.batch * a.heads * ((a.queries + kRows - 1) / kRows);
-  const int64_t want = (token ? 2 : 1) * device_cus();
-  int64_t splits = wgs > 0 ? want / wgs : 1;
-  splits = std::max<int64_t>(1, std::min({splits, a.keys / (token ? 256 : 512), (int64_t)kMaxSplits}));
+  const int64_t cus = device_cus();
+  int64_t splits = 1;
+  if (by_token(a)) {
+    const int64_t wgs = std::max<int64_t>(1, a.batch * a.kv_heads);
+    splits = std::min({2 * cus / wgs, a.keys / 256, (int64_t)kMaxSplits});
+  } else {
+    const double unit = (double)((a.dim + 31) / 32 * 32) / 64;
+    const double alone = (a.dtype == kF32 ? 3.8 : 1.2) * unit, spread = (a.dtype == kF32 ? 3.8 : 0.7) * unit;
+    const int64_t tiles = (a.keys + kKeys - 1) / kKeys;
+    const double wgs = (double)(a.batch * a.heads) * (double)((a.queries + kRows - 1) / kRows);
+    // about half of a square causal call's tiles are walked
+    const double all = wgs * (double)tiles * (a.causal && a.queries * 2 > a.keys ? 0.55 : 1.0) * spread / (double)cus;
+    const double bytes = 8.0 * (double)(a.batch * a.heads) * (double)a.queries * (double)a.dim;  // of a range
+    double best = 0.0;
+    for (int64_t n = 1; n <= std::min<int64_t>(tiles / 4 + 1, kMaxSplits); n = n < 4 ? n + 1 : n + n / 4) {
+      const double walk = (double)((tiles + n - 1) / n) * alone;
+      const double t = std::max(walk, all) + (n > 1 ? 4.0 + (double)n * bytes / 4.5e6 : 0.0);
+      if (n == 1 || t < best) {
+        best = t;
+        splits = n;
+      }
+    }
+  }
+  splits = std::max<int64_t>(1, splits);
   a.split_len = splits > 1 ? ((a.keys + splits - 1) / splits + kKeys - 1) / kKeys * kKeys : std::max<int64_t>(a.keys, 1);
   a.splits = splits > 1 ? (int)((a.keys + a.split_len - 1) / a.split_len) : 1;
 }

@@ -78,7 +78,7 @@ def test_null_pointers_and_workspaces_are_refused():
     assert L.lwl_attention_backward(ctypes.byref(t), None, 0, None) == -1
     for f in ("q", "k", "v", "out", "lse", "grad_out", "grad_q", "grad_k", "grad_v"):
         setattr(t, f, 256)
-    assert L.lwl_attention_backward_workspace_size(ctypes.byref(t)) >= 2 * 4 * 2 * 4 * 9
+    assert L.lwl_attention_backward_workspace_size(ctypes.byref(t)) >= 4 * 2 * 4 * 9
     assert L.lwl_attention_backward(ctypes.byref(t), None, 0, None) == -3
 
 
