@@ -28,8 +28,12 @@ class _AttentionFn(torch.autograd.Function):
         q, k, v, out, lse, lengths = ctx.saved_tensors
         causal, scale, offset = ctx.meta
         # token by token in memory, as the linears before them leave q, k and v
-        grads = [torch.empty_like(t.transpose(1, 2), memory_format=torch.contiguous_format).transpose(1, 2)
-                 for t in (q, k, v)]
+        b, hq, tq, d = q.shape
+        hk, tk = k.shape[1], k.shape[2]
+        dtype, dev = q.dtype, q.device
+        grads = (torch.empty((b, tq, hq, d), dtype=dtype, device=dev).transpose(1, 2),
+                 torch.empty((b, tk, hk, d), dtype=dtype, device=dev).transpose(1, 2),
+                 torch.empty((b, tk, hk, d), dtype=dtype, device=dev).transpose(1, 2))
         layer_ops.attention_backward(q, k, v, out, lse, grad_out, causal, scale, lengths, offset, grads)
         return (*grads, None, None, None, None)
 
@@ -59,32 +63,20 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
     return layer_ops.attention_forward(q, k, v, causal, scale, key_lengths, causal_offset, False)[0]
 
 
-def _split(packed: torch.Tensor, heads: int, kv_heads: int):
-    b, t, width = packed.shape
-    dim = width // (heads + 2 * kv_heads)
-    x = packed.view(b, t, heads + 2 * kv_heads, dim).transpose(1, 2)
-    return x[:, :heads], x[:, heads:heads + kv_heads], x[:, heads + kv_heads:]
-
-
 class _PackedFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, heads, kv_heads, key_lengths, causal, scale, causal_offset):
-        q, k, v = _split(qkv, heads, kv_heads)
-        out, lse = layer_ops.attention_forward(q, k, v, causal, scale, key_lengths, causal_offset, True)
+        out, lse = layer_ops.attention_packed_forward(qkv, heads, kv_heads, causal, scale, key_lengths, causal_offset, True)
         ctx.save_for_backward(qkv, out, lse, key_lengths)
         ctx.meta = (heads, kv_heads, causal, scale, causal_offset)
-        return out.transpose(1, 2).reshape(*qkv.shape[:2], -1)
+        return out
 
     @staticmethod
     @layer_ops.once
     def backward(ctx, grad_out):
         qkv, out, lse, lengths = ctx.saved_tensors
         heads, kv_heads, causal, scale, offset = ctx.meta
-        grad = torch.empty_like(qkv)
-        b, t, width = grad_out.shape
-        g = grad_out.contiguous().view(b, t, heads, width // heads).transpose(1, 2)
-        layer_ops.attention_backward(*_split(qkv, heads, kv_heads), out, lse, g, causal, scale, lengths, offset,
-                                     _split(grad, heads, kv_heads))
+        grad = layer_ops.attention_packed_backward(qkv, out, lse, grad_out, heads, kv_heads, causal, scale, lengths, offset)
         return grad, None, None, None, None, None, None
 
 
@@ -100,9 +92,8 @@ def attention_packed(qkv: torch.Tensor, heads: int, kv_heads: int | None = None,
     if qkv.dim() != 3 or heads <= 0 or kv_heads <= 0 or qkv.shape[2] % (heads + 2 * kv_heads):
         raise N.BlockFHTArgumentError(f"attention_packed: {tuple(qkv.shape)} does not hold {heads} query and twice "
                                       f"{kv_heads} key heads")
-    qkv = qkv.contiguous()
+    if not qkv.is_contiguous():
+        qkv = qkv.contiguous()
     if torch.is_grad_enabled() and qkv.requires_grad:
         return _PackedFn.apply(qkv, heads, kv_heads, key_lengths, bool(causal), scale, causal_offset)
-    q, k, v = _split(qkv, heads, kv_heads)
-    out, _ = layer_ops.attention_forward(q, k, v, causal, scale, key_lengths, causal_offset, False)
-    return out.transpose(1, 2).reshape(*qkv.shape[:2], -1)
+    return layer_ops.attention_packed_forward(qkv, heads, kv_heads, causal, scale, key_lengths, causal_offset, False)[0]

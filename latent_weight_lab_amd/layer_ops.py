@@ -14,7 +14,6 @@ own checks are the only ones of what it checks.
 from __future__ import annotations
 
 import ctypes
-import math
 import struct
 
 import torch
@@ -234,27 +233,46 @@ def _dense_dim(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-def _attention_head(q, k, v, causal, scale, key_lengths, causal_offset):
-    """The first fields of the arguments, up to the scale, and the lengths as int32."""
+def _attention_lengths(key_lengths: torch.Tensor | None, batch: int) -> torch.Tensor | None:
+    if key_lengths is None or (key_lengths.dtype == torch.int32 and key_lengths.shape == (batch,)):
+        return key_lengths if key_lengths is None else _dense(key_lengths)
+    if key_lengths.shape != (batch,) or key_lengths.is_floating_point():
+        raise N.BlockFHTArgumentError(f"attention: key_lengths must be {batch} integers, got {tuple(key_lengths.shape)} of "
+                                      f"{key_lengths.dtype}")
+    return _dense(key_lengths.to(torch.int32))
+
+
+def _attention_shape(dtype, causal, scale, causal_offset, batch, heads, kv_heads, queries, keys, dim):
+    """The arguments' fields up to the scale."""
+    offset = 0 if causal_offset is None else int(causal_offset)
+    if not -(1 << 62) < offset < 1 << 62:
+        raise N.BlockFHTArgumentError(f"attention: causal_offset {offset} is too large")
+    if scale is None:
+        scale = dim ** -0.5 if dim else 0.0
+    return (N.dtype_code(dtype), bool(causal), causal_offset is None, 0, offset, batch, heads, kv_heads, queries, keys, dim,
+            float(scale))
+
+
+def _attention_shape_of(q, k, v, causal, scale, causal_offset):
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         raise N.BlockFHTArgumentError(f"attention: q, k and v must be [batch, heads, tokens, head size], got "
                                       f"{tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
     batch, heads, queries, dim = q.shape
-    if k.shape != v.shape or k.shape[0] != batch or k.shape[3] != dim:
+    kb, kv_heads, keys, kd = shape = k.shape
+    if shape != v.shape or kb != batch or kd != dim:
         raise N.BlockFHTArgumentError(f"attention: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not match")
-    if not q.dtype == k.dtype == v.dtype:
-        raise N.BlockFHTArgumentError(f"attention: q, k and v must have one type, got {q.dtype}, {k.dtype} and {v.dtype}")
-    if key_lengths is not None:
-        if key_lengths.shape != (batch,) or key_lengths.is_floating_point():
-            raise N.BlockFHTArgumentError(f"attention: key_lengths must be {batch} integers, got "
-                                          f"{tuple(key_lengths.shape)} of {key_lengths.dtype}")
-        key_lengths = _dense(key_lengths.to(torch.int32))
-    offset = 0 if causal_offset is None else int(causal_offset)
-    if not -(1 << 62) < offset < 1 << 62:
-        raise N.BlockFHTArgumentError(f"attention: causal_offset {offset} is too large")
-    head = (N.dtype_code(q.dtype), bool(causal), causal_offset is None, 0, offset, batch, heads, k.shape[1], queries,
-            k.shape[2], dim, 1.0 / math.sqrt(dim) if scale is None and dim else float(scale or 0.0))
-    return head, key_lengths
+    dtype = q.dtype
+    if k.dtype != dtype or v.dtype != dtype:
+        raise N.BlockFHTArgumentError(f"attention: q, k and v must have one type, got {dtype}, {k.dtype} and {v.dtype}")
+    return _attention_shape(dtype, causal, scale, causal_offset, batch, heads, kv_heads, queries, keys, dim)
+
+
+def _run_attention(index: int, like: torch.Tensor, forward: bool, *fields) -> None:
+    L = N.lib()
+    args = _ATTENTION.pack(*fields)
+    need = (L.lwl_attention_forward_workspace_size if forward else L.lwl_attention_backward_workspace_size)(args)
+    ws = _scratch(need, like)
+    _launch(index, L.lwl_attention_forward if forward else L.lwl_attention_backward, args, _ptr(ws), need)
 
 
 def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool, scale: float | None,
@@ -262,36 +280,69 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal:
     """``(out, lse)`` for ``[batch, heads, tokens, head size]`` tensors; ``out`` lies in memory token by token
     (all heads of a token together); ``lse`` (float32 ``[batch, heads, queries]``) is None unless ``keep_lse``."""
     index = _device_index(q, k, v, key_lengths)
-    head, lengths = _attention_head(q, k, v, causal, scale, key_lengths, causal_offset)
+    shape = _attention_shape_of(q, k, v, causal, scale, causal_offset)
     batch, heads, queries, dim = q.shape
+    lengths = _attention_lengths(key_lengths, batch)
     q, k, v = _dense_dim(q), _dense_dim(k), _dense_dim(v)
-    dev = q.device
-    out = torch.empty((batch, queries, heads, dim), dtype=q.dtype, device=dev).transpose(1, 2)
-    lse = torch.empty((batch, heads, queries), dtype=torch.float32, device=dev) if keep_lse else None
-    L = N.lib()
-    args = _ATTENTION.pack(*head, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(lengths),
-                           *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], *_NO_GRADS)
-    need = L.lwl_attention_forward_workspace_size(args)
-    ws = _scratch(need, q)
-    _launch(index, L.lwl_attention_forward, args, _ptr(ws), need)
+    out = torch.empty((batch, queries, heads, dim), dtype=q.dtype, device=q.device).transpose(1, 2)
+    lse = torch.empty((batch, heads, queries), dtype=torch.float32, device=q.device) if keep_lse else None
+    _run_attention(index, q, True, *shape, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse),
+                   _ptr(lengths), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], *_NO_GRADS)
     return out, lse
 
 
 def attention_backward(q, k, v, out, lse, grad_out, causal, scale, key_lengths, causal_offset, grads) -> None:
     """Fills ``grads``, the three gradients like q, k and v (any strides, a head's values dense)."""
     index = _device_index(q, k, v, out, lse, grad_out, key_lengths)
-    head, lengths = _attention_head(q, k, v, causal, scale, key_lengths, causal_offset)
+    shape = _attention_shape_of(q, k, v, causal, scale, causal_offset)
+    lengths = _attention_lengths(key_lengths, q.shape[0])
     q, k, v = _dense_dim(q), _dense_dim(k), _dense_dim(v)
     grad_out = _dense_dim(grad_out if grad_out.dtype == q.dtype else grad_out.to(q.dtype))
     gq, gk, gv = grads
-    L = N.lib()
-    args = _ATTENTION.pack(*head, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _ptr(lengths),
-                           *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], grad_out.data_ptr(),
-                           gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), *grad_out.stride()[:3], *gq.stride()[:3],
-                           *gk.stride()[:3], *gv.stride()[:3])
-    need = L.lwl_attention_backward_workspace_size(args)
-    ws = _scratch(need, q)
-    _launch(index, L.lwl_attention_backward, args, _ptr(ws), need)
+    _run_attention(index, q, False, *shape, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
+                   _ptr(lengths), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3],
+                   grad_out.data_ptr(), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), *grad_out.stride()[:3],
+                   *gq.stride()[:3], *gk.stride()[:3], *gv.stride()[:3])
+
+
+def _packed(qkv: torch.Tensor, heads: int, kv_heads: int):
+    """``(head size, strides, byte offsets of k and v)`` of a contiguous ``[batch, tokens, (heads + 2 kv_heads) *
+    head size]``: the pieces by address, without a view of each."""
+    tokens, width = qkv.shape[1], qkv.shape[2]
+    dim = width // (heads + 2 * kv_heads)
+    size = qkv.element_size()
+    return dim, (tokens * width, dim, width), heads * dim * size, (heads + kv_heads) * dim * size
+
+
+def attention_packed_forward(qkv: torch.Tensor, heads: int, kv_heads: int, causal: bool, scale: float | None,
+                             key_lengths: torch.Tensor | None, causal_offset: int | None, keep_lse: bool):
+    """``(out, lse)``; ``qkv`` contiguous, ``out`` ``[batch, tokens, heads * head size]``."""
+    index = _device_index(qkv, key_lengths)
+    dim, st, k_at, v_at = _packed(qkv, heads, kv_heads)
+    batch, tokens = qkv.shape[0], qkv.shape[1]
+    shape = _attention_shape(qkv.dtype, causal, scale, causal_offset, batch, heads, kv_heads, tokens, tokens, dim)
+    lengths = _attention_lengths(key_lengths, batch)
+    out = torch.empty((batch, tokens, heads * dim), dtype=qkv.dtype, device=qkv.device)
+    lse = torch.empty((batch, heads, tokens), dtype=torch.float32, device=qkv.device) if keep_lse else None
+    p = qkv.data_ptr()
+    _run_attention(index, qkv, True, *shape, p, p + k_at, p + v_at, out.data_ptr(), _ptr(lse), _ptr(lengths), *st, *st, *st,
+                   tokens * heads * dim, dim, heads * dim, *_NO_GRADS)
+    return out, lse
+
+
+def attention_packed_backward(qkv, out, lse, grad_out, heads, kv_heads, causal, scale, key_lengths, causal_offset):
+    """The gradient of ``qkv``, in one tensor like it."""
+    index = _device_index(qkv, out, lse, grad_out, key_lengths)
+    dim, st, k_at, v_at = _packed(qkv, heads, kv_heads)
+    batch, tokens = qkv.shape[0], qkv.shape[1]
+    shape = _attention_shape(qkv.dtype, causal, scale, causal_offset, batch, heads, kv_heads, tokens, tokens, dim)
+    lengths = _attention_lengths(key_lengths, batch)
+    grad_out = _dense(grad_out if grad_out.dtype == qkv.dtype else grad_out.to(qkv.dtype))
+    grad = torch.empty_like(qkv)
+    p, g, ost = qkv.data_ptr(), grad.data_ptr(), (tokens * heads * dim, dim, heads * dim)
+    _run_attention(index, qkv, False, *shape, p, p + k_at, p + v_at, out.data_ptr(), lse.data_ptr(), _ptr(lengths),
+                   *st, *st, *st, *ost, grad_out.data_ptr(), g, g + k_at, g + v_at, *ost, *st, *st, *st)
+    return grad
 
 
 def once(backward):
