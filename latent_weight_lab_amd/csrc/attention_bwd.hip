@@ -30,16 +30,17 @@ constexpr int kTile = kTileRows;  // queries (keys) of a tile
 // a key's probabilities over the queries, all of which may be small, and small ones are subnormal in
 // float16 and flushed by the exponential in float32.
 constexpr float kLift = 14.0f, kLower = 0x1p-14f;
+// dS made of them is taken back before it is rounded to float16, whose range it could leave, and with dK
+// at the end otherwise.
+template <class T>
+constexpr bool kLowerLate = !__is_same(T, f16);
 
-// Head sizes up to 64 leave registers for two waves a SIMD, which overlap; larger ones of a 16-bit type run
-// one, whose two halves of a tile the scheduler may interleave.
+// Head sizes up to 96 leave registers for two waves a SIMD, which overlap; 128 of a 16-bit type runs one, whose
+// two halves of a tile the scheduler may interleave.
 template <class T, int DP>
 constexpr int kUnroll = sizeof(T) == 2 && DP > 64 ? 2 : 1;
-
 template <class T, int DP>
-struct BwdTile {
-  static constexpr int S = DP + 16 / (int)sizeof(T);  // LDS row: 16-byte reads of 16 rows on distinct banks
-};
+constexpr int kKeysOccupancy = sizeof(T) == 2 && DP <= 64 ? 2 : 1;
 
 // The workspace: D of every query, then (256-byte aligned) the key gradients' partial sums.
 __host__ __device__ inline int64_t delta_floats(const AttnArgs& a) {
@@ -48,8 +49,8 @@ __host__ __device__ inline int64_t delta_floats(const AttnArgs& a) {
 __device__ __forceinline__ float* partials(const AttnArgs& a) { return a.work + delta_floats(a); }
 
 template <class T, int DP, bool FAST>
-__global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void attention_bwd_keys(const AttnArgs a) {
-  using Tile = BwdTile<T, DP>;
+__global__ __launch_bounds__(256, (kKeysOccupancy<T, DP>)) void attention_bwd_keys(const AttnArgs a) {
+  using Tile = BothWays<T, DP>;
   constexpr int KK = DP / 16, DT = DP / 32;
   __shared__ __attribute__((aligned(16))) T lds_q[2][kTile * Tile::S];
   __shared__ __attribute__((aligned(16))) T lds_g[2][kTile * Tile::S];
@@ -101,8 +102,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void atten
     }
   };
   auto put = [&](int buf) {
-    qt.template put<Tile::S>(lds_q[buf]);
-    gt.template put<Tile::S>(lds_g[buf]);
+    qt.template put<Tile>(lds_q[buf]);
+    gt.template put<Tile>(lds_g[buf]);
     if (threadIdx.x < 2 * kTile) lds_stat[buf][threadIdx.x / kTile][threadIdx.x & (kTile - 1)] = sr;
   };
   int buf = 0;
@@ -139,14 +140,19 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void atten
             }
           }
 #pragma unroll
-          for (int kk = 0; kk < KK; ++kk) {
-            qf[kk] = lds_frag(lq + (lane & 31) * Tile::S + kk * 16 + half * 8);
-            gf[kk] = lds_frag(lg + (lane & 31) * Tile::S + kk * 16 + half * 8);
+          for (int kk = 0; kk < KK; ++kk) qf[kk] = lds_frag(lq + Tile::at(lane & 31, kk * 16 + half * 8));
+          // 96: the two products one after the other, which holds half as many operands at a time
+          if constexpr (DP == 96) {
+            fence_schedule<T>();
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) s = mma32(qf[kk], kf[kk], s);
           }
-          fence_schedule<T, DP>();
+#pragma unroll
+          for (int kk = 0; kk < KK; ++kk) gf[kk] = lds_frag(lg + Tile::at(lane & 31, kk * 16 + half * 8));
+          if constexpr (DP <= 96) fence_schedule<T>();
 #pragma unroll
           for (int kk = 0; kk < KK; ++kk) {
-            s = mma32(qf[kk], kf[kk], s);
+            if constexpr (DP != 96) s = mma32(qf[kk], kf[kk], s);
             dp = mma32(gf[kk], vf[kk], dp);
           }
         }
@@ -156,14 +162,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void atten
 #pragma unroll
           for (int d = 0; d < DT; ++d) {
             const int row = u * 16 + half * 4;
-            gc[u][d] = lds_column_frag(lg, Tile::S, row, row + 8, d * 32 + (lane & 16));
-            qc[u][d] = lds_column_frag(lq, Tile::S, row, row + 8, d * 32 + (lane & 16));
+            gc[u][d] = lds_column_frag<Tile>(lg, row, row + 8, d * 32 + (lane & 16));
+            qc[u][d] = lds_column_frag<Tile>(lq, row, row + 8, d * 32 + (lane & 16));
           }
-        fence_schedule<T, DP>();
+        if constexpr (DP <= 96) fence_schedule<T>();
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           s[r] = exp2_hw(s[r] * c);
-          dp[r] = s[r] * (dp[r] * kLower);
+          dp[r] = s[r] * (kLowerLate<T> ? dp[r] : dp[r] * kLower);
         }
         if (masked) {
           // key < key_end(q), that is q >= key - off
@@ -194,20 +200,22 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void atten
     q0 = next_q;
   }
   if (key >= (int)a.keys) return;
+  const float dk_scale = kLowerLate<T> ? a.scale * kLower : a.scale;
   if (splits > 1) {  // summed by attention_bwd_join
     const int64_t kv_rows = a.batch * a.kv_heads * a.keys, row = (b * a.kv_heads + hk) * a.keys + key;
     float* part = partials(a) + (split * kv_rows + row) * 2 * dim;
-    store_result<float, DP, FAST>(part, dk, a.scale, dim);
+    store_result<float, DP, FAST>(part, dk, dk_scale, dim);
     store_result<float, DP, FAST>(part + dim, dv, kLower, dim);
     return;
   }
-  store_result<T, DP, FAST>((T*)a.dk + b * a.dks[0] + hk * a.dks[1] + (int64_t)key * a.dks[2], dk, a.scale, dim);
+  store_result<T, DP, FAST>((T*)a.dk + b * a.dks[0] + hk * a.dks[1] + (int64_t)key * a.dks[2], dk, dk_scale, dim);
   store_result<T, DP, FAST>((T*)a.dv + b * a.dvs[0] + hk * a.dvs[1] + (int64_t)key * a.dvs[2], dv, kLower, dim);
 }
 
 template <class T, int DP, bool FAST>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_bwd_queries(const AttnArgs a) {
-  using Tile = BwdTile<T, DP>;
+  // rows padded by 16 bytes: one tile in three is read by columns, and BothWays' addresses cost registers
+  using Tile = Padded<T, DP>;
   constexpr int KK = DP / 16, DT = DP / 32;
   __shared__ __attribute__((aligned(16))) T lds_k[2][kTile * Tile::S];
   __shared__ __attribute__((aligned(16))) T lds_v[2][kTile * Tile::S];
@@ -254,8 +262,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_bwd_que
   f32x16 dq[DT] = {};
   const float c = a.scale * kLog2E;
   if (end > 0) {
-    kt.template put<Tile::S>(lds_k[0]);
-    vt.template put<Tile::S>(lds_v[0]);
+    kt.template put<Tile>(lds_k[0]);
+    vt.template put<Tile>(lds_v[0]);
   }
   int buf = 0;
   for (int j0 = 0; j0 < end; j0 += kTile, buf ^= 1) {
@@ -274,7 +282,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_bwd_que
         {
           Frag<T> kf[KK], vf[KK];
 #pragma unroll
-          for (int kk = 0; kk < KK; ++kk) kf[kk] = lds_frag(lk + (lane & 31) * Tile::S + kk * 16 + half * 8);
+          for (int kk = 0; kk < KK; ++kk) kf[kk] = lds_frag(lk + Tile::at(lane & 31, kk * 16 + half * 8));
           // beyond 64 the two products one after the other, which holds half as many operands at a time
           if constexpr (DP > 64) {
             fence_schedule<T>();
@@ -282,7 +290,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_bwd_que
             for (int kk = 0; kk < KK; ++kk) s = mma32(kf[kk], qf[kk], s);
           }
 #pragma unroll
-          for (int kk = 0; kk < KK; ++kk) vf[kk] = lds_frag(lv + (lane & 31) * Tile::S + kk * 16 + half * 8);
+          for (int kk = 0; kk < KK; ++kk) vf[kk] = lds_frag(lv + Tile::at(lane & 31, kk * 16 + half * 8));
           fence_schedule<T>();
 #pragma unroll
           for (int kk = 0; kk < KK; ++kk) {
@@ -295,7 +303,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_bwd_que
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int d = 0; d < DT; ++d)
-            kc[u][d] = lds_column_frag(lk, Tile::S, u * 16 + half * 4, u * 16 + half * 4 + 8, d * 32 + (lane & 16));
+            kc[u][d] = lds_column_frag<Tile>(lk, u * 16 + half * 4, u * 16 + half * 4 + 8, d * 32 + (lane & 16));
         fence_schedule<T>();
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = exp2_hw(fmaf(s[r], c, -lse)) * (dp[r] - delta);
@@ -316,8 +324,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_bwd_que
       }
     }
     if (more) {
-      kt.template put<Tile::S>(lds_k[buf ^ 1]);
-      vt.template put<Tile::S>(lds_v[buf ^ 1]);
+      kt.template put<Tile>(lds_k[buf ^ 1]);
+      vt.template put<Tile>(lds_v[buf ^ 1]);
     }
   }
   if (q >= queries) return;

@@ -66,24 +66,24 @@ __device__ __forceinline__ void lds_put(T* p, const Raw8<T>& v) {
 // Four values of one column from four consecutive rows of an LDS tile, for each of the 16 columns that
 // 16 consecutive lanes ask for: lane i of the 16 gets column col0 + i, rows row0 .. + 3.  16-bit types
 // use the transposing read: lane i names the address of row row0 + i / 4, columns col0 + 4 (i % 4) .. + 3.
-template <class T>
-__device__ __forceinline__ void lds_column4(T (&v)[4], const T* tile, int stride, int row0, int col0) {
+template <class Layout, class T>
+__device__ __forceinline__ void lds_column4(T (&v)[4], const T* tile, int row0, int col0) {
   const int i = threadIdx.x & 15;
   if constexpr (sizeof(T) == 2) {
-    const T* p = tile + (row0 + (i >> 2)) * stride + col0 + (i & 3) * 4;
+    const T* p = tile + Layout::at(row0 + (i >> 2), col0 + (i & 3) * 4);
     const s16x4 t = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)p);
     __builtin_memcpy(v, &t, sizeof(t));
   } else {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) v[r] = tile[(row0 + r) * stride + col0 + i];
+    for (int r = 0; r < 4; ++r) v[r] = tile[Layout::at(row0 + r, col0 + i)];
   }
 }
 // The operand whose eight k are rows a .. a + 3 and b .. b + 3 of a tile, at column col0 + (lane % 16).
-template <class T>
-__device__ __forceinline__ Frag<T> lds_column_frag(const T* tile, int stride, int a, int b, int col0) {
+template <class Layout, class T>
+__device__ __forceinline__ Frag<T> lds_column_frag(const T* tile, int a, int b, int col0) {
   T lo[4], hi[4];
-  lds_column4(lo, tile, stride, a, col0);
-  lds_column4(hi, tile, stride, b, col0);
+  lds_column4<Layout>(lo, tile, a, col0);
+  lds_column4<Layout>(hi, tile, b, col0);
   Frag<T> f;
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
@@ -92,6 +92,36 @@ __device__ __forceinline__ Frag<T> lds_column_frag(const T* tile, int stride, in
   }
   return f;
 }
+
+// Where value (row, col) of a tile lies in LDS when the tile is read both by rows (16 bytes a lane, 16 rows at a
+// time) and by columns (lds_column4: 4 rows of 64 bytes at a time).  16-bit types: a row's chunks of 16 bytes
+// are exchanged by an exclusive or with a number made of the row's, so that either read finds its 16
+// chunks on distinct banks: rows 0 .. 15 have distinct numbers (of those that share banks), and four
+// consecutive rows from a multiple of four differ in the bits that tell blocks of 64 bytes apart.  Rows of
+// 96 are laid out as 128.  float32: rows padded by 16 bytes (columns are read value by value).
+template <class T, int DP>
+struct BothWays {
+  static constexpr int S = sizeof(T) == 4 ? DP + 4 : DP == 96 ? 128 : DP;
+  static __device__ __forceinline__ int at(int row, int col) {
+    if constexpr (sizeof(T) == 4) {
+      return row * S + col;
+    } else {
+      const int f = S == 128 ? ((row & 3) << 2) | ((row >> 2) & 3)
+                    : S == 64 ? ((row & 2) << 1) | ((row >> 2) & 3) : (row >> 2) & 3;
+      return row * S + ((((col >> 3) ^ f) << 3) | (col & 7));
+    }
+  }
+};
+// Rows of a fixed stride.
+template <int STRIDE>
+struct Strided {
+  static constexpr int S = STRIDE;
+  static __device__ __forceinline__ int at(int row, int col) { return row * STRIDE + col; }
+};
+
+// Rows padded by 16 bytes: 16-byte reads of 16 rows fall on distinct banks.
+template <class T, int DP>
+using Padded = Strided<DP + 16 / (int)sizeof(T)>;
 
 // Tiles of 64 rows that a workgroup of 256 threads brings from memory through registers into LDS: fetch()
 // starts the loads, put() stores what came.  Rows from `end` on and columns past the head size are zeros.
@@ -143,12 +173,12 @@ struct TileLoader {
       }
     }
   }
-  template <int STRIDE>
+  template <class Layout>
   __device__ __forceinline__ void put(T* lds) const {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int c = threadIdx.x + i * 256;
-      lds_put(lds + (c / CPR) * STRIDE + (c % CPR) * 8, r[i]);
+      lds_put(lds + Layout::at(c / CPR, (c % CPR) * 8), r[i]);
     }
   }
 };
@@ -201,9 +231,9 @@ __device__ __forceinline__ float max_nan(float a, float b) { return __builtin_el
 // Nothing is moved across this point by the instruction scheduler: loads from LDS issued before it are
 // under way together, where the scheduler would issue each just before its use to save registers.
 // Not for float32, where an operand feeds eight instructions of 64 cycles and its load needs no such lead.
-template <class T, int DP = 64>
+template <class T>
 __device__ __forceinline__ void fence_schedule() {
-  if constexpr (sizeof(T) == 2 && DP <= 64) __builtin_amdgcn_sched_barrier(0);
+  if constexpr (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
 }
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }

@@ -90,8 +90,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_rows(co
   if (begin < end) {
     kt.fetch(begin, end);
     vt.fetch(begin, end);
-    kt.template put<Tile::KS>(lds_k[0]);
-    vt.template put<Tile::VS>(lds_v[0]);
+    kt.template put<Strided<Tile::KS>>(lds_k[0]);
+    vt.template put<Strided<Tile::VS>>(lds_v[0]);
   }
   int buf = 0;
   for (int j0 = begin; j0 < end; j0 += kKeys, buf ^= 1) {
@@ -112,17 +112,19 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_rows(co
 #pragma unroll
           for (int t = 0; t < 2; ++t) kf[t][kk] = lds_frag(lk + t * 32 * Tile::KS + kk * 16);
         fence_schedule<T>();
+        if constexpr (DP > 64) __builtin_amdgcn_s_setprio(1);  // 1 x 8192 x 16 x 128: 548 -> 529 us; slower at 64
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
           for (int t = 0; t < 2; ++t) s[t] = mma32(kf[t][kk], qf[kk], s[t]);
+        if constexpr (DP > 64) __builtin_amdgcn_s_setprio(0);
       }
       Frag<T> vf[4][DT];
 #pragma unroll
       for (int u = 0; u < 4; ++u)
 #pragma unroll
         for (int d = 0; d < DT; ++d)
-          vf[u][d] = lds_column_frag(lv, Tile::VS, u * 16 + half * 4, u * 16 + half * 4 + 8, d * 32 + (lane & 16));
+          vf[u][d] = lds_column_frag<Strided<Tile::VS>>(lv, u * 16 + half * 4, u * 16 + half * 4 + 8, d * 32 + (lane & 16));
       fence_schedule<T>();
       if (j0 + kKeys > free_end) {
         const int lim = std::min(q_end, end) - j0 - half * 4;
@@ -160,8 +162,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_rows(co
       }
     }
     if (more) {
-      kt.template put<Tile::KS>(lds_k[buf ^ 1]);
-      vt.template put<Tile::VS>(lds_v[buf ^ 1]);
+      kt.template put<Strided<Tile::KS>>(lds_k[buf ^ 1]);
+      vt.template put<Strided<Tile::VS>>(lds_v[buf ^ 1]);
     }
   }
   sum += other_half(sum);
@@ -286,7 +288,7 @@ __global__ __launch_bounds__(256) void attention_token(const AttnArgs a) {
     asm volatile("" ::: "memory");
 #pragma unroll
     for (int d = 0; d < DT; ++d)
-      o[d] = mma16(lds_column_frag(lds_v, VS, quad * 4, quad * 4 + 16, d * 16), p, o[d]);
+      o[d] = mma16(lds_column_frag<Strided<VS>>(lds_v, quad * 4, quad * 4 + 16, d * 16), p, o[d]);
     asm volatile("" ::: "memory");
   }
   sum += __shfl_xor(sum, 16, 64);
