@@ -12,6 +12,7 @@ already mapped (same SONAME), and streams and device pointers interoperate.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 import threading
 from pathlib import Path
@@ -85,6 +86,7 @@ class BlockFHTArgumentError(ValueError, RuntimeError):
 
 _lock = threading.Lock()
 _lib = None
+_layers = None
 _error: Exception | None = None
 
 
@@ -157,6 +159,32 @@ def lib():
     if _lib is None:
         raise RuntimeError(f"latent_weight_lab_amd: HIP BlockFHT library unavailable: {_error}") from _error
     return _lib
+
+
+TORCH_EXT_NAME = "lwl_layers"
+
+
+def layers():
+    """The layer operators' torch binding over the loaded library; raises RuntimeError (with the cause) if
+    either cannot load."""
+    global _layers
+    if _layers is not None:
+        return _layers
+    lib()
+    with _lock:
+        if _layers is None:
+            path = LIB_DIR / f"{TORCH_EXT_NAME}.so"
+            try:
+                if not path.exists():
+                    raise FileNotFoundError(f"{path} is missing; build it with `python -m latent_weight_lab_amd.build`")
+                spec = importlib.util.spec_from_file_location(TORCH_EXT_NAME, path)
+                module = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(module)
+                module.bind(str(library_path()), BlockFHTArgumentError)
+            except Exception as exc:  # noqa: BLE001 - re-raised with what it is about
+                raise RuntimeError(f"latent_weight_lab_amd: torch binding of the layer operators unavailable: {exc}") from exc
+            _layers = module
+    return _layers
 
 
 def load_error() -> Exception | None:

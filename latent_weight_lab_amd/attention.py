@@ -11,31 +11,6 @@ from __future__ import annotations
 import torch
 
 from . import _native as N
-from . import layer_ops
-
-
-class _AttentionFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, key_lengths, causal, scale, causal_offset):
-        out, lse = layer_ops.attention_forward(q, k, v, causal, scale, key_lengths, causal_offset, True)
-        ctx.save_for_backward(q, k, v, out, lse, key_lengths)
-        ctx.meta = (causal, scale, causal_offset)
-        return out
-
-    @staticmethod
-    @layer_ops.once
-    def backward(ctx, grad_out):
-        q, k, v, out, lse, lengths = ctx.saved_tensors
-        causal, scale, offset = ctx.meta
-        # token by token in memory, as the linears before them leave q, k and v
-        b, hq, tq, d = q.shape
-        hk, tk = k.shape[1], k.shape[2]
-        dtype, dev = q.dtype, q.device
-        grads = (torch.empty((b, tq, hq, d), dtype=dtype, device=dev).transpose(1, 2),
-                 torch.empty((b, tk, hk, d), dtype=dtype, device=dev).transpose(1, 2),
-                 torch.empty((b, tk, hk, d), dtype=dtype, device=dev).transpose(1, 2))
-        layer_ops.attention_backward(q, k, v, out, lse, grad_out, causal, scale, lengths, offset, grads)
-        return (*grads, None, None, None, None)
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = False, scale: float | None = None,
@@ -58,26 +33,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
     ``out.transpose(1, 2).reshape(batch, queries, -1)`` copies nothing.  Softmax and sums are float32; in 16-bit
     types the probabilities are rounded to the type before the product with v.  Differentiable in q, k
     and v (once)."""
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _AttentionFn.apply(q, k, v, key_lengths, bool(causal), scale, causal_offset)
-    return layer_ops.attention_forward(q, k, v, causal, scale, key_lengths, causal_offset, False)[0]
-
-
-class _PackedFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, qkv, heads, kv_heads, key_lengths, causal, scale, causal_offset):
-        out, lse = layer_ops.attention_packed_forward(qkv, heads, kv_heads, causal, scale, key_lengths, causal_offset, True)
-        ctx.save_for_backward(qkv, out, lse, key_lengths)
-        ctx.meta = (heads, kv_heads, causal, scale, causal_offset)
-        return out
-
-    @staticmethod
-    @layer_ops.once
-    def backward(ctx, grad_out):
-        qkv, out, lse, lengths = ctx.saved_tensors
-        heads, kv_heads, causal, scale, offset = ctx.meta
-        grad = layer_ops.attention_packed_backward(qkv, out, lse, grad_out, heads, kv_heads, causal, scale, lengths, offset)
-        return grad, None, None, None, None, None, None
+    return N.layers().attention(q, k, v, causal, scale, key_lengths, causal_offset)
 
 
 def attention_packed(qkv: torch.Tensor, heads: int, kv_heads: int | None = None, causal: bool = True,
@@ -87,13 +43,5 @@ def attention_packed(qkv: torch.Tensor, heads: int, kv_heads: int | None = None,
     head size]``, queries, keys and values side by side (one linear's output), and the result ``[batch,
     tokens, heads * head size]``.  Nothing is split or copied, and the gradient is one tensor like qkv.  The
     other arguments are ``attention``'s."""
-    heads = int(heads)
-    kv_heads = heads if kv_heads is None else int(kv_heads)
-    if qkv.dim() != 3 or heads <= 0 or kv_heads <= 0 or qkv.shape[2] % (heads + 2 * kv_heads):
-        raise N.BlockFHTArgumentError(f"attention_packed: {tuple(qkv.shape)} does not hold {heads} query and twice "
-                                      f"{kv_heads} key heads")
-    if not qkv.is_contiguous():
-        qkv = qkv.contiguous()
-    if torch.is_grad_enabled() and qkv.requires_grad:
-        return _PackedFn.apply(qkv, heads, kv_heads, key_lengths, bool(causal), scale, causal_offset)
-    return layer_ops.attention_packed_forward(qkv, heads, kv_heads, causal, scale, key_lengths, causal_offset, False)[0]
+    return N.layers().attention_packed(qkv, heads, heads if kv_heads is None else kv_heads, causal, scale, key_lengths,
+                                       causal_offset)

@@ -1,4 +1,5 @@
-"""Build ``lib/liblwl_bfht.so`` from ``csrc/`` with hipcc for gfx950.
+"""Build ``lib/liblwl_bfht.so`` from ``csrc/`` with hipcc for gfx950, and ``lib/lwl_layers.so``, the layer
+operators' torch binding (host code over the library's C entries), from ``csrc/torch_ext/``.
 
 Usage: ``python -m latent_weight_lab_amd.build`` (also called by
 ``__graft_entry__.build()``).  Objects compile in parallel; the library is
@@ -27,6 +28,7 @@ INCLUDE = PKG.parent / "include"
 OUT_DIR = PKG / "lib"
 OBJ_DIR = OUT_DIR / "obj"
 LIB = OUT_DIR / "liblwl_bfht.so"
+TORCH_EXT = OUT_DIR / "lwl_layers.so"
 
 ARCH = "gfx950"
 COMMON_FLAGS = ["-O3", "-std=c++17", "-fPIC", "-Wall", f"-I{INCLUDE}"]
@@ -69,6 +71,27 @@ def _compile(src: Path, obj_dir: Path = OBJ_DIR, sanitize: bool = False) -> Path
     return obj
 
 
+def build_torch_ext() -> Path:
+    """The torch binding, for the torch and Python that run this."""
+    import sysconfig
+
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    cxx = shutil.which("g++") or "g++"
+    tmp = TORCH_EXT.with_suffix(".so.tmp")
+    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}", f"-I{root / 'include'}",
+           f"-I{root / 'include' / 'torch' / 'csrc' / 'api' / 'include'}", f"-I{Path(hipcc()).resolve().parents[1] / 'include'}",
+           f"-I{sysconfig.get_paths()['include']}", str(CSRC / "torch_ext" / "layer_torch.cpp"), f"-L{root / 'lib'}",
+           "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python", "-ldl", "-o", str(tmp)]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"{cxx} failed on layer_torch.cpp:\n{res.stderr}")
+    os.replace(tmp, TORCH_EXT)
+    return TORCH_EXT
+
+
 def build(verbose: bool = False, sanitize: bool = False) -> Path:
     out_dir = OUT_DIR / "sanitize" if sanitize else OUT_DIR
     obj_dir = out_dir / "obj"
@@ -77,7 +100,10 @@ def build(verbose: bool = False, sanitize: bool = False) -> Path:
     srcs = sources()
     jobs = min(len(srcs), int(os.environ.get("MAX_JOBS", os.cpu_count() or 4)))
     with ThreadPoolExecutor(max_workers=max(1, jobs)) as pool:
+        ext = None if sanitize else pool.submit(build_torch_ext)
         objs = list(pool.map(lambda s: _compile(s, obj_dir, sanitize), srcs))
+        if ext is not None:
+            ext.result()
     tmp = lib.with_suffix(".so.tmp")
     link = ["-shared-libasan", "-Xarch_host", "-fsanitize=address", "-Xarch_host", "-fsanitize=undefined"] if sanitize else []
     cmd = [hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", *link, "-o", str(tmp), *map(str, objs)]
@@ -86,7 +112,7 @@ def build(verbose: bool = False, sanitize: bool = False) -> Path:
         raise RuntimeError(f"link failed:\n{res.stderr}")
     os.replace(tmp, lib)
     if verbose:
-        print(f"built {lib}")
+        print(f"built {lib}" + ("" if sanitize else f" and {TORCH_EXT.name}"))
     return lib
 
 

@@ -11,6 +11,7 @@ from __future__ import annotations
 import torch
 from torch import nn
 
+from . import _native as N
 from . import layer_ops
 
 
@@ -18,9 +19,9 @@ class Checkpoint8:
     """What is kept of GELU's input z: int8 ``codes``, float32 ``scales`` for groups of 128 features;
     they stand for ``codes * scale``."""
 
-    def __init__(self, codes, scales, shape, dtype, approximate):
+    def __init__(self, codes, scales, x, approximate):
         self.codes, self.scales = codes, scales
-        self.shape, self.dtype, self.approximate = tuple(shape), dtype, approximate
+        self.shape, self.dtype, self.approximate = tuple(x.shape), x.dtype, approximate
 
     def values(self) -> torch.Tensor:
         """What the codes stand for, in float32 and the input's shape."""
@@ -36,23 +37,6 @@ class Checkpoint8:
         return self.codes.numel() + 4 * self.scales.numel()
 
 
-class _Gelu8Fn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, bias, approximate, holder):
-        out, codes, scales = layer_ops.gelu8_forward(x, bias, approximate, True)
-        holder.append(Checkpoint8(codes, scales, x.shape, x.dtype, approximate))
-        ctx.save_for_backward(codes, scales)
-        ctx.meta = (x.dtype, approximate)
-        return out
-
-    @staticmethod
-    @layer_ops.once
-    def backward(ctx, grad_out):
-        codes, scales = ctx.saved_tensors
-        gx, gb = layer_ops.gelu8_backward(codes, scales, grad_out, *ctx.meta, ctx.needs_input_grad[1])
-        return gx, gb, None, None
-
-
 def gelu_checkpoint8(x: torch.Tensor, bias: torch.Tensor | None = None, approximate: str = "none",
                      return_checkpoint: bool = False):
     """``gelu(x + bias)`` over any leading dimensions; ``approximate`` as ``torch.nn.functional.gelu``'s.
@@ -60,13 +44,8 @@ def gelu_checkpoint8(x: torch.Tensor, bias: torch.Tensor | None = None, approxim
     The forward value is exact (float32, rounded once); the backward pass takes the derivative at
     the 8-bit checkpoint of ``x + bias``.  With ``return_checkpoint`` returns ``(activation,
     Checkpoint8)``.  Where no gradient is recorded and no checkpoint asked for, nothing is kept."""
-    recorded = torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad))
-    if recorded:
-        holder: list[Checkpoint8] = []
-        out = _Gelu8Fn.apply(x, bias, approximate, holder)
-        return (out, holder[0]) if return_checkpoint else out
-    out, codes, scales = layer_ops.gelu8_forward(x, bias, approximate, return_checkpoint)
-    return (out, Checkpoint8(codes, scales, x.shape, x.dtype, approximate)) if return_checkpoint else out
+    out, codes, scales = N.layers().gelu8(x, bias, layer_ops.tanh_form(approximate), return_checkpoint)
+    return (out, Checkpoint8(codes, scales, x, approximate)) if return_checkpoint else out
 
 
 def gelu_linear_checkpoint8(x: torch.Tensor, linear: nn.Module, bias: torch.Tensor | None = None,
