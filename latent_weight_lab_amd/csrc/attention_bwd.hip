@@ -34,6 +34,10 @@ constexpr float kLift = 14.0f, kLower = 0x1p-14f;
 // at the end otherwise.
 template <class T>
 constexpr bool kLowerLate = !__is_same(T, f16);
+// 16-bit products start from what is to be subtracted of them, S - lse / c with c = scale log2(e), and dP - D,
+// which saves an operation a score.  Their sums then round at the size of lse / c: not for float32.
+template <class T>
+constexpr bool kFoldStats = sizeof(T) == 2;
 
 // Head sizes up to 96 leave registers for two waves a SIMD, which overlap; 128 of a 16-bit type runs one, whose
 // two halves of a tile the scheduler may interleave.
@@ -70,7 +74,6 @@ __global__ __launch_bounds__(256, (kKeysOccupancy<T, DP>)) void attention_bwd_ke
   load_operand<T, DP, FAST>(kf, (const T*)a.k + b * a.ks[0] + hk * a.ks[1] + (int64_t)key * a.ks[2], dim, key < seen);
   load_operand<T, DP, FAST>(vf, (const T*)a.v + b * a.vs[0] + hk * a.vs[1] + (int64_t)key * a.vs[2], dim, key < seen);
   f32x16 dk[DT] = {}, dv[DT] = {};
-  // The products start from what is to be subtracted: S - lse / c, with c = scale log2(e), and dP - D.
   const float c = a.scale * kLog2E, inv_c = 1.0f / c;
   // queries before k0 - off see none of the block's keys (so none that sees nothing is ever read), those
   // before wk0 - off none of the wave's
@@ -98,7 +101,7 @@ __global__ __launch_bounds__(256, (kKeysOccupancy<T, DP>)) void attention_bwd_ke
       const bool is_d = threadIdx.x >= kTile;
       const float* stat = (is_d ? a.work : a.lse) + head0 + (int64_t)fg * queries;
       sr = q < queries ? stat[q] : (is_d ? 0.0f : INFINITY);  // past the last: no probabilities
-      sr = is_d ? -sr : (kLift - sr * kLog2E) * inv_c;
+      sr = is_d ? -sr : kFoldStats<T> ? (kLift - sr * kLog2E) * inv_c : kLift - sr * kLog2E;
     }
   };
   auto put = [&](int buf) {
@@ -135,8 +138,8 @@ __global__ __launch_bounds__(256, (kKeysOccupancy<T, DP>)) void attention_bwd_ke
             const f32x4 d = *(const f32x4*)&lds_stat[buf][1][at + r4 * 8 + half * 4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              s[r4 * 4 + r] = l[r];
-              dp[r4 * 4 + r] = d[r];
+              s[r4 * 4 + r] = kFoldStats<T> ? l[r] : 0.0f;
+              dp[r4 * 4 + r] = kFoldStats<T> ? d[r] : 0.0f;
             }
           }
 #pragma unroll
@@ -168,7 +171,13 @@ __global__ __launch_bounds__(256, (kKeysOccupancy<T, DP>)) void attention_bwd_ke
         if constexpr (DP <= 96) fence_schedule<T>();
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          s[r] = exp2_hw(s[r] * c);
+          if constexpr (kFoldStats<T>) {
+            s[r] = exp2_hw(s[r] * c);
+          } else {
+            const int i = at + (r >> 2) * 8 + half * 4 + (r & 3);
+            s[r] = exp2_hw(fmaf(s[r], c, lds_stat[buf][0][i]));
+            dp[r] += lds_stat[buf][1][i];
+          }
           dp[r] = s[r] * (kLowerLate<T> ? dp[r] : dp[r] * kLower);
         }
         if (masked) {
@@ -220,12 +229,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_bwd_que
   __shared__ __attribute__((aligned(16))) T lds_k[2][kTile * Tile::S];
   __shared__ __attribute__((aligned(16))) T lds_v[2][kTile * Tile::S];
   const int lane = threadIdx.x & 63, half = lane >> 5, wave = uniform((int)threadIdx.x >> 6);
-  const uint32_t kvh = (uint32_t)a.kv_heads, kvb = (uint32_t)a.batch * kvh, group = (uint32_t)a.heads / kvh;
-  const uint32_t id = work_order(blockIdx.x, gridDim.x, (uint32_t)a.cus);
-  const uint32_t nbh = kvb * group, bh = id % nbh, kv = bh % kvb;
-  const uint32_t qblocks = (uint32_t)((a.queries + kBlock - 1) / kBlock);
-  const int q0 = uniform((int)(qblocks - 1 - id / nbh)) * kBlock;
-  const int64_t b = uniform((int)(kv / kvh)), hk = uniform((int)(kv % kvh)), h = hk * group + uniform((int)(bh / kvb));
+  const RowsWork w = rows_work(a);
+  const int64_t b = w.b, hk = w.hk, h = w.h;
+  const int q0 = w.block * kBlock;
   const int dim = (int)a.dim;
   const Allowed allow = allowed_keys(a, b);
   const int queries = (int)a.queries, wq0 = q0 + wave * 32, q = wq0 + (lane & 31);
@@ -361,7 +367,9 @@ hipError_t launch(const AttnArgs& a, hipStream_t s) {
   const int64_t kgrid = a.batch * a.kv_heads * ((a.keys + kBlock - 1) / kBlock);
   const int64_t qgrid = a.batch * a.heads * ((a.queries + kBlock - 1) / kBlock);
   if (qgrid > 0) {
-    hipLaunchKernelGGL((attention_bwd_queries<T, DP, FAST>), dim3((unsigned)qgrid), dim3(256), 0, s, a);
+    AttnArgs whole = a;
+    whole.splits = 1;  // the ranges are the key pass's
+    hipLaunchKernelGGL((attention_bwd_queries<T, DP, FAST>), dim3((unsigned)qgrid), dim3(256), 0, s, whole);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
@@ -406,7 +414,8 @@ static void plan_bwd_splits(AttnArgs& a) {
   const double spread = (a.dtype == kF32 ? 8.5 : a.dim <= 64 ? 1.2 : 1.4) * unit;
   const double alone = (a.dtype == kF32 ? 8.5 : a.dim <= 64 ? 1.6 : 1.4) * unit;
   const int64_t tiles = a.heads / a.kv_heads * ((a.queries + kTile - 1) / kTile);
-  const double wgs = (double)(a.batch * a.kv_heads) * (double)((a.keys + kBlock - 1) / kBlock);
+  // with lengths, which only the device knows, about half of the blocks hold keys
+  const double wgs = (double)(a.batch * a.kv_heads) * (double)((a.keys + kBlock - 1) / kBlock) * (a.lengths ? 0.55 : 1.0);
   const bool halves = a.causal && a.keys * 2 > a.queries;
   const double bytes = 16.0 * (double)(a.batch * a.kv_heads) * (double)a.keys * (double)a.dim;
   double best = 0.0;

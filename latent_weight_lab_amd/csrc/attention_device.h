@@ -274,6 +274,33 @@ __device__ __forceinline__ uint32_t work_order(uint32_t block, uint32_t blocks, 
   return first + (cus / 8 - 1 - r / 8) * 8 + r % 8;
 }
 
+// The sequence with the `rank`-th most keys (ties: the lower number), so that workgroups can be numbered longest
+// sequence first although only the device knows the lengths.  Batches of up to 64 (a lane each); others, and
+// those without lengths, in their own order.  Every lane of the wave calls it with the same rank.
+//
+// The rank-th largest of the lanes' numbers length * 64 + 63 - lane, one bit after the other from the top:
+// it is among those with the bit set if they are more than rank, else among the others.
+constexpr int kMostRanked = 64;
+__device__ __forceinline__ int ranked_sequence(const AttnArgs& a, int rank) {
+  if (!a.lengths || a.batch > kMostRanked) return rank;
+  const int lane = threadIdx.x & 63, batch = (int)a.batch, keys = (int)a.keys;
+  int len = lane < batch ? a.lengths[lane] : 0;
+  len = len < 0 ? 0 : len < keys ? len : keys;
+  const uint64_t number = lane < batch ? (uint64_t)len * 64 + (63 - lane) : 0;
+  uint64_t left = batch == 64 ? ~0ull : (1ull << batch) - 1;
+  for (int bit = 37 - __builtin_clz((uint32_t)keys | 1u); bit >= 0; --bit) {
+    const uint64_t set = __ballot((number >> bit) & 1) & left;
+    const int count = __popcll(set);
+    if (rank < count) {
+      left = set;
+    } else {
+      rank -= count;
+      left &= ~set;
+    }
+  }
+  return uniform((int)__builtin_ctzll(left));
+}
+
 // Which keys a sequence's queries may see: j < len, and with causal j <= i + off.  Token numbers are 32 bits
 // (the C entry refuses more than 2^30), so that comparisons of wave-uniform ones are scalar.
 constexpr int kFar = (1 << 30) - 1;  // i + kFar + 1 does not overflow and is past every key
@@ -299,6 +326,31 @@ __device__ __forceinline__ Allowed allowed_keys(const AttnArgs& a, int64_t b) {
 __device__ __forceinline__ int key_end(const Allowed& w, int i) {
   const int e = i + w.off + 1;
   return e < 0 ? 0 : e < w.len ? e : w.len;
+}
+
+// Which block of queries (of 128) of which head a workgroup takes, and which range of keys.  Heads vary fastest,
+// those that share a key head a multiple of the key heads apart, then ranges, then blocks, the last queries
+// (causal: those with the most keys) first.  With lengths the longest sequence's work comes first instead.
+struct RowsWork {
+  int64_t b, hk, h;
+  int block, split;
+};
+__device__ __forceinline__ RowsWork rows_work(const AttnArgs& a) {
+  const uint32_t kvh = (uint32_t)a.kv_heads, group = (uint32_t)a.heads / kvh, splits = (uint32_t)a.splits;
+  const uint32_t blocks = (uint32_t)((a.queries + 127) / 128);
+  const uint32_t id = work_order(blockIdx.x, gridDim.x, (uint32_t)a.cus);
+  const bool ranked = a.lengths && a.batch <= kMostRanked;
+  const uint32_t kvb = ranked ? kvh : (uint32_t)a.batch * kvh, nh = kvb * group;
+  const uint32_t head = id % nh, kv = head % kvb;
+  uint32_t rest = id / nh;
+  RowsWork w;
+  w.split = uniform((int)(rest % splits));
+  rest /= splits;
+  w.block = uniform((int)(blocks - 1 - rest % blocks));
+  w.b = ranked ? ranked_sequence(a, uniform((int)(rest / blocks))) : uniform((int)(kv / kvh));
+  w.hk = uniform((int)(kv % kvh));
+  w.h = w.hk * group + uniform((int)(head / kvb));
+  return w;
 }
 
 }  // namespace lwl

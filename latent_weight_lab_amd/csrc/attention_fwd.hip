@@ -54,16 +54,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_rows(co
   __shared__ __attribute__((aligned(16))) T lds_v[2][kKeys * Tile::VS];
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = uniform((int)threadIdx.x >> 6);
-  // Heads vary fastest, those that share a key head a multiple of the key heads apart; queries with
-  // the most keys first (causal: the last ones).
-  const uint32_t kvh = (uint32_t)a.kv_heads, kvb = (uint32_t)a.batch * kvh, group = (uint32_t)a.heads / kvh;
-  const uint32_t nbh = kvb * group, splits = (uint32_t)a.splits, id = work_order(blockIdx.x, gridDim.x, (uint32_t)a.cus);
-  const uint32_t bh = (uint32_t)uniform((int)(id % nbh)), rest = id / nbh;
-  const int split = uniform((int)(rest % splits));
-  const uint32_t qblocks = (uint32_t)((a.queries + kRows - 1) / kRows);
-  const int q0 = uniform((int)(qblocks - 1 - rest / splits)) * kRows;
-  const uint32_t kv = bh % kvb;
-  const int64_t b = uniform((int)(kv / kvh)), hk = uniform((int)(kv % kvh)), h = hk * group + uniform((int)(bh / kvb));
+  const RowsWork w = rows_work(a);
+  const int64_t b = w.b, hk = w.hk, h = w.h;
+  const int q0 = w.block * kRows, split = w.split;
   const int dim = (int)a.dim;
   const Allowed allow = allowed_keys(a, b);
   const int queries = (int)a.queries, wq0 = q0 + wave * kWaveRows, q = wq0 + (lane & 31);
@@ -198,9 +191,10 @@ __global__ __launch_bounds__(256) void attention_token(const AttnArgs a) {
   const int lane = threadIdx.x & 63, quad = lane >> 4, wave = uniform((int)threadIdx.x >> 6);
   T* lds_v = reinterpret_cast<T*>(lds + wave * kWaveBytes);
   const uint32_t kvh = (uint32_t)a.kv_heads, batch = (uint32_t)a.batch;
+  const uint32_t id = a.lengths ? work_order(blockIdx.x, gridDim.x, (uint32_t)a.cus) : blockIdx.x;
   const int group = uniform((int)((uint32_t)a.heads / kvh));
-  const int64_t hk = uniform((int)(blockIdx.x % kvh)), b = uniform((int)(blockIdx.x / kvh % batch));
-  const int split = uniform((int)(blockIdx.x / kvh / batch));
+  const int64_t hk = uniform((int)(id % kvh)), b = ranked_sequence(a, uniform((int)(id / kvh % batch)));
+  const int split = uniform((int)(id / kvh / batch));
   const int dim = (int)a.dim, queries = (int)a.queries, rows_here = group * queries;
   const Allowed allow = allowed_keys(a, b);
   const int row = lane & 15;  // this lane's column of the products: query row % queries of head row / queries
@@ -407,7 +401,7 @@ bool by_token(const AttnArgs& a) { return a.heads / a.kv_heads * a.queries <= kT
 // 256 keys.  Otherwise what an estimate of the time makes shortest, in us: the larger of a workgroup's
 // own walk (kAlone a tile) and all work spread over the compute units (kSpread a tile), and with more
 // than one range the join.  The rates are measured on MI355X: bfloat16 of head size 64, 0.7 us a tile
-// when a compute unit has three workgroups and 1.2 us alone; float32 3.8 us either way (matrix cores).
+// when a compute unit has three workgroups and 1 us alone; float32 3.8 us either way (matrix cores).
 void plan_splits(AttnArgs& a) {
   const int64_t cus = device_cus();
   int64_t splits = 1;
@@ -416,17 +410,19 @@ void plan_splits(AttnArgs& a) {
     splits = std::min({2 * cus / wgs, a.keys / 256, (int64_t)kMaxSplits});
   } else {
     const double unit = (double)((a.dim + 31) / 32 * 32) / 64;
-    const double alone = (a.dtype == kF32 ? 3.8 : 1.2) * unit, spread = (a.dtype == kF32 ? 3.8 : 0.7) * unit;
+    const double alone = a.dtype == kF32 ? 3.8 * unit : 0.5 + 0.5 * unit, spread = (a.dtype == kF32 ? 3.8 : 0.7) * unit;
     const int64_t tiles = (a.keys + kKeys - 1) / kKeys;
     const double wgs = (double)(a.batch * a.heads) * (double)((a.queries + kRows - 1) / kRows);
     // about half of a square causal call's tiles are walked
-    const double all = wgs * (double)tiles * (a.causal && a.queries * 2 > a.keys ? 0.55 : 1.0) * spread / (double)cus;
+    // (also of ragged sequences' tiles, whose lengths only the device knows)
+    const double all = wgs * (double)tiles * ((a.causal && a.queries * 2 > a.keys) || a.lengths ? 0.55 : 1.0) * spread / (double)cus;
     const double bytes = 8.0 * (double)(a.batch * a.heads) * (double)a.queries * (double)a.dim;  // of a range
     double best = 0.0;
     for (int64_t n = 1; n <= std::min<int64_t>(tiles / 4 + 1, kMaxSplits); n = n < 4 ? n + 1 : n + n / 4) {
       const double walk = (double)((tiles + n - 1) / n) * alone;
       const double t = std::max(walk, all) + (n > 1 ? 4.0 + (double)n * bytes / 4.5e6 : 0.0);
-      if (n == 1 || t < best) {
+      // several only where they gain more than the estimate may be off by
+      if (n == 1 || t < best * (splits == 1 ? 0.85 : 1.0)) {
         best = t;
         splits = n;
       }

@@ -92,7 +92,7 @@ __device__ __forceinline__ float gelu(float z) {
   } else {
     float h, e;
     phi_pair<T>(z, h, e);
-    return fmaf(-fminf(fabsf(z), 16.0f), h, fmaxf(z, 0.0f));
+    return fmaf(-__builtin_elementwise_minimum(fabsf(z), 16.0f), h, __builtin_elementwise_maximum(z, 0.0f));
   }
 }
 
@@ -119,20 +119,42 @@ struct Gelu8Geo {
   static constexpr int ROWS = 256 / CL;
 };
 
-// The codes of the eight values at p as one 8-byte store.
-__device__ __forceinline__ void store_codes(int8_t* p, const float (&q)[8]) {
-  uint32_t w[2];
+// The codes rint(z inv) of eight values as one 8-byte store.  1.5 * 2^23 added to a float32 of up to 2^22
+// rounds it to an integer (to even, as rint) and leaves that integer's low byte as the sum's.
+__device__ __forceinline__ void store_codes(int8_t* p, const float (&z)[8], float inv) {
+  uint32_t b[8], w[2];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const uint32_t b0 = (uint32_t)(int)q[4 * j] & 0xffu, b1 = (uint32_t)(int)q[4 * j + 1] & 0xffu;
-    const uint32_t b2 = (uint32_t)(int)q[4 * j + 2] & 0xffu, b3 = (uint32_t)(int)q[4 * j + 3];
-    w[j] = b0 | (b1 << 8) | (b2 << 16) | (b3 << 24);
+  for (int i = 0; i < 8; ++i) {
+    float v;
+    {
+#pragma clang fp contract(off)
+      v = z[i] * inv;  // rounded before it is rounded to an integer
+      v = v + 12582912.0f;
+    }
+    b[i] = __float_as_uint(v);
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {  // bytes 0 of four registers
+    const uint32_t lo = __builtin_amdgcn_perm(b[4 * j + 1], b[4 * j], 0x0c0c0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(b[4 * j + 3], b[4 * j + 2], 0x04000c0cu);
+    w[j] = lo | hi;
   }
   *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
 }
+// c * scale from the codes: bytes made unsigned (c + 128) convert in one instruction, and (c + 128) scale - 128
+// scale with one rounding is c * scale rounded once (128 scale is exact).
 __device__ __forceinline__ void decode8(float (&z)[8], uint2 w, float scale) {
+  const uint32_t u[2] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u};
+  const float less = -128.0f * scale;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) z[i] = (float)(int8_t)((i < 4 ? w.x : w.y) >> (8 * (i & 3))) * scale;
+  for (int i = 0; i < 8; ++i) z[i] = fmaf((float)((u[i >> 2] >> (8 * (i & 3))) & 0xffu), scale, less);
+}
+// The largest over 16 lanes (a row of the vector unit's lanes), by rotations within them.
+__device__ __forceinline__ uint32_t max_of_16(uint32_t v) {
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, false));  // rotated by 8
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xf, 0xf, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x122, 0xf, 0xf, false));
+  return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x121, 0xf, 0xf, false));
 }
 
 template <class T, bool TANH, int CL, int U>
@@ -167,17 +189,13 @@ __global__ __launch_bounds__(256) void gelu8_fwd(const Gelu8Args a) {
         uint32_t top = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(z[i]) & 0x7fffffffu);
-#pragma unroll
-        for (int m = 8; m > 0; m >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m, 64));
+        top = max_of_16(top);
         const float most = __uint_as_float(top);
         const bool fine = top < 0x7f800000u && most >= kTiny;
         const float scale = top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fine ? most * (1.0f / 127.0f) : 0.0f;
-        const float inv = fine ? 1.0f / scale : 0.0f;
-        float q[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = fine ? rintf(z[i] * inv) : 0.0f;
+        const float inv = fine ? 1.0f / scale : 0.0f;  // not fine: codes of 0, or any under a NaN
         if (live && n > 0) {
-          store_codes(a.codes + row * pitch + col, q);
+          store_codes(a.codes + row * pitch + col, z, inv);
           if ((lane & 15) == 0) a.scales[row * groups + col / kGelu8Group] = scale;
         }
       }
@@ -187,7 +205,7 @@ __global__ __launch_bounds__(256) void gelu8_fwd(const Gelu8Args a) {
 
 // BWD: dx and, with WORK or one row range, the bias's gradient; otherwise the activation again.
 template <class T, bool TANH, int CL, int U, bool BWD>
-__global__ __launch_bounds__(256) void gelu8_use(const Gelu8Args a) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 4 : 1) void gelu8_use(const Gelu8Args a) {
   using Geo = Gelu8Geo<CL>;
   __shared__ float acc[BWD ? 256 * 8 : 1];
   const int lane = threadIdx.x & (CL - 1), sub = threadIdx.x / CL;
@@ -260,11 +278,10 @@ Gelu8Shape gelu8_shape(int64_t rows, int64_t features, int64_t wgs_per_cu) {
   const int64_t per = 256 / s.cl;
   s.u = s.panels * ((rows + per * 4 - 1) / (per * 4)) >= 2 * device_cus() ? 4 : 1;
   const int64_t need = (rows + per * s.u - 1) / (per * s.u);
-  s.ranges = std::max<int64_t>(1, std::min<int64_t>(need, (wgs_per_cu * device_cus() + s.panels - 1) / s.panels));
-  s.ranges = std::min<int64_t>(s.ranges, 65535);
+  s.ranges = even_ranges(need, std::min<int64_t>((wgs_per_cu * device_cus() + s.panels - 1) / s.panels, 65535));
   return s;
 }
-constexpr int64_t kFwdPerCu = 8, kBwdPerCu = 4;
+constexpr int64_t kFwdPerCu = 16, kBwdPerCu = 4;
 
 enum { kGeluFwd, kGeluAgain, kGeluBwd };
 

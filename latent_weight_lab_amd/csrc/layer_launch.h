@@ -17,6 +17,14 @@ int status_ok();
 int status_hip(hipError_t e, const char* what);
 int status_workspace(size_t need, const void* ws, size_t have);
 
+// At most `most` ranges of `works` equal works, as equal as they can be: with one more round for some than for
+// others the last round leaves most of the chip idle.
+inline int64_t even_ranges(int64_t works, int64_t most) {
+  if (works <= 0 || most <= 0) return 1;
+  const int64_t rounds = (works + most - 1) / most;
+  return (works + rounds - 1) / rounds;
+}
+
 // ---------------------------------------------------------------- layer norm
 struct NormArgs {
   int dtype, weight_dtype;

@@ -430,7 +430,7 @@ hipError_t run_norm(const NormArgs& a, bool fwd, hipStream_t s) {
   using Geo = NormGeo<LANES>;
   const int64_t groups = (a.rows + Geo::G - 1) / Geo::G;
   if (fwd) {
-    const unsigned grid = (unsigned)std::min<int64_t>(groups, 4 * device_cus());
+    const unsigned grid = (unsigned)even_ranges(groups, 4 * device_cus());
     hipLaunchKernelGGL((norm_fwd<T, W, LANES, CH>), dim3(grid), dim3(Geo::WG), 0, s, a);
   } else {
     const int64_t part = norm_bwd_partial_rows(a.rows, a.features);
@@ -493,7 +493,7 @@ int64_t norm_bwd_partial_rows(int64_t rows, int64_t features) {
   }
   const int64_t g = kNormWG / sh.lanes, groups = (rows + g - 1) / g;
   if (groups <= 1) return 0;
-  return std::min<int64_t>(groups, 2 * device_cus());
+  return even_ranges(groups, 2 * device_cus());
 }
 
 hipError_t launch_column_sum(const float* part, int64_t rows, int64_t stride, int64_t n0, void* dst0, int64_t n1,
