@@ -54,11 +54,11 @@ __device__ __forceinline__ float* partials(const AttnArgs& a) { return a.work + 
 
 template <class T, int DP, bool FAST>
 __global__ __launch_bounds__(256, (kKeysOccupancy<T, DP>)) void attention_bwd_keys(const AttnArgs a) {
-  using Tile = BothWays<T, DP>;
-  constexpr int KK = DP / 16, DT = DP / 32;
-  __shared__ __attribute__((aligned(16))) T lds_q[2][kTile * Tile::S];
-  __shared__ __attribute__((aligned(16))) T lds_g[2][kTile * Tile::S];
-  __shared__ __attribute__((aligned(16))) float lds_stat[2][2][kTile];
+  using Tile = BothWays<DP>;
+  constexpr int KK = DP / 16, DT = DP / 32, PL = kTile * Tile::S;  // size of a plane
+  __shared__ __attribute__((aligned(16))) Elem<T> lds_q[kBufs<T>][kPlanes<T> * PL];
+  __shared__ __attribute__((aligned(16))) Elem<T> lds_g[kBufs<T>][kPlanes<T> * PL];
+  __shared__ __attribute__((aligned(16))) float lds_stat[kBufs<T>][2][kTile];
   const int lane = threadIdx.x & 63, half = lane >> 5, wave = uniform((int)threadIdx.x >> 6);
   const uint32_t kvh = (uint32_t)a.kv_heads, kvb = (uint32_t)a.batch * kvh, group = (uint32_t)a.heads / kvh;
   const uint32_t id = work_order(blockIdx.x, gridDim.x, (uint32_t)a.cus), bk = id % kvb, splits = (uint32_t)a.splits;
@@ -70,7 +70,7 @@ __global__ __launch_bounds__(256, (kKeysOccupancy<T, DP>)) void attention_bwd_ke
   const int queries = (int)a.queries;
   const int seen = key_end(allow, queries - 1);  // keys that some query sees
   const int wk0 = k0 + wave * 32, key = wk0 + (lane & 31);
-  Frag<T> kf[KK], vf[KK];
+  Opd<T> kf[KK], vf[KK];
   load_operand<T, DP, FAST>(kf, (const T*)a.k + b * a.ks[0] + hk * a.ks[1] + (int64_t)key * a.ks[2], dim, key < seen);
   load_operand<T, DP, FAST>(vf, (const T*)a.v + b * a.vs[0] + hk * a.vs[1] + (int64_t)key * a.vs[2], dim, key < seen);
   f32x16 dk[DT] = {}, dv[DT] = {};
@@ -114,10 +114,14 @@ __global__ __launch_bounds__(256, (kKeysOccupancy<T, DP>)) void attention_bwd_ke
   int q0 = begin < end ? first + (begin - (int)g * per_head) * kTile : 0;
   if (begin < end) {
     fetch(g, q0);
-    put(0);
+    if constexpr (kBufs<T> == 2) put(0);
   }
   for (int i = begin; i < end; ++i) {
     __syncthreads();  // this tile is there, the one before has been read
+    if constexpr (kBufs<T> == 1) {
+      put(0);
+      __syncthreads();
+    }
     const bool last = q0 + kTile >= queries, more = i + 1 < end;
     const uint32_t next_g = last ? g + 1 : g;
     const int next_q = last ? first : q0 + kTile;
@@ -127,11 +131,11 @@ __global__ __launch_bounds__(256, (kKeysOccupancy<T, DP>)) void attention_bwd_ke
 #pragma unroll kUnroll<T, DP>
       for (int t = 0; t < 2; ++t) {
         const int at = t * 32;
-        const T* lq = lds_q[buf] + at * Tile::S;
-        const T* lg = lds_g[buf] + at * Tile::S;
+        const Elem<T>* lq = lds_q[buf] + at * Tile::S;
+        const Elem<T>* lg = lds_g[buf] + at * Tile::S;
         f32x16 s, dp;
         {
-          Frag<T> qf[KK], gf[KK];
+          Opd<T> qf[KK], gf[KK];
 #pragma unroll
           for (int r4 = 0; r4 < 4; ++r4) {
             const f32x4 l = *(const f32x4*)&lds_stat[buf][0][at + r4 * 8 + half * 4];
@@ -142,32 +146,48 @@ __global__ __launch_bounds__(256, (kKeysOccupancy<T, DP>)) void attention_bwd_ke
               dp[r4 * 4 + r] = kFoldStats<T> ? d[r] : 0.0f;
             }
           }
+          const auto load_q = [&](int kk) { qf[kk] = lds_operand<T>(lq + Tile::at(lane & 31, kk * 16 + half * 8), PL); };
+          const auto load_g = [&](int kk) { gf[kk] = lds_operand<T>(lg + Tile::at(lane & 31, kk * 16 + half * 8), PL); };
+          if constexpr (sizeof(T) == 4) {
 #pragma unroll
-          for (int kk = 0; kk < KK; ++kk) qf[kk] = lds_frag(lq + Tile::at(lane & 31, kk * 16 + half * 8));
-          // 96: the two products one after the other, which holds half as many operands at a time
-          if constexpr (DP == 96) {
-            fence_schedule<T>();
+            for (int kk = 0; kk < KK; ++kk) {
+              load_q(kk);
+              load_g(kk);
+              s = mma32(qf[kk], kf[kk], s);
+              dp = mma32(gf[kk], vf[kk], dp);
+              fence_operands<T>();
+            }
+          } else {
 #pragma unroll
-            for (int kk = 0; kk < KK; ++kk) s = mma32(qf[kk], kf[kk], s);
-          }
+            for (int kk = 0; kk < KK; ++kk) load_q(kk);
+            // 96: the two products one after the other, which holds half as many operands at a time
+            if constexpr (DP == 96) {
+              fence_schedule<T>();
 #pragma unroll
-          for (int kk = 0; kk < KK; ++kk) gf[kk] = lds_frag(lg + Tile::at(lane & 31, kk * 16 + half * 8));
-          if constexpr (DP <= 96) fence_schedule<T>();
+              for (int kk = 0; kk < KK; ++kk) s = mma32(qf[kk], kf[kk], s);
+            }
 #pragma unroll
-          for (int kk = 0; kk < KK; ++kk) {
-            if constexpr (DP != 96) s = mma32(qf[kk], kf[kk], s);
-            dp = mma32(gf[kk], vf[kk], dp);
+            for (int kk = 0; kk < KK; ++kk) load_g(kk);
+            if constexpr (DP <= 96) fence_schedule<T>();
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) {
+              if constexpr (DP != 96) s = mma32(qf[kk], kf[kk], s);
+              dp = mma32(gf[kk], vf[kk], dp);
+            }
           }
         }
-        Frag<T> gc[2][DT], qc[2][DT];
+        Opd<T> gc[2][DT], qc[2][DT];
+        const auto load_columns = [&](int u, int d) {
+          const int row = u * 16 + half * 4;
+          gc[u][d] = lds_column_operand<T, Tile>(lg, PL, row, row + 8, d * 32 + (lane & 16));
+          qc[u][d] = lds_column_operand<T, Tile>(lq, PL, row, row + 8, d * 32 + (lane & 16));
+        };
+        if constexpr (sizeof(T) == 2) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+          for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            const int row = u * 16 + half * 4;
-            gc[u][d] = lds_column_frag<Tile>(lg, row, row + 8, d * 32 + (lane & 16));
-            qc[u][d] = lds_column_frag<Tile>(lq, row, row + 8, d * 32 + (lane & 16));
-          }
+            for (int d = 0; d < DT; ++d) load_columns(u, d);
+        }
         if constexpr (DP <= 96) fence_schedule<T>();
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -189,22 +209,25 @@ __global__ __launch_bounds__(256, (kKeysOccupancy<T, DP>)) void attention_bwd_ke
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          Frag<T> p, ds;
+          float e[8], f[8];
 #pragma unroll
           for (int r = 0; r < 8; ++r) {
-            p[r] = (T)s[u * 8 + r];
-            ds[r] = (T)dp[u * 8 + r];
+            e[r] = s[u * 8 + r];
+            f[r] = dp[u * 8 + r];
           }
+          const Opd<T> p = operand_of<T>(e), ds = operand_of<T>(f);
 #pragma unroll
           for (int d = 0; d < DT; ++d) {
+            if constexpr (sizeof(T) == 4) load_columns(u, d);
             dv[d] = mma32(gc[u][d], p, dv[d]);
             dk[d] = mma32(qc[u][d], ds, dk[d]);
+            fence_operands<T>();
           }
         }
       }
     }
-    if (more) put(buf ^ 1);
-    buf ^= 1;
+    if (kBufs<T> == 2 && more) put(buf ^ (kBufs<T> - 1));
+    buf ^= kBufs<T> - 1;
     g = next_g;
     q0 = next_q;
   }
@@ -224,10 +247,10 @@ __global__ __launch_bounds__(256, (kKeysOccupancy<T, DP>)) void attention_bwd_ke
 template <class T, int DP, bool FAST>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_bwd_queries(const AttnArgs a) {
   // rows padded by 16 bytes: one tile in three is read by columns, and BothWays' addresses cost registers
-  using Tile = Padded<T, DP>;
-  constexpr int KK = DP / 16, DT = DP / 32;
-  __shared__ __attribute__((aligned(16))) T lds_k[2][kTile * Tile::S];
-  __shared__ __attribute__((aligned(16))) T lds_v[2][kTile * Tile::S];
+  using Tile = Padded<DP>;
+  constexpr int KK = DP / 16, DT = DP / 32, PL = kTile * Tile::S;  // size of a plane
+  __shared__ __attribute__((aligned(16))) Elem<T> lds_k[kBufs<T>][kPlanes<T> * PL];
+  __shared__ __attribute__((aligned(16))) Elem<T> lds_v[kBufs<T>][kPlanes<T> * PL];
   const int lane = threadIdx.x & 63, half = lane >> 5, wave = uniform((int)threadIdx.x >> 6);
   const RowsWork w = rows_work(a);
   const int64_t b = w.b, hk = w.hk, h = w.h;
@@ -248,32 +271,40 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_bwd_que
     kt.fetch(0, end);
     vt.fetch(0, end);
   }
-  Frag<T> qf[KK], gf[KK];
-  load_operand<T, DP, FAST>(qf, (const T*)a.q + b * a.qs[0] + h * a.qs[1] + (int64_t)q * a.qs[2], dim, q_end > 0);
-  load_operand<T, DP, FAST>(gf, (const T*)a.dout + b * a.dos[0] + h * a.dos[1] + (int64_t)q * a.dos[2], dim, q_end > 0);
   const int64_t row = (b * a.heads + h) * a.queries + q;
   // a query without keys has no probabilities: exp2(-infinity)
   const float lse = q_end > 0 ? a.lse[row] * kLog2E : INFINITY;
+  Opd<T> qf[KK], gf[KK];
+  load_operand<T, DP, FAST>(qf, (const T*)a.q + b * a.qs[0] + h * a.qs[1] + (int64_t)q * a.qs[2], dim, q_end > 0);
   float delta = 0.0f;
-  {
-    Frag<T> of[KK];
-    load_operand<T, DP, FAST>(of, (const T*)a.out + b * a.os[0] + h * a.os[1] + (int64_t)q * a.os[2], dim, q_end > 0);
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk)
+  for (int kk = 0; kk < KK; ++kk) {
+    Raw8<T> gr, orow;
+    load_chunk<T, FAST>(gr, (const T*)a.dout + b * a.dos[0] + h * a.dos[1] + (int64_t)q * a.dos[2], kk, dim, q_end > 0);
+    load_chunk<T, FAST>(orow, (const T*)a.out + b * a.os[0] + h * a.os[1] + (int64_t)q * a.os[2], kk, dim, q_end > 0);
+    gf[kk] = operand_of<T>(gr);
+    float x[8], y[8];
+    unpack8(x, gr);
+    unpack8(y, orow);
 #pragma unroll
-      for (int r = 0; r < 8; ++r) delta += (float)of[kk][r] * (float)gf[kk][r];
-    delta += other_half(delta);
-    if (half == 0 && q < queries) a.work[row] = delta;
+    for (int r = 0; r < 8; ++r) delta += x[r] * y[r];
   }
+  delta += other_half(delta);
+  if (half == 0 && q < queries) a.work[row] = delta;
   f32x16 dq[DT] = {};
   const float c = a.scale * kLog2E;
-  if (end > 0) {
+  if (kBufs<T> == 2 && end > 0) {
     kt.template put<Tile>(lds_k[0]);
     vt.template put<Tile>(lds_v[0]);
   }
   int buf = 0;
-  for (int j0 = 0; j0 < end; j0 += kTile, buf ^= 1) {
+  for (int j0 = 0; j0 < end; j0 += kTile, buf ^= kBufs<T> - 1) {
     __syncthreads();  // this tile is there, the one before has been read
+    if constexpr (kBufs<T> == 1) {
+      kt.template put<Tile>(lds_k[0]);
+      vt.template put<Tile>(lds_v[0]);
+      __syncthreads();
+    }
     const bool more = j0 + kTile < end;
     if (more) {
       kt.fetch(j0 + kTile, end);
@@ -282,34 +313,51 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_bwd_que
     if (j0 < wave_end) {
 #pragma unroll 1
       for (int t = 0; t < 2; ++t) {
-        const T* lk = lds_k[buf] + t * 32 * Tile::S;
-        const T* lv = lds_v[buf] + t * 32 * Tile::S;
+        const Elem<T>* lk = lds_k[buf] + t * 32 * Tile::S;
+        const Elem<T>* lv = lds_v[buf] + t * 32 * Tile::S;
         f32x16 s = {}, dp = {};
         {
-          Frag<T> kf[KK], vf[KK];
+          Opd<T> kf[KK], vf[KK];
+          const auto load_k = [&](int kk) { kf[kk] = lds_operand<T>(lk + Tile::at(lane & 31, kk * 16 + half * 8), PL); };
+          const auto load_v = [&](int kk) { vf[kk] = lds_operand<T>(lv + Tile::at(lane & 31, kk * 16 + half * 8), PL); };
+          if constexpr (sizeof(T) == 4) {
 #pragma unroll
-          for (int kk = 0; kk < KK; ++kk) kf[kk] = lds_frag(lk + Tile::at(lane & 31, kk * 16 + half * 8));
-          // beyond 64 the two products one after the other, which holds half as many operands at a time
-          if constexpr (DP > 64) {
+            for (int kk = 0; kk < KK; ++kk) {
+              load_k(kk);
+              load_v(kk);
+              s = mma32(kf[kk], qf[kk], s);
+              dp = mma32(vf[kk], gf[kk], dp);
+              fence_operands<T>();
+            }
+          } else {
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) load_k(kk);
+            // beyond 64 the two products one after the other, which holds half as many operands at a time
+            if constexpr (DP > 64) {
+              fence_schedule<T>();
+#pragma unroll
+              for (int kk = 0; kk < KK; ++kk) s = mma32(kf[kk], qf[kk], s);
+            }
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) load_v(kk);
             fence_schedule<T>();
 #pragma unroll
-            for (int kk = 0; kk < KK; ++kk) s = mma32(kf[kk], qf[kk], s);
-          }
-#pragma unroll
-          for (int kk = 0; kk < KK; ++kk) vf[kk] = lds_frag(lv + Tile::at(lane & 31, kk * 16 + half * 8));
-          fence_schedule<T>();
-#pragma unroll
-          for (int kk = 0; kk < KK; ++kk) {
-            if constexpr (DP <= 64) s = mma32(kf[kk], qf[kk], s);
-            dp = mma32(vf[kk], gf[kk], dp);
+            for (int kk = 0; kk < KK; ++kk) {
+              if constexpr (DP <= 64) s = mma32(kf[kk], qf[kk], s);
+              dp = mma32(vf[kk], gf[kk], dp);
+            }
           }
         }
-        Frag<T> kc[2][DT];
+        Opd<T> kc[2][DT];
+        const auto load_columns = [&](int u, int d) {
+          kc[u][d] = lds_column_operand<T, Tile>(lk, PL, u * 16 + half * 4, u * 16 + half * 4 + 8, d * 32 + (lane & 16));
+        };
+        if constexpr (sizeof(T) == 2) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+          for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int d = 0; d < DT; ++d)
-            kc[u][d] = lds_column_frag<Tile>(lk, u * 16 + half * 4, u * 16 + half * 4 + 8, d * 32 + (lane & 16));
+            for (int d = 0; d < DT; ++d) load_columns(u, d);
+        }
         fence_schedule<T>();
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = exp2_hw(fmaf(s[r], c, -lse)) * (dp[r] - delta);
@@ -321,17 +369,22 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_bwd_que
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          Frag<T> ds;
+          float e[8];
 #pragma unroll
-          for (int r = 0; r < 8; ++r) ds[r] = (T)s[u * 8 + r];
+          for (int r = 0; r < 8; ++r) e[r] = s[u * 8 + r];
+          const Opd<T> ds = operand_of<T>(e);
 #pragma unroll
-          for (int d = 0; d < DT; ++d) dq[d] = mma32(kc[u][d], ds, dq[d]);
+          for (int d = 0; d < DT; ++d) {
+            if constexpr (sizeof(T) == 4) load_columns(u, d);
+            dq[d] = mma32(kc[u][d], ds, dq[d]);
+            fence_operands<T>();
+          }
         }
       }
     }
-    if (more) {
-      kt.template put<Tile>(lds_k[buf ^ 1]);
-      vt.template put<Tile>(lds_v[buf ^ 1]);
+    if (kBufs<T> == 2 && more) {
+      kt.template put<Tile>(lds_k[buf ^ (kBufs<T> - 1)]);
+      vt.template put<Tile>(lds_v[buf ^ (kBufs<T> - 1)]);
     }
   }
   if (q >= queries) return;
@@ -408,11 +461,11 @@ hipError_t run_dim(const AttnArgs& a, hipStream_t s) {
 // of the time makes shortest, in us, as in the forward pass: the longest walk alone, or all work spread over
 // the compute units, in whole rounds where the works are equal; and with several ranges the join.
 // Measured on MI355X, a tile of 64 queries: bfloat16 of head size 64 1.2 us when a compute unit has two
-// workgroups and 1.6 alone, of size 128 2.8 us (one fits); float32 of size 64 8.5 us.
+// workgroups and 1.6 alone, of size 128 2.8 us (one fits); float32 of size 64 6.8 us.
 static void plan_bwd_splits(AttnArgs& a) {
   const double unit = (double)((a.dim + 31) / 32 * 32) / 64, cus = (double)device_cus();
-  const double spread = (a.dtype == kF32 ? 8.5 : a.dim <= 64 ? 1.2 : 1.4) * unit;
-  const double alone = (a.dtype == kF32 ? 8.5 : a.dim <= 64 ? 1.6 : 1.4) * unit;
+  const double spread = (a.dtype == kF32 ? 6.8 : a.dim <= 64 ? 1.2 : 1.4) * unit;
+  const double alone = (a.dtype == kF32 ? 6.8 : a.dim <= 64 ? 1.6 : 1.4) * unit;
   const int64_t tiles = a.heads / a.kv_heads * ((a.queries + kTile - 1) / kTile);
   // with lengths, which only the device knows, about half of the blocks hold keys
   const double wgs = (double)(a.batch * a.kv_heads) * (double)((a.keys + kBlock - 1) / kBlock) * (a.lengths ? 0.55 : 1.0);

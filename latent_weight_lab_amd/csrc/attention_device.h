@@ -14,15 +14,37 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 // One lane's part of a product operand: eight consecutive k.
 //
 // 32-wide product (32 x 32 x 16): lane l holds row (column) l % 32, k = 8 (l / 32) .. + 7.  16-wide
-// product (16 x 16 x 32): row l % 16, k = 8 (l / 16) .. + 7.  For 16-bit types these are the operands of
-// one matrix instruction.  float32 has none of that depth; the same eight values feed eight
-// instructions of depth 2 (or 4), instruction i taking value i of every lane: each covers k = i, 8 + i
-// (.., 24 + i), and all eight every k once, in both operands alike.
-//
-// Results: lane l holds column l % 32, rows 8 (r / 4) + 4 (l / 32) + r % 4 for r < 16 (32-wide), or
-// column l % 16, rows 4 (l / 16) + r for r < 4 (16-wide).
+// product (16 x 16 x 32): row l % 16, k = 8 (l / 16) .. + 7.  Results: lane l holds column l % 32, rows
+// 8 (r / 4) + 4 (l / 32) + r % 4 for r < 16 (32-wide), or column l % 16, rows 4 (l / 16) + r for r < 4.
 template <class T>
 using Frag = typename Vec8<T>::type;
+
+// What a 32-wide product takes.  For a 16-bit type, one matrix instruction's operand.  A float32 value goes in
+// as a sum of three bfloat16 ones, x = x0 + x1 + x2, each the rounding of what the ones before leave: 24
+// bits, of float32's range.  Of the nine products of two such sums the six largest are taken; the others
+// are below 2^-24 of x y, and the sum is float32 as ever.  Six bfloat16 instructions take 192 cycles
+// where float32's own, of depth 2, take 512 for the same k (1 x 4 x 512 training step: 161 us with those).
+template <class T>
+struct MatrixType {
+  using Elem = T;
+  using Opd = Frag<T>;
+  static constexpr int PLANES = 1;
+};
+struct Frag3 {
+  Frag<bf16> p[3];
+};
+template <>
+struct MatrixType<float> {
+  using Elem = bf16;
+  using Opd = Frag3;
+  static constexpr int PLANES = 3;  // of a tile in LDS
+};
+template <class T>
+using Elem = typename MatrixType<T>::Elem;
+template <class T>
+using Opd = typename MatrixType<T>::Opd;
+template <class T>
+constexpr int kPlanes = MatrixType<T>::PLANES;
 
 __device__ __forceinline__ f32x16 mma32(Frag<bf16> a, Frag<bf16> b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
@@ -30,11 +52,54 @@ __device__ __forceinline__ f32x16 mma32(Frag<bf16> a, Frag<bf16> b, f32x16 c) {
 __device__ __forceinline__ f32x16 mma32(Frag<f16> a, Frag<f16> b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
-__device__ __forceinline__ f32x16 mma32(Frag<float> a, Frag<float> b, f32x16 c) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
-  return c;
+__device__ __forceinline__ f32x16 mma32(const Frag3& a, const Frag3& b, f32x16 c) {
+  // the smallest first
+  c = mma32(a.p[2], b.p[0], c);
+  c = mma32(a.p[0], b.p[2], c);
+  c = mma32(a.p[1], b.p[1], c);
+  c = mma32(a.p[1], b.p[0], c);
+  c = mma32(a.p[0], b.p[1], c);
+  return mma32(a.p[0], b.p[0], c);
 }
+// Eight float32 values as an operand.
+template <class T>
+__device__ __forceinline__ Opd<T> operand_of(const float (&v)[8]) {
+  if constexpr (sizeof(T) == 2) {
+    Frag<T> f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = (T)v[i];
+    return f;
+  } else {
+    Frag3 f;
+    float rest[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) rest[i] = v[i];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f.p[k][i] = (bf16)rest[i];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) rest[i] -= (float)f.p[k][i];
+    }
+    return f;
+  }
+}
+template <class T>
+__device__ __forceinline__ Opd<T> operand_of(const Raw8<T>& r) {
+  if constexpr (sizeof(T) == 2) {
+    Frag<T> f;
+    __builtin_memcpy(&f, &r, sizeof(f));
+    return f;
+  } else {
+    float v[8];
+    unpack8(v, r);
+    return operand_of<T>(v);
+  }
+}
+
+// 16-wide products (single tokens, whose time is the memory's): float32's own instructions, of depth 4.  The same
+// eight values feed eight of them, instruction i taking value i of every lane: each covers k = i, 8 + i, 16
+// + i and 24 + i, and all eight every k once, in both operands alike.
 __device__ __forceinline__ f32x4 mma16(Frag<bf16> a, Frag<bf16> b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
@@ -78,7 +143,7 @@ __device__ __forceinline__ void lds_column4(T (&v)[4], const T* tile, int row0, 
     for (int r = 0; r < 4; ++r) v[r] = tile[Layout::at(row0 + r, col0 + i)];
   }
 }
-// The operand whose eight k are rows a .. a + 3 and b .. b + 3 of a tile, at column col0 + (lane % 16).
+// Eight k as rows a .. a + 3 and b .. b + 3 of a tile, at column col0 + (lane % 16).
 template <class Layout, class T>
 __device__ __forceinline__ Frag<T> lds_column_frag(const T* tile, int a, int b, int col0) {
   T lo[4], hi[4];
@@ -92,24 +157,44 @@ __device__ __forceinline__ Frag<T> lds_column_frag(const T* tile, int a, int b, 
   }
   return f;
 }
+// The same as operands of 32-wide products, from a tile of kPlanes planes `plane` apart: eight values in a row
+// at p, or of a column.
+template <class T>
+__device__ __forceinline__ Opd<T> lds_operand(const Elem<T>* p, int plane) {
+  if constexpr (sizeof(T) == 2) {
+    return lds_frag(p);
+  } else {
+    Frag3 f;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) f.p[k] = lds_frag(p + k * plane);
+    return f;
+  }
+}
+template <class T, class Layout>
+__device__ __forceinline__ Opd<T> lds_column_operand(const Elem<T>* tile, int plane, int a, int b, int col0) {
+  if constexpr (sizeof(T) == 2) {
+    return lds_column_frag<Layout>(tile, a, b, col0);
+  } else {
+    Frag3 f;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) f.p[k] = lds_column_frag<Layout>(tile + k * plane, a, b, col0);
+    return f;
+  }
+}
 
-// Where value (row, col) of a tile lies in LDS when the tile is read both by rows (16 bytes a lane, 16 rows at a
-// time) and by columns (lds_column4: 4 rows of 64 bytes at a time).  16-bit types: a row's chunks of 16 bytes
-// are exchanged by an exclusive or with a number made of the row's, so that either read finds its 16
+// Where value (row, col) of a tile (of 16-bit values) lies in LDS when the tile is read both by rows (16 bytes a
+// lane, 16 rows at a time) and by columns (lds_column4: 4 rows of 64 bytes at a time).  A row's chunks of 16
+// bytes are exchanged by an exclusive or with a number made of the row's, so that either read finds its 16
 // chunks on distinct banks: rows 0 .. 15 have distinct numbers (of those that share banks), and four
 // consecutive rows from a multiple of four differ in the bits that tell blocks of 64 bytes apart.  Rows of
-// 96 are laid out as 128.  float32: rows padded by 16 bytes (columns are read value by value).
-template <class T, int DP>
+// 96 are laid out as 128.
+template <int DP>
 struct BothWays {
-  static constexpr int S = sizeof(T) == 4 ? DP + 4 : DP == 96 ? 128 : DP;
+  static constexpr int S = DP == 96 ? 128 : DP;
   static __device__ __forceinline__ int at(int row, int col) {
-    if constexpr (sizeof(T) == 4) {
-      return row * S + col;
-    } else {
-      const int f = S == 128 ? ((row & 3) << 2) | ((row >> 2) & 3)
-                    : S == 64 ? ((row & 2) << 1) | ((row >> 2) & 3) : (row >> 2) & 3;
-      return row * S + ((((col >> 3) ^ f) << 3) | (col & 7));
-    }
+    const int f = S == 128 ? ((row & 3) << 2) | ((row >> 2) & 3)
+                  : S == 64 ? ((row & 2) << 1) | ((row >> 2) & 3) : (row >> 2) & 3;
+    return row * S + ((((col >> 3) ^ f) << 3) | (col & 7));
   }
 };
 // Rows of a fixed stride.
@@ -118,10 +203,9 @@ struct Strided {
   static constexpr int S = STRIDE;
   static __device__ __forceinline__ int at(int row, int col) { return row * STRIDE + col; }
 };
-
 // Rows padded by 16 bytes: 16-byte reads of 16 rows fall on distinct banks.
-template <class T, int DP>
-using Padded = Strided<DP + 16 / (int)sizeof(T)>;
+template <int DP>
+using Padded = Strided<DP + 8>;
 
 // Tiles of 64 rows that a workgroup of 256 threads brings from memory through registers into LDS: fetch()
 // starts the loads, put() stores what came.  Rows from `end` on and columns past the head size are zeros.
@@ -173,15 +257,26 @@ struct TileLoader {
       }
     }
   }
+  // into a tile of kPlanes planes of kTileRows rows
   template <class Layout>
-  __device__ __forceinline__ void put(T* lds) const {
+  __device__ __forceinline__ void put(Elem<T>* lds) const {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int c = threadIdx.x + i * 256;
-      lds_put(lds + Layout::at(c / CPR, (c % CPR) * 8), r[i]);
+      Elem<T>* p = lds + Layout::at(c / CPR, (c % CPR) * 8);
+      const Opd<T> v = operand_of<T>(r[i]);
+      if constexpr (sizeof(T) == 2) {
+        *reinterpret_cast<Frag<T>*>(p) = v;
+      } else {
+#pragma unroll
+        for (int k = 0; k < 3; ++k) *reinterpret_cast<Frag<bf16>*>(p + k * kTileRows * Layout::S) = v.p[k];
+      }
     }
   }
 };
+// Tiles in LDS: two, one being read while the other is filled, where they fit.
+template <class T>
+constexpr int kBufs = sizeof(T) == 2 ? 2 : 1;
 // Whether a tensor's rows meet FAST's terms (the head size is checked beside it).
 inline bool fast_rows(const void* p, const int64_t (&stride)[3], int64_t size) {
   const int64_t unit = 16 / size;
@@ -191,16 +286,19 @@ inline bool fast_rows(const void* p, const int64_t (&stride)[3], int64_t size) {
 
 // A row of a tensor as operands: lane l holds chunks of eight values, 8 (l / 32) + 16 kk (32-wide products).
 // WHOLE: the head size is a multiple of eight.
+template <class T, bool WHOLE>
+__device__ __forceinline__ void load_chunk(Raw8<T>& r, const T* row, int kk, int dim, bool ok) {
+  const int col = kk * 16 + ((threadIdx.x & 63) >> 5) * 8;
+  if constexpr (WHOLE) load_whole8(r, row + col, ok && col < dim);
+  else load_raw8(r, row + col, ok ? dim - col : 0);
+}
 template <class T, int DP, bool WHOLE>
-__device__ __forceinline__ void load_operand(Frag<T> (&f)[DP / 16], const T* row, int dim, bool ok) {
-  const int half = (threadIdx.x & 63) >> 5;
+__device__ __forceinline__ void load_operand(Opd<T> (&f)[DP / 16], const T* row, int dim, bool ok) {
 #pragma unroll
   for (int kk = 0; kk < DP / 16; ++kk) {
-    const int col = kk * 16 + half * 8;
     Raw8<T> r;
-    if constexpr (WHOLE) load_whole8(r, row + col, ok && col < dim);
-    else load_raw8(r, row + col, ok ? dim - col : 0);
-    f[kk] = frag_of(r);
+    load_chunk<T, WHOLE>(r, row, kk, dim, ok);
+    f[kk] = operand_of<T>(r);
   }
 }
 // A result whose columns are rows of a tensor: the lane's row, values 8 r4 + 4 (l / 32) .. + 3 of each 32.
@@ -228,12 +326,17 @@ __device__ __forceinline__ void store_result(T* row, const f32x16 (&v)[DP / 32],
 // The larger of the two; a NaN stays a NaN (one instruction for three operands).
 __device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
-// Nothing is moved across this point by the instruction scheduler: loads from LDS issued before it are
-// under way together, where the scheduler would issue each just before its use to save registers.
-// Not for float32, where an operand feeds eight instructions of 64 cycles and its load needs no such lead.
+// Nothing is moved across these points by the instruction scheduler.  16-bit types: loads from LDS issued before
+// one are under way together, where the scheduler would issue each just before its use to save registers.
+// float32, whose operands are three times as large and feed six instructions each: few are held at a time,
+// where it would load all of them at once.
 template <class T>
 __device__ __forceinline__ void fence_schedule() {
   if constexpr (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
+}
+template <class T>
+__device__ __forceinline__ void fence_operands() {
+  if constexpr (sizeof(T) == 4) __builtin_amdgcn_sched_barrier(0);
 }
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }

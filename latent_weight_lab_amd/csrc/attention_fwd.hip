@@ -36,22 +36,21 @@ constexpr int kWaveRows = 32;
 constexpr int kWaves = 4;
 constexpr int kRows = kWaves * kWaveRows;
 
-// LDS row lengths in elements.  Keys are read 16 bytes a lane, 16 lanes at a time from 16 rows: 16
-// bytes of padding put these on distinct banks.  Values are read by columns: 16-bit rows of 16 dwords
-// more than a multiple of 32, so that a transposing read's four rows of 64 bytes fall on distinct
-// banks; float32 rows of 8 more than a multiple of 16.
-template <class T, int DP>
-struct RowsTile {
-  static constexpr int KS = DP + 16 / (int)sizeof(T);
-  static constexpr int VS = sizeof(T) == 2 ? DP + ((DP / 32) % 2 ? 0 : 32) : DP + 8;
-};
+// LDS row lengths in (16-bit) elements.  Keys are read 16 bytes a lane, 16 lanes at a time from 16 rows: 16
+// bytes of padding put these on distinct banks.  Values are read by columns: rows of 16 dwords more than a
+// multiple of 32, so that a transposing read's four rows of 64 bytes fall on distinct banks.
+template <int DP>
+using KeyRows = Padded<DP>;
+template <int DP>
+using ValueRows = Strided<DP + ((DP / 32) % 2 ? 0 : 32)>;
 
 template <class T, int DP, bool FAST>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_rows(const AttnArgs a) {
-  using Tile = RowsTile<T, DP>;
-  constexpr int KK = DP / 16, DT = DP / 32;
-  __shared__ __attribute__((aligned(16))) T lds_k[2][kKeys * Tile::KS];
-  __shared__ __attribute__((aligned(16))) T lds_v[2][kKeys * Tile::VS];
+  using KL = KeyRows<DP>;
+  using VL = ValueRows<DP>;
+  constexpr int KK = DP / 16, DT = DP / 32, KP = kKeys * KL::S, VP = kKeys * VL::S;  // sizes of a plane
+  __shared__ __attribute__((aligned(16))) Elem<T> lds_k[kBufs<T>][kPlanes<T> * KP];
+  __shared__ __attribute__((aligned(16))) Elem<T> lds_v[kBufs<T>][kPlanes<T> * VP];
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = uniform((int)threadIdx.x >> 6);
   const RowsWork w = rows_work(a);
@@ -70,7 +69,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_rows(co
   const T* qp = (const T*)a.q + b * a.qs[0] + h * a.qs[1];
   const T* kp = (const T*)a.k + b * a.ks[0] + hk * a.ks[1];
   const T* vp = (const T*)a.v + b * a.vs[0] + hk * a.vs[1];
-  Frag<T> qf[KK];
+  Opd<T> qf[KK];
   load_operand<T, DP, FAST>(qf, qp + (int64_t)q * a.qs[2], dim, q < queries);
   f32x16 o[DT] = {};
   float top = -FLT_MAX, sum = 0.0f;  // subtracted, in units of log2; sum of this lane's half of the keys
@@ -83,42 +82,60 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_rows(co
   if (begin < end) {
     kt.fetch(begin, end);
     vt.fetch(begin, end);
-    kt.template put<Strided<Tile::KS>>(lds_k[0]);
-    vt.template put<Strided<Tile::VS>>(lds_v[0]);
+    if constexpr (kBufs<T> == 2) {
+      kt.template put<KL>(lds_k[0]);
+      vt.template put<VL>(lds_v[0]);
+    }
   }
   int buf = 0;
-  for (int j0 = begin; j0 < end; j0 += kKeys, buf ^= 1) {
+  for (int j0 = begin; j0 < end; j0 += kKeys, buf ^= kBufs<T> - 1) {
     __syncthreads();  // this tile is there, the one before has been read
+    if constexpr (kBufs<T> == 1) {
+      kt.template put<KL>(lds_k[0]);
+      vt.template put<VL>(lds_v[0]);
+      __syncthreads();
+    }
     const bool more = j0 + kKeys < end;
     if (more) {
       kt.fetch(j0 + kKeys, end);
       vt.fetch(j0 + kKeys, end);
     }
     if (j0 < wave_end) {
-      const T* lk = lds_k[buf] + (lane & 31) * Tile::KS + half * 8;
-      const T* lv = lds_v[buf];
+      const Elem<T>* lk = lds_k[buf] + KL::at(lane & 31, half * 8);
+      const Elem<T>* lv = lds_v[buf];
       f32x16 s[2] = {};
       {
-        Frag<T> kf[2][KK];
+        Opd<T> kf[2][KK];
+        if constexpr (sizeof(T) == 2) {
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk)
+          for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
-          for (int t = 0; t < 2; ++t) kf[t][kk] = lds_frag(lk + t * 32 * Tile::KS + kk * 16);
-        fence_schedule<T>();
+            for (int t = 0; t < 2; ++t) kf[t][kk] = lds_operand<T>(lk + t * 32 * KL::S + kk * 16, KP);
+          fence_schedule<T>();
+        }
         if constexpr (DP > 64) __builtin_amdgcn_s_setprio(1);  // 1 x 8192 x 16 x 128: 548 -> 529 us; slower at 64
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk)
+        for (int kk = 0; kk < KK; ++kk) {
 #pragma unroll
-          for (int t = 0; t < 2; ++t) s[t] = mma32(kf[t][kk], qf[kk], s[t]);
+          for (int t = 0; t < 2; ++t) {
+            if constexpr (sizeof(T) == 4) kf[t][kk] = lds_operand<T>(lk + t * 32 * KL::S + kk * 16, KP);
+            s[t] = mma32(kf[t][kk], qf[kk], s[t]);
+          }
+          fence_operands<T>();
+        }
         if constexpr (DP > 64) __builtin_amdgcn_s_setprio(0);
       }
-      Frag<T> vf[4][DT];
+      Opd<T> vf[4][DT];
+      const auto load_v = [&](int u, int d) {
+        vf[u][d] = lds_column_operand<T, VL>(lv, VP, u * 16 + half * 4, u * 16 + half * 4 + 8, d * 32 + (lane & 16));
+      };
+      if constexpr (sizeof(T) == 2) {
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < 4; ++u)
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
-          vf[u][d] = lds_column_frag<Strided<Tile::VS>>(lv, u * 16 + half * 4, u * 16 + half * 4 + 8, d * 32 + (lane & 16));
-      fence_schedule<T>();
+          for (int d = 0; d < DT; ++d) load_v(u, d);
+        fence_schedule<T>();
+      }
       if (j0 + kKeys > free_end) {
         const int lim = std::min(q_end, end) - j0 - half * 4;
 #pragma unroll
@@ -143,20 +160,24 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_rows(co
       }
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        Frag<T> p;
+        float e[8];
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
-          const float e = exp2_hw(fmaf(s[u >> 1][(u & 1) * 8 + r], c, -top));
-          sum += e;
-          p[r] = (T)e;
+          e[r] = exp2_hw(fmaf(s[u >> 1][(u & 1) * 8 + r], c, -top));
+          sum += e[r];
         }
+        const Opd<T> p = operand_of<T>(e);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) o[d] = mma32(vf[u][d], p, o[d]);
+        for (int d = 0; d < DT; ++d) {
+          if constexpr (sizeof(T) == 4) load_v(u, d);
+          o[d] = mma32(vf[u][d], p, o[d]);
+        }
+        fence_operands<T>();
       }
     }
-    if (more) {
-      kt.template put<Strided<Tile::KS>>(lds_k[buf ^ 1]);
-      vt.template put<Strided<Tile::VS>>(lds_v[buf ^ 1]);
+    if (kBufs<T> == 2 && more) {
+      kt.template put<KL>(lds_k[buf ^ (kBufs<T> - 1)]);
+      vt.template put<VL>(lds_v[buf ^ (kBufs<T> - 1)]);
     }
   }
   sum += other_half(sum);
@@ -401,7 +422,7 @@ bool by_token(const AttnArgs& a) { return a.heads / a.kv_heads * a.queries <= kT
 // 256 keys.  Otherwise what an estimate of the time makes shortest, in us: the larger of a workgroup's
 // own walk (kAlone a tile) and all work spread over the compute units (kSpread a tile), and with more
 // than one range the join.  The rates are measured on MI355X: bfloat16 of head size 64, 0.7 us a tile
-// when a compute unit has three workgroups and 1 us alone; float32 3.8 us either way (matrix cores).
+// when a compute unit has three workgroups and 1 us alone; float32 2.9 and 3.3 us.
 void plan_splits(AttnArgs& a) {
   const int64_t cus = device_cus();
   int64_t splits = 1;
@@ -410,7 +431,7 @@ void plan_splits(AttnArgs& a) {
     splits = std::min({2 * cus / wgs, a.keys / 256, (int64_t)kMaxSplits});
   } else {
     const double unit = (double)((a.dim + 31) / 32 * 32) / 64;
-    const double alone = a.dtype == kF32 ? 3.8 * unit : 0.5 + 0.5 * unit, spread = (a.dtype == kF32 ? 3.8 : 0.7) * unit;
+    const double alone = a.dtype == kF32 ? 3.3 * unit : 0.5 + 0.5 * unit, spread = (a.dtype == kF32 ? 2.9 : 0.7) * unit;
     const int64_t tiles = (a.keys + kKeys - 1) / kKeys;
     const double wgs = (double)(a.batch * a.heads) * (double)((a.queries + kRows - 1) / kRows);
     // about half of a square causal call's tiles are walked
