@@ -273,10 +273,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_bwd_que
   }
   const int64_t row = (b * a.heads + h) * a.queries + q;
   // a query without keys has no probabilities: exp2(-infinity)
-  const float lse = q_end > 0 ? a.lse[row] * kLog2E : INFINITY;
+  float lse = q_end > 0 ? a.lse[row] * kLog2E : INFINITY;
   Opd<T> qf[KK], gf[KK];
   load_operand<T, DP, FAST>(qf, (const T*)a.q + b * a.qs[0] + h * a.qs[1] + (int64_t)q * a.qs[2], dim, q_end > 0);
-  float delta = 0.0f;
+  float delta = 0.0f, norm = 0.0f;
 #pragma unroll
   for (int kk = 0; kk < KK; ++kk) {
     Raw8<T> gr, orow;
@@ -287,9 +287,24 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_bwd_que
     unpack8(x, gr);
     unpack8(y, orow);
 #pragma unroll
-    for (int r = 0; r < 8; ++r) delta += x[r] * y[r];
+    for (int r = 0; r < 8; ++r) {
+      delta += x[r] * y[r];
+      norm += x[r] * x[r];
+    }
   }
   delta += other_half(delta);
+  // float16 scores' gradients are held 2^-e times as large, 2^e about the length of this query's row of dout: they
+  // are then not subnormal where gradients are small, and |dS| <= 4 max |v| (lengths again).  It costs nothing:
+  // the power goes into lse and back out with dQ's scale.
+  float unscale = a.scale;
+  if constexpr (__is_same(T, f16)) {
+    norm += other_half(norm);
+    if (norm > 0x1p-60f && norm < 0x1p60f) {
+      const int e = (((int)(__float_as_uint(norm) >> 23) & 0xff) - 127) >> 1;
+      lse += (float)e;
+      unscale = ldexpf(a.scale, e);
+    }
+  }
   if (half == 0 && q < queries) a.work[row] = delta;
   f32x16 dq[DT] = {};
   const float c = a.scale * kLog2E;
@@ -388,7 +403,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_bwd_que
     }
   }
   if (q >= queries) return;
-  store_result<T, DP, FAST>((T*)a.dq + b * a.dqs[0] + h * a.dqs[1] + (int64_t)q * a.dqs[2], dq, a.scale, dim);
+  store_result<T, DP, FAST>((T*)a.dq + b * a.dqs[0] + h * a.dqs[1] + (int64_t)q * a.dqs[2], dq, unscale, dim);
 }
 
 // dK and dV of a key from the ranges' partial sums, in the ranges' order: 32 lanes of eight values for the two
