@@ -46,9 +46,15 @@ constexpr int kUnroll = sizeof(T) == 2 && DP > 64 ? 2 : 1;
 template <class T, int DP>
 constexpr int kKeysOccupancy = sizeof(T) == 2 && DP <= 64 ? 2 : 1;
 
-// The workspace: D of every query, then (256-byte aligned) the key gradients' partial sums.
+// float32 keeps of every query, beside D, the factor that makes its probabilities sum to 1.  lse is one rounded
+// number, so exp2(s - lse) is off by the same 2^-24 |lse| for a whole row, more than all else here together; the
+// query pass meets every key of a row, so it sums what it computes and passes 1 / sum on.
+template <class T>
+constexpr bool kRenorm = sizeof(T) == 4;
+
+// The workspace: D of every query (float32: and its factor), then (256-byte aligned) the key gradients' partial sums.
 __host__ __device__ inline int64_t delta_floats(const AttnArgs& a) {
-  return (a.batch * a.heads * a.queries + 63) / 64 * 64;
+  return ((a.dtype == kF32 ? 2 : 1) * a.batch * a.heads * a.queries + 63) / 64 * 64;
 }
 __device__ __forceinline__ float* partials(const AttnArgs& a) { return a.work + delta_floats(a); }
 
@@ -58,7 +64,8 @@ __global__ __launch_bounds__(256, (kKeysOccupancy<T, DP>)) void attention_bwd_ke
   constexpr int KK = DP / 16, DT = DP / 32, PL = kTile * Tile::S;  // size of a plane
   __shared__ __attribute__((aligned(16))) Elem<T> lds_q[kBufs<T>][kPlanes<T> * PL];
   __shared__ __attribute__((aligned(16))) Elem<T> lds_g[kBufs<T>][kPlanes<T> * PL];
-  __shared__ __attribute__((aligned(16))) float lds_stat[kBufs<T>][2][kTile];
+  constexpr int kStats = kRenorm<T> ? 3 : 2;  // lse, D and float32's factor, kTile of each
+  __shared__ __attribute__((aligned(16))) float lds_stat[kBufs<T>][kStats][kTile];
   const int lane = threadIdx.x & 63, half = lane >> 5, wave = uniform((int)threadIdx.x >> 6);
   const uint32_t kvh = (uint32_t)a.kv_heads, kvb = (uint32_t)a.batch * kvh, group = (uint32_t)a.heads / kvh;
   const uint32_t id = work_order(blockIdx.x, gridDim.x, (uint32_t)a.cus), bk = id % kvb, splits = (uint32_t)a.splits;
@@ -96,18 +103,19 @@ __global__ __launch_bounds__(256, (kKeysOccupancy<T, DP>)) void attention_bwd_ke
     gt.base = gp + fg * a.dos[1];
     qt.fetch(fq, queries);
     gt.fetch(fq, queries);
-    if (threadIdx.x < 2 * kTile) {
+    if (threadIdx.x < kStats * kTile) {
       const int q = fq + (threadIdx.x & (kTile - 1));
-      const bool is_d = threadIdx.x >= kTile;
+      const bool is_d = threadIdx.x >= kTile, is_factor = threadIdx.x >= 2 * kTile;
       const float* stat = (is_d ? a.work : a.lse) + head0 + (int64_t)fg * queries;
+      if (is_factor) stat += a.batch * a.heads * a.queries;
       sr = q < queries ? stat[q] : (is_d ? 0.0f : INFINITY);  // past the last: no probabilities
-      sr = is_d ? -sr : kFoldStats<T> ? (kLift - sr * kLog2E) * inv_c : kLift - sr * kLog2E;
+      sr = is_factor ? sr : is_d ? -sr : kFoldStats<T> ? (kLift - sr * kLog2E) * inv_c : kLift - sr * kLog2E;
     }
   };
   auto put = [&](int buf) {
     qt.template put<Tile>(lds_q[buf]);
     gt.template put<Tile>(lds_g[buf]);
-    if (threadIdx.x < 2 * kTile) lds_stat[buf][threadIdx.x / kTile][threadIdx.x & (kTile - 1)] = sr;
+    if (threadIdx.x < kStats * kTile) lds_stat[buf][threadIdx.x / kTile][threadIdx.x & (kTile - 1)] = sr;
   };
   int buf = 0;
   uint32_t g = begin < end ? (uint32_t)uniform(begin / per_head) : 0;
@@ -195,7 +203,7 @@ __global__ __launch_bounds__(256, (kKeysOccupancy<T, DP>)) void attention_bwd_ke
             s[r] = exp2_hw(s[r] * c);
           } else {
             const int i = at + (r >> 2) * 8 + half * 4 + (r & 3);
-            s[r] = exp2_hw(fmaf(s[r], c, lds_stat[buf][0][i]));
+            s[r] = exp2_hw(fmaf(s[r], c, lds_stat[buf][0][i])) * lds_stat[buf][kStats - 1][i];
             dp[r] += lds_stat[buf][1][i];
           }
           dp[r] = s[r] * (kLowerLate<T> ? dp[r] : dp[r] * kLower);
@@ -307,6 +315,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_bwd_que
   }
   if (half == 0 && q < queries) a.work[row] = delta;
   f32x16 dq[DT] = {};
+  float total = 0.0f;  // of the query's probabilities
   const float c = a.scale * kLog2E;
   if (kBufs<T> == 2 && end > 0) {
     kt.template put<Tile>(lds_k[0]);
@@ -375,12 +384,24 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_bwd_que
         }
         fence_schedule<T>();
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = exp2_hw(fmaf(s[r], c, -lse)) * (dp[r] - delta);
+        for (int r = 0; r < 16; ++r) {
+          s[r] = exp2_hw(fmaf(s[r], c, -lse));
+          if constexpr (!kRenorm<T>) s[r] *= dp[r] - delta;
+        }
         if (j0 + kTile > free_end) {
           const int lim = q_end - j0 - t * 32 - half * 4;
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            if ((r >> 2) * 8 + (r & 3) >= lim) s[r] = 0.0f;
+            if ((r >> 2) * 8 + (r & 3) >= lim) s[r] = dp[r] = 0.0f;  // dp: may be NaN where masked
+        }
+        if constexpr (kRenorm<T>) {
+          float sum = 0.0f;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            sum += s[r];
+            s[r] *= dp[r] - delta;
+          }
+          total += sum;
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -401,6 +422,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_bwd_que
       kt.template put<Tile>(lds_k[buf ^ (kBufs<T> - 1)]);
       vt.template put<Tile>(lds_v[buf ^ (kBufs<T> - 1)]);
     }
+  }
+  if constexpr (kRenorm<T>) {
+    total += other_half(total);
+    const float factor = total == 0.0f ? 0.0f : 1.0f / total;  // 0: no keys
+    if (half == 0 && q < queries) a.work[a.batch * a.heads * a.queries + row] = factor;
+    unscale *= factor;
   }
   if (q >= queries) return;
   store_result<T, DP, FAST>((T*)a.dq + b * a.dqs[0] + h * a.dqs[1] + (int64_t)q * a.dqs[2], dq, unscale, dim);
