@@ -347,72 +347,67 @@ __global__ __launch_bounds__(256) void attention_token(const AttnArgs a) {
   }
 }
 
-// The ranges' outputs weighed by their sums.  32 lanes of four columns each hold a row; GROUPS groups of lanes
-// share a row's ranges, taking every GROUPS-th, and join through LDS in the groups' order: eight (one row a
-// workgroup) where there are many ranges, one (eight rows) where there are few.
-constexpr int kMaxSplits = 512;
-template <class T, int GROUPS>
+// The ranges' outputs weighed by their sums: a thread joins eight values of a row, its chunk, and computes the
+// weights for itself.  Where there are few ranges every thread of a workgroup has another chunk (kSplitsAlone);
+// where there are many the workgroup has 16 chunks or fewer, one row's, and its SHARE = 16 threads of a chunk take every
+// 16th range each and add up through LDS in their order.
+constexpr int kMaxSplits = 512, kSplitsAlone = 16;
+template <class T, int SHARE>
 __global__ __launch_bounds__(256) void attention_join(const AttnArgs a) {
-  constexpr int ROWS = 8 / GROUPS, WIDTH = 32 * GROUPS;  // rows of a workgroup, threads of a row
-  __shared__ float lds_w[ROWS][kMaxSplits / ROWS], lds_v[ROWS][GROUPS][kAttnMaxDim], lds_t[2][8];
-  const int r = threadIdx.x / WIDTH, t = threadIdx.x % WIDTH, group = t >> 5, col = (t & 31) * 4;
-  const uint32_t rows = (uint32_t)(a.batch * a.heads * a.queries), row = blockIdx.x * ROWS + r;
-  const int dim = (int)a.dim, splits = a.splits;
-  const bool live = row < rows;
+  constexpr int CHUNKS = 256 / SHARE;
+  static_assert(SHARE == 1 || CHUNKS * 8 == kAttnMaxDim);
+  __shared__ float lds_v[SHARE][CHUNKS][8], lds_m[SHARE], lds_t[SHARE];
+  const int dim = (int)a.dim, splits = a.splits, per_row = (dim + 7) / 8;
+  const uint32_t rows_wg = SHARE == 1 ? 256 / per_row : 1, rows = (uint32_t)(a.batch * a.heads * a.queries);
+  const int part_no = threadIdx.x / CHUNKS, chunk = threadIdx.x % CHUNKS, r = chunk / per_row;
+  const int col = (chunk - r * per_row) * 8;
+  const uint32_t row = blockIdx.x * rows_wg + r;
+  const bool live = (uint32_t)r < rows_wg && row < rows;
   const int64_t first = (int64_t)(live ? row : 0) * splits;
   const float* lses = a.work + (int64_t)rows * splits * dim + first;
-  float m = -FLT_MAX, total = 0.0f;
-  for (int s = t; s < splits; s += WIDTH) m = max_nan(m, lses[s]);
-#pragma unroll
-  for (int k = 16; k > 0; k >>= 1) m = max_nan(m, __shfl_xor(m, k, 64));
-  if constexpr (GROUPS > 1) {
-    if ((t & 31) == 0) lds_t[0][group] = m;
+  const float* part = a.work + first * dim + col;
+  float m = -FLT_MAX, total = 0.0f, v[8] = {};
+  for (int s = part_no; s < splits; s += SHARE) m = max_nan(m, lses[s]);
+  if constexpr (SHARE > 1) {
+    if (chunk == 0) lds_m[part_no] = m;
     __syncthreads();
 #pragma unroll
-    for (int g = 0; g < GROUPS; ++g) m = max_nan(m, lds_t[0][g]);
+    for (int g = 0; g < SHARE; ++g) m = max_nan(m, lds_m[g]);
   }
-  for (int s = t; s < splits; s += WIDTH) {
-    const float w = exp2_hw(lses[s] - m);  // 0 for a range that holds nothing
-    lds_w[r][s] = w;
-    total += w;
-  }
-  total = lanes_sum<32>(total);
-  if ((t & 31) == 0) lds_t[1][threadIdx.x >> 5] = total;
-  __syncthreads();
-  float v[4] = {};
-  const float* part = a.work + first * dim;
-#pragma unroll 8
-  for (int s = group; s < splits; s += GROUPS) {
-    const float w = lds_w[r][s];
+  if (live) {
+#pragma unroll 4
+    for (int s = part_no; s < splits; s += SHARE) {
+      float x[8];
+      load8(x, part + (int64_t)s * dim, dim - col);  // written, zeros where nothing is held
+      const float w = exp2_hw(lses[s] - m);          // 0 for a range that holds nothing
+      total += w;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float x = col + i < dim ? part[(int64_t)s * dim + col + i] : 0.0f;  // written, zeros where nothing is held
-      v[i] += w * x;
+      for (int i = 0; i < 8; ++i) v[i] += w * x[i];
     }
   }
-  if constexpr (GROUPS > 1) {
+  if constexpr (SHARE > 1) {
+    if (chunk == 0) lds_t[part_no] = total;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) lds_v[r][group][col + i] = v[i];
+    for (int i = 0; i < 8; ++i) lds_v[part_no][chunk][i] = v[i];
     __syncthreads();
     total = 0.0f;
 #pragma unroll
-    for (int g = 0; g < GROUPS; ++g) total += lds_t[1][g];
+    for (int g = 0; g < SHARE; ++g) total += lds_t[g];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 8; ++i) {
       v[i] = 0.0f;
 #pragma unroll
-      for (int g = 0; g < GROUPS; ++g) v[i] += lds_v[r][g][col + i];
+      for (int g = 0; g < SHARE; ++g) v[i] += lds_v[g][chunk][i];
     }
   }
-  if (!live || group != 0) return;
+  if (!live || part_no != 0) return;
   const uint32_t queries = (uint32_t)a.queries, heads = (uint32_t)a.heads, bh = row / queries, q = row - bh * queries;
   const int64_t b = bh / heads, h = bh % heads;
   const float inv = total > 0.0f ? 1.0f / total : (total == 0.0f ? 0.0f : total);
-  T* op = (T*)a.out + b * a.os[0] + h * a.os[1] + (int64_t)q * a.os[2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (col + i < dim) op[col + i] = (T)(v[i] * inv);
-  if (a.lse && t == 0)
+  for (int i = 0; i < 8; ++i) v[i] *= inv;
+  store8((T*)a.out + b * a.os[0] + h * a.os[1] + (int64_t)q * a.os[2] + col, v, dim - col);
+  if (a.lse && col == 0)
     a.lse[row] = total > 0.0f ? (m + log2_hw(total)) * kLn2 : (total == 0.0f ? -INFINITY : total);
 }
 
@@ -420,9 +415,11 @@ bool by_token(const AttnArgs& a) { return a.heads / a.kv_heads * a.queries <= kT
 
 // Ranges of keys.  Single tokens: as many as make two workgroups for each compute unit, none shorter than
 // 256 keys.  Otherwise what an estimate of the time makes shortest, in us: the larger of a workgroup's
-// own walk (kAlone a tile) and all work spread over the compute units (kSpread a tile), and with more
-// than one range the join.  The rates are measured on MI355X: bfloat16 of head size 64, 0.7 us a tile
-// when a compute unit has three workgroups and 1 us alone; float32 2.9 and 3.3 us.
+// own walk (`alone` a tile, and as much as a tile before its first) and all work spread over the compute units
+// (`spread` a tile), and with more than one range the join.  The rates are measured on MI355X: bfloat16 of head
+// size 64, 0.7 us a tile when a compute unit has three workgroups and 1 us alone; float32 2.9 and 3.3 us.
+// 4 x 512 x 12 x 64 in float32: 1, 2, 3, 4 ranges 31.8, 27.2, 30.4, 31.0 us with the join, 2 are taken;
+// float16 6 x 515 over up to 1531 keys x 12 x 80: 34.4, 37.4, 44.0, 47.7 us, 1 is taken.
 void plan_splits(AttnArgs& a) {
   const int64_t cus = device_cus();
   int64_t splits = 1;
@@ -436,12 +433,13 @@ void plan_splits(AttnArgs& a) {
     const double wgs = (double)(a.batch * a.heads) * (double)((a.queries + kRows - 1) / kRows);
     // about half of a square causal call's tiles are walked
     // (also of ragged sequences' tiles, whose lengths only the device knows)
-    const double all = wgs * (double)tiles * ((a.causal && a.queries * 2 > a.keys) || a.lengths ? 0.55 : 1.0) * spread / (double)cus;
+    const double walked = (double)tiles * ((a.causal && a.queries * 2 > a.keys) || a.lengths ? 0.55 : 1.0);
     const double bytes = 8.0 * (double)(a.batch * a.heads) * (double)a.queries * (double)a.dim;  // of a range
     double best = 0.0;
     for (int64_t n = 1; n <= std::min<int64_t>(tiles / 4 + 1, kMaxSplits); n = n < 4 ? n + 1 : n + n / 4) {
-      const double walk = (double)((tiles + n - 1) / n) * alone;
-      const double t = std::max(walk, all) + (n > 1 ? 4.0 + (double)n * bytes / 4.5e6 : 0.0);
+      const double walk = (double)((tiles + n - 1) / n + 1) * alone;
+      const double all = wgs * ((double)n + walked) * spread / (double)cus;
+      const double t = std::max(walk, all) + (n > 1 ? 2.5 + (double)n * bytes / 9e6 : 0.0);
       // several only where they gain more than the estimate may be off by
       if (n == 1 || t < best * (splits == 1 ? 0.85 : 1.0)) {
         best = t;
@@ -470,8 +468,11 @@ hipError_t run(const AttnArgs& a, hipStream_t s) {
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.splits == 1) return e;
   const int64_t rows = a.batch * a.heads * a.queries;
-  if (a.splits > 16) hipLaunchKernelGGL((attention_join<T, 8>), dim3((unsigned)rows), dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((attention_join<T, 1>), dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s, a);
+  const int64_t rows_wg = 256 / ((a.dim + 7) / 8);
+  if (a.splits > kSplitsAlone)
+    hipLaunchKernelGGL((attention_join<T, 16>), dim3((unsigned)rows), dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((attention_join<T, 1>), dim3((unsigned)((rows + rows_wg - 1) / rows_wg)), dim3(256), 0, s, a);
   return hipGetLastError();
 }
 
