@@ -505,12 +505,15 @@ hipError_t run_dim(const AttnArgs& a, hipStream_t s) {
 // of the time makes shortest, in us, as in the forward pass: the longest walk alone, or all work spread over
 // the compute units, in whole rounds where the works are equal; and with several ranges the join.
 // Measured on MI355X, a tile of 64 queries: bfloat16 of head size 64 1.2 us when a compute unit has two
-// workgroups and 1.6 alone, of size 128 2.8 us (one fits); float32 of size 64 6.8 us.
-// 4 x 512 x 12 x 64 in float32: 1, 2, 3, 4 ranges 60.9, 51.1, 59.1, 61.2 us with the join, 2 are taken.
+// workgroups and 1.6 alone, of size 128 2.8 us (one fits); float32 of size 64 6.8 us; and what a workgroup
+// takes before its first tile and for its results, 7 and 10 us at size 64.  Of 1, 2, 3, 4 ranges, with the join:
+// 4 x 512 x 12 x 64 in float32 60.9, 51.1, 59.1, 61.2 us, 2 are taken; float16 6 x 515 queries over up to 1531 keys,
+// 12 heads on 4, of size 80: 63.1, 80.9, 87.6, 91.7 us, 1 is taken; bfloat16 8 x 1024 x 12 x 64: 47 us and up from 85, 1.
 static void plan_bwd_splits(AttnArgs& a) {
   const double unit = (double)((a.dim + 31) / 32 * 32) / 64, cus = (double)device_cus();
   const double spread = (a.dtype == kF32 ? 6.8 : a.dim <= 64 ? 1.2 : 1.4) * unit;
   const double alone = (a.dtype == kF32 ? 6.8 : a.dim <= 64 ? 1.6 : 1.4) * unit;
+  const double fixed = (a.dtype == kF32 ? 10.0 : 7.0) * unit;
   const int64_t tiles = a.heads / a.kv_heads * ((a.queries + kTile - 1) / kTile);
   // with lengths, which only the device knows, about half of the blocks hold keys
   const double wgs = (double)(a.batch * a.kv_heads) * (double)((a.keys + kBlock - 1) / kBlock) * (a.lengths ? 0.55 : 1.0);
@@ -521,8 +524,9 @@ static void plan_bwd_splits(AttnArgs& a) {
   for (int64_t n = 1; n <= std::min<int64_t>(tiles / 4 + 1, 256); n = n < 4 ? n + 1 : n + n / 4) {
     const double walk = (double)((tiles + n - 1) / n);
     const double slots = a.dtype != kF32 && a.dim <= 64 ? 2 * cus : cus, rounds = std::ceil(wgs * (double)n / slots);
-    const double all = halves ? 0.55 * wgs * (double)tiles / cus * spread : rounds * walk * spread * slots / cus;
-    const double t = std::max(walk * alone, all) + (n > 1 ? 4.0 + (double)n * bytes / 11e6 : 0.0);
+    const double all = halves ? 0.55 * wgs * (double)tiles / cus * spread + wgs * (double)n / slots * fixed
+                              : rounds * (walk * spread * slots / cus + fixed);
+    const double t = std::max(walk * alone + fixed, all) + (n > 1 ? 4.0 + (double)n * bytes / 11e6 : 0.0);
     if (n == 1 || t < best) {
       best = t;
       a.splits = (int)n;
