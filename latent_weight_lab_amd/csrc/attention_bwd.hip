@@ -14,7 +14,8 @@
 // column a query (bwd_queries: S^T = K Q^T) dS^T is the operand of dQ^T = K^T dS^T.  The other operand of
 // these is a column of the tile in LDS (the transposing read).
 //
-// bwd_queries runs first and leaves each query's D in the workspace for bwd_keys.
+// bwd_queries runs first and leaves each query's D in the workspace for bwd_keys.  Where blocks are too few for the
+// compute units, both take ranges of what they walk over and leave float32 sums to be joined.
 #include <algorithm>
 #include <cmath>
 
@@ -25,6 +26,7 @@ namespace {
 
 constexpr int kBlock = 128;  // keys (queries) of a workgroup: 32 for each of four waves
 constexpr int kTile = kTileRows;  // queries (keys) of a tile
+constexpr int kMostQuerySplits = 64;
 
 // In dV's product the probabilities are 2^kLift times too large (exact, and taken back at the end): dV sums
 // a key's probabilities over the queries, all of which may be small, and small ones are subnormal in
@@ -51,8 +53,12 @@ constexpr int kKeysOccupancy = sizeof(T) == 2 && DP <= 64 ? 2 : 1;
 // query pass meets every key of a row, so it sums what it computes and passes 1 / sum on.
 template <class T>
 constexpr bool kRenorm = sizeof(T) == 4;
+__device__ __forceinline__ float renorm_factor(float total) {
+  return total == 0.0f ? 0.0f : 1.0f / total;  // 0: no keys
+}
 
-// The workspace: D of every query (float32: and its factor), then (256-byte aligned) the key gradients' partial sums.
+// The workspace: D of every query (float32: and its factor), then (256-byte aligned) the partial sums of a pass that
+// is split: the query pass's until attention_bwd_join_queries has run, then the key pass's.
 __host__ __device__ inline int64_t delta_floats(const AttnArgs& a) {
   return ((a.dtype == kF32 ? 2 : 1) * a.batch * a.heads * a.queries + 63) / 64 * 64;
 }
@@ -90,8 +96,8 @@ __global__ __launch_bounds__(256, (kKeysOccupancy<T, DP>)) void attention_bwd_ke
   const T* gp = (const T*)a.dout + b * a.dos[0] + hk * group * a.dos[1];
   const int64_t head0 = (b * a.heads + hk * group) * a.queries;
   TileLoader<T, DP, FAST> qt, gt;
-  qt.init(qp, a.qs[2], dim);
-  gt.init(gp, a.dos[2], dim);
+  qt.init(qp, a.qs[2], dim, queries);
+  gt.init(gp, a.dos[2], dim, queries);
   float sr = 0.0f;
   // Tiles of the first head, then of the next one of the group: one sequence, of which this workgroup
   // takes the tiles begin .. end.
@@ -267,17 +273,18 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_bwd_que
   const Allowed allow = allowed_keys(a, b);
   const int queries = (int)a.queries, wq0 = q0 + wave * 32, q = wq0 + (lane & 31);
   const int q_end = q < queries ? key_end(allow, q) : 0;
-  const int end = key_end(allow, std::min(q0 + kBlock, queries) - 1);
+  const int begin = w.split * (int)a.split_len;
+  const int end = std::min(key_end(allow, std::min(q0 + kBlock, queries) - 1), begin + (int)a.split_len);
   const int free_end = wq0 < queries ? key_end(allow, wq0) : 0;
   const int wave_end = wq0 < queries ? key_end(allow, std::min(wq0 + 32, queries) - 1) : 0;
   const T* kp = (const T*)a.k + b * a.ks[0] + hk * a.ks[1];
   const T* vp = (const T*)a.v + b * a.vs[0] + hk * a.vs[1];
   TileLoader<T, DP, FAST> kt, vt;
-  kt.init(kp, a.ks[2], dim);
-  vt.init(vp, a.vs[2], dim);
-  if (end > 0) {
-    kt.fetch(0, end);
-    vt.fetch(0, end);
+  kt.init(kp, a.ks[2], dim, (int)a.keys);
+  vt.init(vp, a.vs[2], dim, (int)a.keys);
+  if (begin < end) {
+    kt.fetch(begin, end);
+    vt.fetch(begin, end);
   }
   const int64_t row = (b * a.heads + h) * a.queries + q;
   // a query without keys has no probabilities: exp2(-infinity)
@@ -313,16 +320,16 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_bwd_que
       unscale = ldexpf(a.scale, e);
     }
   }
-  if (half == 0 && q < queries) a.work[row] = delta;
+  if (half == 0 && q < queries && w.split == 0) a.work[row] = delta;
   f32x16 dq[DT] = {};
   float total = 0.0f;  // of the query's probabilities
   const float c = a.scale * kLog2E;
-  if (kBufs<T> == 2 && end > 0) {
+  if (kBufs<T> == 2 && begin < end) {
     kt.template put<Tile>(lds_k[0]);
     vt.template put<Tile>(lds_v[0]);
   }
   int buf = 0;
-  for (int j0 = 0; j0 < end; j0 += kTile, buf ^= kBufs<T> - 1) {
+  for (int j0 = begin; j0 < end; j0 += kTile, buf ^= kBufs<T> - 1) {
     __syncthreads();  // this tile is there, the one before has been read
     if constexpr (kBufs<T> == 1) {
       kt.template put<Tile>(lds_k[0]);
@@ -423,14 +430,52 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_bwd_que
       vt.template put<Tile>(lds_v[buf ^ (kBufs<T> - 1)]);
     }
   }
+  if constexpr (kRenorm<T>) total += other_half(total);
+  if (q >= queries) return;
+  const int64_t rows = a.batch * a.heads * a.queries;
+  if (a.splits > 1) {  // summed by attention_bwd_join_queries
+    const int64_t part = row * a.splits + w.split;
+    if (kRenorm<T> && half == 0) partials(a)[rows * a.splits * dim + part] = total;
+    store_result<float, DP, FAST>(partials(a) + part * dim, dq, unscale, dim);
+    return;
+  }
   if constexpr (kRenorm<T>) {
-    total += other_half(total);
-    const float factor = total == 0.0f ? 0.0f : 1.0f / total;  // 0: no keys
-    if (half == 0 && q < queries) a.work[a.batch * a.heads * a.queries + row] = factor;
+    const float factor = renorm_factor(total);
+    if (half == 0) a.work[rows + row] = factor;
     unscale *= factor;
   }
-  if (q >= queries) return;
   store_result<T, DP, FAST>((T*)a.dq + b * a.dqs[0] + h * a.dqs[1] + (int64_t)q * a.dqs[2], dq, unscale, dim);
+}
+
+// dQ of a query, and float32's factor, from the ranges of keys, in their order: a thread sums eight values.
+template <class T>
+__global__ __launch_bounds__(256) void attention_bwd_join_queries(const AttnArgs a) {
+  const int dim = (int)a.dim, chunks = (dim + 7) / 8, rows_wg = 256 / chunks, r = threadIdx.x / chunks;
+  const int col = (threadIdx.x - r * chunks) * 8, splits = a.splits;
+  const int64_t rows = a.batch * a.heads * a.queries, row = (int64_t)blockIdx.x * rows_wg + r;
+  if (r >= rows_wg || row >= rows) return;
+  const float* part = partials(a) + row * splits * dim + col;
+  float sum[8] = {}, factor = 1.0f;
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) {
+    float v[8];
+    load8(v, part + s * dim, dim - col);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum[i] += v[i];
+  }
+  if constexpr (kRenorm<T>) {
+    const float* totals = partials(a) + rows * splits * dim + row * splits;
+    float total = 0.0f;
+    for (int s = 0; s < splits; ++s) total += totals[s];
+    factor = renorm_factor(total);
+    if (col == 0) a.work[rows + row] = factor;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum[i] *= factor;
+  const uint32_t queries = (uint32_t)a.queries, heads = (uint32_t)a.heads, bh = (uint32_t)row / queries;
+  const uint32_t q = (uint32_t)row - bh * queries;
+  const int64_t b = bh / heads, h = bh % heads;
+  store8((T*)a.dq + b * a.dqs[0] + h * a.dqs[1] + (int64_t)q * a.dqs[2] + col, sum, dim - col);
 }
 
 // dK and dV of a key from the ranges' partial sums, in the ranges' order: a thread sums eight values of them.
@@ -458,16 +503,50 @@ __global__ __launch_bounds__(256) void attention_bwd_join(const AttnArgs a) {
   store8(dst + col, sum, dim - col);
 }
 
+// Ranges of a query block's keys, where blocks are too few for the compute units: the estimate of the forward pass,
+// with this pass's times, in us.  Of 1, 2, 3, 4, 10 ranges, with the join: float32 5 x 65 queries over up to 2641
+// keys, 6 heads on 2, of size 32: 114, 66, 49, 41, 26 us, 11 are taken; float32 4 x 512 x 12 x 64: 46, 38, 42, 46,
+// 56 us, 2; bfloat16 3 x 1807 x 4 x 96: 46, 39, 40, 41, 60 us, 3; 8 x 1024 x 12 x 64: 34, 53, 62, 72, 120 us, 1.
+void plan_query_splits(AttnArgs& a) {
+  const double unit = (double)((a.dim + 31) / 32 * 32) / 64, cus = (double)device_cus();
+  const double alone = (a.dtype == kF32 ? 5.1 : 1.1) * unit, spread = (a.dtype == kF32 ? 4.8 : 1.0) * unit;
+  const int64_t tiles = (a.keys + kTile - 1) / kTile;
+  const double wgs = (double)(a.batch * a.heads) * (double)((a.queries + kBlock - 1) / kBlock);
+  const double walked = (double)tiles * ((a.causal && a.queries * 2 > a.keys) || a.lengths ? 0.55 : 1.0);
+  const double bytes = 8.0 * (double)(a.batch * a.heads) * (double)a.queries * (double)a.dim;
+  double best = 0.0;
+  int64_t splits = 1;
+  for (int64_t n = 1; n <= std::min<int64_t>(tiles / 4 + 1, kMostQuerySplits); n = n < 4 ? n + 1 : n + n / 4) {
+    const double walk = (double)((tiles + n - 1) / n + 1) * alone, all = wgs * ((double)n + walked) * spread / cus;
+    const double t = std::max(walk, all) + (n > 1 ? 4.5 + (double)n * bytes / 18e6 : 0.0);
+    // several only where they gain more than the estimate may be off by
+    if (n == 1 || t < best * (splits == 1 ? 0.85 : 1.0)) {
+      best = t;
+      splits = n;
+    }
+  }
+  a.split_len = splits > 1 ? ((a.keys + splits - 1) / splits + kTile - 1) / kTile * kTile : std::max<int64_t>(a.keys, 1);
+  a.splits = splits > 1 ? (int)((a.keys + a.split_len - 1) / a.split_len) : 1;
+}
+
 template <class T, int DP, bool FAST>
 hipError_t launch(const AttnArgs& a, hipStream_t s) {
   const int64_t kgrid = a.batch * a.kv_heads * ((a.keys + kBlock - 1) / kBlock);
   const int64_t qgrid = a.batch * a.heads * ((a.queries + kBlock - 1) / kBlock);
   if (qgrid > 0) {
-    AttnArgs whole = a;
-    whole.splits = 1;  // the ranges are the key pass's
-    hipLaunchKernelGGL((attention_bwd_queries<T, DP, FAST>), dim3((unsigned)qgrid), dim3(256), 0, s, whole);
-    const hipError_t e = hipGetLastError();
+    AttnArgs by_keys = a;  // a's ranges are the key pass's
+    plan_query_splits(by_keys);
+    hipLaunchKernelGGL((attention_bwd_queries<T, DP, FAST>), dim3((unsigned)(qgrid * by_keys.splits)), dim3(256), 0, s,
+                       by_keys);
+    hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
+    if (by_keys.splits > 1) {
+      const int64_t rows = a.batch * a.heads * a.queries, rows_wg = 256 / ((a.dim + 7) / 8);
+      hipLaunchKernelGGL((attention_bwd_join_queries<T>), dim3((unsigned)((rows + rows_wg - 1) / rows_wg)), dim3(256), 0,
+                         s, by_keys);
+      e = hipGetLastError();
+      if (e != hipSuccess) return e;
+    }
   }
   if (kgrid > 0) {
     hipLaunchKernelGGL((attention_bwd_keys<T, DP, FAST>), dim3((unsigned)(kgrid * a.splits)), dim3(256), 0, s, a);
@@ -535,9 +614,12 @@ static void plan_bwd_splits(AttnArgs& a) {
 }
 
 int64_t attention_bwd_work(const AttnArgs& args) {
-  AttnArgs a = args;
+  AttnArgs a = args, by_keys = args;
   plan_bwd_splits(a);
-  return delta_floats(a) + (a.splits > 1 ? (int64_t)a.splits * 2 * a.batch * a.kv_heads * a.keys * a.dim : 0);
+  plan_query_splits(by_keys);
+  const int64_t keys = a.splits > 1 ? (int64_t)a.splits * 2 * a.batch * a.kv_heads * a.keys * a.dim : 0;
+  const int64_t queries = by_keys.splits > 1 ? (int64_t)by_keys.splits * a.batch * a.heads * a.queries * (a.dim + 1) : 0;
+  return delta_floats(a) + std::max(keys, queries);
 }
 
 hipError_t launch_attention_bwd(AttnArgs a, hipStream_t s) {

@@ -77,8 +77,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_rows(co
 
   // one tile's products in LDS while the next one's loads are under way, a barrier a tile
   TileLoader<T, DP, FAST> kt, vt;
-  kt.init(kp, a.ks[2], dim);
-  vt.init(vp, a.vs[2], dim);
+  kt.init(kp, a.ks[2], dim, (int)a.keys);
+  vt.init(vp, a.vs[2], dim, (int)a.keys);
   if (begin < end) {
     kt.fetch(begin, end);
     vt.fetch(begin, end);
@@ -228,18 +228,21 @@ __global__ __launch_bounds__(256) void attention_token(const AttnArgs a) {
   const T* kp = (const T*)a.k + b * a.ks[0] + hk * a.ks[1];
   const T* vp = (const T*)a.v + b * a.vs[0] + hk * a.vs[1];
   const T* qp = (const T*)a.q + b * a.qs[0] + h * a.qs[1] + qi * a.qs[2];
-  auto load8_or = [](Raw8<T>& r, const T* p, bool ok, int left) {  // zeros where not ok
-    if constexpr (WHOLE) load_whole8(r, p, ok && left > 0);
-    else load_raw8(r, p, ok ? left : 0);
-  };
   Frag<T> qf[KK];
 #pragma unroll
   for (int kk = 0; kk < KK; ++kk) {
     const int col = kk * 32 + quad * 8;
     Raw8<T> r;
-    load8_or(r, qp + col, live, dim - col);
+    load_raw8(r, qp + col, live ? dim - col : 0);
     qf[kk] = frag_of(r);
   }
+  // of key j; zeros where not ok.  What a key's row reads past it is cleared before the product, a value's
+  // makes columns that are not stored.
+  const int keys = (int)a.keys;
+  auto load8_or = [&](Raw8<T>& r, const T* p, int64_t stride, int j, bool ok, int left) {
+    if constexpr (WHOLE) load_whole8(r, p, ok && left > 0);
+    else load_ahead8(r, p, ok ? left : 0, stride >= 8 && j + 1 < keys);
+  };
   Raw8<T> kr[2][KK], vr[PER];
   auto fetch = [&](int j0) {
 #pragma unroll
@@ -247,12 +250,12 @@ __global__ __launch_bounds__(256) void attention_token(const AttnArgs a) {
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
         const int j = j0 + t * 16 + row, col = kk * 32 + quad * 8;
-        load8_or(kr[t][kk], kp + (int64_t)j * a.ks[2] + col, j < end, dim - col);
+        load8_or(kr[t][kk], kp + (int64_t)j * a.ks[2] + col, a.ks[2], j, j < end, dim - col);
       }
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int cc = lane + i * 64, j = j0 + cc / CPR, col = (cc % CPR) * 8;
-      load8_or(vr[i], vp + (int64_t)j * a.vs[2] + col, j < end, dim - col);
+      load8_or(vr[i], vp + (int64_t)j * a.vs[2] + col, a.vs[2], j, j < end, dim - col);
     }
   };
   f32x4 o[DT] = {};
@@ -265,7 +268,10 @@ __global__ __launch_bounds__(256) void attention_token(const AttnArgs a) {
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk) s[t] = mma16(frag_of(kr[t][kk]), qf[kk], s[t]);
+      for (int kk = 0; kk < KK; ++kk) {
+        if constexpr (!WHOLE) keep8(kr[t][kk], dim - kk * 32 - quad * 8);
+        s[t] = mma16(frag_of(kr[t][kk]), qf[kk], s[t]);
+      }
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int cc = lane + i * 64;

@@ -246,3 +246,37 @@ def test_empty_tensors(tq, tk, b):
     assert o.shape == q.shape and (o == 0).all()
     for g, t in zip(torch.autograd.grad(o.sum(), (q, k, v)), (q, k, v)):
         assert g.shape == t.shape and (g == 0).all()
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("shape", [(2, 2, 1, 70, 130, 7), (1, 2, 2, 33, 65, 21), (1, 2, 1, 140, 200, 69),
+                                   (2, 2, 2, 66, 64, 102), (2, 4, 2, 1, 150, 43), (1, 2, 1, 3, 70, 86)])
+@pytest.mark.parametrize("gap", [1, 9])
+def test_nothing_beside_a_row_counts(dtype, shape, gap):
+    """Head sizes that fill no eight values, in rows `gap` values apart that hold NaN, as does all around the
+    tensor: the results are those of the tensors alone."""
+    b, h, hk, tq, tk, d = shape
+    clean = [t.cuda() for t in make(*shape, DT[dtype], 5)]
+
+    def hidden(t):
+        room = torch.full((t.shape[0], t.shape[1] + 2, t.shape[2] + 2, d + gap), float("nan"), dtype=t.dtype, device="cuda")
+        view = room[:, 1:-1, 1:-1, :d]
+        view.copy_(t)
+        return view
+
+    def step(q, k, v, do):
+        out, lse = layer_ops.attention_forward(q, k, v, True, None, None, None, True)
+        return out, *layer_ops.attention_backward(q, k, v, out, lse, do, True, None, None, None)
+
+    for want, got in zip(step(*clean), step(*map(hidden, clean))):
+        assert torch.isfinite(got).all() and torch.equal(want, got)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("shape", [(1, 2, 1, 40, 1500, 32), (2, 3, 1, 65, 1030, 64), (1, 1, 1, 129, 2100, 100)])
+@pytest.mark.parametrize("lengths,causal", [(False, True), (True, True), (True, False)])
+def test_few_queries_over_many_keys(dtype, shape, lengths, causal):
+    """Both passes of the backward in ranges, of which some hold no key."""
+    b, h, hk, tq, tk, d = shape
+    q, k, v, do = make(*shape, DT[dtype], sum(shape))
+    run(q, k, v, do, DT[dtype], causal=causal, lengths=[tk // 3, 0][:b] if lengths else None)
