@@ -89,6 +89,11 @@ int lwl_gelu8_backward(const int8_t* codes, const float* scales, const void* gra
  * consecutive values along dim; any order, sharing (stride 0 of an input) and alignment of an element.
  * dim is 1 .. LWL_ATTENTION_MAX_DIM, heads a multiple of kv_heads, scale positive and finite.  lse
  * (float32 [batch][heads][queries], contiguous) may be NULL in the forward.
+ *
+ * Not finite: a NaN in a key or value that some query may see reaches that query's results, and may reach
+ * those of other queries whose `causal` limit hides it (its probability 0 is multiplied by it), as
+ * it does where a masked score matrix is multiplied out.  float32 tensors that hold infinities give NaN:
+ * their products are those of bfloat16 parts.
  */
 #define LWL_ATTENTION_MAX_DIM 128
 typedef struct lwl_attention_args {
@@ -111,7 +116,8 @@ int lwl_attention_check(const lwl_attention_args* args); /* host only; does not 
 size_t lwl_attention_forward_workspace_size(const lwl_attention_args* args);
 int lwl_attention_forward(const lwl_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);
 /* The probabilities are computed again from q, k and lse.  grad_k and grad_v are summed over the query
- * heads that share a key head; all three gradients are overwritten whole (zeros where nothing reaches). */
+ * heads that share a key head; all three gradients are overwritten whole (zeros where nothing reaches).
+ * float32 divides each row of probabilities by its sum, so that lse's rounding does not count. */
 size_t lwl_attention_backward_workspace_size(const lwl_attention_args* args);
 int lwl_attention_backward(const lwl_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);
 

@@ -32,7 +32,10 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
     ``[batch, heads, queries, head size]`` and lies token by token in memory, so that
     ``out.transpose(1, 2).reshape(batch, queries, -1)`` copies nothing.  Softmax and sums are float32; in 16-bit
     types the probabilities are rounded to the type before the product with v.  Differentiable in q, k
-    and v (once)."""
+    and v (once).
+
+    A NaN in a key or value that some query sees may also reach queries from which ``causal`` hides it, as where
+    a masked score matrix is multiplied out; float32 infinities in k, q or v give NaN."""
     return N.layers().attention(q, k, v, causal, scale, key_lengths, causal_offset)
 
 

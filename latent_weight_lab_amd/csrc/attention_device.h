@@ -23,7 +23,8 @@ using Frag = typename Vec8<T>::type;
 // as a sum of three bfloat16 ones, x = x0 + x1 + x2, each the rounding of what the ones before leave: 24
 // bits, of float32's range.  Of the nine products of two such sums the six largest are taken; the others
 // are below 2^-24 of x y, and the sum is float32 as ever.  Six bfloat16 instructions take 192 cycles
-// where float32's own, of depth 2, take 512 for the same k (1 x 4 x 512 training step: 161 us with those).
+// where float32's own, of depth 2, take 512 for the same k (4 x 512 x 12 x 64 training step: 161 us with
+// those, 108 with these).  An infinite float32 value leaves NaN (infinity less infinity).
 template <class T>
 struct MatrixType {
   using Elem = T;

@@ -22,6 +22,13 @@
 // kSlack) = 2^14, the accumulators are rarely rescaled, and of float16's range the upper part is used, so
 // that a probability 2^-20 of the largest keeps its digits.  The first value is -FLT_MAX, not -infinity, so
 // that a row with no allowed key sums zeros: exp2(-inf + FLT_MAX) is 0 and nothing is NaN.
+//
+// Measured on MI355X: prompts are bound by the matrix cores and by what stands between their instructions, the
+// exponentials (a quarter of the vector rate) and LDS reads: bfloat16 1 x 8192 x 16 on 4 x 128, causal, 297 us, 925
+// TFLOP/s of the pairs needed, where a library product of 8192^3 runs at 1030; 8 x 1024 x 12 x 64 23 us, 560 TFLOP/s,
+// two rounds of walks of unequal lengths.  Float32 4 x 512 x 12 x 64 22.6 us and 5.7 for the join.  Tokens are bound
+// by memory: bfloat16 64 sequences of up to 1024 tokens x 12 x 64 19.4 us (101 MB, 5.2 TB/s); float16 2 x 65536 x 4 x
+// 128 42.6 us (268 MB, 6.3 TB/s) and 4.7 for the join.
 #include <algorithm>
 #include <cfloat>
 

@@ -81,7 +81,7 @@ struct AttnArgs {
   int64_t dos[3], dqs[3], dks[3], dvs[3];
   float* work;
   // filled in by the launchers
-  int splits;         // ranges of keys that different workgroups take (forward)
+  int splits;         // ranges of what is walked over that different workgroups take
   int64_t split_len;  // keys of a range
   int cus;            // compute units
 };

@@ -577,10 +577,6 @@ PYBIND11_MODULE(lwl_layers, m) {
   using release = py::call_guard<py::gil_scoped_release>;
   m.def("bind", &bind);
   m.def("layer_norm", &layer_norm, release());
-  m.def("norm_forward", [](const Tensor& x, const Tensor& w, const MaybeTensor& b, double eps, const MaybeTensor& r) {
-    const Normed n = norm_forward(x, w, b, eps, r, true);
-    return std::make_tuple(n.out, kept(n.sum), n.stats);
-  }, release());
   m.def("gelu8", &gelu8, release());
   m.def("gelu8_activation", &gelu8_activation, release());
   m.def("gelu8_backward", &gelu8_backward, release());

@@ -14,7 +14,6 @@ import torch
 from . import _native as N
 
 GELU8_GROUP = 128
-ATTENTION_MAX_DIM = 128
 
 _Strides = ctypes.c_int64 * 3
 
