@@ -49,9 +49,13 @@ constexpr bool kFoldStats = sizeof(T) == 2;
 // Head sizes up to 96 leave registers for two waves a SIMD, which overlap; 128 of a 16-bit type runs one, whose
 // two halves of a tile the scheduler may interleave.
 template <class T, int DP>
-constexpr int kUnroll = sizeof(T) == 2 && DP > 64 ? 2 : 1;
+constexpr int kUnroll = sizeof(T) == 2 && DP > 96 ? 2 : 1;
 template <class T, int DP>
-constexpr int kKeysOccupancy = sizeof(T) == 2 && DP <= 64 ? 2 : 1;
+constexpr int kKeysOccupancy = sizeof(T) == 2 && DP <= 96 ? 2 : 1;
+// The key pass loads a product's operands from LDS just before it, where all of them ahead would not fit the
+// registers.  At 96 that makes room for the second wave: bfloat16 4 x 2048 x 16 x 96, causal, 195 -> 153 us.
+template <class T, int DP>
+constexpr bool kLoadLate = sizeof(T) == 4 || DP == 96;
 
 // float32 keeps of every query, beside D, the factor that makes its probabilities sum to 1.  lse is one rounded
 // number, so exp2(s - lse) is off by the same 2^-24 |lse| for a whole row, more than all else here together; the
@@ -167,7 +171,7 @@ __global__ __launch_bounds__(256, (kKeysOccupancy<T, DP>)) void attention_bwd_ke
           }
           const auto load_q = [&](int kk) { qf[kk] = lds_operand<T>(lq + Tile::at(lane & 31, kk * 16 + half * 8), PL); };
           const auto load_g = [&](int kk) { gf[kk] = lds_operand<T>(lg + Tile::at(lane & 31, kk * 16 + half * 8), PL); };
-          if constexpr (sizeof(T) == 4) {
+          if constexpr (kLoadLate<T, DP>) {
 #pragma unroll
             for (int kk = 0; kk < KK; ++kk) {
               load_q(kk);
@@ -175,22 +179,18 @@ __global__ __launch_bounds__(256, (kKeysOccupancy<T, DP>)) void attention_bwd_ke
               s = mma32(qf[kk], kf[kk], s);
               dp = mma32(gf[kk], vf[kk], dp);
               fence_operands<T>();
+              if (kk % 2) fence_schedule<T>();  // two steps' operands at a time
             }
           } else {
 #pragma unroll
-            for (int kk = 0; kk < KK; ++kk) load_q(kk);
-            // 96: the two products one after the other, which holds half as many operands at a time
-            if constexpr (DP == 96) {
-              fence_schedule<T>();
-#pragma unroll
-              for (int kk = 0; kk < KK; ++kk) s = mma32(qf[kk], kf[kk], s);
+            for (int kk = 0; kk < KK; ++kk) {
+              load_q(kk);
+              load_g(kk);
             }
-#pragma unroll
-            for (int kk = 0; kk < KK; ++kk) load_g(kk);
-            if constexpr (DP <= 96) fence_schedule<T>();
+            if constexpr (DP <= 64) fence_schedule<T>();
 #pragma unroll
             for (int kk = 0; kk < KK; ++kk) {
-              if constexpr (DP != 96) s = mma32(qf[kk], kf[kk], s);
+              s = mma32(qf[kk], kf[kk], s);
               dp = mma32(gf[kk], vf[kk], dp);
             }
           }
@@ -201,7 +201,7 @@ __global__ __launch_bounds__(256, (kKeysOccupancy<T, DP>)) void attention_bwd_ke
           gc[u][d] = lds_column_operand<T, Tile>(lg, PL, row, row + 8, d * 32 + (lane & 16));
           qc[u][d] = lds_column_operand<T, Tile>(lq, PL, row, row + 8, d * 32 + (lane & 16));
         };
-        if constexpr (sizeof(T) == 2) {
+        if constexpr (!kLoadLate<T, DP>) {
 #pragma unroll
           for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -237,7 +237,7 @@ __global__ __launch_bounds__(256, (kKeysOccupancy<T, DP>)) void attention_bwd_ke
           const Opd<T> p = operand_of<T>(e), ds = operand_of<T>(f);
 #pragma unroll
           for (int d = 0; d < DT; ++d) {
-            if constexpr (sizeof(T) == 4) load_columns(u, d);
+            if constexpr (kLoadLate<T, DP>) load_columns(u, d);
             dv[d] = mma32(gc[u][d], p, dv[d]);
             dk[d] = mma32(qc[u][d], ds, dk[d]);
             fence_operands<T>();
@@ -252,7 +252,8 @@ __global__ __launch_bounds__(256, (kKeysOccupancy<T, DP>)) void attention_bwd_ke
   }
   if (key >= (int)a.keys) return;
   const float dk_scale = kLowerLate<T> ? a.scale * kLower : a.scale;
-  if (splits > 1) {  // summed by attention_bwd_join
+  if (splits > 1) {  // summed by attention_bwd_join, which takes keys that no query sees for zeros
+    if (key >= seen) return;
     const int64_t kv_rows = a.batch * a.kv_heads * a.keys, row = (b * a.kv_heads + hk) * a.keys + key;
     float* part = partials(a) + (split * kv_rows + row) * 2 * dim;
     store_result<float, DP, FAST>(part, dk, dk_scale, dim);
@@ -496,8 +497,9 @@ __global__ __launch_bounds__(256) void attention_bwd_join(const AttnArgs a) {
   const int64_t kv_rows = a.batch * a.kv_heads * a.keys, row = (int64_t)bk * keys + key, b = bk / kvh, hk = bk % kvh;
   const float* part = partials(a) + row * 2 * dim + (is_v ? dim : 0) + col;
   float sum[8] = {};
+  const int splits = (int)key < key_end(allowed_keys(a, b), (int)a.queries - 1) ? a.splits : 0;
 #pragma unroll 4
-  for (int s = 0; s < a.splits; ++s) {
+  for (int s = 0; s < splits; ++s) {
     float v[8];
     load8(v, part + s * kv_rows * 2 * dim, dim - col);
 #pragma unroll
@@ -587,29 +589,31 @@ hipError_t run_dim(const AttnArgs& a, hipStream_t s) {
 
 // Ranges of a key block's queries (all query heads that share the key head in one sequence): what an estimate
 // of the time makes shortest, in us, as in the forward pass: the longest walk alone, or all work spread over
-// the compute units, in whole rounds where the works are equal; and with several ranges the join.
+// the compute units, in rounds where the works are equal; and with several ranges the join.
 // Measured on MI355X, a tile of 64 queries: bfloat16 of head size 64 1.2 us when a compute unit has two
 // workgroups and 1.6 alone, of size 128 2.8 us (one fits); float32 of size 64 6.8 us; and what a workgroup
 // takes before its first tile and for its results, 7 and 10 us at size 64.  Of 1, 2, 3, 4 ranges, with the join:
 // 4 x 512 x 12 x 64 in float32 60.9, 51.1, 59.1, 61.2 us, 2 are taken; float16 6 x 515 queries over up to 1531 keys,
-// 12 heads on 4, of size 80: 63.1, 80.9, 87.6, 91.7 us, 1 is taken; bfloat16 8 x 1024 x 12 x 64: 47 us and up from 85, 1.
+// 12 heads on 4, of size 80: 70.4, 63.3, 77.7, 74.3 us, 2; bfloat16 8 x 1024 x 12 x 64: 47 us and up from 85, 1.
 static void plan_bwd_splits(AttnArgs& a) {
   const double unit = (double)((a.dim + 31) / 32 * 32) / 64, cus = (double)device_cus();
-  const double spread = (a.dtype == kF32 ? 6.8 : a.dim <= 64 ? 1.2 : 1.4) * unit;
-  const double alone = (a.dtype == kF32 ? 6.8 : a.dim <= 64 ? 1.6 : 1.4) * unit;
-  const double fixed = (a.dtype == kF32 ? 10.0 : 7.0) * unit;
+  const bool two = a.dtype != kF32 && a.dim <= 96;  // workgroups on a compute unit
+  const double spread = (a.dtype == kF32 ? 6.8 : two ? 1.2 : 1.4) * unit;
+  const double alone = (a.dtype == kF32 ? 6.8 : two ? 1.6 : 1.4) * unit;
+  const double fixed = (a.dtype == kF32 ? 10.0 : 7.0) * unit, slots = two ? 2 * cus : cus;
   const int64_t tiles = a.heads / a.kv_heads * ((a.queries + kTile - 1) / kTile);
-  // with lengths, which only the device knows, about half of the blocks hold keys
-  const double wgs = (double)(a.batch * a.kv_heads) * (double)((a.keys + kBlock - 1) / kBlock) * (a.lengths ? 0.55 : 1.0);
+  // with lengths, which only the device knows, about half of the blocks hold keys; the others take a little
+  const double wgs = (double)(a.batch * a.kv_heads) * (double)((a.keys + kBlock - 1) / kBlock) * (a.lengths ? 0.7 : 1.0);
   const bool halves = a.causal && a.keys * 2 > a.queries;
   const double bytes = 16.0 * (double)(a.batch * a.kv_heads) * (double)a.keys * (double)a.dim;
   double best = 0.0;
   a.splits = 1;
   for (int64_t n = 1; n <= std::min<int64_t>(tiles / 4 + 1, 256); n = n < 4 ? n + 1 : n + n / 4) {
-    const double walk = (double)((tiles + n - 1) / n);
-    const double slots = a.dtype != kF32 && a.dim <= 64 ? 2 * cus : cus, rounds = std::ceil(wgs * (double)n / slots);
-    const double all = halves ? 0.55 * wgs * (double)tiles / cus * spread + wgs * (double)n / slots * fixed
-                              : rounds * (walk * spread * slots / cus + fixed);
+    const double walk = (double)((tiles + n - 1) / n), works = wgs * (double)n;
+    const double whole = std::floor(works / slots), rest = works - whole * slots;
+    const double round = walk * spread * slots / cus + fixed;
+    const double all = halves ? 0.55 * wgs * (double)tiles / cus * spread + works / slots * fixed
+                              : whole * round + (rest > cus ? round : rest > 0.0 ? walk * alone + fixed : 0.0);
     const double t = std::max(walk * alone + fixed, all) + (n > 1 ? 4.0 + (double)n * bytes / 11e6 : 0.0);
     if (n == 1 || t < best) {
       best = t;
