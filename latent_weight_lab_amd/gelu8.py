@@ -54,15 +54,18 @@ def gelu_linear_checkpoint8(x: torch.Tensor, linear: nn.Module, bias: torch.Tens
 
     What ``linear`` (a ``BlockFHTLinear``, cached or not, or any other module) saves of its input for the
     backward pass is replaced by the checkpoint and computed again from it there; the weight's (or
-    latent's) gradient is then that of the checkpoint's activation."""
+    latent's) gradient is then that of the checkpoint's activation.  What it saves of its input after
+    changing it in place (a dropout with ``inplace=True``, say) is kept as it is.
+    """
     if not torch.is_grad_enabled():
         return linear(gelu_checkpoint8(x, bias, approximate))
     y, checkpoint = gelu_checkpoint8(x, bias, approximate, return_checkpoint=True)
-    span = (y.data_ptr(), y.numel(), y.dtype)
+    span = (y.data_ptr(), y.numel(), y.dtype, y._version)
 
     def pack(t):
-        # the activation itself or a dense view of all of it (flattened rows)
-        if t.is_cuda and (t.data_ptr(), t.numel(), t.dtype) == span and t.is_contiguous() and t.numel():
+        # the activation itself or a dense view of all of it (flattened rows), not written to since: views
+        # count their base's changes
+        if t.is_cuda and (t.data_ptr(), t.numel(), t.dtype, t._version) == span and t.is_contiguous() and t.numel():
             return tuple(t.shape)
         return t
 

@@ -175,3 +175,23 @@ def test_refusals():
                 lambda: gelu_checkpoint8(x, approximate="sigmoid"), lambda: gelu_checkpoint8(x[:, :0])):
         with pytest.raises((RuntimeError, ValueError)):
             bad()
+
+
+@pytest.mark.parametrize("cached", [False, True])
+@pytest.mark.parametrize("first", [torch.nn.Hardtanh, torch.nn.ReLU])
+def test_module_that_changes_its_input_in_place(cached, first):
+    """The gradients are those of the input that the linear saw, bit for bit.  Not in place, the linear's input is
+    a tensor of its own and kept; what the first module saves may be the activation and stand for the checkpoint's."""
+    torch.manual_seed(0)
+    lin = BlockFHTLinear(256, 96, latent_dim=512, seed=4).cuda()
+    x = torch.randn(2, 50, 256, device="cuda", requires_grad=True)
+    dy = torch.randn(2, 50, 96, device="cuda")
+    if cached:
+        prepare_block_fht_weight_cache(lin)
+    p = lin._cached_weight if cached else lin.generator.latent
+    apart = first()(gelu_checkpoint8(x))
+    want = torch.autograd.grad(lin(apart), (p, x), dy)
+    got = torch.autograd.grad(gelu_linear_checkpoint8(x, torch.nn.Sequential(first(inplace=True), lin)), (p, x), dy)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    got = torch.autograd.grad(gelu_linear_checkpoint8(x, torch.nn.Sequential(first(), lin)), p, dy)
+    assert torch.equal(got[0], want[0])
