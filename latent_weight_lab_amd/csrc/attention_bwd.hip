@@ -37,10 +37,17 @@ constexpr int kMostQuerySplits = 64;
 // a key's probabilities over the queries, all of which may be small, and small ones are subnormal in
 // float16 and flushed by the exponential in float32.
 constexpr float kLift = 14.0f, kLower = 0x1p-14f;
-// dS made of them is taken back before it is rounded to float16, whose range it could leave, and with dK
-// at the end otherwise.
+// float16 holds the dS of a key times a power of two, `held`, that puts the largest met so far at 2^kHeldTop or
+// more: unscaled, probabilities of long rows times small dout are subnormal or zero (relative error of dK,
+// 2048 queries over 4096 keys, dout of 1e-4: 5.3e-2; 4.7e-3 so, which is dK's own rounding), and dS of large
+// dout is infinite where dK fits.  As with the forward's maximum, a key is a lane's column: the sums are
+// rescaled when a score's gradient leaves the range, and what leaves it at the bottom is 2^-36 of the largest.
+// Until the first, 2^kHeldStart; the power is taken back with dK's scale.
 template <class T>
-constexpr bool kLowerLate = !__is_same(T, f16);
+constexpr bool kHold = __is_same(T, f16);
+constexpr int kHeldStart = 60, kHeldTop = 12;
+constexpr float kMostF16 = 65504.0f;
+__device__ __forceinline__ int exponent_bits(float v) { return (int)(__float_as_uint(v) >> 23) & 0xff; }
 // 16-bit products start from what is to be subtracted of them, S - lse / c with c = scale log2(e), and dP - D,
 // which saves an operation a score.  Their sums then round at the size of lse / c: not for float32.
 template <class T>
@@ -96,6 +103,7 @@ __global__ __launch_bounds__(256, (kKeysOccupancy<T, DP>)) void attention_bwd_ke
   load_operand<T, DP, FAST>(kf, (const T*)a.k + b * a.ks[0] + hk * a.ks[1] + (int64_t)key * a.ks[2], dim, key < seen);
   load_operand<T, DP, FAST>(vf, (const T*)a.v + b * a.vs[0] + hk * a.vs[1] + (int64_t)key * a.vs[2], dim, key < seen);
   f32x16 dk[DT] = {}, dv[DT] = {};
+  float held = __builtin_ldexpf(1.0f, kHeldStart);
   const float c = a.scale * kLog2E, inv_c = 1.0f / c;
   // queries before k0 - off see none of the block's keys (so none that sees nothing is ever read), those
   // before wk0 - off none of the wave's
@@ -217,7 +225,7 @@ __global__ __launch_bounds__(256, (kKeysOccupancy<T, DP>)) void attention_bwd_ke
             s[r] = exp2_hw(fmaf(s[r], c, lds_stat[buf][0][i])) * lds_stat[buf][kStats - 1][i];
             dp[r] += lds_stat[buf][1][i];
           }
-          dp[r] = s[r] * (kLowerLate<T> ? dp[r] : dp[r] * kLower);
+          dp[r] *= s[r];
         }
         if (masked) {
           // key < key_end(q), that is q >= key - off
@@ -225,6 +233,25 @@ __global__ __launch_bounds__(256, (kKeysOccupancy<T, DP>)) void attention_bwd_ke
 #pragma unroll
           for (int r = 0; r < 16; ++r)
             if ((r >> 2) * 8 + (r & 3) < from) s[r] = dp[r] = 0.0f;
+        }
+        if constexpr (kHold<T>) {
+          float most = 0.0f;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(dp[r]));
+          if (__any(most * held > kMostF16)) {
+            most = max_halves(most);
+            if (most * held > kMostF16) {
+              const float next = __uint_as_float((uint32_t)(254 + kHeldTop - exponent_bits(most)) << 23);
+              const int shrink = exponent_bits(next) - exponent_bits(held);
+              held = next;
+#pragma unroll
+              for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) dk[d][r] = __builtin_ldexpf(dk[d][r], shrink);
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < 16; ++r) dp[r] *= held;
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -251,7 +278,7 @@ __global__ __launch_bounds__(256, (kKeysOccupancy<T, DP>)) void attention_bwd_ke
     q0 = next_q;
   }
   if (key >= (int)a.keys) return;
-  const float dk_scale = kLowerLate<T> ? a.scale * kLower : a.scale;
+  const float dk_scale = kHold<T> ? __builtin_ldexpf(a.scale * kLower, 127 - exponent_bits(held)) : a.scale * kLower;
   if (splits > 1) {  // summed by attention_bwd_join, which takes keys that no query sees for zeros
     if (key >= seen) return;
     const int64_t kv_rows = a.batch * a.kv_heads * a.keys, row = (b * a.kv_heads + hk) * a.keys + key;

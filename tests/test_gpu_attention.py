@@ -280,3 +280,32 @@ def test_few_queries_over_many_keys(dtype, shape, lengths, causal):
     b, h, hk, tq, tk, d = shape
     q, k, v, do = make(*shape, DT[dtype], sum(shape))
     run(q, k, v, do, DT[dtype], causal=causal, lengths=[tk // 3, 0][:b] if lengths else None)
+
+
+@pytest.mark.parametrize("std", [1.0, 1e-3, 1e-4])
+@pytest.mark.parametrize("shape", [(1, 4, 1, 2048, 4096, 64), (1, 2, 2, 1100, 3000, 128), (1, 2, 2, 1500, 2000, 80)])
+def test_float16_gradients_of_small_dout(shape, std):
+    """Long rows times small gradients, where probability times gradient is below float16's normal range.
+
+    In the L2 norm the gradients are off by their own rounding, which is what the exact ones rounded are off by, and by
+    the relative error of their terms: a rounding (2^-11) each of P or dS, of out inside D and of the product's
+    start, doubled for the float32 steps between."""
+    q, k, v, do = make(*shape, torch.float16, 3)
+    do = (do.float() * std).half()
+    d = shape[-1]
+    res = R.attention(q, k, v, d ** -0.5, torch.ones(1, *shape[3:5], dtype=torch.bool), do)
+    leaves = [t.cuda().requires_grad_() for t in (q, k, v)]
+    for name, g in zip(("dq", "dk", "dv"), torch.autograd.grad(attention(*leaves), leaves, do.cuda())):
+        want = res[name]
+        off, least = (g.double().cpu() - want).norm(), (want.half().double() - want).norm()
+        assert off <= least + 6 * R.U[torch.float16] * want.norm(), (name, (off / want.norm()).item())
+
+
+def test_float16_gradients_of_large_dout():
+    """Gradients of scores past float16's range, of which those of q, k and v are well inside."""
+    q, k, v, do = make(1, 2, 1, 200, 3, 64, torch.float16, 3)
+    q, k, v, do = (0.05 * q).half(), (0.05 * k).half(), (4 * v).half(), (1000 * do).half()
+    do[:, :, 100:] *= 4  # later tiles larger: the sums are rescaled
+    ds = (do.double() @ v.double().transpose(2, 3).repeat_interleave(2, 1)) / 3
+    assert ds.abs().max() > 65504
+    run(q, k, v, do, torch.float16)
