@@ -343,7 +343,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_bwd_que
   delta += other_half(delta);
   // float16 scores' gradients are held 2^-e times as large, 2^e about the length of this query's row of dout: they
   // are then not subnormal where gradients are small, and |dS| <= 4 max |v| (lengths again).  It costs nothing:
-  // the power goes into lse and back out with dQ's scale.
+  // the power goes into lse and back out with dQ's scale.  Where values longer than 16000 take them past
+  // float16's range all the same, the power is raised and what is summed so far taken down.
   float unscale = a.scale;
   if constexpr (__is_same(T, f16)) {
     norm += other_half(norm);
@@ -442,6 +443,23 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_bwd_que
             s[r] *= dp[r] - delta;
           }
           total += sum;
+        }
+        if constexpr (kHold<T>) {
+          float most = 0.0f;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(s[r]));
+          if (__any(most > kMostF16)) {
+            most = max_halves(most);
+            const int n = most > kMostF16 ? exponent_bits(most) - 127 - kHeldTop : 0;
+            lse += (float)n;
+            unscale = __builtin_ldexpf(unscale, n);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = __builtin_ldexpf(s[r], -n);
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+              for (int r = 0; r < 16; ++r) dq[d][r] = __builtin_ldexpf(dq[d][r], -n);
+          }
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {

@@ -309,3 +309,17 @@ def test_float16_gradients_of_large_dout():
     ds = (do.double() @ v.double().transpose(2, 3).repeat_interleave(2, 1)) / 3
     assert ds.abs().max() > 65504
     run(q, k, v, do, torch.float16)
+
+
+def test_float16_gradients_of_large_values():
+    """Values whose rows are longer than float16's range, upstream gradients along them: the scores' gradients over
+    the length of dout's row leave it too, and dQ does not."""
+    q, k, _, _ = make(1, 1, 1, 70, 2, 64, torch.float16, 4)
+    v = (20000 * torch.sign(make(1, 1, 1, 2, 2, 64, torch.float16, 5)[1])).half()
+    v[:, :, 1] = -v[:, :, 0]
+    do = (1e-6 * v[:, :, :1]).expand(-1, -1, 70, -1).clone()
+    for tk in (2, 130):  # the second: in a later tile, beside small ones
+        kk, vv = torch.zeros(1, 1, tk, 64).half(), torch.zeros(1, 1, tk, 64).half()
+        kk[:, :, -2:], vv[:, :, -2:] = k, v
+        vv[:, :, :-2] = 1.0
+        run(q, kk, vv, do, torch.float16, scale=0.01)
