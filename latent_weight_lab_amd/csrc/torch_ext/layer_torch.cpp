@@ -75,10 +75,13 @@ int dtype_code(at::ScalarType t) {
   }
 }
 
-// Every tensor on one GPU.
+// Every tensor on one GPU, none with a forward-mode tangent: outputs are filled through pointers and would have
+// none, which is a derivative of zero (and holds without gradient recording too, which does not end this mode).
 void on_one_gpu(const Tensor& first) {
   if (!first.is_cuda())
     throw std::runtime_error("latent_weight_lab_amd runs on the GPU only; move the inputs to a cuda device");
+  TORCH_CHECK_NOT_IMPLEMENTED(!first._fw_grad(/*level=*/0).defined(),
+                              "latent_weight_lab_amd: the layer operators have no forward-mode derivatives");
 }
 template <class... Rest>
 void on_one_gpu(const Tensor& first, const Rest&... rest) {
@@ -511,6 +514,7 @@ struct PackedFn : torch::autograd::Function<PackedFn> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto s = ctx->get_saved_variables();
     const Tensor &qkv = s[0], &out = s[1], &lse = s[2];
+    on_one_gpu(qkv, grads[0]);
     const int64_t heads = ctx->saved_data["heads"].toInt(), kv_heads = ctx->saved_data["kv_heads"].toInt();
     lwl_attention_args a = packed_args(qkv, heads, kv_heads, kept_how(ctx));
     const c10::DeviceGuard guard(qkv.device());
@@ -572,6 +576,8 @@ PYBIND11_MODULE(lwl_layers, m) {
       if (p) std::rethrow_exception(p);
     } catch (const ArgumentError& e) {
       PyErr_SetString(argument_error ? argument_error : PyExc_ValueError, e.what());
+    } catch (const c10::NotImplementedError& e) {
+      PyErr_SetString(PyExc_NotImplementedError, e.what_without_backtrace());
     }
   });
   using release = py::call_guard<py::gil_scoped_release>;
