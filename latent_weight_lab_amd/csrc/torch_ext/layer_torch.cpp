@@ -170,13 +170,18 @@ Normed norm_forward(const Tensor& x0, const Tensor& weight0, const MaybeTensor& 
   return r;
 }
 
-std::tuple<Tensor, Tensor, Tensor> norm_backward(const Tensor& h, const Tensor& weight0, const Tensor& stats,
+std::tuple<Tensor, Tensor, Tensor> norm_backward(const Tensor& h0, const Tensor& weight0, const Tensor& stats,
                                                  const Tensor& grad_out0, const MaybeTensor& grad_sum0, bool need_x,
                                                  bool need_weight, bool need_bias) {
-  on_one_gpu(h, weight0, stats, grad_out0, grad_sum0);
-  const int64_t f = features_of("layer norm", h), rows = h.numel() / f;
-  const c10::DeviceGuard guard(h.device());
-  const Tensor weight = weight0.contiguous(), grad_out = typed(grad_out0, h.scalar_type()).contiguous();
+  on_one_gpu(h0, weight0, stats, grad_out0, grad_sum0);
+  const int64_t f = features_of("layer norm", h0), rows = h0.numel() / f;
+  // saved tensors come back as a caller's hooks left them
+  if (stats.scalar_type() != at::kFloat || !stats.is_contiguous() || stats.sizes() != at::IntArrayRef({2, rows}) ||
+      weight0.numel() != f)
+    refuse("layer norm backward: statistics ", stats.sizes(), " of ", stats.scalar_type(), " and weight ", weight0.sizes(),
+           " are not those of ", h0.sizes());
+  const c10::DeviceGuard guard(h0.device());
+  const Tensor h = h0.contiguous(), weight = weight0.contiguous(), grad_out = typed(grad_out0, h.scalar_type()).contiguous();
   MaybeTensor grad_sum;
   if (grad_sum0) grad_sum = typed(*grad_sum0, h.scalar_type()).contiguous();
   Tensor gx, gw, gb;
@@ -244,18 +249,26 @@ std::tuple<Tensor, MaybeTensor, MaybeTensor> gelu8_forward(const Tensor& x0, con
   return {out, codes, scales};
 }
 
+// The kernels read both by these shapes alone.
+void hold_checkpoint(const Tensor& codes, const Tensor& scales, int64_t rows, int64_t f, at::IntArrayRef shape) {
+  const int64_t groups = (f + LWL_GELU8_GROUP - 1) / LWL_GELU8_GROUP;
+  if (codes.scalar_type() != at::kChar || scales.scalar_type() != at::kFloat || !codes.is_contiguous() ||
+      !scales.is_contiguous() || codes.sizes() != at::IntArrayRef({rows, lib.gelu8_pitch(f)}) ||
+      scales.sizes() != at::IntArrayRef({rows, groups}))
+    refuse("GELU checkpoint: codes ", codes.sizes(), " of ", codes.scalar_type(), " and scales ", scales.sizes(), " of ",
+           scales.scalar_type(), " do not hold ", shape, " as contiguous int8 rows of ", lib.gelu8_pitch(f),
+           " and float32 rows of ", groups);
+}
+
 Tensor gelu8_activation(const Tensor& codes, const Tensor& scales, std::vector<int64_t> shape, at::ScalarType dtype,
                         bool tanh_form) {
   on_one_gpu(codes, scales);
   const c10::DeviceGuard guard(codes.device());
-  const int64_t f = shape.empty() ? 0 : shape.back();
   const Tensor out = at::empty(shape, codes.options().dtype(dtype));
-  if (codes.dim() != 2 || scales.dim() != 2 || f <= 0 || out.numel() != codes.size(0) * f ||
-      codes.size(1) != lib.gelu8_pitch(f) || scales.size(0) != codes.size(0) ||
-      scales.size(1) != (f + LWL_GELU8_GROUP - 1) / LWL_GELU8_GROUP)
-    refuse("GELU checkpoint: codes ", codes.sizes(), " and scales ", scales.sizes(), " do not hold ", out.sizes());
+  const int64_t f = features_of("GELU checkpoint", out);
+  hold_checkpoint(codes, scales, out.numel() / f, f, out.sizes());
   check(lib.gelu8_activation((const int8_t*)codes.data_ptr(), (const float*)scales.data_ptr(), dtype_code(dtype), tanh_form,
-                             codes.size(0), f, out.data_ptr(), stream_of(codes)));
+                             out.numel() / f, f, out.data_ptr(), stream_of(codes)));
   return out;
 }
 
@@ -264,8 +277,7 @@ std::tuple<Tensor, MaybeTensor> gelu8_backward(const Tensor& codes, const Tensor
   on_one_gpu(codes, scales, grad_out0);
   const c10::DeviceGuard guard(codes.device());
   const int64_t f = features_of("GELU checkpoint", grad_out0), rows = grad_out0.numel() / f;
-  if (codes.dim() != 2 || codes.size(0) != rows || codes.size(1) != lib.gelu8_pitch(f))
-    refuse("GELU checkpoint: codes ", codes.sizes(), " do not hold ", grad_out0.sizes());
+  hold_checkpoint(codes, scales, rows, f, grad_out0.sizes());
   const Tensor grad_out = typed(grad_out0, dtype).contiguous(), gx = at::empty(grad_out.sizes(), grad_out.options());
   MaybeTensor gb;
   if (need_bias) gb = at::empty({f}, grad_out.options());
@@ -391,14 +403,24 @@ std::tuple<Tensor, MaybeTensor> attention_forward(const Tensor& q0, const Tensor
   return {out, lse};
 }
 
+// What the forward left for the backward: out like q (`shape`), lse float32 for each query of each head.
+void check_left(const lwl_attention_args& a, const Tensor& q, at::IntArrayRef shape, const Tensor& out, const Tensor& lse,
+                const Tensor& grad_out) {
+  if (out.sizes() != shape || grad_out.sizes() != shape || out.scalar_type() != q.scalar_type())
+    refuse("attention backward: out ", out.sizes(), " of ", out.scalar_type(), " and grad_out ", grad_out.sizes(),
+           " must be ", shape, ", out of ", q.scalar_type());
+  if (lse.scalar_type() != at::kFloat || !lse.is_contiguous() || lse.sizes() != at::IntArrayRef({a.batch, a.heads, a.queries}))
+    refuse("attention backward: lse must be contiguous float32 [", a.batch, ", ", a.heads, ", ", a.queries, "], got ",
+           lse.sizes(), " of ", lse.scalar_type());
+}
+
 std::tuple<Tensor, Tensor, Tensor> attention_backward(const Tensor& q0, const Tensor& k0, const Tensor& v0,
                                                       const Tensor& out, const Tensor& lse, const Tensor& grad_out0,
                                                       bool causal, std::optional<double> scale,
                                                       const MaybeTensor& lengths0, std::optional<int64_t> offset) {
   on_one_gpu(q0, k0, v0, out, lse, grad_out0, lengths0);
   lwl_attention_args a = heads_args(q0, k0, v0, {causal, scale, offset});
-  if (out.sizes() != q0.sizes() || grad_out0.sizes() != q0.sizes() || lse.numel() != a.batch * a.heads * a.queries)
-    refuse("attention backward: out ", out.sizes(), " and grad_out ", grad_out0.sizes(), " must be like q ", q0.sizes());
+  check_left(a, q0, q0.sizes(), out, lse, grad_out0);
   const c10::DeviceGuard guard(q0.device());
   const MaybeTensor lengths = lengths_of(lengths0, a.batch);
   const Tensor q = dense_dim(q0), k = dense_dim(k0), v = dense_dim(v0), o = dense_dim(out);
@@ -513,10 +535,11 @@ struct PackedFn : torch::autograd::Function<PackedFn> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto s = ctx->get_saved_variables();
-    const Tensor &qkv = s[0], &out = s[1], &lse = s[2];
-    on_one_gpu(qkv, grads[0]);
+    on_one_gpu(s[0], s[1], s[2], kept(s[3]), grads[0]);
+    const Tensor qkv = s[0].contiguous(), out = s[1].contiguous(), lse = s[2];
     const int64_t heads = ctx->saved_data["heads"].toInt(), kv_heads = ctx->saved_data["kv_heads"].toInt();
     lwl_attention_args a = packed_args(qkv, heads, kv_heads, kept_how(ctx));
+    check_left(a, qkv, {a.batch, a.queries, heads * a.dim}, out, lse, grads[0]);
     const c10::DeviceGuard guard(qkv.device());
     const MaybeTensor lengths = lengths_of(kept(s[3]), a.batch);
     const Tensor grad_out = typed(grads[0], qkv.scalar_type()).contiguous(), grad = at::empty(qkv.sizes(), qkv.options());

@@ -323,3 +323,32 @@ def test_float16_gradients_of_large_values():
         kk[:, :, -2:], vv[:, :, -2:] = k, v
         vv[:, :, :-2] = 1.0
         run(q, kk, vv, do, torch.float16, scale=0.01)
+
+
+def test_what_does_not_fit_the_forward_is_refused():
+    q, k, v, do = (t.cuda() for t in make(2, 4, 2, 9, 12, 32, torch.float16, 1))
+    out, lse = layer_ops.attention_forward(q, k, v, False, None, None, None, True)
+    back = lambda out, lse, do: layer_ops.attention_backward(q, k, v, out, lse, do, False, None, None, None)
+    back(out, lse, do)
+    back(out, lse, do.float())  # converted
+    for args in [(out, lse.half(), do), (out, lse.double(), do), (out, lse.view(-1), do), (out, lse[:, :2], do),
+                 (out, lse.transpose(0, 1), do), (out, torch.cat([lse, lse], 2)[:, :, ::2], do), (out.float(), lse, do),
+                 (out.bfloat16(), lse, do), (out[:, :, :8], lse, do), (out, lse, do[:1]), (out, lse.cpu(), do)]:
+        with pytest.raises(RuntimeError):
+            back(*args)
+
+
+def test_saved_tensors_in_another_layout_or_type():
+    """A caller's hooks may give saved tensors back in another layout, not in another type."""
+    x = torch.randn(2, 20, 3 * 64, device="cuda", requires_grad=True)
+    y = attention_packed(x, 2)
+    want = torch.autograd.grad(y.sum(), x)[0]
+    apart = lambda t: torch.stack([t, t], -1)[..., 0] if t.is_floating_point() else t
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: apart(t) if t.shape[-1] != 20 else t):
+        y = attention_packed(x, 2)
+    assert torch.equal(torch.autograd.grad(y.sum(), x)[0], want)
+    for change in (apart, torch.Tensor.half):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: change(t) if t.shape[-1] == 20 else t):
+            y = attention_packed(x, 2)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(y.sum(), x)

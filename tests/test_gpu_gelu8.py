@@ -195,3 +195,29 @@ def test_module_that_changes_its_input_in_place(cached, first):
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     got = torch.autograd.grad(gelu_linear_checkpoint8(x, torch.nn.Sequential(first(), lin)), p, dy)
     assert torch.equal(got[0], want[0])
+
+
+def test_checkpoints_that_do_not_fit_are_refused():
+    """Codes and scales of another shape, type or layout than the call's would be read out of range."""
+    x = torch.randn(40, 300, device="cuda")
+    _, kept = gelu_checkpoint8(x, return_checkpoint=True)
+    c, s = kept.codes, kept.scales
+    assert c.shape == (40, 304) and s.shape == (40, 3)
+    wide, tall = torch.zeros(40, 8, device="cuda"), torch.zeros(80, 304, dtype=torch.int8, device="cuda")
+    for codes, scales in [(c, s[:, :2]), (c, s[:, :2].contiguous()), (c, s[:39]), (c, s.half()), (c, s.double()), (c, wide[:, :3]),
+                          (c[:39], s), (c[:, :296].contiguous(), s), (c.float(), s), (c.to(torch.uint8), s), (tall[::2], s),
+                          (c.view(-1), s), (c, s.view(-1)), (c, s.t().contiguous().t()), (c.cpu(), s), (c, s.cpu())]:
+        with pytest.raises(RuntimeError):
+            layer_ops.gelu8_activation(codes, scales, (40, 300), x.dtype, "none")
+        with pytest.raises(RuntimeError):
+            layer_ops.gelu8_backward(codes, scales, x, x.dtype, "none", True)
+    for shape in [(40, 305), (41, 300), (40, 0), ()]:
+        with pytest.raises(RuntimeError):
+            layer_ops.gelu8_activation(c, s, shape, x.dtype, "none")
+        with pytest.raises(RuntimeError):
+            layer_ops.gelu8_backward(c, s, torch.ones(shape, device="cuda"), x.dtype, "none", True)
+    kept.scales = s.bfloat16()
+    with pytest.raises(ValueError):
+        kept.activation()
+    assert torch.equal(layer_ops.gelu8_activation(c, s, (2, 20, 300), x.dtype, "none").view(40, 300),
+                       layer_ops.gelu8_activation(c, s, (40, 300), x.dtype, "none"))

@@ -164,3 +164,19 @@ def test_module_and_refusals():
     with pytest.raises(RuntimeError):
         g.sum().backward()
     assert issubclass(N.BlockFHTArgumentError, ValueError)
+
+
+def test_saved_tensors_in_another_layout_or_type():
+    """A caller's hooks may give saved tensors back in another layout, statistics only as they were."""
+    x, w = torch.randn(30, 100, device="cuda", requires_grad=True), torch.randn(100, device="cuda", requires_grad=True)
+    dy = torch.randn(30, 100, device="cuda")
+    want = torch.autograd.grad(layer_norm(x, w), (x, w), dy)
+    apart = lambda t: torch.stack([t, t], -1)[..., 0]
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t if t.shape == (2, 30) else apart(t)):
+        y = layer_norm(x, w)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, (x, w), dy), want))
+    for change in (apart, torch.Tensor.half, lambda t: t[:, :29].contiguous()):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: change(t) if t.shape == (2, 30) else t):
+            y = layer_norm(x, w)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(y, (x, w), dy)
