@@ -211,11 +211,10 @@ using Padded = Strided<DP + 8>;
 // Tiles of 64 rows that a workgroup of 256 threads brings from memory through registers into LDS: fetch()
 // starts the loads, put() stores what came.  Rows from `end` on and columns past the head size are zeros.
 //
-// FAST: head size, strides and addresses are multiples of 16 bytes and a tile spans less than 2 GiB.  A
+// FAST: the head size is a multiple of eight and fast_rows() holds of the tensor.  A
 // thread's byte offsets within a tile are then the same for every tile, the tile's address is scalar,
 // and the buffer's range check makes the zeros: no vector arithmetic for a tile.  Otherwise
 // load_ahead8 with 64-bit addresses for every row, and keep8 when it goes to LDS.
-constexpr int kTileRows = 64;
 
 // Eight values of a row of a tensor whose first n belong to it, without waiting for them: all eight are read where
 // that is in the tensor (`inside`: a row follows, and rows are at least eight values apart), and keep8 clears
@@ -307,12 +306,6 @@ struct TileLoader {
 // Tiles in LDS: two, one being read while the other is filled, where they fit.
 template <class T>
 constexpr int kBufs = sizeof(T) == 2 ? 2 : 1;
-// Whether a tensor's rows meet FAST's terms (the head size is checked beside it).
-inline bool fast_rows(const void* p, const int64_t (&stride)[3], int64_t size) {
-  const int64_t unit = 16 / size;
-  return (uintptr_t)p % 16 == 0 && stride[0] % unit == 0 && stride[1] % unit == 0 && stride[2] % unit == 0 &&
-         stride[2] * size * kTileRows < ((int64_t)1 << 31);
-}
 
 // A row of a tensor as operands: lane l holds chunks of eight values, 8 (l / 32) + 16 kk (32-wide products).
 // WHOLE: the head size is a multiple of eight.

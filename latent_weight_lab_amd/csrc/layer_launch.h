@@ -85,6 +85,15 @@ struct AttnArgs {
   int64_t split_len;  // keys of a range
   int cus;            // compute units
 };
+constexpr int kTileRows = 64;  // tokens of a tile
+// Whether a tensor of values of `size` bytes can be read in tiles by 32-bit offsets from a tile's first row:
+// addresses and strides are multiples of 16 bytes, rows lie in ascending order (the offsets are unsigned),
+// and a tile spans less than 2 GiB.
+inline bool fast_rows(const void* p, const int64_t (&stride)[3], int64_t size) {
+  const int64_t unit = 16 / size;
+  return (uintptr_t)p % 16 == 0 && stride[0] % unit == 0 && stride[1] % unit == 0 && stride[2] % unit == 0 &&
+         stride[2] >= 0 && stride[2] < ((int64_t)1 << 31) / (size * kTileRows);
+}
 // float32 values in the workspace
 int64_t attention_fwd_work(const AttnArgs& a);
 int64_t attention_bwd_work(const AttnArgs& a);

@@ -7,11 +7,14 @@ result's terms: |error| <= (2 u + gamma) T + u |result| forward, (4 u + 4 gamma)
 """
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
 import layer_oracle as R
 from conftest import gpu_available
+from latent_weight_lab_amd import _native as N
 from latent_weight_lab_amd import attention, attention_packed, layer_ops
 
 pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not gpu_available(), reason="needs a GPU")]
@@ -352,3 +355,38 @@ def test_saved_tensors_in_another_layout_or_type():
             y = attention_packed(x, 2)
         with pytest.raises(RuntimeError):
             torch.autograd.grad(y.sum(), x)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("tq,tk,d", [(1, 300, 64), (70, 150, 64), (70, 150, 61)])
+def test_rows_in_descending_order(dtype, tq, tk, d):
+    """Negative token strides (which the C entry takes and torch cannot make) give what ascending rows give."""
+    dt, dev = DT[dtype], "cuda"
+    q, k, v, do = (t.to(dev).contiguous() for t in make(2, 2, 1, tq, tk, d, dt, 7))
+    out, lse = layer_ops.attention_forward(q, k, v, True, None, None, None, True)
+    want = (out, *layer_ops.attention_backward(q, k, v, out, lse, do, True, None, None, None))
+    a = layer_ops.AttentionArgs()
+    a.dtype, a.causal, a.bottom_right = {"f32": 0, "f16": 1, "bf16": 2}[dtype], 1, 1
+    a.batch, a.heads, a.kv_heads, a.queries, a.keys, a.dim, a.scale = 2, 2, 1, tq, tk, d, d ** -0.5
+    held = []
+
+    def place(name, t):  # tokens from the last to the first
+        t = t.flip(2).contiguous()
+        held.append(t)
+        setattr(a, name, t.data_ptr() + (t.shape[2] - 1) * d * t.element_size())
+        getattr(a, name + "_stride")[:] = [t.stride(0), t.stride(1), -d]
+        return t
+
+    for name, t in (("q", q), ("k", k), ("v", v), ("grad_out", do)):
+        place(name, t)
+    outs = [place(name, torch.zeros_like(t)) for name, t in (("out", q), ("grad_q", q), ("grad_k", k), ("grad_v", k))]
+    log = torch.zeros(2, 2, tq, device=dev)
+    a.lse = log.data_ptr()
+    lib, stream = N.lib(), torch.cuda.current_stream().cuda_stream
+    for step in ("forward", "backward"):
+        size = getattr(lib, f"lwl_attention_{step}_workspace_size")(ctypes.byref(a))
+        ws = torch.empty(max(size, 1), dtype=torch.uint8, device=dev)
+        assert getattr(lib, f"lwl_attention_{step}")(ctypes.byref(a), ws.data_ptr(), size, stream) == 0
+    torch.cuda.synchronize()
+    for got, ref in zip(outs, want):
+        assert torch.allclose(got.flip(2).float(), ref.float(), rtol=0, atol=2 * R.U[dt] * float(ref.abs().max()))

@@ -134,3 +134,36 @@ def test_formulas_match_differences():
         val, slope = R.gelu(z, form)
         assert torch.allclose(central(lambda x: R.gelu(x, form)[0], z, torch.ones_like(z)), slope, atol=1e-8)
         assert torch.allclose(val, torch.nn.functional.gelu(z, approximate=form), atol=1e-12)
+
+
+def test_tiles_by_32_bit_offsets_only_where_they_reach(tmp_path):
+    """A tile's rows are read at unsigned 32-bit byte offsets from its first, inside a range of (rows - 1) * stride +
+    dim values: with descending rows offsets wrap, some of them into the range."""
+    from latent_weight_lab_amd.build import hipcc
+
+    strides = [s * m for s in (0, 8, 64, 120, 1 << 19, 1 << 23, (1 << 24) - 8, 1 << 24, 1 << 40, 1 << 57, 1 << 62)
+               for m in (1, -1)]
+    src = tmp_path / "t.cpp"
+    src.write_text(f'''#include <cstdio>
+#include "layer_launch.h"
+int main() {{
+  for (int64_t s : {{{", ".join(f"{s}LL" for s in strides)}}})
+    for (int64_t size : {{2, 4}}) {{
+      const int64_t stride[3] = {{0, 0, s}};
+      std::printf("%lld %lld %d\\n", (long long)s, (long long)size, lwl::fast_rows((void*)256, stride, size));
+    }}
+}}''')
+    rocm = Path(hipcc()).resolve().parents[1]
+    subprocess.run([str(rocm / "llvm" / "bin" / "clang++"), "-std=c++17", "-D__HIP_PLATFORM_AMD__",
+                    f"-I{ROOT / 'latent_weight_lab_amd' / 'csrc'}", f"-I{rocm / 'include'}", str(src), "-o",
+                    str(tmp_path / "t")], check=True)
+    out = subprocess.run([str(tmp_path / "t")], capture_output=True, text=True, check=True).stdout.split()
+    rows = [tuple(map(int, out[i:i + 3])) for i in range(0, len(out), 3)]
+    assert len(rows) == 2 * len(strides)
+    for stride, size, fast in rows:
+        # every offset is the distance itself, and below the range that the hardware checks it against
+        reach = [row * stride * size for row in range(64)]
+        sound = all(0 <= r <= 63 * stride * size < 1 << 31 for r in reach)
+        assert not fast or sound, (stride, size)
+        if 0 <= stride <= 1 << 19:
+            assert fast
