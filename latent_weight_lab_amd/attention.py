@@ -45,6 +45,7 @@ def attention_packed(qkv: torch.Tensor, heads: int, kv_heads: int | None = None,
     """Self-attention straight from and to a block's linears: ``qkv`` is ``[batch, tokens, (heads + 2 kv_heads) *
     head size]``, queries, keys and values side by side (one linear's output), and the result ``[batch,
     tokens, heads * head size]``.  Nothing is split or copied, and the gradient is one tensor like qkv.  The
-    other arguments are ``attention``'s."""
+    other arguments are ``attention``'s, but for ``causal_offset``: queries and keys are the same tokens, so it
+    defaults to 0, also in a batch padded at its ends (``key_lengths``)."""
     return N.layers().attention_packed(qkv, heads, heads if kv_heads is None else kv_heads, causal, scale, key_lengths,
                                        causal_offset)

@@ -491,7 +491,9 @@ lwl_attention_args packed_args(const Tensor& qkv, int64_t heads, int64_t kv_head
   if (qkv.dim() != 3 || heads <= 0 || kv_heads <= 0 || qkv.size(2) % (heads + 2 * kv_heads))
     refuse("attention_packed: ", qkv.sizes(), " does not hold ", heads, " query and twice ", kv_heads, " key heads");
   const int64_t tokens = qkv.size(1), width = qkv.size(2), dim = width / (heads + 2 * kv_heads);
-  lwl_attention_args a = shape_args(qkv.scalar_type(), how, qkv.size(0), heads, kv_heads, tokens, tokens, dim);
+  // queries and keys are the same tokens, whatever a sequence's length
+  const How same{how.causal, how.scale, how.offset.value_or(0)};
+  lwl_attention_args a = shape_args(qkv.scalar_type(), same, qkv.size(0), heads, kv_heads, tokens, tokens, dim);
   const int64_t in[3] = {tokens * width, dim, width}, res[3] = {tokens * heads * dim, dim, heads * dim};
   for (int i = 0; i < 3; ++i) {
     a.q_stride[i] = a.k_stride[i] = a.v_stride[i] = a.grad_q_stride[i] = a.grad_k_stride[i] = a.grad_v_stride[i] = in[i];

@@ -390,3 +390,23 @@ def test_rows_in_descending_order(dtype, tq, tk, d):
     torch.cuda.synchronize()
     for got, ref in zip(outs, want):
         assert torch.allclose(got.flip(2).float(), ref.float(), rtol=0, atol=2 * R.U[dt] * float(ref.abs().max()))
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_packed_batch_padded_at_its_ends(causal):
+    """Each sequence's tokens see what they see alone, and what pads them takes no part, in both directions."""
+    lengths, heads, kv_heads, d = [70, 41, 1, 0, 64], 4, 2, 32
+    x = torch.randn(5, 70, (heads + 2 * kv_heads) * d, device="cuda")
+    lens = torch.tensor(lengths, device="cuda")
+    dy = torch.randn(5, 70, heads * d, device="cuda") * (torch.arange(70, device="cuda")[None] < lens[:, None]).unsqueeze(-1)
+    x.requires_grad_()
+    y = attention_packed(x, heads, kv_heads, causal=causal, key_lengths=lens)
+    (gx,) = torch.autograd.grad(y, x, dy)
+    for b, n in enumerate(lengths):
+        alone = x[b:b + 1, :n].detach().requires_grad_()
+        want = attention_packed(alone, heads, kv_heads, causal=causal)
+        (g,) = torch.autograd.grad(want, alone, dy[b:b + 1, :n])
+        # the same float32 sums over a sequence's keys in another split at most: some 70 roundings of terms of size 1
+        assert torch.allclose(y[b:b + 1, :n], want, rtol=0, atol=1e-5)
+        assert torch.allclose(gx[b:b + 1, :n], g, rtol=0, atol=1e-4)
+        assert (gx[b, n:] == 0).all()
