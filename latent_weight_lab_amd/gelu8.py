@@ -55,7 +55,9 @@ def gelu_linear_checkpoint8(x: torch.Tensor, linear: nn.Module, bias: torch.Tens
     What ``linear`` (a ``BlockFHTLinear``, cached or not, or any other module) saves of its input for the
     backward pass is replaced by the checkpoint and computed again from it there; the weight's (or
     latent's) gradient is then that of the checkpoint's activation.  What it saves of its input after
-    changing it in place (a dropout with ``inplace=True``, say) is kept as it is.
+    changing it in place (a dropout with ``inplace=True``, say) is kept as it is.  Saved-tensor hooks around the
+    call (offloading to the host) see the codes and scales, not what ``linear`` saves: hooks of torch do not
+    nest.
     """
     if not torch.is_grad_enabled():
         return linear(gelu_checkpoint8(x, bias, approximate))

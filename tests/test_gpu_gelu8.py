@@ -221,3 +221,27 @@ def test_checkpoints_that_do_not_fit_are_refused():
         kept.activation()
     assert torch.equal(layer_ops.gelu8_activation(c, s, (2, 20, 300), x.dtype, "none").view(40, 300),
                        layer_ops.gelu8_activation(c, s, (40, 300), x.dtype, "none"))
+
+
+@pytest.mark.parametrize("kind", ["torch", "generated", "cached"])
+def test_activation_is_not_held(kind):
+    """What a step holds for its backward pass, in bytes asked of the allocator: codes, scales and the result.  The
+    same linear on the activation holds that as well."""
+    rows, f, out = 2000, 1024, 8
+    lin = torch.nn.Linear(f, out, device="cuda") if kind == "torch" else BlockFHTLinear(f, out, latent_dim=512, seed=4).cuda()
+    if kind == "cached":
+        prepare_block_fht_weight_cache(lin)
+    x = torch.randn(2, rows // 2, f, device="cuda", requires_grad=True)
+    asked = lambda: torch.cuda.memory_stats()["requested_bytes.all.current"]
+
+    def held(step):
+        step()  # library workspaces
+        before = asked()
+        y = step()
+        return asked() - before, y
+
+    kept = rows * f + rows * (f // 128) * 4 + rows * out * 4
+    got, _ = held(lambda: gelu_linear_checkpoint8(x, lin))
+    assert kept <= got < kept + 100_000
+    got, _ = held(lambda: lin(gelu_checkpoint8(x)))
+    assert kept + rows * f * 4 <= got < kept + rows * f * 4 + 100_000
