@@ -142,7 +142,7 @@ bool records(const MaybeTensor& t) { return t && t->requires_grad(); }
 
 // ---------------------------------------------------------------- layer norm
 struct Normed {
-  Tensor out, sum, stats;  // sum: undefined without a residual, stats: unless kept
+  Tensor h, out, sum, stats;  // h: what was normed, dense; sum: undefined without a residual, stats: unless kept
 };
 
 Normed norm_forward(const Tensor& x0, const Tensor& weight0, const MaybeTensor& bias0, double eps,
@@ -164,6 +164,7 @@ Normed norm_forward(const Tensor& x0, const Tensor& weight0, const MaybeTensor& 
   Normed r;
   r.out = at::empty(x.sizes(), x.options());
   if (residual) r.sum = at::empty(x.sizes(), x.options());
+  r.h = residual ? r.sum : x;
   if (keep_stats) r.stats = at::empty({2, rows}, x.options().dtype(at::kFloat));
   check(lib.norm_forward(x.data_ptr(), ptr(residual), ptr(weight), ptr(bias), code, weight_code, rows, f, eps,
                          r.out.data_ptr(), ptr(r.sum), (float*)ptr(r.stats), stream_of(x)));
@@ -200,7 +201,7 @@ struct NormFn : torch::autograd::Function<NormFn> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const MaybeTensor& bias,
                                const MaybeTensor& residual, double eps) {
     const Normed r = norm_forward(x, weight, bias, eps, residual, true);
-    ctx->save_for_backward({residual ? r.sum : x.contiguous(), weight, r.stats});
+    ctx->save_for_backward({r.h, weight, r.stats});
     ctx->saved_data["bias"] = bias.has_value();
     ctx->saved_data["residual"] = residual.has_value();
     ctx->set_materialize_grads(false);

@@ -180,3 +180,19 @@ def test_saved_tensors_in_another_layout_or_type():
             y = layer_norm(x, w)
         with pytest.raises(RuntimeError):
             torch.autograd.grad(y, (x, w), dy)
+
+
+def test_rows_that_are_not_dense_are_made_so_once():
+    """The copy that the kernel reads is the one kept for the backward pass."""
+    wide = torch.randn(2000, 1500, device="cuda", requires_grad=True)
+    w = torch.ones(1000, device="cuda")
+    layer_norm(wide[:, :1000], w)
+    before = torch.cuda.memory_stats()["requested_bytes.all.allocated"]
+    y = layer_norm(wide[:, :1000], w)
+    asked = torch.cuda.memory_stats()["requested_bytes.all.allocated"] - before
+    assert asked == 2 * 2000 * 1000 * 4 + 2 * 2000 * 4
+    dy = torch.randn_like(y)
+    dense = wide[:, :1000].detach().contiguous().requires_grad_()
+    want = torch.autograd.grad(layer_norm(dense, w), dense, dy)[0]
+    got = torch.autograd.grad(y, wide, dy)[0]
+    assert torch.equal(got[:, :1000], want) and (got[:, 1000:] == 0).all()
