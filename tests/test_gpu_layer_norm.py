@@ -182,6 +182,33 @@ def test_saved_tensors_in_another_layout_or_type():
             torch.autograd.grad(y, (x, w), dy)
 
 
+@pytest.mark.parametrize("rows,f", [(1, 768), (70, 300), (3, 9000)])
+@pytest.mark.parametrize("dtype,wtype", [("f32", "f32"), ("bf16", "f32"), ("f16", "f16")])
+@pytest.mark.parametrize("frozen", [False, True])
+def test_residual_without_bias(rows, f, dtype, wtype, frozen):
+    """The residual is the third tensor then; with x frozen its gradient is the residual's alone."""
+    dt, wt = DT[dtype], DT[wtype]
+    x, w, _, res, dy, dh = make(rows, f, dt, wt, rows + f, bias=False)
+    gx, gw, gr = gpu(x, not frozen), gpu(w, True), gpu(res, True)
+    out = layer_norm(gx, gw, None, EPS, gr)
+    wanted = (gw, gr) if frozen else (gx, gw, gr)
+    grads = torch.autograd.grad(out, wanted, (dy.cuda(), dh.cuda()))
+    if not frozen:
+        assert torch.equal(grads[0], grads[2])
+    # As check()'s bounds, and the error of the mean's sum, 2^-19 of the mean size: a row whose mean is almost zero
+    # and that has no bias holds nothing else to measure a small n by.
+    h, u, uw = (x.float() + res.float()).to(dt), R.U[dt], R.U[wt]
+    y, n, rstd = R.layer_norm(h, w, None, EPS)
+    _, dx, dw, _ = R.layer_norm(h, w, None, EPS, dy, dh)
+    off_mean, wd = h.double().abs().mean(-1, keepdim=True) * rstd, w.double()
+    assert torch.equal(out[1].cpu(), h)
+    assert ((out[0].double().cpu() - y).abs() <= u * y.abs() + 2.0 ** -19 * (n.abs() + off_mean) * wd.abs() + R.TINY[dt]).all()
+    a, nn = (dy.double() * wd).abs(), n.abs() + off_mean
+    size = rstd * (a + a.mean(-1, keepdim=True) + nn * (a * nn).mean(-1, keepdim=True)) + dh.double().abs()
+    assert ((grads[-1].double().cpu() - dx).abs() <= u * dx.abs() + 2.0 ** -18 * size + R.TINY[dt]).all()
+    assert ((grads[-2].double().cpu() - dw).abs() <= uw * dw.abs() + 2.0 ** -18 * (dy.double().abs() * nn).sum(0) + R.TINY[wt]).all()
+
+
 def test_rows_that_are_not_dense_are_made_so_once():
     """The copy that the kernel reads is the one kept for the backward pass."""
     wide = torch.randn(2000, 1500, device="cuda", requires_grad=True)
