@@ -366,8 +366,6 @@ __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2
 __device__ __forceinline__ float log2_hw(float x) { return __builtin_amdgcn_logf(x); }
 constexpr float kLog2E = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-__device__ __forceinline__ float max_nan(float a, float b);
-
 // The other half's value: lane l gets lane l ^ 32's.
 __device__ __forceinline__ float other_half(float v) {
   const uint32_t u = __float_as_uint(v);
