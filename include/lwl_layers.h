@@ -87,7 +87,7 @@ int lwl_gelu8_backward(const int8_t* codes, const float* scales, const void* gra
  *
  * Tensors are [batch, heads, tokens, dim] with the given strides in elements (batch, head, token) and
  * consecutive values along dim; any order, sharing (stride 0 of an input) and alignment of an element.
- * dim is 1 .. LWL_ATTENTION_MAX_DIM, heads a multiple of kv_heads, scale positive and finite.  lse
+ * dim is 1 .. LWL_ATTENTION_MAX_DIM, heads a multiple of kv_heads, scale from 2^-100 to 2^100.  lse
  * (float32 [batch][heads][queries], contiguous) may be NULL in the forward.
  *
  * Not finite: a NaN in a key or value that some query may see reaches that query's results, and may reach

@@ -20,7 +20,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
     ``q`` is ``[batch, heads, queries, head size]``, ``k`` and ``v`` ``[batch, kv_heads, keys, head size]``; ``heads`` is a
     multiple of ``kv_heads``, and consecutive query heads share a key head.  Head sizes up to 128;
     float32, float16 or bfloat16; any strides (a head's values are made dense if they are not).
-    ``scale`` defaults to ``1 / sqrt(head size)`` and must be positive.
+    ``scale`` defaults to ``1 / sqrt(head size)`` and must be positive (from 2^-100 to 2^100).
 
     ``key_lengths`` (integers on the device, ``[batch]``): keys of each sequence; what lies past them in k and
     v is not read into any result (a cache's unused end).  ``causal``: query i sees keys up to

@@ -86,8 +86,9 @@ int check_attention(const lwl_attention_args* a) {
   if (a->dim > LWL_ATTENTION_MAX_DIM)
     return status_fail(LWL_ERR_UNSUPPORTED, "attention supports head sizes up to %d (got %lld)", LWL_ATTENTION_MAX_DIM,
                        (long long)a->dim);
-  if (!(a->scale > 0.0) || !std::isfinite((float)a->scale) || (float)a->scale == 0.0f)
-    return status_fail(LWL_ERR_INVALID, "attention: scale must be positive and finite");
+  // the kernels multiply by scale * log2(e) and, in 16-bit types' backward, by its reciprocal times log sums
+  if (!(a->scale >= 0x1p-100 && a->scale <= 0x1p100))
+    return status_fail(LWL_ERR_INVALID, "attention: scale must be positive, from 2^-100 to 2^100");
   // token indexes are 32 bits in the kernels, workgroups are counted in 32 bits
   const int64_t kTokens = (int64_t)1 << 30, kCount = (int64_t)1 << 31;
   if (a->keys > kTokens || a->queries > kTokens || a->heads > kTokens || a->batch > kTokens)

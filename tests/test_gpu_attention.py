@@ -410,3 +410,19 @@ def test_packed_batch_padded_at_its_ends(causal):
         assert torch.allclose(y[b:b + 1, :n], want, rtol=0, atol=1e-5)
         assert torch.allclose(gx[b:b + 1, :n], g, rtol=0, atol=1e-4)
         assert (gx[b, n:] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("scale", [2.0 ** -100, 2.0 ** 100])
+def test_the_extreme_scales(dtype, scale):
+    """Of scores that are all but equal and of scores that are zero: uniform probabilities, all gradients finite."""
+    q, k, v, do = make(1, 2, 1, 40, 70, 64, DT[dtype], 6)
+    if scale > 1:
+        q = torch.zeros_like(q)
+    out, lse = layer_ops.attention_forward(q.cuda(), k.cuda(), v.cuda(), False, scale, None, None, True)
+    gq, gk, gv = layer_ops.attention_backward(q.cuda(), k.cuda(), v.cuda(), out, lse, do.cuda(), False, scale, None, None)
+    want = v.double().mean(2, keepdim=True).expand_as(out)
+    assert (out.double().cpu() - want).abs().max() <= 2 * R.U[DT[dtype]] * 4
+    if scale < 1 or dtype != "f16":  # else dQ, 2^100 times sums of size 1, is past the type
+        assert torch.isfinite(gq).all()
+    assert torch.isfinite(gk).all() and torch.isfinite(gv).all()

@@ -167,3 +167,9 @@ int main() {{
         assert not fast or sound, (stride, size)
         if 0 <= stride <= 1 << 19:
             assert fast
+
+
+@pytest.mark.parametrize("scale,rc", [(2.0 ** -100, 0), (2.0 ** 100, 0), (1e-39, -1), (3e38, -1), (float("inf"), -1)])
+def test_scales_that_the_exponent_cannot_take_are_refused(scale, rc):
+    """scale * log2(e) past float32's range gives 0 * infinity, its reciprocal past it log sums that are infinite."""
+    assert N.lib().lwl_attention_check(ctypes.byref(attn_args(scale=scale))) == rc
