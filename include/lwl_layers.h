@@ -92,8 +92,9 @@ int lwl_gelu8_backward(const int8_t* codes, const float* scales, const void* gra
  *
  * Not finite: a NaN in a key or value that some query may see reaches that query's results, and may reach
  * those of other queries whose `causal` limit hides it (its probability 0 is multiplied by it), as
- * it does where a masked score matrix is multiplied out.  float32 tensors that hold infinities give NaN:
- * their products are those of bfloat16 parts.
+ * it does where a masked score matrix is multiplied out; in the backward so may one in a query or its gradient
+ * reach the gradients of keys hidden from it.  float32 tensors that hold infinities give NaN: their products
+ * are those of bfloat16 parts.
  */
 #define LWL_ATTENTION_MAX_DIM 128
 typedef struct lwl_attention_args {
@@ -117,7 +118,9 @@ size_t lwl_attention_forward_workspace_size(const lwl_attention_args* args);
 int lwl_attention_forward(const lwl_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);
 /* The probabilities are computed again from q, k and lse.  grad_k and grad_v are summed over the query
  * heads that share a key head; all three gradients are overwritten whole (zeros where nothing reaches).
- * float32 divides each row of probabilities by its sum, so that lse's rounding does not count. */
+ * float32 divides each row of probabilities by its sum, so that lse's rounding does not count.  16-bit types
+ * round probabilities and scores' gradients to the type before their products; float16 holds the latter
+ * times powers of two, so that they neither leave its range nor lose digits at its lower end. */
 size_t lwl_attention_backward_workspace_size(const lwl_attention_args* args);
 int lwl_attention_backward(const lwl_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);
 

@@ -31,11 +31,12 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
     A query that sees no key gives zeros and takes no part in the gradients.  The result is
     ``[batch, heads, queries, head size]`` and lies token by token in memory, so that
     ``out.transpose(1, 2).reshape(batch, queries, -1)`` copies nothing.  Softmax and sums are float32; in 16-bit
-    types the probabilities are rounded to the type before the product with v.  Differentiable in q, k
-    and v (once).
+    types the probabilities are rounded to the type before the product with v, and in the backward pass the
+    probabilities and the scores' gradients before theirs.  Differentiable in q, k and v (once, in reverse mode).
 
     A NaN in a key or value that some query sees may also reach queries from which ``causal`` hides it, as where
-    a masked score matrix is multiplied out; float32 infinities in k, q or v give NaN."""
+    a masked score matrix is multiplied out, and one in a query or its gradient the gradients of keys hidden from it;
+    float32 infinities in k, q or v give NaN."""
     return N.layers().attention(q, k, v, causal, scale, key_lengths, causal_offset)
 
 

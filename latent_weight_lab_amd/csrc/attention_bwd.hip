@@ -17,10 +17,13 @@
 // bwd_queries runs first and leaves each query's D in the workspace for bwd_keys.  Where blocks are too few for the
 // compute units, both take ranges of what they walk over and leave float32 sums to be joined.
 //
-// Measured on MI355X, bfloat16 8 x 1024 x 12 x 64, causal: queries 33.6 us, keys 46.9 (45 GFLOP together, 560
+// 16-bit types: probabilities and dS are rounded to the type before their products (float16's dS in range, below),
+// D comes from the rounded output.
+//
+// Measured on MI355X, bfloat16 8 x 1024 x 12 x 64, causal: queries 34.1 us, keys 48.0 (45 GFLOP together, 550
 // TFLOP/s); 1 x 8192 x 16 x 128, all pairs: queries 790, keys 1280 us (1040 and 860 TFLOP/s of their products).  Matrix
 // instructions, exponentials and transposing LDS reads of the key pass share the time; registers hold it to one or two
-// waves a SIMD.  Float32 4 x 512 x 12 x 64: queries 31.6 + 6.3 us, keys 44.0 + 8.8.
+// waves a SIMD.  Float32 4 x 512 x 12 x 64: queries 31.4 + 6.3 us, keys 43.4 + 8.9.
 #include <algorithm>
 #include <cmath>
 

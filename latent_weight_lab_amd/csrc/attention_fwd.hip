@@ -27,8 +27,9 @@
 // exponentials (a quarter of the vector rate) and LDS reads: bfloat16 1 x 8192 x 16 on 4 x 128, causal, 297 us, 925
 // TFLOP/s of the pairs needed, where a library product of 8192^3 runs at 1030; 8 x 1024 x 12 x 64 23 us, 560 TFLOP/s,
 // two rounds of walks of unequal lengths.  Float32 4 x 512 x 12 x 64 22.6 us and 5.7 for the join.  Tokens are bound
-// by memory: bfloat16 64 sequences of up to 1024 tokens x 12 x 64 19.4 us (101 MB, 5.2 TB/s); float16 2 x 65536 x 4 x
-// 128 42.6 us (268 MB, 6.3 TB/s) and 4.7 for the join.
+// by memory: bfloat16 64 sequences of up to 1024 tokens x 12 x 64 19.6 us (101 MB, 5.2 TB/s), float32 38.3 us (202 MB,
+// 5.3 TB/s); float16 2 x 65536 x 4 x 128 42.6 us (268 MB, 6.3 TB/s, in part from the last-level cache) and 4.6 for the
+// join.
 #include <algorithm>
 #include <cfloat>
 
@@ -202,7 +203,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_rows(co
 }
 
 // ---------------------------------------------------------------- few queries
-constexpr int kTokenRows = 16;  // queries times heads that share a key head
+// Queries times heads that share a key head: the columns of one product.  More of them take attention_rows, where a
+// workgroup holds one query head and each reads the cache for itself: bfloat16 8 sequences of 8192 tokens of size 128, 16
+// heads on one 10.8 us and 3.9 for the join, 32 heads on one 146 us; 8 heads on one with 4 tokens each 34 and 4.6 us.
+constexpr int kTokenRows = 16;
 constexpr int kStep = 32;       // keys of a wave's step
 
 template <class T, int DP, bool WHOLE>

@@ -17,9 +17,9 @@
 // infinity or a NaN has s = NaN and stands for NaN, so that what went wrong in the forward pass
 // shows in the gradients.
 //
-// Measured on MI355X, bfloat16 8192 x 3072 with a bias: forward 27.3 us (126 MB, 4.6 TB/s), activation 19.8 us (76 MB,
-// 3.8 TB/s), backward 29.8 us (126 MB, 4.2 TB/s) and 3.9 us for the bias's sums, where a copy runs at 4.8-5.2 TB/s
-// from memory.  The two uses read what the forward left in the last-level cache; the instructions to unpack, evaluate
+// Measured on MI355X, bfloat16 8192 x 3072 with a bias: forward 27.6 us (126 MB, 4.6 TB/s), activation 19.8 us (76 MB,
+// 3.8 TB/s), backward 30.2 us (126 MB, 4.2 TB/s) and 3.9 us for the bias's sums, where a copy runs at 4.8-5.2 TB/s
+// from memory; float16 27.6, 18.4 and 28.6 us; float32 4096 x 3072 (113, 63 and 113 MB) 26.5, 21.0 and 27.0 us.  The two uses read what the forward left in the last-level cache; the instructions to unpack, evaluate
 // and pack again fill what is left of their time.
 #include <algorithm>
 

@@ -18,9 +18,9 @@
 // the partial rows in a fixed order (the result does not depend on which workgroup ends first).
 //
 // Measured on MI355X (a copy of as many bytes, which lie in the last-level cache, runs at 8 TB/s, one from memory at
-// 4.8-5.2): bfloat16 8192 x 768 with residual, forward 13.2 us (50 MB, 3.8 TB/s), backward 16.4 us (38 MB and
-// two partial rows a workgroup) and 5.4 us for the sums; float32 1021 x 3072, forward 8.2 us (25 MB), backward 13.0
-// and 5.3 us; one to a few rows 3.6 us, a launch and a round trip to memory.
+// 4.8-5.2): bfloat16 8192 x 768 with residual, forward 13.1 us (50 MB, 3.8 TB/s), backward 16.6 us (50 MB, 3.0 TB/s,
+// and two partial rows a workgroup) and 5.4 us for the sums; float32 1021 x 3072 without, forward 8.2 us (25 MB),
+// backward 12.6 (38 MB) and 5.3 us; one to a few rows 3.6 us, a launch and a round trip to memory.
 #include <algorithm>
 
 #include "layer_device.h"
