@@ -43,7 +43,8 @@ def gelu_checkpoint8(x: torch.Tensor, bias: torch.Tensor | None = None, approxim
 
     The forward value is exact (float32, rounded once); the backward pass takes the derivative at
     the 8-bit checkpoint of ``x + bias``.  With ``return_checkpoint`` returns ``(activation,
-    Checkpoint8)``.  Where no gradient is recorded and no checkpoint asked for, nothing is kept."""
+    Checkpoint8)``.  Where no gradient is recorded and no checkpoint asked for, nothing is kept.
+    Differentiable once, in reverse mode; ``bias`` has x's type."""
     out, codes, scales = N.layers().gelu8(x, bias, layer_ops.tanh_form(approximate), return_checkpoint)
     return (out, Checkpoint8(codes, scales, x, approximate)) if return_checkpoint else out
 

@@ -19,7 +19,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     Without ``residual`` h is x, and the normed tensor is returned.  With it h is ``x + residual``, rounded
     to x's type, and ``(normed, h)`` is returned: h is the residual stream that goes on.  ``x`` is
     float32, float16 or bfloat16; ``weight`` and ``bias`` have its type or are float32; mean, variance
-    and the gradients' sums are float32.  Differentiable in all four tensors."""
+    and the gradients' sums are float32.  Differentiable in all four tensors (once, in reverse mode)."""
     out = N.layers().layer_norm(x, weight, bias, eps, residual)
     return out[0] if residual is None else (out[0], out[1])
 
