@@ -21,9 +21,10 @@ from .block_fht import (
     signs_for,
     suspend_block_fht_weight_cache,
 )
-from .attention import attention, attention_packed
+from .attention import attention, attention_packed, attention_tree
 from .batched import block_fht_grouped_input_linear, block_fht_headwise_linear
 from .gelu8 import Checkpoint8, gelu_checkpoint8, gelu_linear_checkpoint8
+from .log_probs import token_log_probs
 from .mix import FixedFHTMix, fixed_fht_mix
 from .norm import LayerNorm, layer_norm
 
@@ -35,6 +36,7 @@ __all__ = [
     "LayerNorm",
     "attention",
     "attention_packed",
+    "attention_tree",
     "block_fht_grad_latent",
     "block_fht_grouped_input_linear",
     "block_fht_headwise_linear",
@@ -53,4 +55,5 @@ __all__ = [
     "sign_word_for",
     "signs_for",
     "suspend_block_fht_weight_cache",
+    "token_log_probs",
 ]

@@ -133,9 +133,10 @@ def _bind(lib) -> None:
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args
-    from . import layer_ops  # its structures name this module's types
+    from . import layer_ops, token_ops  # their structures name this module's types
 
     layer_ops.bind(lib)
+    token_ops.bind(lib)
 
 
 def lib():

@@ -2,6 +2,8 @@
 // element types, tiles in LDS.
 #pragma once
 
+#include <algorithm>
+
 #include "layer_device.h"
 #include "layer_launch.h"
 
@@ -428,9 +430,15 @@ __device__ __forceinline__ int ranked_sequence(const AttnArgs& a, int rank) {
 // Which keys a sequence's queries may see: j < len, and with causal j <= i + off.  Token numbers are 32 bits
 // (the C entry refuses more than 2^30), so that comparisons of wave-uniform ones are scalar.
 constexpr int kFar = (1 << 30) - 1;  // i + kFar + 1 does not overflow and is past every key
+//
+// Within a window (kWindow) a query at position p = i + off sees of these the last `window` and the first
+// `sinks`.  Of a tree (kTree) query i is node i, the key base + i is its own; it sees the keys below base, and of the
+// nodes those in its line of ancestors.
+enum Mask { kAll, kWindow, kTree };
 struct Allowed {
   int len;  // keys of this sequence
   int off;
+  int window, sinks;
 };
 // For the sequence b that a whole wave works on.
 __device__ __forceinline__ Allowed allowed_keys(const AttnArgs& a, int64_t b) {
@@ -444,12 +452,69 @@ __device__ __forceinline__ Allowed allowed_keys(const AttnArgs& a, int64_t b) {
   w.len = len;
   const int given = a.causal_offset > kFar ? kFar : (int)a.causal_offset;
   w.off = !a.causal ? kFar : a.bottom_right ? len - (int)a.queries : given;
+  w.window = (int)a.window;
+  w.sinks = (int)a.sinks;
   return w;
 }
 // First key that query i may not see.
 __device__ __forceinline__ int key_end(const Allowed& w, int i) {
   const int e = i + w.off + 1;
   return e < 0 ? 0 : e < w.len ? e : w.len;
+}
+
+// First key of query i's window.
+__device__ __forceinline__ int window_begin(const Allowed& w, int i) {
+  const int p = i + w.off;
+  return p < w.window ? 0 : p - w.window + 1;
+}
+
+// The keys that a block of queries walks over, STEP at a time, every STRIDE-th step: begin .. end; within a
+// window 0 .. head, the sinks before it, and then from the first query's window on.  j is a step's first
+// key, and keys from stop() on are not of it.
+template <int MASK, int STEP, int STRIDE = 1>
+struct Walk {
+  int j, end;
+  __device__ __forceinline__ bool live() const { return j < end; }
+  __device__ __forceinline__ bool more() const { return j + STEP * STRIDE < end; }
+  __device__ __forceinline__ int stop() const { return end; }
+  __device__ __forceinline__ int next() const { return j + STEP * STRIDE; }
+  __device__ __forceinline__ int next_stop() const { return end; }
+  __device__ __forceinline__ void step() { j += STEP * STRIDE; }
+};
+template <int STEP, int STRIDE>
+struct Walk<kWindow, STEP, STRIDE> {
+  int t, t_end, head_steps, head, lo, end, j;
+  __device__ __forceinline__ bool live() const { return t < t_end; }
+  __device__ __forceinline__ bool more() const { return t + STRIDE < t_end; }
+  __device__ __forceinline__ int at(int n) const { return n < head_steps ? n * STEP : lo + (n - head_steps) * STEP; }
+  __device__ __forceinline__ int stop_at(int n) const { return n < head_steps ? head : end; }
+  __device__ __forceinline__ int stop() const { return stop_at(t); }
+  __device__ __forceinline__ int next() const { return at(t + STRIDE); }
+  __device__ __forceinline__ int next_stop() const { return stop_at(t + STRIDE); }
+  __device__ __forceinline__ void step() { j = at(t += STRIDE); }
+};
+// Range `split` of split_len keys (a multiple of 64, or all) of the walk of queries first .. last, step `at` of it.
+template <int STEP, int STRIDE = 1>
+__device__ __forceinline__ Walk<kWindow, STEP, STRIDE> window_walk(const AttnArgs& a, const Allowed& w, int first, int last,
+                                                                   int split, int at) {
+  Walk<kWindow, STEP, STRIDE> k;
+  k.end = key_end(w, last);
+  k.lo = window_begin(w, first);
+  k.head = w.sinks < k.lo ? w.sinks : k.lo;
+  if (k.head > k.end) k.head = k.end;
+  if (w.sinks >= k.lo) k.lo = k.head = 0;  // nothing between sinks and window
+  k.head_steps = (k.head + STEP - 1) / STEP;
+  const int steps = k.head_steps + (k.end > k.lo ? (k.end - k.lo + STEP - 1) / STEP : 0);
+  const int per_range = a.splits > 1 ? (int)(a.split_len / STEP) : steps, begin = split * per_range;
+  k.t_end = begin + per_range < steps ? begin + per_range : steps;
+  k.t = begin + at;
+  k.j = k.at(k.t);
+  return k;
+}
+// Tiles that the longest walk of a block of `block` queries takes (host).
+inline int64_t window_tiles(const AttnArgs& a, int64_t block) {
+  const int64_t most = a.window + std::min(a.queries, block) - 1;
+  return (std::min(most, a.keys) + kTileRows - 1) / kTileRows + (std::min(a.sinks, a.keys) + kTileRows - 1) / kTileRows;
 }
 
 // Which block of queries (of 128) of which head a workgroup takes, and which range of keys.  Heads vary fastest,

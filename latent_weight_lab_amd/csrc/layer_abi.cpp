@@ -11,6 +11,8 @@
 
 namespace {
 
+using lwl::attention_args;
+using lwl::check_attention;
 using lwl::status_fail;
 using lwl::status_hip;
 using lwl::status_ok;
@@ -72,6 +74,10 @@ lwl::Gelu8Args gelu8_args(int dtype, int tanh_form, int64_t rows, int64_t featur
   return g;
 }
 
+}  // namespace
+
+namespace lwl {
+
 int check_attention(const lwl_attention_args* a) {
   if (!a) return status_fail(LWL_ERR_INVALID, "attention: args must be non-null");
   if (!valid_dtype(a->dtype))
@@ -101,8 +107,8 @@ int check_attention(const lwl_attention_args* a) {
   return LWL_OK;
 }
 
-lwl::AttnArgs attention_args(const lwl_attention_args* a) {
-  lwl::AttnArgs t{};
+AttnArgs attention_args(const lwl_attention_args* a) {
+  AttnArgs t{};
   t.dtype = a->dtype;
   t.causal = a->causal != 0;
   t.bottom_right = a->bottom_right != 0;
@@ -137,7 +143,7 @@ lwl::AttnArgs attention_args(const lwl_attention_args* a) {
   return t;
 }
 
-}  // namespace
+}  // namespace lwl
 
 extern "C" {
 

@@ -1,6 +1,7 @@
 // Internal interface between the C ABI of the layer operators (layer_abi.cpp) and their kernel
 // files: layer norm (layer_norm.hip), GELU with an 8-bit checkpoint (gelu8.hip), attention
-// (attention_fwd.hip, attention_bwd.hip).
+// (attention_fwd.hip, attention_bwd.hip; within a window attention_window.hip, attention_window_bwd.hip; of a tree
+// attention_tree.hip), log probabilities of tokens (log_probs.hip).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -8,6 +9,8 @@
 #include <stdint.h>
 
 #include "bfht_launch.h"
+
+struct lwl_attention_args;
 
 namespace lwl {
 
@@ -84,6 +87,12 @@ struct AttnArgs {
   int splits;         // ranges of what is walked over that different workgroups take
   int64_t split_len;  // keys of a range
   int cus;            // compute units
+  // within a window: of the keys up to its own position a query sees the last `window` and the first `sinks`
+  int64_t window, sinks;
+  int sink_splits;  // backward: ranges of the key blocks that hold sinks, whose queries are all later ones
+  // of a tree: [batch][queries]
+  const int32_t* parents;
+  int64_t parents_stride;
 };
 constexpr int kTileRows = 64;  // tokens of a tile
 // Whether a tensor of values of `size` bytes can be read in tiles by 32-bit offsets from a tile's first row:
@@ -94,11 +103,39 @@ inline bool fast_rows(const void* p, const int64_t (&stride)[3], int64_t size) {
   return (uintptr_t)p % 16 == 0 && stride[0] % unit == 0 && stride[1] % unit == 0 && stride[2] % unit == 0 &&
          stride[2] >= 0 && stride[2] < ((int64_t)1 << 31) / (size * kTileRows);
 }
+// A caller's arguments (layer_abi.cpp): refused with a status, or taken.
+int check_attention(const lwl_attention_args* a);
+AttnArgs attention_args(const lwl_attention_args* a);
 // float32 values in the workspace
 int64_t attention_fwd_work(const AttnArgs& a);
 int64_t attention_bwd_work(const AttnArgs& a);
 hipError_t launch_attention_fwd(AttnArgs a, hipStream_t s);
 hipError_t launch_attention_bwd(AttnArgs a, hipStream_t s);
+
+// The same within a window, and of a tree.
+int64_t attention_window_fwd_work(const AttnArgs& a);
+int64_t attention_window_bwd_work(const AttnArgs& a);
+hipError_t launch_attention_window_fwd(AttnArgs a, hipStream_t s);
+hipError_t launch_attention_window_bwd(AttnArgs a, hipStream_t s);
+int64_t attention_tree_work(const AttnArgs& a);
+hipError_t launch_attention_tree(AttnArgs a, hipStream_t s);
+
+// ---------------------------------------------------------------- log probabilities of tokens
+struct LogProbArgs {
+  int dtype, each, top;
+  int64_t outer, inner, vocab, outer_stride, inner_stride;
+  const void* logits;
+  const int64_t* tokens;
+  float *log_probs, *entropy, *top_log_probs;  // entropy may be null in the forward
+  int64_t* top_tokens;
+  float* stats;  // [rows][2]: the largest logit, lse less that; may be null in the forward
+  // backward; the first three may be null
+  const float *grad_log_probs, *grad_entropy, *grad_top;
+  void* grad_logits;
+};
+hipError_t launch_log_probs_fwd(const LogProbArgs& a, hipStream_t s);
+hipError_t launch_log_probs_bwd(const LogProbArgs& a, hipStream_t s);
+int64_t log_probs_bwd_ranges(int64_t vocab);  // workgroups of a row
 
 // Column sums of `rows` float32 rows of `stride` values, in a fixed order: columns [0, n0) to dst0,
 // [n0, n0 + n1) to dst1, in `dtype` (layer_norm.hip).  A null destination is skipped.

@@ -1,0 +1,367 @@
+// Log probabilities of given tokens, the entropy and the most probable alternatives, and their gradient.
+//
+// Forward: one pass over a row with a running maximum m, S = sum exp(z - m) and A = sum exp(z - m) (z - m) a thread,
+// joined at the end in a fixed order:
+//
+//   log p_t = (z_t - m) - log S,  H = log S - A / S   (A <= 0: nothing cancels)
+//
+// m starts at -FLT_MAX, so that a row of minus infinities sums zeros and nothing is NaN.
+//
+// The alternatives need no second pass over the row.  Each thread also keeps the largest of its values and the
+// chunk of eight it first met it in.  The top-th largest of these pairs bounds the answer from below, and exactly `top`
+// threads hold values that reach it: only they look at their part of the row again.  Pairs are ordered by value,
+// then by the lower index, so of equal values no more than the first few pass.  What passes is ranked by counting.
+//
+// Backward: one pass that reads the logits and writes their gradient; tokens that are asked about are written once more
+// afterwards by the workgroup whose range they lie in, with all gradients given for them in the order given.
+#include <algorithm>
+#include <cfloat>
+
+#include "layer_device.h"
+#include "layer_launch.h"
+
+namespace lwl {
+namespace {
+
+constexpr float kLog2E = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+template <class T>
+__device__ __forceinline__ const T* row_of(const LogProbArgs& a, int64_t r) {
+  return (const T*)a.logits + r / a.inner * a.outer_stride + r % a.inner * a.inner_stride;
+}
+
+// Numbers in the order of the values, all above 0: NaN is the largest, both zeros are one.
+__device__ __forceinline__ uint32_t order_of(float v) {
+  const uint32_t u = __float_as_uint(v + 0.0f);
+  return v != v ? 0xffffffffu : u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(uint32_t order) {
+  return __uint_as_float(order & 0x80000000u ? order & 0x7fffffffu : ~order);
+}
+// A value and where it lies, in the order wanted: larger values, then lower places, are larger numbers.
+__device__ __forceinline__ uint64_t pair_of(uint32_t order, uint32_t place) {
+  return (uint64_t)order << 32 | (uint32_t)~place;
+}
+
+// Eight values of a row from chunk `c` on; minus infinity past its end.
+template <class T>
+__device__ __forceinline__ void chunk_values(float (&v)[8], const Raw8<T>& raw, int64_t left) {
+  unpack8(v, raw);
+  if (left < 8) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < left ? v[i] : -INFINITY;
+  }
+}
+
+struct Sums {
+  float m, s, a;
+};
+template <bool ENTROPY>
+__device__ __forceinline__ void raise(Sums& t, float next) {
+  const float shrink = exp2_hw((t.m - next) * kLog2E);
+  if constexpr (ENTROPY) t.a = shrink > 0.0f ? (t.a + t.s * (t.m - next)) * shrink : 0.0f;
+  t.s *= shrink;
+  t.m = next;
+}
+
+constexpr int kCandidates = 1024;
+
+template <class T, int THREADS, bool ENTROPY, bool TOP>
+__global__ __launch_bounds__(THREADS) void log_probs_forward(const LogProbArgs a) {
+  constexpr int WAVES = THREADS / 64, U = 4;  // chunks of a thread under way
+  __shared__ float lds_m[WAVES], lds_s[WAVES], lds_a[WAVES];
+  __shared__ uint64_t lds_best[TOP ? THREADS : 1], lds_cand[TOP ? kCandidates : 1], lds_bound;
+  __shared__ int lds_count;
+  const int64_t row = blockIdx.x;
+  const T* x = row_of<T>(a, row);
+  const int vocab = (int)a.vocab, chunks = (vocab + 7) / 8;
+  int64_t token = -1;
+  float asked = 0.0f;
+  if ((int)threadIdx.x < a.each) {
+    token = a.tokens[row * a.each + threadIdx.x];
+    if (token >= 0 && token < vocab) asked = (float)x[token];
+  }
+  Sums t = {-FLT_MAX, 0.0f, 0.0f};
+  float best = -INFINITY;
+  uint32_t best_chunk = 0;
+  bool any = false;
+  for (int c0 = threadIdx.x; c0 < chunks; c0 += THREADS * U) {
+    Raw8<T> raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int c = c0 + u * THREADS;
+      load_raw8(raw[u], x + (int64_t)c * 8, c < chunks ? vocab - c * 8 : 0);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int c = c0 + u * THREADS;
+      float v[8];
+      chunk_values(v, raw[u], vocab - c * 8);
+      const float most = max_nan(max_nan(max_nan(v[0], v[1]), max_nan(v[2], v[3])),
+                                 max_nan(max_nan(v[4], v[5]), max_nan(v[6], v[7])));
+      if constexpr (TOP) {
+        if (c < chunks && (!any || !(most <= best) && best == best)) {  // the first NaN stays
+          best = most;
+          best_chunk = (uint32_t)c;
+          any = true;
+        }
+      }
+      if (__any(most > t.m)) raise<ENTROPY>(t, fmaxf(t.m, most));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float d = v[i] - t.m, e = exp2_hw(d * kLog2E);
+        t.s += e;
+        if constexpr (ENTROPY) t.a = fmaf(e, fmaxf(d, -FLT_MAX), t.a);
+      }
+    }
+  }
+  // over the wave, then over the waves
+#pragma unroll
+  for (int k = 1; k < 64; k *= 2) {
+    const float m = __shfl_xor(t.m, k, 64), next = fmaxf(t.m, m);
+    Sums o = {m, __shfl_xor(t.s, k, 64), ENTROPY ? __shfl_xor(t.a, k, 64) : 0.0f};
+    raise<ENTROPY>(t, next);
+    raise<ENTROPY>(o, next);
+    t.s += o.s;
+    t.a += o.a;
+  }
+  if ((threadIdx.x & 63) == 0) {
+    lds_m[threadIdx.x >> 6] = t.m;
+    lds_s[threadIdx.x >> 6] = t.s;
+    lds_a[threadIdx.x >> 6] = t.a;
+  }
+  if constexpr (TOP) {
+    // threads without a chunk come last
+    lds_best[threadIdx.x] = any ? pair_of(order_of(best), best_chunk) : (uint64_t)threadIdx.x;
+    if (threadIdx.x == 0) lds_count = 0;
+  }
+  __syncthreads();
+  t = {lds_m[0], lds_s[0], lds_a[0]};
+#pragma unroll
+  for (int w = 1; w < WAVES; ++w) {
+    Sums o = {lds_m[w], lds_s[w], lds_a[w]};
+    const float next = fmaxf(t.m, o.m);
+    raise<ENTROPY>(t, next);
+    raise<ENTROPY>(o, next);
+    t.s += o.s;
+    t.a += o.a;
+  }
+  const bool empty = t.s == 0.0f;  // nothing but minus infinities
+  const float log_s = __logf(t.s);
+  if ((int)threadIdx.x < a.each) {
+    const float lp = token >= vocab ? NAN : empty ? -INFINITY : (asked - t.m) - log_s;
+    a.log_probs[row * a.each + threadIdx.x] = token < 0 ? 0.0f : lp;
+  }
+  if (threadIdx.x == 0) {
+    if (ENTROPY && a.entropy) a.entropy[row] = empty ? 0.0f : log_s - t.a / t.s;
+    if (a.stats) {
+      a.stats[row * 2] = t.m;
+      a.stats[row * 2 + 1] = log_s;
+    }
+  }
+  if constexpr (TOP) {
+    const int top = a.top;
+    const uint64_t mine = lds_best[threadIdx.x];
+    int rank = 0;
+    for (int i = 0; i < THREADS; ++i) rank += lds_best[i] > mine;
+    if (rank == top - 1) lds_bound = mine;
+    __syncthreads();
+    uint64_t bound = lds_bound;
+    const auto candidates = [&](int c, const Raw8<T>& raw) {
+      float v[8];
+      chunk_values(v, raw, vocab - c * 8);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t order = order_of(v[i]);
+        // the bound names a chunk, or after a selection a place in one
+        if (c * 8 + i < vocab && pair_of(order, (uint32_t)c) >= bound) {
+          const int at = atomicAdd(&lds_count, 1);
+          if (at < kCandidates) lds_cand[at] = pair_of(order, (uint32_t)(c * 8 + i));
+        }
+      }
+    };
+    if (mine >= bound && any) {
+      for (int c0 = threadIdx.x; c0 < chunks; c0 += THREADS * U) {
+        Raw8<T> raw[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int c = c0 + u * THREADS;
+          load_raw8(raw[u], x + (int64_t)c * 8, c < chunks ? vocab - c * 8 : 0);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (c0 + u * THREADS < chunks) candidates(c0 + u * THREADS, raw[u]);
+      }
+    }
+    __syncthreads();
+    int count = lds_count;
+    if (count > kCandidates) {
+      // Few threads hold many of the largest values (sorted rows): the same chunk by chunk in step, and whenever the
+      // next chunks may not fit, all but the `top` largest so far are dropped.
+      __syncthreads();
+      if (threadIdx.x == 0) lds_count = 0;
+      __syncthreads();
+      for (int c0 = 0; c0 < chunks; c0 += THREADS) {
+        const int c = c0 + (int)threadIdx.x;
+        if (c < chunks && mine >= bound) {
+          Raw8<T> raw;
+          load_raw8(raw, x + (int64_t)c * 8, vocab - c * 8);
+          candidates(c, raw);
+        }
+        __syncthreads();
+        count = lds_count;
+        __syncthreads();  // all have read it
+        if (count + top * 8 > kCandidates) {
+          uint64_t keep[kCandidates / THREADS];
+          int at[kCandidates / THREADS];
+#pragma unroll
+          for (int k = 0; k < kCandidates / THREADS; ++k) {
+            const int i = threadIdx.x + k * THREADS;
+            keep[k] = i < count ? lds_cand[i] : 0;
+            at[k] = 0;
+            if (i < count)
+              for (int j = 0; j < count; ++j) at[k] += lds_cand[j] > keep[k];
+          }
+          __syncthreads();
+#pragma unroll
+          for (int k = 0; k < kCandidates / THREADS; ++k)
+            if ((int)threadIdx.x + k * THREADS < count && at[k] < top) lds_cand[at[k]] = keep[k];
+          if (threadIdx.x == 0) lds_count = top;
+          __syncthreads();
+          count = top;
+        }
+      }
+    }
+    for (int i = threadIdx.x; i < count; i += THREADS) {
+      const uint64_t one = lds_cand[i];
+      int place = 0;
+      for (int j = 0; j < count; ++j) place += lds_cand[j] > one;
+      if (place < top) {
+        a.top_log_probs[row * top + place] = empty ? -INFINITY : (value_of((uint32_t)(one >> 32)) - t.m) - log_s;
+        a.top_tokens[row * top + place] = (int64_t)(uint32_t)~(uint32_t)one;
+      }
+    }
+  }
+}
+
+constexpr int kListed = 128;  // tokens that a row's gradients are given for
+constexpr int kBwdChunks = 8; // of a thread
+constexpr int kBwdRange = 256 * 8 * kBwdChunks;  // logits of a workgroup
+
+template <class T, bool ENTROPY>
+__global__ __launch_bounds__(256) void log_probs_backward(const LogProbArgs a, uint32_t ranges) {
+  __shared__ int lds_token[kListed];
+  __shared__ float lds_grad[kListed];
+  const int64_t row = blockIdx.x / ranges;
+  const int begin = (int)(blockIdx.x % ranges) * kBwdRange;
+  const T* x = row_of<T>(a, row);
+  T* dz = (T*)a.grad_logits + row * a.vocab;
+  const int vocab = (int)a.vocab, end = vocab - begin < kBwdRange ? vocab : begin + kBwdRange;
+  const int listed = a.each + a.top;
+  if ((int)threadIdx.x < listed) {
+    const int i = threadIdx.x;
+    const bool is_top = i >= a.each;
+    const float* g = is_top ? a.grad_top : a.grad_log_probs;
+    int64_t token = -1;
+    if (g) token = is_top ? a.top_tokens[row * a.top + i - a.each] : a.tokens[row * a.each + i];
+    const bool ok = token >= 0 && token < vocab;
+    lds_token[i] = ok ? (int)token : -1;
+    lds_grad[i] = ok ? g[is_top ? row * a.top + i - a.each : row * a.each + i] : 0.0f;
+  }
+  const float m = a.stats[row * 2], log_s = a.stats[row * 2 + 1];
+  const bool empty = log_s == -INFINITY;
+  const float gh = ENTROPY ? a.grad_entropy[row] : 0.0f, entropy = ENTROPY ? a.entropy[row] : 0.0f;
+  __syncthreads();
+  float total = 0.0f;
+  for (int i = 0; i < listed; ++i) total += lds_grad[i];
+  // what a logit's gradient is without those given for its token
+  const auto spread = [&](float z) {
+    const float lp = (z - m) - log_s, p = exp2_hw(lp * kLog2E);
+    float f = -total;
+    if constexpr (ENTROPY) f -= gh * (fmaxf(lp, -200.0f) + entropy);  // below that p is 0
+    return empty ? 0.0f : p * f;
+  };
+  Raw8<T> raw[kBwdChunks];
+#pragma unroll
+  for (int u = 0; u < kBwdChunks; ++u) {
+    const int at = begin + (u * 256 + (int)threadIdx.x) * 8;
+    load_raw8(raw[u], x + at, end - at);
+  }
+#pragma unroll
+  for (int u = 0; u < kBwdChunks; ++u) {
+    const int at = begin + (u * 256 + (int)threadIdx.x) * 8;
+    float v[8];
+    unpack8(v, raw[u]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = spread(v[i]);
+    store8(dz + at, v, end - at);
+  }
+  __syncthreads();
+  if ((int)threadIdx.x < listed && !empty) {
+    const int token = lds_token[threadIdx.x];
+    if (token >= begin && token < end) {
+      float g = 0.0f;
+      int first = -1;
+      for (int j = 0; j < listed; ++j)
+        if (lds_token[j] == token) {
+          g += lds_grad[j];
+          if (first < 0) first = j;
+        }
+      if (first == (int)threadIdx.x) dz[token] = (T)(spread((float)x[token]) + g);
+    }
+  }
+}
+
+template <class T, int THREADS>
+void forward(const LogProbArgs& a, hipStream_t s) {
+  const dim3 grid((unsigned)(a.outer * a.inner)), block(THREADS);
+  if (a.top > 0) {
+    if (a.entropy) hipLaunchKernelGGL((log_probs_forward<T, THREADS, true, true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((log_probs_forward<T, THREADS, false, true>), grid, block, 0, s, a);
+  } else {
+    if (a.entropy) hipLaunchKernelGGL((log_probs_forward<T, THREADS, true, false>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((log_probs_forward<T, THREADS, false, false>), grid, block, 0, s, a);
+  }
+}
+template <class T>
+hipError_t run_forward(const LogProbArgs& a, hipStream_t s) {
+  forward<T, 256>(a, s);
+  return hipGetLastError();
+}
+
+template <class T>
+hipError_t run_backward(const LogProbArgs& a, hipStream_t s) {
+  const int64_t ranges = log_probs_bwd_ranges(a.vocab);
+  const dim3 grid((unsigned)(a.outer * a.inner * ranges));
+  if (a.grad_entropy)
+    hipLaunchKernelGGL((log_probs_backward<T, true>), grid, dim3(256), 0, s, a, (uint32_t)ranges);
+  else
+    hipLaunchKernelGGL((log_probs_backward<T, false>), grid, dim3(256), 0, s, a, (uint32_t)ranges);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+int64_t log_probs_bwd_ranges(int64_t vocab) { return (vocab + kBwdRange - 1) / kBwdRange; }
+
+hipError_t launch_log_probs_fwd(const LogProbArgs& a, hipStream_t s) {
+  switch (a.dtype) {
+    case kF32: return run_forward<float>(a, s);
+    case kF16: return run_forward<f16>(a, s);
+    case kBF16: return run_forward<bf16>(a, s);
+  }
+  return hipErrorInvalidValue;
+}
+
+hipError_t launch_log_probs_bwd(const LogProbArgs& a, hipStream_t s) {
+  switch (a.dtype) {
+    case kF32: return run_backward<float>(a, s);
+    case kF16: return run_backward<f16>(a, s);
+    case kBF16: return run_backward<bf16>(a, s);
+  }
+  return hipErrorInvalidValue;
+}
+
+}  // namespace lwl

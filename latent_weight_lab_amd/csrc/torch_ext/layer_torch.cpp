@@ -1,5 +1,5 @@
 // The layer operators on torch tensors: argument checks, outputs and scratch from torch's caching allocator,
-// the current stream, and autograd, over the C entries of include/lwl_layers.h.
+// the current stream, and autograd, over the C entries of include/lwl_layers.h and include/lwl_tokens.h.
 //
 // These calls are short on the GPU (a layer norm's training step of 8192 x 768 is 36 us of kernels).  Through
 // ctypes and Python autograd functions such a step took 130 us of host time, most of it in Python
@@ -22,6 +22,7 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include "lwl_layers.h"
+#include "lwl_tokens.h"
 
 namespace {
 
@@ -45,6 +46,14 @@ struct Library {
   decltype(&lwl_attention_forward) attention_forward = nullptr;
   decltype(&lwl_attention_backward_workspace_size) attention_backward_workspace = nullptr;
   decltype(&lwl_attention_backward) attention_backward = nullptr;
+  decltype(&lwl_attention_window_forward_workspace_size) window_forward_workspace = nullptr;
+  decltype(&lwl_attention_window_forward) window_forward = nullptr;
+  decltype(&lwl_attention_window_backward_workspace_size) window_backward_workspace = nullptr;
+  decltype(&lwl_attention_window_backward) window_backward = nullptr;
+  decltype(&lwl_attention_tree_workspace_size) tree_workspace = nullptr;
+  decltype(&lwl_attention_tree_forward) tree_forward = nullptr;
+  decltype(&lwl_log_probs_forward) log_probs_forward = nullptr;
+  decltype(&lwl_log_probs_backward) log_probs_backward = nullptr;
 } lib;
 
 // An invalid argument: the package's BlockFHTArgumentError (a ValueError and a RuntimeError).
@@ -325,6 +334,8 @@ struct How {
   bool causal;
   std::optional<double> scale;
   std::optional<int64_t> offset;
+  std::optional<int64_t> window;
+  int64_t sinks;
 };
 
 Tensor dense_dim(const Tensor& t) {
@@ -357,7 +368,16 @@ lwl_attention_args shape_args(at::ScalarType dtype, const How& how, int64_t batc
 void strides(int64_t (&s)[3], const Tensor& t) {
   for (int i = 0; i < 3; ++i) s[i] = t.stride(i);
 }
-void run(const lwl_attention_args& a, bool forward, const Tensor& like) {
+void run(const lwl_attention_args& a, const How& how, bool forward, const Tensor& like) {
+  if (how.window) {
+    const size_t need =
+        (forward ? lib.window_forward_workspace : lib.window_backward_workspace)(&a, *how.window, how.sinks);
+    const Tensor ws = scratch(need, like);
+    check((forward ? lib.window_forward : lib.window_backward)(&a, *how.window, how.sinks, ptr(ws), need,
+                                                               stream_of(like)));
+    return;
+  }
+  if (how.sinks != 0) refuse("attention: sinks without a window");
   const size_t need = (forward ? lib.attention_forward_workspace : lib.attention_backward_workspace)(&a);
   const Tensor ws = scratch(need, like);
   check((forward ? lib.attention_forward : lib.attention_backward)(&a, ptr(ws), need, stream_of(like)));
@@ -382,9 +402,11 @@ Tensor empty_heads(const lwl_attention_args& a, int64_t tokens, int64_t heads, c
 
 std::tuple<Tensor, MaybeTensor> attention_forward(const Tensor& q0, const Tensor& k0, const Tensor& v0, bool causal,
                                                   std::optional<double> scale, const MaybeTensor& lengths0,
-                                                  std::optional<int64_t> offset, bool keep_lse) {
+                                                  std::optional<int64_t> offset, bool keep_lse,
+                                                  std::optional<int64_t> window, int64_t sinks) {
   on_one_gpu(q0, k0, v0, lengths0);
-  lwl_attention_args a = heads_args(q0, k0, v0, {causal, scale, offset});
+  const How how{causal, scale, offset, window, sinks};
+  lwl_attention_args a = heads_args(q0, k0, v0, how);
   const c10::DeviceGuard guard(q0.device());
   const MaybeTensor lengths = lengths_of(lengths0, a.batch);
   const Tensor q = dense_dim(q0), k = dense_dim(k0), v = dense_dim(v0), out = empty_heads(a, a.queries, a.heads, q);
@@ -400,7 +422,7 @@ std::tuple<Tensor, MaybeTensor> attention_forward(const Tensor& q0, const Tensor
   strides(a.k_stride, k);
   strides(a.v_stride, v);
   strides(a.out_stride, out);
-  run(a, true, q);
+  run(a, how, true, q);
   return {out, lse};
 }
 
@@ -418,9 +440,11 @@ void check_left(const lwl_attention_args& a, const Tensor& q, at::IntArrayRef sh
 std::tuple<Tensor, Tensor, Tensor> attention_backward(const Tensor& q0, const Tensor& k0, const Tensor& v0,
                                                       const Tensor& out, const Tensor& lse, const Tensor& grad_out0,
                                                       bool causal, std::optional<double> scale,
-                                                      const MaybeTensor& lengths0, std::optional<int64_t> offset) {
+                                                      const MaybeTensor& lengths0, std::optional<int64_t> offset,
+                                                      std::optional<int64_t> window, int64_t sinks) {
   on_one_gpu(q0, k0, v0, out, lse, grad_out0, lengths0);
-  lwl_attention_args a = heads_args(q0, k0, v0, {causal, scale, offset});
+  const How how{causal, scale, offset, window, sinks};
+  lwl_attention_args a = heads_args(q0, k0, v0, how);
   check_left(a, q0, q0.sizes(), out, lse, grad_out0);
   const c10::DeviceGuard guard(q0.device());
   const MaybeTensor lengths = lengths_of(lengths0, a.batch);
@@ -446,7 +470,7 @@ std::tuple<Tensor, Tensor, Tensor> attention_backward(const Tensor& q0, const Te
   strides(a.grad_q_stride, gq);
   strides(a.grad_k_stride, gk);
   strides(a.grad_v_stride, gv);
-  run(a, false, q);
+  run(a, how, false, q);
   return {gq, gk, gv};
 }
 
@@ -455,36 +479,41 @@ void keep_how(AutogradContext* ctx, const How& how) {
   ctx->saved_data["causal"] = how.causal;
   ctx->saved_data["scale"] = how.scale ? c10::IValue(*how.scale) : c10::IValue();
   ctx->saved_data["offset"] = how.offset ? c10::IValue(*how.offset) : c10::IValue();
+  ctx->saved_data["window"] = how.window ? c10::IValue(*how.window) : c10::IValue();
+  ctx->saved_data["sinks"] = how.sinks;
 }
 How kept_how(AutogradContext* ctx) {
-  const auto &scale = ctx->saved_data["scale"], &offset = ctx->saved_data["offset"];
+  const auto number = [](const c10::IValue& v) { return v.isNone() ? std::nullopt : std::optional<int64_t>(v.toInt()); };
+  const auto& scale = ctx->saved_data["scale"];
   return {ctx->saved_data["causal"].toBool(), scale.isNone() ? std::nullopt : std::optional<double>(scale.toDouble()),
-          offset.isNone() ? std::nullopt : std::optional<int64_t>(offset.toInt())};
+          number(ctx->saved_data["offset"]), number(ctx->saved_data["window"]), ctx->saved_data["sinks"].toInt()};
 }
 MaybeTensor kept(const Tensor& t) { return t.defined() ? MaybeTensor(t) : MaybeTensor(); }
 
 struct AttentionFn : torch::autograd::Function<AttentionFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, bool causal,
-                        std::optional<double> scale, const MaybeTensor& lengths, std::optional<int64_t> offset) {
-    const auto [out, lse] = attention_forward(q, k, v, causal, scale, lengths, offset, true);
+                        std::optional<double> scale, const MaybeTensor& lengths, std::optional<int64_t> offset,
+                        std::optional<int64_t> window, int64_t sinks) {
+    const auto [out, lse] = attention_forward(q, k, v, causal, scale, lengths, offset, true, window, sinks);
     ctx->save_for_backward({q, k, v, out, *lse, lengths ? *lengths : Tensor()});
-    keep_how(ctx, {causal, scale, offset});
+    keep_how(ctx, {causal, scale, offset, window, sinks});
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto s = ctx->get_saved_variables();
     const How how = kept_how(ctx);
     const auto [gq, gk, gv] =
-        attention_backward(s[0], s[1], s[2], s[3], s[4], grads[0], how.causal, how.scale, kept(s[5]), how.offset);
-    return once({gq, gk, gv, Tensor(), Tensor(), Tensor(), Tensor()});
+        attention_backward(s[0], s[1], s[2], s[3], s[4], grads[0], how.causal, how.scale, kept(s[5]), how.offset,
+                           how.window, how.sinks);
+    return once({gq, gk, gv, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
   }
 };
 
 Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, bool causal, std::optional<double> scale,
-                 const MaybeTensor& lengths, std::optional<int64_t> offset) {
+                 const MaybeTensor& lengths, std::optional<int64_t> offset, std::optional<int64_t> window, int64_t sinks) {
   if (at::GradMode::is_enabled() && (records(q) || records(k) || records(v)))
-    return AttentionFn::apply(q, k, v, causal, scale, lengths, offset);
-  return std::get<0>(attention_forward(q, k, v, causal, scale, lengths, offset, false));
+    return AttentionFn::apply(q, k, v, causal, scale, lengths, offset, window, sinks);
+  return std::get<0>(attention_forward(q, k, v, causal, scale, lengths, offset, false, window, sinks));
 }
 
 // Queries, keys and values side by side in one contiguous [batch, tokens, (heads + 2 kv_heads) * dim].
@@ -493,7 +522,7 @@ lwl_attention_args packed_args(const Tensor& qkv, int64_t heads, int64_t kv_head
     refuse("attention_packed: ", qkv.sizes(), " does not hold ", heads, " query and twice ", kv_heads, " key heads");
   const int64_t tokens = qkv.size(1), width = qkv.size(2), dim = width / (heads + 2 * kv_heads);
   // queries and keys are the same tokens, whatever a sequence's length
-  const How same{how.causal, how.scale, how.offset.value_or(0)};
+  const How same{how.causal, how.scale, how.offset.value_or(0), how.window, how.sinks};
   lwl_attention_args a = shape_args(qkv.scalar_type(), same, qkv.size(0), heads, kv_heads, tokens, tokens, dim);
   const int64_t in[3] = {tokens * width, dim, width}, res[3] = {tokens * heads * dim, dim, heads * dim};
   for (int i = 0; i < 3; ++i) {
@@ -508,9 +537,11 @@ char* head_of(const Tensor& qkv, const lwl_attention_args& a, int64_t head) {
 
 std::tuple<Tensor, MaybeTensor> packed_forward(const Tensor& qkv, int64_t heads, int64_t kv_heads, bool causal,
                                                std::optional<double> scale, const MaybeTensor& lengths0,
-                                               std::optional<int64_t> offset, bool keep_lse) {
+                                               std::optional<int64_t> offset, bool keep_lse,
+                                               std::optional<int64_t> window, int64_t sinks) {
   on_one_gpu(qkv, lengths0);
-  lwl_attention_args a = packed_args(qkv, heads, kv_heads, {causal, scale, offset});
+  const How how{causal, scale, offset, window, sinks};
+  lwl_attention_args a = packed_args(qkv, heads, kv_heads, how);
   const c10::DeviceGuard guard(qkv.device());
   const MaybeTensor lengths = lengths_of(lengths0, a.batch);
   const Tensor out = at::empty({a.batch, a.queries, heads * a.dim}, qkv.options());
@@ -522,16 +553,17 @@ std::tuple<Tensor, MaybeTensor> packed_forward(const Tensor& qkv, int64_t heads,
   a.out = out.data_ptr();
   a.lse = (float*)ptr(lse);
   a.key_lengths = (const int32_t*)ptr(lengths);
-  run(a, true, qkv);
+  run(a, how, true, qkv);
   return {out, lse};
 }
 
 struct PackedFn : torch::autograd::Function<PackedFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& qkv, int64_t heads, int64_t kv_heads, bool causal,
-                        std::optional<double> scale, const MaybeTensor& lengths, std::optional<int64_t> offset) {
-    const auto [out, lse] = packed_forward(qkv, heads, kv_heads, causal, scale, lengths, offset, true);
+                        std::optional<double> scale, const MaybeTensor& lengths, std::optional<int64_t> offset,
+                        std::optional<int64_t> window, int64_t sinks) {
+    const auto [out, lse] = packed_forward(qkv, heads, kv_heads, causal, scale, lengths, offset, true, window, sinks);
     ctx->save_for_backward({qkv, out, *lse, lengths ? *lengths : Tensor()});
-    keep_how(ctx, {causal, scale, offset});
+    keep_how(ctx, {causal, scale, offset, window, sinks});
     ctx->saved_data["heads"] = heads;
     ctx->saved_data["kv_heads"] = kv_heads;
     return out;
@@ -541,7 +573,8 @@ struct PackedFn : torch::autograd::Function<PackedFn> {
     on_one_gpu(s[0], s[1], s[2], kept(s[3]), grads[0]);
     const Tensor qkv = s[0].contiguous(), out = s[1].contiguous(), lse = s[2];
     const int64_t heads = ctx->saved_data["heads"].toInt(), kv_heads = ctx->saved_data["kv_heads"].toInt();
-    lwl_attention_args a = packed_args(qkv, heads, kv_heads, kept_how(ctx));
+    const How how = kept_how(ctx);
+    lwl_attention_args a = packed_args(qkv, heads, kv_heads, how);
     check_left(a, qkv, {a.batch, a.queries, heads * a.dim}, out, lse, grads[0]);
     const c10::DeviceGuard guard(qkv.device());
     const MaybeTensor lengths = lengths_of(kept(s[3]), a.batch);
@@ -556,17 +589,211 @@ struct PackedFn : torch::autograd::Function<PackedFn> {
     a.grad_q = grad.data_ptr();
     a.grad_k = head_of(grad, a, heads);
     a.grad_v = head_of(grad, a, heads + kv_heads);
-    run(a, false, qkv);
-    return once({grad, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
+    run(a, how, false, qkv);
+    return once({grad, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
   }
 };
 
 Tensor attention_packed(const Tensor& qkv0, int64_t heads, int64_t kv_heads, bool causal, std::optional<double> scale,
-                        const MaybeTensor& lengths, std::optional<int64_t> offset) {
+                        const MaybeTensor& lengths, std::optional<int64_t> offset, std::optional<int64_t> window,
+                        int64_t sinks) {
   const Tensor qkv = qkv0.contiguous();
   if (at::GradMode::is_enabled() && records(qkv))
-    return PackedFn::apply(qkv, heads, kv_heads, causal, scale, lengths, offset);
-  return std::get<0>(packed_forward(qkv, heads, kv_heads, causal, scale, lengths, offset, false));
+    return PackedFn::apply(qkv, heads, kv_heads, causal, scale, lengths, offset, window, sinks);
+  return std::get<0>(packed_forward(qkv, heads, kv_heads, causal, scale, lengths, offset, false, window, sinks));
+}
+
+// Of a tree of drafted tokens over a cache.
+Tensor attention_tree(const Tensor& q0, const Tensor& k0, const Tensor& v0, const Tensor& parents0,
+                      std::optional<double> scale, const MaybeTensor& lengths0) {
+  on_one_gpu(q0, k0, v0, parents0, lengths0);
+  if (at::GradMode::is_enabled() && (records(q0) || records(k0) || records(v0)))
+    TORCH_CHECK_NOT_IMPLEMENTED(false, "latent_weight_lab_amd: attention_tree has no derivatives; call it without gradients");
+  lwl_attention_args a = heads_args(q0, k0, v0, {false, scale, 0, std::nullopt, 0});
+  const bool own_trees = parents0.dim() == 2;
+  if ((!own_trees && parents0.dim() != 1) || parents0.size(-1) != a.queries || (own_trees && parents0.size(0) != a.batch) ||
+      !at::isIntegralType(parents0.scalar_type(), /*includeBool=*/false))
+    refuse("attention_tree: parents must be [", a.queries, "] or [", a.batch, ", ", a.queries, "] integers, got ",
+           parents0.sizes(), " of ", parents0.scalar_type());
+  const c10::DeviceGuard guard(q0.device());
+  const MaybeTensor lengths = lengths_of(lengths0, a.batch);
+  Tensor parents = parents0;
+  if (parents.scalar_type() != at::kInt)  // numbers that are no node's stay so in 32 bits
+    parents = parents.scalar_type() == at::kLong ? parents.clamp(-1, LWL_ATTENTION_MAX_NODES).to(at::kInt) : parents.to(at::kInt);
+  parents = parents.contiguous();
+  const Tensor q = dense_dim(q0), k = dense_dim(k0), v = dense_dim(v0), out = empty_heads(a, a.queries, a.heads, q);
+  a.q = q.data_ptr();
+  a.k = k.data_ptr();
+  a.v = v.data_ptr();
+  a.out = out.data_ptr();
+  a.key_lengths = (const int32_t*)ptr(lengths);
+  strides(a.q_stride, q);
+  strides(a.k_stride, k);
+  strides(a.v_stride, v);
+  strides(a.out_stride, out);
+  const size_t need = lib.tree_workspace(&a);
+  const Tensor ws = scratch(need, q);
+  check(lib.tree_forward(&a, (const int32_t*)parents.data_ptr(), own_trees ? a.queries : 0, ptr(ws), need, stream_of(q)));
+  return out;
+}
+
+// ---------------------------------------------------------------- log probabilities of tokens
+// Logits as outer x inner rows, where their leading axes lie so; a copy otherwise.
+struct LogitRows {
+  Tensor logits;
+  int64_t outer = 1, inner = 1, outer_stride = 0, inner_stride = 0;
+};
+LogitRows logit_rows(const Tensor& logits0) {
+  LogitRows r;
+  const auto two_axes = [&](const Tensor& t) {
+    r = {t};
+    if (t.size(-1) != 1 && t.stride(-1) != 1) return false;
+    int axes = 0;  // met so far, from the last
+    for (int64_t d = t.dim() - 2; d >= 0; --d) {
+      const int64_t n = t.size(d), s = t.stride(d);
+      if (n == 1) continue;
+      if (axes == 0) {
+        r.inner = n;
+        r.inner_stride = s;
+        axes = 1;
+      } else if (axes == 1 && s == r.inner_stride * r.inner) {
+        r.inner *= n;
+      } else if (axes == 1) {
+        r.outer = n;
+        r.outer_stride = s;
+        axes = 2;
+      } else if (s == r.outer_stride * r.outer) {
+        r.outer *= n;
+      } else {
+        return false;
+      }
+    }
+    return true;
+  };
+  if (!two_axes(logits0)) two_axes(logits0.contiguous());
+  return r;
+}
+
+// What the forward leaves; undefined where not asked for.
+struct Judged {
+  Tensor log_probs, entropy, top_log_probs, top_tokens, stats;
+};
+lwl_log_probs_args log_probs_args(const LogitRows& r, const Tensor& tokens, int64_t each, int64_t top) {
+  lwl_log_probs_args a{};
+  a.dtype = dtype_code(r.logits.scalar_type());
+  a.each = (int32_t)each;
+  a.top = (int32_t)top;
+  a.outer = r.outer;
+  a.inner = r.inner;
+  a.vocab = r.logits.size(-1);
+  a.outer_stride = r.outer_stride;
+  a.inner_stride = r.inner_stride;
+  a.logits = r.logits.data_ptr();
+  a.tokens = (const int64_t*)tokens.data_ptr();
+  return a;
+}
+// Tokens of a row.
+int64_t tokens_each(const Tensor& logits, const Tensor& tokens) {
+  if (logits.dim() < 1) refuse("token_log_probs: logits need an axis of tokens, got a single number");
+  const auto rows = logits.sizes().slice(0, logits.dim() - 1);
+  const bool one = tokens.dim() == logits.dim() - 1;
+  if (!at::isIntegralType(tokens.scalar_type(), /*includeBool=*/false) ||
+      (one ? tokens.sizes() != rows
+           : tokens.dim() != logits.dim() || tokens.sizes().slice(0, logits.dim() - 1) != rows))
+    refuse("token_log_probs: tokens must be integers of ", rows, ", or of that with one more axis, for logits ",
+           logits.sizes(), "; got ", tokens.sizes(), " of ", tokens.scalar_type());
+  return one ? 1 : tokens.size(-1);
+}
+
+Judged log_probs_forward(const Tensor& logits0, const Tensor& tokens0, bool entropy, int64_t top, bool keep_stats) {
+  on_one_gpu(logits0, tokens0);
+  const int64_t each = tokens_each(logits0, tokens0);
+  if (each > LWL_LOG_PROBS_MAX_EACH || top > LWL_LOG_PROBS_MAX_TOP || top < 0)
+    refuse("token_log_probs: up to ", LWL_LOG_PROBS_MAX_EACH, " tokens a row and 0 to ", LWL_LOG_PROBS_MAX_TOP,
+           " alternatives, got ", each, " and ", top);
+  const c10::DeviceGuard guard(logits0.device());
+  const LogitRows r = logit_rows(logits0);
+  const Tensor tokens = typed(tokens0, at::kLong).contiguous();
+  lwl_log_probs_args a = log_probs_args(r, tokens, each, top);
+  const auto floats = logits0.options().dtype(at::kFloat).requires_grad(false);
+  const auto rows = logits0.sizes().slice(0, logits0.dim() - 1);
+  std::vector<int64_t> tops(rows.begin(), rows.end());
+  tops.push_back(top);
+  Judged j;
+  j.log_probs = at::empty(tokens.sizes(), floats);
+  if (entropy) j.entropy = at::empty(rows, floats);
+  if (top > 0) {
+    j.top_log_probs = at::empty(tops, floats);
+    j.top_tokens = at::empty(tops, floats.dtype(at::kLong));
+  }
+  if (keep_stats) j.stats = at::empty({r.outer * r.inner, 2}, floats);
+  a.log_probs = each > 0 ? (float*)j.log_probs.data_ptr() : nullptr;
+  if (each == 0) a.tokens = nullptr;
+  a.entropy = (float*)ptr(j.entropy);
+  a.top_log_probs = (float*)ptr(j.top_log_probs);
+  a.top_tokens = (int64_t*)ptr(j.top_tokens);
+  a.stats = (float*)ptr(j.stats);
+  check(lib.log_probs_forward(&a, stream_of(r.logits)));
+  return j;
+}
+
+variable_list results(const Judged& j) {
+  variable_list out{j.log_probs};
+  for (const Tensor& t : {j.entropy, j.top_log_probs, j.top_tokens})
+    if (t.defined()) out.push_back(t);
+  return out;
+}
+
+struct LogProbsFn : torch::autograd::Function<LogProbsFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& tokens, bool entropy, int64_t top) {
+    const Judged j = log_probs_forward(logits, tokens, entropy, top, true);
+    if (top > 0) ctx->mark_non_differentiable({j.top_tokens});
+    ctx->save_for_backward({logits, tokens, j.stats, j.entropy, j.top_tokens});
+    ctx->set_materialize_grads(false);
+    return results(j);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    const Tensor &logits = s[0], &stats = s[2], &entropy = s[3], &top_tokens = s[4];
+    const Tensor grad_entropy = entropy.defined() ? grads[1] : Tensor();
+    const Tensor grad_top = top_tokens.defined() ? grads[entropy.defined() ? 2 : 1] : Tensor();
+    if (!grads[0].defined() && !grad_entropy.defined() && !grad_top.defined())
+      return {Tensor(), Tensor(), Tensor(), Tensor()};
+    on_one_gpu(logits, s[1], stats, kept(entropy), kept(top_tokens), kept(grads[0]), kept(grad_entropy), kept(grad_top));
+    const int64_t each = tokens_each(logits, s[1]), top = top_tokens.defined() ? top_tokens.size(-1) : 0;
+    const c10::DeviceGuard guard(logits.device());
+    const LogitRows r = logit_rows(logits);
+    const Tensor tokens = typed(s[1], at::kLong).contiguous();
+    const auto rows = logits.sizes().slice(0, logits.dim() - 1);
+    std::vector<int64_t> tops(rows.begin(), rows.end());
+    tops.push_back(top);
+    // saved tensors come back as a caller's hooks left them
+    const auto left = [](const Tensor& t, at::IntArrayRef sizes, at::ScalarType type) {
+      return !t.defined() || (t.sizes() == sizes && t.scalar_type() == type && t.is_contiguous());
+    };
+    if (!left(stats, {r.outer * r.inner, 2}, at::kFloat) || !left(entropy, rows, at::kFloat) ||
+        !left(top_tokens, tops, at::kLong))
+      refuse("token_log_probs backward: statistics ", stats.sizes(), " are not those of logits ", logits.sizes());
+    const auto given = [](const Tensor& g) { return g.defined() ? typed(g, at::kFloat).contiguous() : g; };
+    const Tensor g = given(grads[0]), gh = given(grad_entropy), gt = given(grad_top);
+    const Tensor grad = at::empty(logits.sizes(), logits.options().requires_grad(false));
+    lwl_log_probs_args a = log_probs_args(r, tokens, each, top);
+    a.entropy = (float*)ptr(entropy);
+    a.top_tokens = (int64_t*)ptr(top_tokens);
+    a.stats = (float*)stats.data_ptr();
+    a.grad_log_probs = each > 0 ? (const float*)ptr(g) : nullptr;
+    a.grad_entropy = (const float*)ptr(gh);
+    a.grad_top = (const float*)ptr(gt);
+    a.grad_logits = grad.data_ptr();
+    check(lib.log_probs_backward(&a, stream_of(logits)));
+    return once({grad, Tensor(), Tensor(), Tensor()});
+  }
+};
+
+// (log_probs[, entropy][, top_log_probs, top_tokens])
+variable_list token_log_probs(const Tensor& logits, const Tensor& tokens, bool entropy, int64_t top) {
+  if (at::GradMode::is_enabled() && records(logits)) return LogProbsFn::apply(logits, tokens, entropy, top);
+  return results(log_probs_forward(logits, tokens, entropy, top, false));
 }
 
 // Takes the entries from the library at `path`, which the package has loaded, and the class of its
@@ -591,6 +818,14 @@ void bind(const std::string& path, py::object error_class) {
   get(lib.attention_forward, "lwl_attention_forward");
   get(lib.attention_backward_workspace, "lwl_attention_backward_workspace_size");
   get(lib.attention_backward, "lwl_attention_backward");
+  get(lib.window_forward_workspace, "lwl_attention_window_forward_workspace_size");
+  get(lib.window_forward, "lwl_attention_window_forward");
+  get(lib.window_backward_workspace, "lwl_attention_window_backward_workspace_size");
+  get(lib.window_backward, "lwl_attention_window_backward");
+  get(lib.tree_workspace, "lwl_attention_tree_workspace_size");
+  get(lib.tree_forward, "lwl_attention_tree_forward");
+  get(lib.log_probs_forward, "lwl_log_probs_forward");
+  get(lib.log_probs_backward, "lwl_log_probs_backward");
   argument_error = error_class.release().ptr();
 }
 
@@ -616,4 +851,6 @@ PYBIND11_MODULE(lwl_layers, m) {
   m.def("attention_backward", &attention_backward, release());
   m.def("attention", &attention, release());
   m.def("attention_packed", &attention_packed, release());
+  m.def("attention_tree", &attention_tree, release());
+  m.def("token_log_probs", &token_log_probs, release());
 }

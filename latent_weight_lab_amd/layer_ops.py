@@ -81,12 +81,14 @@ def gelu8_backward(codes: torch.Tensor, scales: torch.Tensor, grad_out: torch.Te
 
 
 def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool, scale: float | None,
-                      key_lengths: torch.Tensor | None, causal_offset: int | None, keep_lse: bool):
+                      key_lengths: torch.Tensor | None, causal_offset: int | None, keep_lse: bool,
+                      window: int | None = None, sinks: int = 0):
     """``(out, lse)`` for ``[batch, heads, tokens, head size]`` tensors; ``out`` lies in memory token by token
     (all heads of a token together); ``lse`` (float32 ``[batch, heads, queries]``) is None unless ``keep_lse``."""
-    return N.layers().attention_forward(q, k, v, causal, scale, key_lengths, causal_offset, keep_lse)
+    return N.layers().attention_forward(q, k, v, causal, scale, key_lengths, causal_offset, keep_lse, window, sinks)
 
 
-def attention_backward(q, k, v, out, lse, grad_out, causal, scale, key_lengths, causal_offset):
+def attention_backward(q, k, v, out, lse, grad_out, causal, scale, key_lengths, causal_offset, window=None, sinks=0):
     """The gradients of q, k and v; each lies in memory token by token, as ``out``."""
-    return N.layers().attention_backward(q, k, v, out, lse, grad_out, causal, scale, key_lengths, causal_offset)
+    return N.layers().attention_backward(q, k, v, out, lse, grad_out, causal, scale, key_lengths, causal_offset, window,
+                                         sinks)
