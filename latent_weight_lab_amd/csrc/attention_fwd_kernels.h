@@ -93,26 +93,93 @@ __device__ __forceinline__ uint64_t line_from(const Line& line, int from) {
   return from < 128 ? line.high >> (from - 64) : 0;
 }
 
-// A tree's rows: those of every query head that shares a key head, so that a workgroup reads the cache for all of
-// them.  The blocks of 128 rows of one range of a key head's cache go to the same die, one after the other.
-struct TreeWork {
-  int64_t b, hk;
-  int block, split;
+// How the sequences' caches are cut into a tree's ranges.  Only the device knows lengths, so the host gives a number of
+// ranges for all sequences together, one for each and `spare` more, and these go to the sequences by their lengths: ranges
+// of `per` tiles, the least number with which `spare` of them hold all tiles.  Lane b gets sequence b's first range
+// and how many it has.
+struct TreeShare {
+  int first, count, per;
+};
+constexpr int kLeastTiles = 4;  // of a range
+__device__ __forceinline__ TreeShare tree_share(const AttnArgs& a) {
+  const int lane = threadIdx.x & 63, keys = (int)a.keys;
+  int len = lane < (int)a.batch ? a.lengths[lane] : 0;
+  len = len < 0 ? 0 : len < keys ? len : keys;
+  const int tiles = (len + kKeys - 1) / kKeys;
+  int total = tiles;
+#pragma unroll
+  for (int k = 1; k < 64; k *= 2) total += __shfl_xor(total, k, 64);
+  total = uniform(total);
+  TreeShare s;
+  s.per = (int)(((uint32_t)total + a.spare - 1) / (uint32_t)a.spare);
+  if (s.per < kLeastTiles) s.per = kLeastTiles;
+  s.count = lane < (int)a.batch ? (int)((uint32_t)(tiles + s.per - 1) / (uint32_t)s.per) : 0;
+  if (lane < (int)a.batch && s.count == 0) s.count = 1;  // writes zeros
+  int last = s.count;
+#pragma unroll
+  for (int k = 1; k < 64; k *= 2) {
+    const int before = __shfl_up(last, k, 64);
+    if (lane >= k) last += before;
+  }
+  s.first = last - s.count;
+  return s;
+}
+
+// A tree's work: range `slot`, keys begin .. end of sequence b.  Without lengths, and for batches of more than 64, every
+// sequence has a.splits ranges of split_len keys.
+struct TreeRange {
   bool any;
+  int64_t b;
+  int slot, begin, end;  // end: as far as the sequence goes
+};
+__device__ __forceinline__ TreeRange tree_range(const AttnArgs& a, int number) {
+  TreeRange r = {false, 0, number, 0, 0};
+  if (a.spare > 0) {
+    const TreeShare s = tree_share(a);
+    const uint64_t hit = __ballot(number >= s.first && number < s.first + s.count);
+    if (hit == 0) return r;
+    const int b = (int)__builtin_ctzll(hit), split = number - uniform(__shfl(s.first, b, 64));
+    r.any = true;
+    r.b = b;
+    r.begin = split * s.per * kKeys;
+    r.end = r.begin + s.per * kKeys;
+  } else {
+    const int rank = (int)((uint32_t)number / (uint32_t)a.splits), split = number - rank * a.splits;
+    r.any = rank < (int)a.batch;
+    if (!r.any) return r;
+    r.b = ranked_sequence(a, rank);
+    r.slot = (int)r.b * a.splits + split;
+    r.begin = split * (int)a.split_len;
+    r.end = r.begin + (int)a.split_len;
+  }
+  return r;
+}
+// A tree's rows are those of every query head that shares a key head, so that a workgroup reads the cache for all of
+// them.  Where rows fill more than one block of 128, the blocks of a range go to the same die, one after the other.
+struct TreeWork {
+  TreeRange range;
+  int hk, block;
 };
 __device__ __forceinline__ TreeWork tree_work(const AttnArgs& a) {
-  const uint32_t kvh = (uint32_t)a.kv_heads, splits = (uint32_t)a.splits, units = (uint32_t)a.batch * kvh * splits;
+  const uint32_t kvh = (uint32_t)a.kv_heads;
   const uint32_t blocks = ((uint32_t)(a.heads / a.kv_heads) * (uint32_t)a.queries + kRows - 1) / kRows;
-  const uint32_t id = blocks == 1 ? work_order(blockIdx.x, gridDim.x, (uint32_t)a.cus) : blockIdx.x;
-  const uint32_t eight = id / (8 * blocks), in = id - eight * 8 * blocks;
-  const uint32_t unit = blocks == 1 ? id : eight * 8 + in % 8;
+  uint32_t unit = blockIdx.x, block = 0;
+  if (blocks > 1) {
+    const uint32_t eight = unit / (8 * blocks), in = unit - eight * 8 * blocks;
+    unit = eight * 8 + in % 8;
+    block = in / 8;
+  }
+  const uint32_t slot = unit / kvh;
   TreeWork w;
-  w.any = unit < units;
-  w.block = uniform((int)(blocks == 1 ? 0 : in / 8));
-  w.hk = uniform((int)(unit % kvh));
-  w.split = uniform((int)(unit / kvh % splits));
-  w.b = w.any ? ranked_sequence(a, uniform((int)(unit / kvh / splits))) : 0;
+  w.hk = uniform((int)(unit - slot * kvh));
+  w.block = uniform((int)block);
+  w.range = tree_range(a, uniform((int)slot));
   return w;
+}
+// Where range `slot` of key head hk leaves row r of it for the join: log sums follow all the outputs.
+__host__ __device__ inline int64_t tree_rows(const AttnArgs& a) { return a.heads / a.kv_heads * a.queries; }
+__device__ __forceinline__ int64_t tree_partial(const AttnArgs& a, int slot, int64_t hk, int64_t r) {
+  return ((int64_t)slot * a.kv_heads + hk) * tree_rows(a) + r;
 }
 
 template <class T, int DP, bool FAST, int MASK>
@@ -125,11 +192,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_rows(co
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = uniform((int)threadIdx.x >> 6);
   int64_t b, hk, h;
-  int block, split;
+  int block, split, tree_begin = 0, tree_end = 0;
   if constexpr (MASK == kTree) {
     const TreeWork w = tree_work(a);
-    if (!w.any) return;
-    b = w.b, hk = w.hk, h = 0, block = w.block, split = w.split;
+    if (!w.range.any) return;
+    b = w.range.b, hk = w.hk, h = 0, block = w.block, split = w.range.slot;
+    tree_begin = w.range.begin, tree_end = w.range.end;
   } else {
     const RowsWork w = rows_work(a);
     b = w.b, hk = w.hk, h = w.h, block = w.block, split = w.split;
@@ -153,10 +221,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_rows(co
   Walk<MASK, kKeys> at;
   if constexpr (MASK == kWindow) {
     at = window_walk<kKeys>(a, allow, q0, std::min(q0 + kRows, queries) - 1, split, 0);
+  } else if constexpr (MASK == kTree) {
+    at.j = std::min(tree_begin, allow.len);
+    at.end = std::min(tree_end, allow.len);
   } else {
     at.j = std::min(split * (int)a.split_len, allow.len);
-    at.end = std::min(MASK == kTree ? allow.len : key_end(allow, std::min(q0 + kRows, queries) - 1),
-                      at.j + (int)a.split_len);
+    at.end = std::min(key_end(allow, std::min(q0 + kRows, queries) - 1), at.j + (int)a.split_len);
   }
   const int end = at.end;
   // keys below free_end are seen by every query of the wave, keys from wave_end on by none; within a window also, but
@@ -326,10 +396,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_rows(co
   if (!live) return;
   const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
   const float lse = sum > 0.0f ? top + log2_hw(sum) : (sum == 0.0f ? -INFINITY : sum);
-  const int64_t rows = a.batch * a.heads * a.queries, row = (b * a.heads + h) * a.queries + q;
-  if (a.splits > 1) {
-    if (half == 0) a.work[rows * a.splits * dim + row * a.splits + split] = lse;
-    store_result<float, DP, FAST>(a.work + (row * a.splits + split) * dim, o, inv, dim);
+  const int64_t row = (b * a.heads + h) * a.queries + q;
+  const int64_t rows = MASK == kTree ? a.kv_heads * tree_rows(a) : a.batch * a.heads * a.queries;
+  const bool ranges = MASK == kTree ? a.slots > a.batch : a.splits > 1;
+  if (ranges) {
+    const int64_t part = MASK == kTree ? tree_partial(a, split, hk, wave_row) : row * a.splits + split;
+    if (half == 0) a.work[rows * (MASK == kTree ? a.slots : a.splits) * dim + part] = lse;
+    if (MASK != kAll && lse == -INFINITY) return;  // the join does not read it
+    store_result<float, DP, FAST>(a.work + part * dim, o, inv, dim);
     return;
   }
   if (a.lse && half == 0) a.lse[row] = lse * kLn2;
@@ -359,8 +433,17 @@ __global__ __launch_bounds__(256) void attention_token(const AttnArgs a) {
   const uint32_t kvh = (uint32_t)a.kv_heads, batch = (uint32_t)a.batch;
   const uint32_t id = a.lengths ? work_order(blockIdx.x, gridDim.x, (uint32_t)a.cus) : blockIdx.x;
   const int group = uniform((int)((uint32_t)a.heads / kvh));
-  const int64_t hk = uniform((int)(id % kvh)), b = ranked_sequence(a, uniform((int)(id / kvh % batch)));
-  const int split = uniform((int)(id / kvh / batch));
+  const int64_t hk = uniform((int)(id % kvh));
+  int64_t b;
+  int split, tree_begin = 0, tree_end = 0;
+  if constexpr (MASK == kTree) {
+    const TreeRange r = tree_range(a, uniform((int)(id / kvh)));
+    if (!r.any) return;
+    b = r.b, split = r.slot, tree_begin = r.begin, tree_end = r.end;
+  } else {
+    b = ranked_sequence(a, uniform((int)(id / kvh % batch)));
+    split = uniform((int)(id / kvh / batch));
+  }
   const int dim = (int)a.dim, queries = (int)a.queries, rows_here = group * queries;
   const Allowed allow = allowed_keys(a, b);
   const int row = lane & 15;  // this lane's column of the products: query row % queries of head row / queries
@@ -373,10 +456,13 @@ __global__ __launch_bounds__(256) void attention_token(const AttnArgs a) {
   Walk<MASK, kStep, kWaves> at;
   if constexpr (MASK == kWindow) {
     at = window_walk<kStep, kWaves>(a, allow, 0, queries - 1, split, wave);
+  } else if constexpr (MASK == kTree) {
+    at.j = std::min(tree_begin, allow.len) + wave * kStep;
+    at.end = std::min(tree_end, allow.len);
   } else {
     const int begin = std::min(split * (int)a.split_len, allow.len);
     at.j = begin + wave * kStep;
-    at.end = std::min(MASK == kTree ? allow.len : key_end(allow, queries - 1), begin + (int)a.split_len);
+    at.end = std::min(key_end(allow, queries - 1), begin + (int)a.split_len);
   }
   const T* kp = (const T*)a.k + b * a.ks[0] + hk * a.ks[1];
   const T* vp = (const T*)a.v + b * a.vs[0] + hk * a.vs[1];
@@ -501,7 +587,8 @@ __global__ __launch_bounds__(256) void attention_token(const AttnArgs a) {
     lds_stat[wave][1][row] = sum;
   }
   __syncthreads();
-  const int64_t rows = a.batch * a.heads * a.queries;
+  const int64_t rows = MASK == kTree ? a.kv_heads * tree_rows(a) : a.batch * a.heads * a.queries;
+  const bool ranges = MASK == kTree ? a.slots > a.batch : a.splits > 1;
   for (int i = threadIdx.x; i < rows_here * DP; i += 256) {
     const int rr = i / DP, col = i % DP;
     float m = lds_stat[0][0][rr];
@@ -518,9 +605,10 @@ __global__ __launch_bounds__(256) void attention_token(const AttnArgs a) {
     const float lse = total > 0.0f ? m + log2_hw(total) : (total == 0.0f ? -INFINITY : total);
     const int64_t hh = hk * group + rr / queries, qq = rr % queries, out_row = (b * a.heads + hh) * queries + qq;
     if (col >= dim) continue;
-    if (a.splits > 1) {
-      a.work[(out_row * a.splits + split) * dim + col] = v;
-      if (col == 0) a.work[rows * a.splits * dim + out_row * a.splits + split] = lse;
+    if (ranges) {
+      const int64_t part = MASK == kTree ? tree_partial(a, split, hk, rr) : out_row * a.splits + split;
+      if (MASK == kAll || lse != -INFINITY) a.work[part * dim + col] = v;
+      if (col == 0) a.work[rows * (MASK == kTree ? a.slots : a.splits) * dim + part] = lse;
     } else {
       ((T*)a.out)[b * a.os[0] + hh * a.os[1] + qq * a.os[2] + col] = (T)v;
       if (a.lse && col == 0) a.lse[out_row] = lse * kLn2;
@@ -533,47 +621,65 @@ __global__ __launch_bounds__(256) void attention_token(const AttnArgs a) {
 // where there are many the workgroup has 16 chunks or fewer, one row's, and its SHARE = 16 threads of a chunk take every
 // 16th range each and add up through LDS in their order.
 constexpr int kMaxSplits = 512, kSplitsAlone = 16;
-template <class T, int SHARE>
+template <class T, int SHARE, int MASK>
 __global__ __launch_bounds__(256) void attention_join(const AttnArgs a) {
   constexpr int CHUNKS = 256 / SHARE;
-  static_assert(SHARE == 1 || CHUNKS * 8 == kAttnMaxDim);
-  __shared__ float lds_v[SHARE][CHUNKS][8], lds_m[SHARE], lds_t[SHARE];
-  const int dim = (int)a.dim, splits = a.splits, per_row = (dim + 7) / 8;
-  const uint32_t rows_wg = SHARE == 1 ? 256 / per_row : 1, rows = (uint32_t)(a.batch * a.heads * a.queries);
+  static_assert(CHUNKS * 8 >= kAttnMaxDim);
+  __shared__ float lds_v[SHARE][CHUNKS][8], lds_m[SHARE][CHUNKS], lds_t[SHARE][CHUNKS];
+  const int dim = (int)a.dim, per_row = (dim + 7) / 8;
+  const uint32_t rows_wg = CHUNKS / per_row, rows = (uint32_t)(a.batch * a.heads * a.queries);
   const int part_no = threadIdx.x / CHUNKS, chunk = threadIdx.x % CHUNKS, r = chunk / per_row;
   const int col = (chunk - r * per_row) * 8;
   const uint32_t row = blockIdx.x * rows_wg + r;
   const bool live = (uint32_t)r < rows_wg && row < rows;
-  const int64_t first = (int64_t)(live ? row : 0) * splits;
-  const float* lses = a.work + (int64_t)rows * splits * dim + first;
+  int splits = a.splits;
+  int64_t first = (int64_t)(live ? row : 0) * splits, step = 1, all = (int64_t)rows * splits;  // partial rows
+  if constexpr (MASK == kTree) {
+    const uint32_t head_row = live ? row : 0, q = head_row % (uint32_t)a.queries, head = head_row / (uint32_t)a.queries;
+    const uint32_t group = (uint32_t)(a.heads / a.kv_heads), b = head / (uint32_t)a.heads, h = head - b * (uint32_t)a.heads;
+    int slot = (int)b * splits;
+    if (a.spare > 0) {
+      const TreeShare s = tree_share(a);
+      slot = __shfl(s.first, (int)b, 64);
+      splits = __shfl(s.count, (int)b, 64);
+    }
+    first = tree_partial(a, slot, h / group, (int64_t)(h % group) * a.queries + q);
+    step = a.kv_heads * tree_rows(a);
+    all = step * a.slots;
+  }
+  const float* lses = a.work + all * dim + first;
   const float* part = a.work + first * dim + col;
   float m = -FLT_MAX, total = 0.0f, v[8] = {};
-  for (int s = part_no; s < splits; s += SHARE) m = max_nan(m, lses[s]);
+  for (int s = part_no; s < splits; s += SHARE) m = max_nan(m, lses[s * step]);
   if constexpr (SHARE > 1) {
-    if (chunk == 0) lds_m[part_no] = m;
+    lds_m[part_no][chunk] = m;
     __syncthreads();
 #pragma unroll
-    for (int g = 0; g < SHARE; ++g) m = max_nan(m, lds_m[g]);
+    for (int g = 0; g < SHARE; ++g) m = max_nan(m, lds_m[g][chunk]);
   }
   if (live) {
 #pragma unroll 4
     for (int s = part_no; s < splits; s += SHARE) {
       float x[8];
-      load8(x, part + (int64_t)s * dim, dim - col);  // written, zeros where nothing is held
-      const float w = exp2_hw(lses[s] - m);          // 0 for a range that holds nothing
+      load8(x, part + s * step * dim, dim - col);
+      const float w = exp2_hw(lses[s * step] - m);  // 0 for a range that holds nothing
+      if constexpr (MASK != kAll) {                 // whose output is not written
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = w > 0.0f ? x[i] : 0.0f;
+      }
       total += w;
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] += w * x[i];
     }
   }
   if constexpr (SHARE > 1) {
-    if (chunk == 0) lds_t[part_no] = total;
+    lds_t[part_no][chunk] = total;
 #pragma unroll
     for (int i = 0; i < 8; ++i) lds_v[part_no][chunk][i] = v[i];
     __syncthreads();
     total = 0.0f;
 #pragma unroll
-    for (int g = 0; g < SHARE; ++g) total += lds_t[g];
+    for (int g = 0; g < SHARE; ++g) total += lds_t[g][chunk];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       v[i] = 0.0f;
@@ -609,8 +715,8 @@ void plan_splits(AttnArgs& a) {
   int64_t splits = 1;
   // keys of the longest walk
   const int64_t keys = MASK == kWindow ? window_tiles(a, kRows) * kKeys : a.keys;
-  if (MASK == kTree || by_token(a)) {
-    const int64_t wgs = std::max<int64_t>(1, a.batch * a.kv_heads * (MASK == kTree ? tree_blocks(a) : 1));
+  if (by_token(a)) {
+    const int64_t wgs = std::max<int64_t>(1, a.batch * a.kv_heads);
     splits = std::min({2 * cus / wgs, keys / 256, (int64_t)kMaxSplits});
   } else {
     const double unit = (double)((a.dim + 31) / 32 * 32) / 64;
@@ -640,16 +746,48 @@ void plan_splits(AttnArgs& a) {
   a.splits = splits > 1 ? (int)((keys + a.split_len - 1) / a.split_len) : 1;
 }
 
+// A tree's ranges (tree_share): as many as make one workgroup for each compute unit, for a workgroup leaves up to 128 rows
+// of float32 outputs however short its range, or two where one would leave sequences whole; single tokens' kernel
+// two.  Where sequences alone are as many, none is cut.  bfloat16, us with the join: 16 sequences of up to 8192 tokens, 32
+// nodes, 16 heads on 4 of size 128, 48 more ranges than sequences 51 (one workgroup), 112 more 55, none 161; 65536 tokens,
+// 61 nodes, 16 heads on 2 of size 128, 32 ranges (one workgroup) 59, 64 59, 16 94; 64 x 12 sequences and heads of up to 1024
+// tokens of size 64, 20 nodes, none cut 27, with ranges 34.
+inline void plan_tree(AttnArgs& a) {
+  const int64_t cus = device_cus(), units = std::max<int64_t>(1, a.kv_heads * tree_blocks(a)), batch = a.batch;
+  const int64_t tiles = (a.keys + kKeys - 1) / kKeys;
+  a.splits = 1;
+  a.spare = 0;
+  a.split_len = std::max<int64_t>(a.keys, 1);
+  int64_t ranges = (by_token(a) ? 2 : 1) * cus / units;
+  if (ranges < 2 * batch) ranges = 2 * cus / units;
+  if (ranges >= 2 * batch && tiles >= 2 * kLeastTiles) {
+    if (a.lengths && batch <= kMostRanked) {
+      // no more than there are tiles for; sequences' own come on top
+      a.spare = (int)std::min(ranges - batch, batch * ((tiles + kLeastTiles - 1) / kLeastTiles));
+    } else {
+      const int64_t per = std::max<int64_t>(kLeastTiles, (tiles + ranges / batch - 1) / (ranges / batch));
+      a.splits = (int)((tiles + per - 1) / per);
+      a.split_len = per * kKeys;
+    }
+  }
+  a.slots = (int)(a.spare > 0 ? batch + a.spare : batch * a.splits);
+}
+template <int MASK>
+void plan(AttnArgs& a) {
+  if constexpr (MASK == kTree) plan_tree(a);
+  else plan_splits<MASK>(a);
+}
+
 template <class T, int DP, int MASK>
 hipError_t run(const AttnArgs& a, hipStream_t s) {
   if (by_token(a)) {
-    const int64_t grid = a.batch * a.kv_heads * a.splits;
+    const int64_t grid = a.kv_heads * (MASK == kTree ? (int64_t)a.slots : a.batch * a.splits);
     if (a.dim % 8 == 0) hipLaunchKernelGGL((attention_token<T, DP, true, MASK>), dim3((unsigned)grid), dim3(256), 0, s, a);
     else hipLaunchKernelGGL((attention_token<T, DP, false, MASK>), dim3((unsigned)grid), dim3(256), 0, s, a);
   } else {
     int64_t works = a.batch * a.heads * a.splits * ((a.queries + kRows - 1) / kRows);
     if (MASK == kTree) {
-      const int64_t units = a.batch * a.kv_heads * a.splits, blocks = tree_blocks(a);
+      const int64_t units = a.kv_heads * a.slots, blocks = tree_blocks(a);
       works = blocks == 1 ? units : (units + 7) / 8 * 8 * blocks;
     }
     const dim3 grid((unsigned)works);
@@ -659,13 +797,18 @@ hipError_t run(const AttnArgs& a, hipStream_t s) {
       hipLaunchKernelGGL((attention_rows<T, DP, false, MASK>), grid, dim3(256), 0, s, a);
   }
   hipError_t e = hipGetLastError();
-  if (e != hipSuccess || a.splits == 1) return e;
+  if (e != hipSuccess || !(MASK == kTree ? a.slots > a.batch : a.splits > 1)) return e;
   const int64_t rows = a.batch * a.heads * a.queries;
-  const int64_t rows_wg = 256 / ((a.dim + 7) / 8);
-  if (a.splits > kSplitsAlone)
-    hipLaunchKernelGGL((attention_join<T, 16>), dim3((unsigned)rows), dim3(256), 0, s, a);
+  const int64_t per_row = (a.dim + 7) / 8, ranges = MASK == kTree ? a.slots / a.batch : a.splits;
+  const auto grid = [&](int64_t chunks) { return dim3((unsigned)((rows + chunks / per_row - 1) / (chunks / per_row))); };
+  // Threads for a chunk of a row.  A tree's ranges of 4 for each, where 1024 workgroups hold them: 4096 rows of size 128 with
+  // 8 ranges 7.1, 5.6 and 15 us with 1, 4 and 16, 976 rows with 64 ranges 29, 12 and 11, 8192 rows with 4 ranges 7.6, 9.2 and 37.
+  if (MASK == kTree && ranges >= 4 && ranges <= 2 * kSplitsAlone && grid(64).x <= 1024)
+    hipLaunchKernelGGL((attention_join<T, 4, MASK>), grid(64), dim3(256), 0, s, a);
+  else if (ranges > kSplitsAlone)
+    hipLaunchKernelGGL((attention_join<T, 16, MASK>), grid(16), dim3(256), 0, s, a);
   else
-    hipLaunchKernelGGL((attention_join<T, 1>), dim3((unsigned)((rows + rows_wg - 1) / rows_wg)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((attention_join<T, 1, MASK>), grid(256), dim3(256), 0, s, a);
   return hipGetLastError();
 }
 
@@ -682,12 +825,13 @@ hipError_t run_dim(const AttnArgs& a, hipStream_t s) {
 
 template <int MASK>
 int64_t fwd_work(AttnArgs a) {
-  plan_splits<MASK>(a);
+  plan<MASK>(a);
+  if (MASK == kTree) return a.slots > a.batch ? (int64_t)a.slots * a.kv_heads * tree_rows(a) * (a.dim + 1) : 0;
   return a.splits > 1 ? (int64_t)a.splits * a.batch * a.heads * a.queries * (a.dim + 1) : 0;
 }
 template <int MASK>
 hipError_t launch_fwd(AttnArgs a, hipStream_t s) {
-  plan_splits<MASK>(a);
+  plan<MASK>(a);
   a.cus = (int)device_cus();
   switch (a.dtype) {
     case kF32: return run_dim<float, MASK>(a, s);

@@ -93,6 +93,7 @@ struct AttnArgs {
   // of a tree: [batch][queries]
   const int32_t* parents;
   int64_t parents_stride;
+  int slots, spare;  // ranges of a key head's caches, all sequences together; of these more than one for each
 };
 constexpr int kTileRows = 64;  // tokens of a tile
 // Whether a tensor of values of `size` bytes can be read in tiles by 32-bit offsets from a tile's first row:

@@ -65,18 +65,41 @@ __device__ __forceinline__ void raise(Sums& t, float next) {
   t.s *= shrink;
   t.m = next;
 }
+// Over LANES consecutive lanes; all of them get it.
+template <bool ENTROPY, int LANES>
+__device__ __forceinline__ void join_lanes(Sums& t) {
+  float m = t.m;
+#pragma unroll
+  for (int k = 1; k < LANES; k *= 2) m = fmaxf(m, __shfl_xor(m, k, 64));
+  raise<ENTROPY>(t, m);
+  t.s = lanes_sum<LANES>(t.s);
+  if constexpr (ENTROPY) t.a = lanes_sum<LANES>(t.a);
+}
 
+// A thread's sums are taken relative to its largest value when that was last raised, which happens where one lies more
+// than this above it, and to the largest at the end.
+constexpr float kSlack = 8.0f;
 constexpr int kCandidates = 1024;
+constexpr int kGroups = 128;  // of threads, whose largest values bound the alternatives: more than of these
 
-template <class T, int THREADS, bool ENTROPY, bool TOP>
+template <class T, int THREADS, int U, bool ENTROPY, bool TOP>
 __global__ __launch_bounds__(THREADS) void log_probs_forward(const LogProbArgs a) {
-  constexpr int WAVES = THREADS / 64, U = 4;  // chunks of a thread under way
-  __shared__ float lds_m[WAVES], lds_s[WAVES], lds_a[WAVES];
+  constexpr int WAVES = THREADS / 64;
+  __shared__ float lds_sums[3][WAVES];
   __shared__ uint64_t lds_best[TOP ? THREADS : 1], lds_cand[TOP ? kCandidates : 1], lds_bound;
-  __shared__ int lds_count;
+  __shared__ int lds_count, lds_hot[TOP ? THREADS : 1], lds_hot_count;
   const int64_t row = blockIdx.x;
   const T* x = row_of<T>(a, row);
   const int vocab = (int)a.vocab, chunks = (vocab + 7) / 8;
+  Raw8<T> raw[U];
+  const auto load = [&](int base) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int c = base + u * THREADS + (int)threadIdx.x;
+      load_raw8(raw[u], x + (int64_t)c * 8, c < chunks ? vocab - c * 8 : 0);
+    }
+  };
+  load(0);
   int64_t token = -1;
   float asked = 0.0f;
   if ((int)threadIdx.x < a.each) {
@@ -85,68 +108,60 @@ __global__ __launch_bounds__(THREADS) void log_probs_forward(const LogProbArgs a
   }
   Sums t = {-FLT_MAX, 0.0f, 0.0f};
   float best = -INFINITY;
-  uint32_t best_chunk = 0;
-  bool any = false;
-  for (int c0 = threadIdx.x; c0 < chunks; c0 += THREADS * U) {
-    Raw8<T> raw[U];
+  uint32_t best_chunk = threadIdx.x;
+  for (int base = 0; base < chunks; base += THREADS * U) {
+    if (base > 0) load(base);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int c = c0 + u * THREADS;
-      load_raw8(raw[u], x + (int64_t)c * 8, c < chunks ? vocab - c * 8 : 0);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int c = c0 + u * THREADS;
+      const int c = base + u * THREADS + (int)threadIdx.x;
+      if (c >= chunks) break;
       float v[8];
       chunk_values(v, raw[u], vocab - c * 8);
       const float most = max_nan(max_nan(max_nan(v[0], v[1]), max_nan(v[2], v[3])),
                                  max_nan(max_nan(v[4], v[5]), max_nan(v[6], v[7])));
       if constexpr (TOP) {
-        if (c < chunks && (!any || !(most <= best) && best == best)) {  // the first NaN stays
+        if (!(most <= best) && best == best) {  // the first of equal ones; a NaN stays
           best = most;
           best_chunk = (uint32_t)c;
-          any = true;
         }
+      } else {
+        best = max_nan(best, most);
       }
-      if (__any(most > t.m)) raise<ENTROPY>(t, fmaxf(t.m, most));
+      if (__any(most > t.m + kSlack)) raise<ENTROPY>(t, fmaxf(t.m, most));
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float d = v[i] - t.m, e = exp2_hw(d * kLog2E);
         t.s += e;
-        if constexpr (ENTROPY) t.a = fmaf(e, fmaxf(d, -FLT_MAX), t.a);
+        if constexpr (ENTROPY) t.a = fmaf(e, max_nan(d, -FLT_MAX), t.a);
       }
     }
   }
-  // over the wave, then over the waves
-#pragma unroll
-  for (int k = 1; k < 64; k *= 2) {
-    const float m = __shfl_xor(t.m, k, 64), next = fmaxf(t.m, m);
-    Sums o = {m, __shfl_xor(t.s, k, 64), ENTROPY ? __shfl_xor(t.a, k, 64) : 0.0f};
-    raise<ENTROPY>(t, next);
-    raise<ENTROPY>(o, next);
-    t.s += o.s;
-    t.a += o.a;
-  }
+  raise<ENTROPY>(t, fmaxf(t.m, best));
+  join_lanes<ENTROPY, 64>(t);
   if ((threadIdx.x & 63) == 0) {
-    lds_m[threadIdx.x >> 6] = t.m;
-    lds_s[threadIdx.x >> 6] = t.s;
-    lds_a[threadIdx.x >> 6] = t.a;
+    lds_sums[0][threadIdx.x >> 6] = t.m;
+    lds_sums[1][threadIdx.x >> 6] = t.s;
+    lds_sums[2][threadIdx.x >> 6] = t.a;
   }
+  uint64_t mine = 0;
   if constexpr (TOP) {
-    // threads without a chunk come last
-    lds_best[threadIdx.x] = any ? pair_of(order_of(best), best_chunk) : (uint64_t)threadIdx.x;
-    if (threadIdx.x == 0) lds_count = 0;
+    // threads without a value come last, each with a number of its own
+    mine = (int)threadIdx.x < chunks ? pair_of(order_of(best), best_chunk) : (uint64_t)threadIdx.x;
+    uint64_t group = mine;
+#pragma unroll
+    for (int k = 1; k < THREADS / kGroups; k *= 2) {
+      const uint64_t other = (uint64_t)__shfl_xor((unsigned long long)group, k, 64);
+      group = other > group ? other : group;
+    }
+    lds_best[threadIdx.x] = mine;
+    if (threadIdx.x % (THREADS / kGroups) == 0) lds_cand[threadIdx.x / (THREADS / kGroups)] = group;
+    if (threadIdx.x == 0) lds_count = lds_hot_count = 0;
   }
   __syncthreads();
-  t = {lds_m[0], lds_s[0], lds_a[0]};
-#pragma unroll
-  for (int w = 1; w < WAVES; ++w) {
-    Sums o = {lds_m[w], lds_s[w], lds_a[w]};
-    const float next = fmaxf(t.m, o.m);
-    raise<ENTROPY>(t, next);
-    raise<ENTROPY>(o, next);
-    t.s += o.s;
-    t.a += o.a;
+  {
+    const int w = threadIdx.x % WAVES;
+    t = {lds_sums[0][w], lds_sums[1][w], lds_sums[2][w]};
+    join_lanes<ENTROPY, WAVES>(t);
   }
   const bool empty = t.s == 0.0f;  // nothing but minus infinities
   const float log_s = __logf(t.s);
@@ -163,61 +178,74 @@ __global__ __launch_bounds__(THREADS) void log_probs_forward(const LogProbArgs a
   }
   if constexpr (TOP) {
     const int top = a.top;
-    const uint64_t mine = lds_best[threadIdx.x];
-    int rank = 0;
-    for (int i = 0; i < THREADS; ++i) rank += lds_best[i] > mine;
-    if (rank == top - 1) lds_bound = mine;
+    {
+      // the groups' ranks, each counted by a few lanes
+      constexpr int LANES = THREADS / kGroups, PER = kGroups / LANES;
+      const int part = threadIdx.x % LANES;
+      const uint64_t group = lds_cand[threadIdx.x / LANES];
+      int rank = 0;
+#pragma unroll 16
+      for (int i = 0; i < PER; ++i) rank += lds_cand[i * LANES + part] > group;
+#pragma unroll
+      for (int k = 1; k < LANES; k *= 2) rank += __shfl_xor(rank, k, 64);
+      if (rank == top - 1 && part == 0) lds_bound = group;
+    }
     __syncthreads();
     uint64_t bound = lds_bound;
-    const auto candidates = [&](int c, const Raw8<T>& raw) {
+    // lds_cand held the groups
+    const auto candidates = [&](int c, const Raw8<T>& chunk) {
       float v[8];
-      chunk_values(v, raw, vocab - c * 8);
+      chunk_values(v, chunk, vocab - c * 8);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const uint32_t order = order_of(v[i]);
-        // the bound names a chunk, or after a selection a place in one
         if (c * 8 + i < vocab && pair_of(order, (uint32_t)c) >= bound) {
           const int at = atomicAdd(&lds_count, 1);
           if (at < kCandidates) lds_cand[at] = pair_of(order, (uint32_t)(c * 8 + i));
         }
       }
     };
-    if (mine >= bound && any) {
-      for (int c0 = threadIdx.x; c0 < chunks; c0 += THREADS * U) {
-        Raw8<T> raw[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int c = c0 + u * THREADS;
-          load_raw8(raw[u], x + (int64_t)c * 8, c < chunks ? vocab - c * 8 : 0);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-          if (c0 + u * THREADS < chunks) candidates(c0 + u * THREADS, raw[u]);
+    // The chunks of the threads that pass are looked at by all threads: their own would read them one after the other.
+    if (mine >= bound && (int)threadIdx.x < chunks) lds_hot[atomicAdd(&lds_hot_count, 1)] = (int)threadIdx.x;
+    __syncthreads();
+    const int hot = lds_hot_count, looks = hot * ((chunks + THREADS - 1) / THREADS);
+    for (int i = threadIdx.x; i < looks; i += THREADS) {
+      const int n = i / hot, c = n * THREADS + lds_hot[i - n * hot];
+      if (c < chunks) {
+        Raw8<T> chunk;
+        load_raw8(chunk, x + (int64_t)c * 8, vocab - c * 8);
+        candidates(c, chunk);
       }
     }
     __syncthreads();
     int count = lds_count;
     if (count > kCandidates) {
-      // Few threads hold many of the largest values (sorted rows): the same chunk by chunk in step, and whenever the
-      // next chunks may not fit, all but the `top` largest so far are dropped.
-      __syncthreads();
+      // Few threads hold many of the largest values (sorted rows).  With the bound of single threads no more than `top` of
+      // them pass; they go chunk by chunk in step, and whenever the next chunks may not fit, all but the `top` largest
+      // so far are dropped.
+      int rank = 0;
+      for (int i = 0; i < THREADS; ++i) rank += lds_best[i] > mine;
+      __syncthreads();  // all have read count
       if (threadIdx.x == 0) lds_count = 0;
+      if (rank == top - 1) lds_bound = mine;
       __syncthreads();
-      for (int c0 = 0; c0 < chunks; c0 += THREADS) {
-        const int c = c0 + (int)threadIdx.x;
+      bound = lds_bound;
+      for (int base = 0; base < chunks; base += THREADS) {
+        const int c = base + (int)threadIdx.x;
         if (c < chunks && mine >= bound) {
-          Raw8<T> raw;
-          load_raw8(raw, x + (int64_t)c * 8, vocab - c * 8);
-          candidates(c, raw);
+          Raw8<T> chunk;
+          load_raw8(chunk, x + (int64_t)c * 8, vocab - c * 8);
+          candidates(c, chunk);
         }
         __syncthreads();
         count = lds_count;
         __syncthreads();  // all have read it
         if (count + top * 8 > kCandidates) {
-          uint64_t keep[kCandidates / THREADS];
-          int at[kCandidates / THREADS];
+          constexpr int PER = (kCandidates + THREADS - 1) / THREADS;
+          uint64_t keep[PER];
+          int at[PER];
 #pragma unroll
-          for (int k = 0; k < kCandidates / THREADS; ++k) {
+          for (int k = 0; k < PER; ++k) {
             const int i = threadIdx.x + k * THREADS;
             keep[k] = i < count ? lds_cand[i] : 0;
             at[k] = 0;
@@ -226,7 +254,7 @@ __global__ __launch_bounds__(THREADS) void log_probs_forward(const LogProbArgs a
           }
           __syncthreads();
 #pragma unroll
-          for (int k = 0; k < kCandidates / THREADS; ++k)
+          for (int k = 0; k < PER; ++k)
             if ((int)threadIdx.x + k * THREADS < count && at[k] < top) lds_cand[at[k]] = keep[k];
           if (threadIdx.x == 0) lds_count = top;
           __syncthreads();
@@ -237,6 +265,7 @@ __global__ __launch_bounds__(THREADS) void log_probs_forward(const LogProbArgs a
     for (int i = threadIdx.x; i < count; i += THREADS) {
       const uint64_t one = lds_cand[i];
       int place = 0;
+#pragma unroll 4
       for (int j = 0; j < count; ++j) place += lds_cand[j] > one;
       if (place < top) {
         a.top_log_probs[row * top + place] = empty ? -INFINITY : (value_of((uint32_t)(one >> 32)) - t.m) - log_s;
@@ -314,20 +343,24 @@ __global__ __launch_bounds__(256) void log_probs_backward(const LogProbArgs a, u
   }
 }
 
-template <class T, int THREADS>
+template <class T, int THREADS, int U>
 void forward(const LogProbArgs& a, hipStream_t s) {
   const dim3 grid((unsigned)(a.outer * a.inner)), block(THREADS);
   if (a.top > 0) {
-    if (a.entropy) hipLaunchKernelGGL((log_probs_forward<T, THREADS, true, true>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((log_probs_forward<T, THREADS, false, true>), grid, block, 0, s, a);
+    if (a.entropy) hipLaunchKernelGGL((log_probs_forward<T, THREADS, U, true, true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((log_probs_forward<T, THREADS, U, false, true>), grid, block, 0, s, a);
   } else {
-    if (a.entropy) hipLaunchKernelGGL((log_probs_forward<T, THREADS, true, false>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((log_probs_forward<T, THREADS, false, false>), grid, block, 0, s, a);
+    if (a.entropy) hipLaunchKernelGGL((log_probs_forward<T, THREADS, U, true, false>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((log_probs_forward<T, THREADS, U, false, false>), grid, block, 0, s, a);
   }
 }
+// 512 threads hold 16384 logits of a row at a time, which keeps memory busy; 256 lose less at the ends of short rows.
+// bfloat16, 512 and 256 threads: 8192 x 50257 168 and 172 us; with five alternatives and the entropy 1 x 200000 21 and
+// 32 us, 16 x 50304 10.1 and 12.4, 2048 x 16000 21 and 20, 2048 x 4000 16 and 13.  With 1024: 184, 20, 10.0, 32, 28 us.
 template <class T>
 hipError_t run_forward(const LogProbArgs& a, hipStream_t s) {
-  forward<T, 256>(a, s);
+  if (a.vocab > 16384) forward<T, 512, 4>(a, s);
+  else forward<T, 256, 4>(a, s);
   return hipGetLastError();
 }
 
