@@ -207,9 +207,8 @@ __global__ __launch_bounds__(256, (kKeysOccupancy<T, DP>)) void attention_bwd_ke
     if (more) fetch(next_g, next_q);
     if (q0 + kTile > wave_first && (MASK != kWindow || q0 < wave_last)) {
       // some pair of the tile is not allowed
-      bool masked = key_end(allow, q0) < wk0 + 32;
-      if constexpr (MASK == kWindow)
-        masked |= window_begin(allow, q0 + kTile - 1) > wk0 && wk0 + 32 > allow.sinks;
+      const bool masked = key_end(allow, q0) < wk0 + 32;
+      const bool passed = MASK == kWindow && window_begin(allow, q0 + kTile - 1) > wk0 && wk0 + 32 > allow.sinks;
 #pragma unroll kUnroll<T, DP>
       for (int t = 0; t < 2; ++t) {
         const int at = t * 32;
@@ -278,15 +277,24 @@ __global__ __launch_bounds__(256, (kKeysOccupancy<T, DP>)) void attention_bwd_ke
           }
           dp[r] *= s[r];
         }
-        if (masked) {
+        if constexpr (MASK == kWindow) {
+          if (masked || passed) {
+            // the queries from this key's position on, as far as its window reaches: their tile's bits
+            const int from = key < allow.len ? key - allow.off : queries;
+            const Seen seen = seen_keys(q0, lane_last, from, INT32_MIN);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const uint32_t mask = bit_mask(t ? seen.w[1] : seen.w[0], (r >> 2) * 8 + (r & 3));
+              s[r] = masked_term(s[r], mask);
+              dp[r] = masked_term(dp[r], mask);
+            }
+          }
+        } else if (masked) {
           // key < key_end(q), that is q >= key - off
           const int from = key < allow.len ? key - allow.off - q0 - at - half * 4 : kTile;
-          const int to = lane_last - q0 - at - half * 4;  // and within a window, q < lane_last
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int n = (r >> 2) * 8 + (r & 3);
-            if (n < from || (MASK == kWindow && n >= to)) s[r] = dp[r] = 0.0f;
-          }
+          for (int r = 0; r < 16; ++r)
+            if ((r >> 2) * 8 + (r & 3) < from) s[r] = dp[r] = 0.0f;
         }
         if constexpr (kHold<T>) {
           float most = 0.0f;
@@ -498,13 +506,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_bwd_que
         }
         // dp: may be NaN where masked
         if constexpr (MASK == kWindow) {
-          if (j0 + kTile > std::min(free_end, at.stop()) || (j0 < free_begin && j0 + kTile > allow.sinks)) {
-            const int first = j0 + t * 32 + half * 4, lim = std::min(q_end, at.stop()) - first, from = q_begin - first,
-                      sinks = allow.sinks - first;
+          if (j0 + kTile > std::min(free_end, at.stop()) ||
+              (j0 < free_begin && std::min(j0 + kTile, at.stop()) > allow.sinks)) {
+            const Seen seen = seen_keys(j0, std::min(q_end, at.stop()), q_begin, allow.sinks);
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-              const int n = (r >> 2) * 8 + (r & 3);
-              if (n >= lim || (n < from && n >= sinks)) s[r] = dp[r] = 0.0f;
+              const uint32_t mask = bit_mask(t ? seen.w[1] : seen.w[0], (r >> 2) * 8 + (r & 3));
+              s[r] = masked_term(s[r], mask);
+              dp[r] = masked_term(dp[r], mask);
             }
           }
         } else if (j0 + kTile > free_end) {
@@ -762,10 +771,14 @@ void plan_bwd_splits(AttnArgs& a) {
       a.splits = (int)n;
     }
   }
-  // the sinks' blocks in ranges about as long as the others
-  const int64_t range = std::max<int64_t>(4, (tiles + a.splits - 1) / a.splits);
-  a.sink_splits = MASK == kWindow ? (int)std::min<int64_t>((all_tiles + range - 1) / range, 256) : 1;
-  if (a.sink_splits < 1) a.sink_splits = 1;
+  // Sinks' blocks walk over all later queries: in ranges where that would take longer than all other work.
+  a.sink_splits = 1;
+  if (MASK == kWindow) {
+    const int64_t least = 4, most = std::max<int64_t>(1, std::min<int64_t>(all_tiles / least, 256));
+    const double sinks = (double)(a.batch * a.kv_heads * sink_blocks(a)) * ((double)all_tiles * spread * 0.5 + fixed);
+    const double rest = std::max(best, (double)tiles * alone + fixed) + sinks / slots;
+    while (a.sink_splits < most && (double)(all_tiles / a.sink_splits) * alone + fixed > rest) ++a.sink_splits;
+  }
 }
 
 template <int MASK>

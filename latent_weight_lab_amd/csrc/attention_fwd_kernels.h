@@ -329,16 +329,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_rows(co
         fence_schedule<T>();
       }
       if constexpr (MASK == kWindow) {
-        const int stop = std::min(q_end, at.stop());
-        if (j0 + kKeys > std::min(free_end, at.stop()) || (j0 < free_begin && j0 + kKeys > allow.sinks)) {
-          const int lim = stop - j0 - half * 4, from = q_begin - j0 - half * 4, sinks = allow.sinks - j0 - half * 4;
+        if (j0 + kKeys > std::min(free_end, at.stop()) || (j0 < free_begin && std::min(j0 + kKeys, at.stop()) > allow.sinks)) {
+          const Seen seen = seen_keys(j0, std::min(q_end, at.stop()), q_begin, allow.sinks);
 #pragma unroll
           for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const int n = t * 32 + (r >> 2) * 8 + (r & 3);
-              s[t][r] = n < lim && (n >= from || n < sinks) ? s[t][r] : -INFINITY;
-            }
+            for (int r = 0; r < 16; ++r) s[t][r] = masked_score(s[t][r], bit_mask(seen.w[t], (r >> 2) * 8 + (r & 3)));
         }
       } else if (j0 + kKeys > free_end) {
         const int lim = std::min(q_end, end) - j0 - half * 4;
