@@ -162,6 +162,10 @@ __global__ __launch_bounds__(THREADS) void log_probs_forward(const LogProbArgs a
     const int w = threadIdx.x % WAVES;
     t = {lds_sums[0][w], lds_sums[1][w], lds_sums[2][w]};
     join_lanes<ENTROPY, WAVES>(t);
+    // The first lane's for all: a lane's own term may enter its sum unrounded (a fused multiply and add), so lanes may
+    // differ in the last bit, and which thread writes an alternative varies.
+    const auto first = [](float v) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v))); };
+    t = {first(t.m), first(t.s), first(t.a)};
   }
   const bool empty = t.s == 0.0f;  // nothing but minus infinities
   const float log_s = __logf(t.s);
