@@ -46,6 +46,8 @@ int lwl_attention_window_backward(const lwl_attention_args* args, int64_t window
  * number makes node i a root.  parents_stride 0: one tree for all sequences.  A sequence shorter than the tree
  * lacks the nodes at negative positions; a node that sees nothing gives zeros.
  *
+ * A NaN in a node's key or value may reach nodes that do not see it.
+ *
  * args as in lwl_attention_forward, with causal, bottom_right and causal_offset 0 and at most
  * LWL_ATTENTION_MAX_NODES queries.  lse may be NULL.  Forward only.
  */

@@ -71,5 +71,6 @@ def attention_tree(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, parents: t
     A sequence shorter than the tree lacks its first nodes; one that sees nothing gives zeros.
 
     The cache is read once for all query heads that share a key head.  The result lies in memory as ``attention``'s.
+    A NaN in a node's key or value may reach nodes that do not see it, as where a masked score matrix is multiplied out.
     There is no gradient: inputs that require one raise ``NotImplementedError`` where gradients are recorded."""
     return N.layers().attention_tree(q, k, v, parents, scale, key_lengths)

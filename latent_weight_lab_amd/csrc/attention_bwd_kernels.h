@@ -208,7 +208,7 @@ __global__ __launch_bounds__(256, (kKeysOccupancy<T, DP>)) void attention_bwd_ke
     if (q0 + kTile > wave_first && (MASK != kWindow || q0 < wave_last)) {
       // some pair of the tile is not allowed
       const bool masked = key_end(allow, q0) < wk0 + 32;
-      const bool passed = MASK == kWindow && window_begin(allow, q0 + kTile - 1) > wk0 && wk0 + 32 > allow.sinks;
+      const bool passed = MASK == kWindow && window_begin(allow, std::min(q0 + kTile, queries) - 1) > wk0 && wk0 + 32 > allow.sinks;
 #pragma unroll kUnroll<T, DP>
       for (int t = 0; t < 2; ++t) {
         const int at = t * 32;
@@ -281,7 +281,7 @@ __global__ __launch_bounds__(256, (kKeysOccupancy<T, DP>)) void attention_bwd_ke
           if (masked || passed) {
             // the queries from this key's position on, as far as its window reaches: their tile's bits
             const int from = key < allow.len ? key - allow.off : queries;
-            const Seen seen = seen_keys(q0, lane_last, from, INT32_MIN);
+            const Seen seen = seen_keys(q0, lane_last, from, q0);
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
               const uint32_t mask = bit_mask(t ? seen.w[1] : seen.w[0], (r >> 2) * 8 + (r & 3));

@@ -2,13 +2,16 @@
 bounds as in ``test_gpu_attention``."""
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
 import layer_oracle as R
 import token_oracle as T
 from conftest import gpu_available
-from latent_weight_lab_amd import attention, attention_tree
+from latent_weight_lab_amd import _native as N
+from latent_weight_lab_amd import attention, attention_tree, layer_ops
 from test_gpu_attention import DT, compare, make
 
 pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not gpu_available(), reason="needs a GPU")]
@@ -136,6 +139,45 @@ def test_offsets_past_32_bits():
     parents = torch.tensor(some_tree(60, 1, 2)[0], device="cuda")
     for n in (60, 3):
         assert torch.equal(attention_tree(q[:, :, :n], bk, bv, parents[:n]), attention_tree(q[:, :, :n], k, v, parents[:n]))
+
+
+@pytest.mark.parametrize("nodes,d,hk", [(4, 64, 2), (40, 32, 1)])
+def test_large_batches(nodes, d, hk):
+    """More sequences than a wave has lanes, and as many, of all lengths."""
+    for b in (64, 65, 130):
+        q, k, v, _ = make(b, 2, hk, nodes, 600, d, torch.bfloat16, b)
+        lengths = [(i * 97) % 601 for i in range(b)]
+        run(q, k, v, torch.bfloat16, some_tree(nodes, b, b), lengths)
+
+
+@pytest.mark.parametrize("nodes,d", [(2, 64), (30, 128)])
+def test_log_sums_of_the_c_entry(nodes, d):
+    """lse, which only C callers ask for, from one range and from several."""
+    for tk in (100, 3000):
+        q, k, v, _ = make(2, 4, 2, nodes, tk, d, torch.float16, 3)
+        parents = some_tree(nodes, 2, 1)
+        lengths = [tk, nodes - 1]
+        ok = T.tree_allowed(parents, tk, lengths, 2)
+        res = R.attention(q, k, v, d ** -0.5, ok)
+        q, k, v = (t.cuda().contiguous() for t in (q, k, v))
+        out, lse = torch.empty_like(q), torch.empty(2, 4, nodes, device="cuda")
+        lens, par = (torch.tensor(t, dtype=torch.int32, device="cuda") for t in (lengths, parents))
+        a = layer_ops.AttentionArgs()
+        a.dtype, a.batch, a.heads, a.kv_heads, a.queries, a.keys, a.dim, a.scale = 1, 2, 4, 2, nodes, tk, d, d ** -0.5
+        a.q, a.k, a.v, a.out, a.lse, a.key_lengths = (t.data_ptr() for t in (q, k, v, out, lse, lens))
+        for f, t in (("q_stride", q), ("k_stride", k), ("v_stride", v), ("out_stride", out)):
+            for i in range(3):
+                getattr(a, f)[i] = t.stride(i)
+        need = N.lib().lwl_attention_tree_workspace_size(ctypes.byref(a))
+        ws = torch.empty(max(need, 1), dtype=torch.uint8, device="cuda")
+        N.check(N.lib().lwl_attention_tree_forward(ctypes.byref(a), par.data_ptr(), nodes, ws.data_ptr(), need,
+                                                   torch.cuda.current_stream().cuda_stream))
+        torch.cuda.synchronize()
+        compare(out, res, "o", torch.float16, 2, res["gamma"])
+        some = ok.any(2).unsqueeze(1).expand(-1, 4, -1)
+        assert (lse.cpu()[~some] == float("-inf")).all()
+        off = (lse.double().cpu() - res["lse"]).abs()[some]
+        assert (off <= res["gamma"].squeeze(-1)[some] + 2.0 ** -20 * (1 + res["lse"].abs()[some])).all()
 
 
 def test_streams_and_graphs():

@@ -79,6 +79,14 @@ def test_sinks_of_long_sequences(dtype, shape):
 
 
 @pytest.mark.parametrize("dtype", list(DT))
+def test_large_batches(dtype):
+    """More sequences than a wave has lanes."""
+    for tq in (1, 40):
+        q, k, v, do = make(70, 2, 1, tq, 300, 32, DT[dtype], tq)
+        run(q, k, v, do, DT[dtype], 37, 3, lengths=[(i * 41) % 301 for i in range(70)])
+
+
+@pytest.mark.parametrize("dtype", list(DT))
 def test_a_wide_window_is_none(dtype):
     """A window that hides nothing gives what causal order alone gives, to its rounding."""
     q, k, v, do = (t.cuda() for t in make(2, 4, 2, 150, 200, 64, DT[dtype], 7))

@@ -190,6 +190,28 @@ def test_layouts(dtype):
     assert token_log_probs(base, torch.zeros(4, 6, 0, dtype=torch.long, device="cuda")).shape == (4, 6, 0)
 
 
+def test_no_tokens_asked_about():
+    """Entropies and alternatives alone, with their gradients."""
+    z, _, g = make(6, 2500, 1, torch.float32, 14)
+    none = torch.zeros(6, 0, dtype=torch.long)
+    run(z, none, 3, True, None, torch.randn(6, generator=g), torch.randn(6, 3, generator=g))
+
+
+def test_two_streams_at_once():
+    xs = [torch.randn(64, 30_000, device="cuda").bfloat16() for _ in range(2)]
+    toks = torch.randint(30_000, (64,), device="cuda")
+    want = [token_log_probs(x, toks, entropy=True, top=4) for x in xs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = []
+        for s, x in zip(streams, xs):
+            with torch.cuda.stream(s):
+                got.append(token_log_probs(x, toks, entropy=True, top=4))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for w, o in zip(want, got) for a, b in zip(w, o))
+
+
 def test_nothing_around_a_row_counts():
     z, tokens, _ = make(9, 1001, 1, torch.bfloat16, 4)
     buf = torch.full((11, 1040), math.nan, dtype=torch.bfloat16, device="cuda")
