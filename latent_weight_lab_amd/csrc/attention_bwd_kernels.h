@@ -771,13 +771,25 @@ void plan_bwd_splits(AttnArgs& a) {
       a.splits = (int)n;
     }
   }
-  // Sinks' blocks walk over all later queries: in ranges where that would take longer than all other work.
+  // Sinks' blocks walk over all later queries: in ranges where one alone, sharing its compute unit, would outlast all work
+  // spread over the compute units and the join.  bfloat16, a training step with 4 sinks, us: 8 x 1024 x 12 x 64, window
+  // 256, in 1, 2, 3 ranges 86, 92, 92, 1 is taken; 1 x 8192 x 12 x 64, window 512, in 1, 2, 4, 8, 16 ranges 289, 183, 130, 120,
+  // 120, 8.
   a.sink_splits = 1;
   if (MASK == kWindow) {
-    const int64_t least = 4, most = std::max<int64_t>(1, std::min<int64_t>(all_tiles / least, 256));
-    const double sinks = (double)(a.batch * a.kv_heads * sink_blocks(a)) * ((double)all_tiles * spread * 0.5 + fixed);
-    const double rest = std::max(best, (double)tiles * alone + fixed) + sinks / slots;
-    while (a.sink_splits < most && (double)(all_tiles / a.sink_splits) * alone + fixed > rest) ++a.sink_splits;
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(all_tiles / 4, 256));
+    const double sinks = (double)(a.batch * a.kv_heads * sink_blocks(a)), shared = two ? 1.8 * spread : alone;
+    const double all = (wgs * (double)tiles + sinks * (double)all_tiles) * spread / cus + (wgs + sinks) / slots * fixed;
+    const double part = 16.0 * sinks * (double)kBlock * (double)a.dim / 11e6;
+    double least = 0.0;
+    for (int64_t n = 1; n <= most; n = n < 4 ? n + 1 : n + n / 4) {
+      const double walk = (double)((all_tiles + n - 1) / n) * shared + fixed;
+      const double t = std::max(walk, all + (double)(n - 1) * sinks / slots * fixed) + (n > 1 ? 5.0 + (double)n * part : 0.0);
+      if (n == 1 || t < least) {
+        least = t;
+        a.sink_splits = (int)n;
+      }
+    }
   }
 }
 
