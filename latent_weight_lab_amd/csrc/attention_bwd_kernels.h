@@ -92,6 +92,11 @@ __host__ __device__ inline int64_t sink_blocks(const AttnArgs& a) {
   return (sinks + kBlock - 1) / kBlock;
 }
 __host__ __device__ inline int64_t partial_rows(const AttnArgs& a) { return a.batch * a.kv_heads * a.keys; }
+// Whether some query sees a key: `seen` is the end of those that the last query sees.
+template <int MASK>
+__device__ __forceinline__ bool key_seen(const Allowed& w, int key, int seen) {
+  return key < seen && (MASK != kWindow || key < w.sinks || key >= window_begin(w, 0));
+}
 // Where the partial sums of range `split` of key `key` of the key head number bk lie, two rows of dim.
 template <int MASK>
 __device__ __forceinline__ float* key_partial(const AttnArgs& a, int64_t bk, int64_t key, int split, bool sinks) {
@@ -137,8 +142,10 @@ __global__ __launch_bounds__(256, (kKeysOccupancy<T, DP>)) void attention_bwd_ke
   const int seen = key_end(allow, queries - 1);  // keys that some query sees
   const int wk0 = k0 + wave * 32, key = wk0 + (lane & 31);
   Opd<T> kf[KK], vf[KK];
-  load_operand<T, DP, FAST>(kf, (const T*)a.k + b * a.ks[0] + hk * a.ks[1] + (int64_t)key * a.ks[2], dim, key < seen);
-  load_operand<T, DP, FAST>(vf, (const T*)a.v + b * a.vs[0] + hk * a.vs[1] + (int64_t)key * a.vs[2], dim, key < seen);
+  load_operand<T, DP, FAST>(kf, (const T*)a.k + b * a.ks[0] + hk * a.ks[1] + (int64_t)key * a.ks[2], dim,
+                           key_seen<MASK>(allow, key, seen));
+  load_operand<T, DP, FAST>(vf, (const T*)a.v + b * a.vs[0] + hk * a.vs[1] + (int64_t)key * a.vs[2], dim,
+                           key_seen<MASK>(allow, key, seen));
   f32x16 dk[DT] = {}, dv[DT] = {};
   float held = __builtin_ldexpf(1.0f, kHeldStart);
   const float c = a.scale * kLog2E, inv_c = 1.0f / c;
@@ -342,7 +349,7 @@ __global__ __launch_bounds__(256, (kKeysOccupancy<T, DP>)) void attention_bwd_ke
   if (key >= (int)a.keys) return;
   const float dk_scale = kHold<T> ? __builtin_ldexpf(a.scale * kLower, 127 - exponent_bits(held)) : a.scale * kLower;
   if (splits > 1) {  // summed by attention_bwd_join, which takes keys that no query sees for zeros
-    if (key >= seen) return;
+    if (!key_seen<MASK>(allow, key, seen)) return;
     float* sums = key_partial<MASK>(a, b * a.kv_heads + hk, key, split, of_sinks);
     store_result<float, DP, FAST>(sums, dk, dk_scale, dim);
     store_result<float, DP, FAST>(sums + dim, dv, kLower, dim);
@@ -641,7 +648,8 @@ __global__ __launch_bounds__(256) void attention_bwd_join(const AttnArgs a) {
   const int64_t next = key_partial<MASK>(a, 0, 0, 1, of_sinks) - key_partial<MASK>(a, 0, 0, 0, of_sinks);
   const float* part = key_partial<MASK>(a, bk, key, 0, of_sinks) + (is_v ? dim : 0) + col;
   float sum[8] = {};
-  if ((int)key >= key_end(allowed_keys(a, b), (int)a.queries - 1)) splits = 0;
+  const Allowed allow = allowed_keys(a, b);
+  if (!key_seen<MASK>(allow, (int)key, key_end(allow, (int)a.queries - 1))) splits = 0;
 #pragma unroll 4
   for (int s = 0; s < splits; ++s) {
     float v[8];

@@ -799,9 +799,13 @@ hipError_t run(const AttnArgs& a, hipStream_t s) {
   const auto grid = [&](int64_t chunks) { return dim3((unsigned)((rows + chunks / per_row - 1) / (chunks / per_row))); };
   // Threads for a chunk of a row.  A tree's ranges of 4 for each, where 1024 workgroups hold them: 4096 rows of size 128 with
   // 8 ranges 7.1, 5.6 and 15 us with 1, 4 and 16, 976 rows with 64 ranges 29, 12 and 11, 8192 rows with 4 ranges 7.6, 9.2 and 37.
-  if (MASK == kTree && ranges >= 4 && ranges <= 2 * kSplitsAlone && grid(64).x <= 1024)
-    hipLaunchKernelGGL((attention_join<T, 4, MASK>), grid(64), dim3(256), 0, s, a);
-  else if (ranges > kSplitsAlone)
+  if constexpr (MASK == kTree) {
+    if (ranges >= 4 && ranges <= 2 * kSplitsAlone && grid(64).x <= 1024) {
+      hipLaunchKernelGGL((attention_join<T, 4, MASK>), grid(64), dim3(256), 0, s, a);
+      return hipGetLastError();
+    }
+  }
+  if (ranges > kSplitsAlone)
     hipLaunchKernelGGL((attention_join<T, 16, MASK>), grid(16), dim3(256), 0, s, a);
   else
     hipLaunchKernelGGL((attention_join<T, 1, MASK>), grid(256), dim3(256), 0, s, a);
