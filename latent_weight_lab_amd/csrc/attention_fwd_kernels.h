@@ -17,6 +17,11 @@
 // Where heads and rows give too few workgroups, ranges of keys are given to different workgroups,
 // which leave normalized float32 outputs and log sums; attention_join weighs them.
 //
+// MASK says which pairs count (attention_device.h): all that lengths and causal order leave, a window, or a tree's.  Within
+// a window a block of queries walks over the sinks' tiles and its windows' only (Walk).  A tree's block of rows are the
+// nodes of all query heads that share a key head, so that the cache is read once for them, and its ranges are cut
+// by the sequences' lengths (tree_share).
+//
 // What is subtracted from the scores is the maximum less kLift when it was last raised, and it is raised
 // only for a score more than kSlack above that maximum: probabilities then stay below 2^(kLift +
 // kSlack) = 2^14, the accumulators are rarely rescaled, and of float16's range the upper part is used, so
@@ -29,7 +34,10 @@
 // two rounds of walks of unequal lengths.  Float32 4 x 512 x 12 x 64 22.6 us and 5.7 for the join.  Tokens are bound
 // by memory: bfloat16 64 sequences of up to 1024 tokens x 12 x 64 19.6 us (101 MB, 5.2 TB/s), float32 38.3 us (202 MB,
 // 5.3 TB/s); float16 2 x 65536 x 4 x 128 42.6 us (268 MB, 6.3 TB/s, in part from the last-level cache) and 4.6 for the
-// join.
+// join.  Windows: 1 x 16384 x 16 on 4 x 128, window 4096, 4 sinks 503 us, 957 TFLOP/s of the pairs needed; 64 tokens over up
+// to 8192 x 12 x 64, window 1024, 39.5 us (188 MB, 4.8 TB/s).  Trees: 16 sequences of up to 8192 x 4 x 128, 32 nodes of 16
+// heads, 38 us and 7.5 for the join (138 MB; one token over the same caches 40 us in all); 65536 x 2 x 128, 61 nodes of 16
+// heads, 53 us and 7.4 (620 TFLOP/s: bound by the products).
 #pragma once
 
 #include <algorithm>

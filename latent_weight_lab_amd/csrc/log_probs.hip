@@ -7,13 +7,21 @@
 //
 // m starts at -FLT_MAX, so that a row of minus infinities sums zeros and nothing is NaN.
 //
-// The alternatives need no second pass over the row.  Each thread also keeps the largest of its values and the
-// chunk of eight it first met it in.  The top-th largest of these pairs bounds the answer from below, and exactly `top`
-// threads hold values that reach it: only they look at their part of the row again.  Pairs are ordered by value,
-// then by the lower index, so of equal values no more than the first few pass.  What passes is ranked by counting.
+// m is raised lazily (kSlack), and to the largest value at the end.
+//
+// The alternatives need no second pass over the row.  Each thread also keeps the largest of its values and the chunk of
+// eight that it first met it in; groups of threads keep the largest of these pairs.  The top-th largest group's bounds the
+// answer from below.  The chunks of the few threads that reach it are looked at again, by all threads, and what reaches it
+// there is ranked by counting.  Pairs are ordered by value, then by the lower index, so that of equal values no more than
+// the first few pass.  (Each such thread reading its own part again: 16 x 50304 with five alternatives 37 us, so 10.)
+//
+// Bound by memory where rows are many: bfloat16 8192 x 50257 in rows of 50304 139 us (5.9 TB/s), float32 264 us (6.2);
+// 512 x 50304 with one alternative 14.0 us (3.7 TB/s, two rows for a compute unit at once).  Few rows are bound by one
+// compute unit: 16 x 50304 with the entropy and five alternatives 9.6 us, some 4 of them after the row has been read.
 //
 // Backward: one pass that reads the logits and writes their gradient; tokens that are asked about are written once more
-// afterwards by the workgroup whose range they lie in, with all gradients given for them in the order given.
+// afterwards by the workgroup whose range they lie in, with all gradients given for them in the order given.  8192 x 50257
+// bfloat16 285 us (5.8 TB/s of reading and writing), float32 584 (5.6).
 #include <algorithm>
 #include <cfloat>
 
@@ -45,7 +53,9 @@ __device__ __forceinline__ uint64_t pair_of(uint32_t order, uint32_t place) {
   return (uint64_t)order << 32 | (uint32_t)~place;
 }
 
-// Eight values of a row from chunk `c` on; minus infinity past its end.
+// Eight values of a row, minus infinity past its end.  Chunks begin with the row, at any alignment, so that a row's results
+// have the same bits wherever it lies.  Dense rows of odd length cost that a sixth of the time: bfloat16 8192 x 50257, dense,
+// 166 us, in rows of 50304 142; with chunks at multiples of 16 bytes 141 both.
 template <class T>
 __device__ __forceinline__ void chunk_values(float (&v)[8], const Raw8<T>& raw, int64_t left) {
   unpack8(v, raw);
@@ -360,13 +370,14 @@ void forward(const LogProbArgs& a, hipStream_t s) {
     else hipLaunchKernelGGL((log_probs_forward<T, THREADS, U, false, false>), grid, block, 0, s, a);
   }
 }
-// 512 threads hold 16384 logits of a row at a time, which keeps memory busy; 256 lose less at the ends of short rows.
-// bfloat16, 512 and 256 threads: 8192 x 50257 168 and 172 us; with five alternatives and the entropy 1 x 200000 21 and
-// 32 us, 16 x 50304 10.1 and 12.4, 2048 x 16000 21 and 20, 2048 x 4000 16 and 13.  With 1024: 184, 20, 10.0, 32, 28 us.
+// Threads of a row: few lose less at the ends of short rows, many bring more of a long row at a time.  bfloat16, us with 256,
+// 512 and 1024: 2048 x 4000 with the entropy and five alternatives 12.5, 16, 27; 2048 x 16000 19.7, 23, 31; 8192 x 50257 in
+// rows of 50304, neither, 140, 142, 142; 16 x 50304 13.0, 9.6, 9.6; 1 x 200000 37, 22, 19.
 template <class T>
 hipError_t run_forward(const LogProbArgs& a, hipStream_t s) {
-  if (a.vocab > 16384) forward<T, 512, 4>(a, s);
-  else forward<T, 256, 4>(a, s);
+  if (a.vocab > 65536 && a.outer * a.inner <= device_cus()) forward<T, 1024, 2>(a, s);
+  else if (a.vocab > 16384) forward<T, 512, 2>(a, s);
+  else forward<T, 256, 2>(a, s);
   return hipGetLastError();
 }
 
