@@ -764,7 +764,7 @@ inline void plan_tree(AttnArgs& a) {
   a.split_len = std::max<int64_t>(a.keys, 1);
   int64_t ranges = (by_token(a) ? 2 : 1) * cus / units;
   if (ranges < 2 * batch) ranges = 2 * cus / units;
-  if (ranges >= 2 * batch && tiles >= 2 * kLeastTiles) {
+  if (batch > 0 && ranges >= 2 * batch && tiles >= 2 * kLeastTiles) {
     if (a.lengths && batch <= kMostRanked) {
       // no more than there are tiles for; sequences' own come on top
       a.spare = (int)std::min(ranges - batch, batch * ((tiles + kLeastTiles - 1) / kLeastTiles));

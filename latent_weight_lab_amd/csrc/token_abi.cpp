@@ -44,6 +44,9 @@ int check_tree(const lwl_attention_args* a) {
   if (a->queries > LWL_ATTENTION_MAX_NODES)
     return status_fail(LWL_ERR_UNSUPPORTED, "attention of a tree supports up to %d nodes (got %lld)",
                        LWL_ATTENTION_MAX_NODES, (long long)a->queries);
+  // the rows on a key head are counted in 32 bits
+  if (a->heads / a->kv_heads * a->queries > (int64_t)1 << 30)
+    return status_fail(LWL_ERR_UNSUPPORTED, "attention of a tree: more than 2^30 rows on a key head");
   return LWL_OK;
 }
 

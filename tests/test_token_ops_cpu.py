@@ -54,7 +54,8 @@ def test_window_refusals(kw, window, sinks, rc):
 
 
 @pytest.mark.parametrize("kw,rc", [({}, 0), ({"causal": 1}, -1), ({"bottom_right": 1}, -1), ({"causal_offset": 3}, -1),
-                                   ({"queries": 128}, 0), ({"queries": 129}, -2), ({"heads": 3}, -1), ({"keys": 0}, 0)])
+                                   ({"queries": 128}, 0), ({"queries": 129}, -2),
+                                   ({"batch": 1, "queries": 128, "heads": 1 << 27, "kv_heads": 1, "keys": 1}, -2), ({"heads": 3}, -1), ({"keys": 0}, 0)])
 def test_tree_refusals(kw, rc):
     L = N.lib()
     a = ctypes.byref(attn_args(**kw))
@@ -110,6 +111,19 @@ def test_null_pointers_and_workspaces_are_refused():
     for kw in ({}, {"stats": 256}, {"stats": 256, "grad_logits": 256, "grad_log_probs": 256},
                {"stats": 256, "grad_logits": 256, "grad_entropy": 256}, {"stats": 256, "grad_logits": 256, "grad_top": 256}):
         assert L.lwl_log_probs_backward(ctypes.byref(log_args(logits=256, **kw)), None) == -1
+
+
+@pytest.mark.parametrize("kw", [{"batch": 0, "keys": 100_000}, {"batch": 0, "keys": 100_000, "queries": 40},
+                                {"batch": 0, "keys": 0, "queries": 0}, {"keys": 0}, {"queries": 0, "keys": 100_000}])
+def test_workspaces_of_empty_calls(kw):
+    L = N.lib()
+    for lengths in (None, 256):
+        a = attn_args(**kw)
+        a.key_lengths = lengths
+        assert L.lwl_attention_tree_workspace_size(ctypes.byref(a)) < 1 << 31
+        a.causal = 1
+        assert L.lwl_attention_window_forward_workspace_size(ctypes.byref(a), 100, 4) < 1 << 31
+        assert L.lwl_attention_window_backward_workspace_size(ctypes.byref(a), 100, 4) < 1 << 31
 
 
 def test_workspaces_grow_with_the_window_only():
