@@ -751,19 +751,22 @@ void plan_splits(AttnArgs& a) {
 }
 
 // A tree's ranges (tree_share): as many as make one workgroup for each compute unit, for a workgroup leaves up to 128 rows
-// of float32 outputs however short its range, or two where one would leave sequences whole; single tokens' kernel
-// two.  Where sequences alone are as many, none is cut.  bfloat16, us with the join: 16 sequences of up to 8192 tokens, 32
-// nodes, 16 heads on 4 of size 128, 48 more ranges than sequences 51 (one workgroup), 112 more 55, none 161; 65536 tokens,
-// 61 nodes, 16 heads on 2 of size 128, 32 ranges (one workgroup) 59, 64 59, 16 94; 64 x 12 sequences and heads of up to 1024
-// tokens of size 64, 20 nodes, none cut 27, with ranges 34.
+// of float32 outputs however short its range; two for head sizes up to 64, whose rows are short and whose exponentials
+// take longer than their products, where one would leave sequences whole, and for single tokens' kernel; no more than 256
+// of a sequence, for the join.  Where sequences alone are as many, none is cut.  16-bit types, us with the join, one and two
+// workgroups: 16 sequences of up to 8192 tokens, 32 nodes, 16 heads on 4 of size 128 51 and 55 (uncut 161); 65536 tokens, 61
+// nodes, 16 heads on 2 of size 128 60 and 60; the former of size 64 31 and 30, of size 32 25 and 24; 2 x 64208 tokens, 67 nodes,
+// 32 heads on 8 of size 32 146 and 101 to 117; 131072 tokens, 32 nodes, 4 heads on 1 of size 64, 256 ranges 23, 512 31; 64 x 12
+// sequences and heads of up to 1024 tokens of size 64, 20 nodes, uncut 27, cut 34.
 inline void plan_tree(AttnArgs& a) {
   const int64_t cus = device_cus(), units = std::max<int64_t>(1, a.kv_heads * tree_blocks(a)), batch = a.batch;
   const int64_t tiles = (a.keys + kKeys - 1) / kKeys;
   a.splits = 1;
   a.spare = 0;
   a.split_len = std::max<int64_t>(a.keys, 1);
-  int64_t ranges = (by_token(a) ? 2 : 1) * cus / units;
+  int64_t ranges = (by_token(a) || a.dim <= 64 ? 2 : 1) * cus / units;
   if (ranges < 2 * batch) ranges = 2 * cus / units;
+  if (!by_token(a)) ranges = std::min(ranges, 256 * batch);
   if (batch > 0 && ranges >= 2 * batch && tiles >= 2 * kLeastTiles) {
     if (a.lengths && batch <= kMostRanked) {
       // no more than there are tiles for; sequences' own come on top
