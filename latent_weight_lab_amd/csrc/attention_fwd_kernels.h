@@ -190,11 +190,16 @@ __device__ __forceinline__ int64_t tree_partial(const AttnArgs& a, int slot, int
   return ((int64_t)slot * a.kv_heads + hk) * tree_rows(a) + r;
 }
 
-template <class T, int DP, bool FAST, int MASK>
+// HALVES of 2, for a tree's calls of at most 64 rows, which would leave half the waves without any: two waves hold the same
+// 32 rows and take 32 keys of every tile each; their sums meet in LDS at the end.  us with the join, 1 and 2: float32
+// 85810 tokens, 60 nodes, 12 heads of size 128 447 and 337, 16 sequences of up to 1024 x 12 x 64, 20 nodes 34.6 and 29.5; bfloat16,
+// which memory bounds, 8 sequences of up to 8192 x 8 x 128, 32 nodes 44.1 and 42.5, 64 of up to 1024 x 12 x 64 27 and 26.6.
+template <class T, int DP, bool FAST, int MASK, int HALVES = 1>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_rows(const AttnArgs a) {
   using KL = KeyRows<DP>;
   using VL = ValueRows<DP>;
   constexpr int KK = DP / 16, DT = DP / 32, KP = kKeys * KL::S, VP = kKeys * VL::S;  // sizes of a plane
+  constexpr int MINE = kKeys / HALVES, TS = MINE / 32;                                // a wave's keys of a tile
   __shared__ __attribute__((aligned(16))) Elem<T> lds_k[kBufs<T>][kPlanes<T> * KP];
   __shared__ __attribute__((aligned(16))) Elem<T> lds_v[kBufs<T>][kPlanes<T> * VP];
   const int lane = threadIdx.x & 63, half = lane >> 5;
@@ -215,7 +220,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_rows(co
   const Allowed allow = allowed_keys(a, b);
   // a tree's rows: the nodes of the first of the heads that share the key head, then of the next
   const int queries = (int)a.queries, rows_here = MASK == kTree ? queries * (int)(a.heads / a.kv_heads) : queries;
-  const int wq0 = q0 + wave * kWaveRows, wave_row = wq0 + (lane & 31);
+  const int team = HALVES == 1 ? wave : wave & 1, first = HALVES == 1 ? 0 : (wave >> 1) * MINE;  // of a tile's keys
+  const int wq0 = q0 + team * kWaveRows, wave_row = wq0 + (lane & 31);
   const bool live = wave_row < rows_here;
   int q = wave_row;
   if constexpr (MASK == kTree) {
@@ -301,23 +307,23 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_rows(co
       vt.fetch(at.next(), at.next_stop());
     }
     if (j0 < wave_end && (MASK != kWindow || j0 + kKeys > wave_begin || j0 < allow.sinks)) {
-      const Elem<T>* lk = lds_k[buf] + KL::at(lane & 31, half * 8);
+      const Elem<T>* lk = lds_k[buf] + KL::at(first + (lane & 31), half * 8);
       const Elem<T>* lv = lds_v[buf];
-      f32x16 s[2] = {};
+      f32x16 s[TS] = {};
       {
-        Opd<T> kf[2][KK];
+        Opd<T> kf[TS][KK];
         if constexpr (sizeof(T) == 2) {
 #pragma unroll
           for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
-            for (int t = 0; t < 2; ++t) kf[t][kk] = lds_operand<T>(lk + t * 32 * KL::S + kk * 16, KP);
+            for (int t = 0; t < TS; ++t) kf[t][kk] = lds_operand<T>(lk + t * 32 * KL::S + kk * 16, KP);
           fence_schedule<T>();
         }
         if constexpr (DP > 64) __builtin_amdgcn_s_setprio(1);  // 1 x 8192 x 16 x 128: 548 -> 529 us; slower at 64
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) {
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
+          for (int t = 0; t < TS; ++t) {
             if constexpr (sizeof(T) == 4) kf[t][kk] = lds_operand<T>(lk + t * 32 * KL::S + kk * 16, KP);
             s[t] = mma32(kf[t][kk], qf[kk], s[t]);
           }
@@ -325,13 +331,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_rows(co
         }
         if constexpr (DP > 64) __builtin_amdgcn_s_setprio(0);
       }
-      Opd<T> vf[4][DT];
+      Opd<T> vf[TS * 2][DT];
       const auto load_v = [&](int u, int d) {
-        vf[u][d] = lds_column_operand<T, VL>(lv, VP, u * 16 + half * 4, u * 16 + half * 4 + 8, d * 32 + (lane & 16));
+        const int key = first + u * 16 + half * 4;
+        vf[u][d] = lds_column_operand<T, VL>(lv, VP, key, key + 8, d * 32 + (lane & 16));
       };
       if constexpr (sizeof(T) == 2) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < TS * 2; ++u)
 #pragma unroll
           for (int d = 0; d < DT; ++d) load_v(u, d);
         fence_schedule<T>();
@@ -340,16 +347,16 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_rows(co
         if (j0 + kKeys > std::min(free_end, at.stop()) || (j0 < free_begin && std::min(j0 + kKeys, at.stop()) > allow.sinks)) {
           const Seen seen = seen_keys(j0, std::min(q_end, at.stop()), q_begin, allow.sinks);
 #pragma unroll
-          for (int t = 0; t < 2; ++t)
+          for (int t = 0; t < TS; ++t)
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[t][r] = masked_score(s[t][r], bit_mask(seen.w[t], (r >> 2) * 8 + (r & 3)));
         }
       } else if (j0 + kKeys > free_end) {
-        const int lim = std::min(q_end, end) - j0 - half * 4;
+        const int lim = std::min(q_end, end) - j0 - first - half * 4;
         uint64_t bits = 0;
-        if constexpr (MASK == kTree) bits = line_from(line, j0 - base);
+        if constexpr (MASK == kTree) bits = line_from(line, j0 + first - base);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int t = 0; t < TS; ++t) {
           const uint32_t seen = (uint32_t)(bits >> (t * 32)) >> (half * 4);
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
@@ -361,7 +368,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_rows(co
       }
       float most = s[0][0];
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < TS; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r) most = max_nan(most, s[t][r]);
       most = max_halves(most) * c;
@@ -375,7 +382,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_rows(co
           for (int r = 0; r < 16; ++r) o[d][r] *= shrink;
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < TS * 2; ++u) {
         float e[8];
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
@@ -395,6 +402,30 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_rows(co
       kt.template put<KL>(lds_k[buf ^ (kBufs<T> - 1)]);
       vt.template put<VL>(lds_v[buf ^ (kBufs<T> - 1)]);
     }
+  }
+  if constexpr (HALVES == 2) {
+    // The second half's waves leave theirs where keys and values were.
+    __syncthreads();
+    float* theirs = (float*)&lds_k[0][0] + team * DT * 16 * 64 + lane;
+    float* stat = (float*)&lds_v[0][0] + team * 2 * 64 + lane;
+    static_assert(sizeof(lds_k) >= 2 * DT * 16 * 64 * sizeof(float) && sizeof(lds_v) >= 4 * 64 * sizeof(float), "");
+    if (first > 0) {
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) theirs[(d * 16 + r) * 64] = o[d][r];
+      stat[0] = top;
+      stat[64] = sum;
+    }
+    __syncthreads();
+    if (first > 0) return;
+    const float next = fmaxf(top, stat[0]), mine = exp2_hw(top - next), other = exp2_hw(stat[0] - next);
+    top = next;
+    sum = sum * mine + stat[64] * other;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[d][r] = o[d][r] * mine + theirs[(d * 16 + r) * 64] * other;
   }
   sum += other_half(sum);
   if (!live) return;
@@ -798,10 +829,18 @@ hipError_t run(const AttnArgs& a, hipStream_t s) {
       works = blocks == 1 ? units : (units + 7) / 8 * 8 * blocks;
     }
     const dim3 grid((unsigned)works);
-    if (a.dim % 8 == 0 && fast_rows(a.k, a.ks, sizeof(T)) && fast_rows(a.v, a.vs, sizeof(T)))
-      hipLaunchKernelGGL((attention_rows<T, DP, true, MASK>), grid, dim3(256), 0, s, a);
-    else
-      hipLaunchKernelGGL((attention_rows<T, DP, false, MASK>), grid, dim3(256), 0, s, a);
+    const bool fast = a.dim % 8 == 0 && fast_rows(a.k, a.ks, sizeof(T)) && fast_rows(a.v, a.vs, sizeof(T));
+    const auto launch = [&](auto halves) {
+      constexpr int H = decltype(halves)::value;
+      if (fast) hipLaunchKernelGGL((attention_rows<T, DP, true, MASK, H>), grid, dim3(256), 0, s, a);
+      else hipLaunchKernelGGL((attention_rows<T, DP, false, MASK, H>), grid, dim3(256), 0, s, a);
+    };
+    if constexpr (MASK == kTree) {
+      if (tree_rows(a) <= 2 * kWaveRows) launch(std::integral_constant<int, 2>{});
+      else launch(std::integral_constant<int, 1>{});
+    } else {
+      launch(std::integral_constant<int, 1>{});
+    }
   }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !(MASK == kTree ? a.slots > a.batch : a.splits > 1)) return e;

@@ -70,6 +70,24 @@ def test_lengths(dtype, nodes, tk, lengths):
 
 
 @pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("heads,nodes,tk", [(2, 32, 31), (2, 32, 32), (2, 32, 33), (1, 64, 95), (1, 64, 96), (1, 17, 97),
+                                            (4, 9, 1024 + 31), (1, 33, 2048 + 33)])
+def test_halves_of_a_tile(dtype, heads, nodes, tk):
+    """Up to 64 rows: sequences that end in either half of 64 keys; scores of one half far above the other's, either way."""
+    q, k, v, _ = make(4, heads, 1, nodes, tk, 40, DT[dtype], heads + nodes + tk)
+    lengths = [tk, max(0, tk - 32), tk, tk - 1]
+    k = k.clone()
+    q = q.clone()
+    q[..., 0] = 8.0
+    k[..., 0] = 0.0
+    k[0, :, torch.arange(tk) % 64 < 32, 0] = 4.0
+    k[2, :, torch.arange(tk) % 64 >= 32, 0] = 4.0
+    parents = some_tree(nodes, 4, nodes)
+    q.permute(0, 2, 1, 3)[~T.tree_allowed(parents, tk, lengths, 4).any(2)] = float("nan")
+    run(q, k, v, DT[dtype], parents, lengths, 1.0)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
 @pytest.mark.parametrize("nodes", [3, 40])
 def test_a_chain_is_causal(dtype, nodes):
     q, k, v, _ = (t.cuda() for t in make(2, 4, 2, nodes, 500, 64, DT[dtype], 1))
