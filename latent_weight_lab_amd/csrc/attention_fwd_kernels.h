@@ -53,6 +53,7 @@ constexpr int kKeys = kTileRows;  // keys of a tile
 constexpr int kWaveRows = 32;
 constexpr int kWaves = 4;
 constexpr int kRows = kWaves * kWaveRows;
+constexpr int kHalvedRows = kRows / 2;  // of a tree, up to which waves halve the tiles
 
 // LDS row lengths in (16-bit) elements.  Keys are read 16 bytes a lane, 16 lanes at a time from 16 rows: 16
 // bytes of padding put these on distinct banks.  Values are read by columns: rows of 16 dwords more than a
@@ -782,20 +783,23 @@ void plan_splits(AttnArgs& a) {
 }
 
 // A tree's ranges (tree_share): as many as make one workgroup for each compute unit, for a workgroup leaves up to 128 rows
-// of float32 outputs however short its range; two for head sizes up to 64, whose rows are short and whose exponentials
-// take longer than their products, where one would leave sequences whole, and for single tokens' kernel; no more than 256
-// of a sequence, for the join.  Where sequences alone are as many, none is cut.  16-bit types, us with the join, one and two
-// workgroups: 16 sequences of up to 8192 tokens, 32 nodes, 16 heads on 4 of size 128 51 and 55 (uncut 161); 65536 tokens, 61
-// nodes, 16 heads on 2 of size 128 60 and 60; the former of size 64 31 and 30, of size 32 25 and 24; 2 x 64208 tokens, 67 nodes,
-// 32 heads on 8 of size 32 146 and 101 to 117; 131072 tokens, 32 nodes, 4 heads on 1 of size 64, 256 ranges 23, 512 31; 64 x 12
-// sequences and heads of up to 1024 tokens of size 64, 20 nodes, uncut 27, cut 34.
+// of float32 outputs however short its range.  Two where one would leave sequences whole, for single tokens' kernel, and
+// where rows are short or at most 64 and ranges still long; no more than 256 of a sequence, for the join.  Where sequences
+// alone are as many, none is cut.  us with the join, one and two workgroups; bfloat16: 16 sequences of up to 8192 tokens, 32
+// nodes, 16 heads on 4 of size 128 51 and 55 (uncut 161), of size 64 31 and 30; 8 of up to 8192 x 8 x 128, 32 nodes 42 and 38;
+// 2 of 8192 x 12 x 64, 60 nodes, ranges of 6 tiles 17.4 and 18.4; 64 x 12 sequences and heads of up to 1024 tokens of size 64, 20
+// nodes, uncut 27, cut 34.  Float16: 65536 tokens, 61 nodes, 16 heads on 2 of size 128 60 and 60; 2 x 64208, 67 nodes, 32 heads
+// on 8 of size 32 146 and 101 to 117.  Float32: 2 x 16384 x 8 x 96, 40 nodes, ranges of 8 tiles 73 and 66.  131072 tokens, 32
+// nodes, 4 heads on 1 of size 64, 256 ranges 23, 512 31.
 inline void plan_tree(AttnArgs& a) {
   const int64_t cus = device_cus(), units = std::max<int64_t>(1, a.kv_heads * tree_blocks(a)), batch = a.batch;
   const int64_t tiles = (a.keys + kKeys - 1) / kKeys;
   a.splits = 1;
   a.spare = 0;
   a.split_len = std::max<int64_t>(a.keys, 1);
-  int64_t ranges = (by_token(a) || a.dim <= 64 ? 2 : 1) * cus / units;
+  const bool few = a.dim <= 64 || tree_rows(a) <= kHalvedRows;
+  const bool lasting = tiles * batch * units >= (a.dtype == kF32 ? 8 : 12) * 2 * cus;  // a float32 tile takes longer
+  int64_t ranges = (by_token(a) || (few && lasting) ? 2 : 1) * cus / units;
   if (ranges < 2 * batch) ranges = 2 * cus / units;
   if (!by_token(a)) ranges = std::min(ranges, 256 * batch);
   if (batch > 0 && ranges >= 2 * batch && tiles >= 2 * kLeastTiles) {
@@ -836,7 +840,7 @@ hipError_t run(const AttnArgs& a, hipStream_t s) {
       else hipLaunchKernelGGL((attention_rows<T, DP, false, MASK, H>), grid, dim3(256), 0, s, a);
     };
     if constexpr (MASK == kTree) {
-      if (tree_rows(a) <= 2 * kWaveRows) launch(std::integral_constant<int, 2>{});
+      if (tree_rows(a) <= kHalvedRows) launch(std::integral_constant<int, 2>{});
       else launch(std::integral_constant<int, 1>{});
     } else {
       launch(std::integral_constant<int, 1>{});
