@@ -189,12 +189,17 @@ __global__ __launch_bounds__(256, (kKeysOccupancy<T, DP>)) void attention_bwd_ke
       const float* stat = (is_d ? a.work : a.lse) + head0 + (int64_t)fg * queries;
       if (is_factor) stat += a.batch * a.heads * a.queries;
       sr = q < last ? stat[q] : (is_d ? 0.0f : INFINITY);  // past the last: no probabilities
-      sr = is_factor ? sr : is_d ? -sr : kFoldStats<T> ? (kLift - sr * kLog2E) * inv_c : kLift - sr * kLog2E;
+      if constexpr (!kReadAhead<T, FAST>)
+        sr = is_factor ? sr : is_d ? -sr : kFoldStats<T> ? (kLift - sr * kLog2E) * inv_c : kLift - sr * kLog2E;
     }
   };
   auto put = [&](int buf) {
     qt.template put<Tile>(lds_q[buf]);
     gt.template put<Tile>(lds_g[buf]);
+    if constexpr (kReadAhead<T, FAST>) {  // not before, for it would wait for the tile's loads
+      const bool is_d = threadIdx.x >= kTile, is_factor = threadIdx.x >= 2 * kTile;
+      sr = is_factor ? sr : is_d ? -sr : kFoldStats<T> ? (kLift - sr * kLog2E) * inv_c : kLift - sr * kLog2E;
+    }
     if (threadIdx.x < kStats * kTile) lds_stat[buf][threadIdx.x / kTile][threadIdx.x & (kTile - 1)] = sr;
   };
   int buf = 0;
@@ -204,6 +209,8 @@ __global__ __launch_bounds__(256, (kKeysOccupancy<T, DP>)) void attention_bwd_ke
     fetch(g, q0);
     if constexpr (kBufs<T> == 2) put(0);
   }
+  wait_operands<T, FAST>(kf);
+  wait_operands<T, FAST>(vf);
   for (int i = begin; i < end; ++i) {
     __syncthreads();  // this tile is there, the one before has been read
     if constexpr (kBufs<T> == 1) {
@@ -408,11 +415,21 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_bwd_que
   Opd<T> qf[KK], gf[KK];
   load_operand<T, DP, FAST>(qf, (const T*)a.q + b * a.qs[0] + h * a.qs[1] + (int64_t)q * a.qs[2], dim, q_end > 0);
   float delta = 0.0f, norm = 0.0f;
+  Raw8<T> g_chunks[KK], o_chunks[KK];
+  if constexpr (kReadAhead<T, FAST>) {
+    load_chunks(g_chunks, (const T*)a.dout + b * a.dos[0] + h * a.dos[1] + (int64_t)q * a.dos[2], dim, q_end > 0);
+    load_chunks(o_chunks, (const T*)a.out + b * a.os[0] + h * a.os[1] + (int64_t)q * a.os[2], dim, q_end > 0);
+  }
 #pragma unroll
   for (int kk = 0; kk < KK; ++kk) {
     Raw8<T> gr, orow;
-    load_chunk<T, FAST>(gr, (const T*)a.dout + b * a.dos[0] + h * a.dos[1] + (int64_t)q * a.dos[2], kk, dim, q_end > 0);
-    load_chunk<T, FAST>(orow, (const T*)a.out + b * a.os[0] + h * a.os[1] + (int64_t)q * a.os[2], kk, dim, q_end > 0);
+    if constexpr (!kReadAhead<T, FAST>) {
+      load_chunk<T, FAST>(gr, (const T*)a.dout + b * a.dos[0] + h * a.dos[1] + (int64_t)q * a.dos[2], kk, dim, q_end > 0);
+      load_chunk<T, FAST>(orow, (const T*)a.out + b * a.os[0] + h * a.os[1] + (int64_t)q * a.os[2], kk, dim, q_end > 0);
+    } else {
+      gr = g_chunks[kk];
+      orow = o_chunks[kk];
+    }
     gf[kk] = operand_of<T>(gr);
     float x[8], y[8];
     unpack8(x, gr);
@@ -445,6 +462,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_bwd_que
     kt.template put<Tile>(lds_k[0]);
     vt.template put<Tile>(lds_v[0]);
   }
+  wait_operands<T, FAST>(qf);
+  wait_operands<T, FAST>(gf);
   int buf = 0;
   for (; at.live(); at.step(), buf ^= kBufs<T> - 1) {
     const int j0 = at.j;

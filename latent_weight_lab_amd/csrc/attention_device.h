@@ -215,8 +215,8 @@ using Padded = Strided<DP + 8>;
 //
 // FAST: the head size is a multiple of eight and fast_rows() holds of the tensor.  A
 // thread's byte offsets within a tile are then the same for every tile, the tile's address is scalar,
-// and the buffer's range check makes the zeros: no vector arithmetic for a tile.  Otherwise
-// load_ahead8 with 64-bit addresses for every row, and keep8 when it goes to LDS.
+// and the buffer's range check makes the zeros: no vector arithmetic for a tile.  Otherwise 16-bit types read ahead
+// (kReadAhead), float32 takes load_ahead8 with 64-bit addresses for every row, and keep8 when it goes to LDS.
 
 // Eight values of a row of a tensor whose first n belong to it, without waiting for them: all eight are read where
 // that is in the tensor (`inside`: a row follows, and rows are at least eight values apart), and keep8 clears
@@ -242,10 +242,39 @@ __device__ __forceinline__ void keep8(Raw8<T>& r, int n) {
       r.q[i][j] &= n >= first + per ? 0xffffffffu : part;
     }
 }
+// Whether rows that are not FAST are read ahead without a branch a chunk, whose loads are waited for where the branches
+// meet.  Every lane reads eight values of its tensor (TileLoader: those of the last row that would end past it end with
+// it; load_chunks: those of a row's last chunk end with the row), and what does not belong is cleared on the way to LDS.
+// Not so float32, whose tiles are short of vector instructions, not of loads.
+// us, with a branch a chunk and without: 8 x 1024 x 12 x 81, window 256, a step 207 and 183; 2 x 2048 x 8 x 115, causal,
+// forward 80.5 and 61, backward 208 and 190; a tree of 64 nodes, 24 heads on 8 of size 97 over 68762 tokens 342 and 166;
+// float32 2 x 1024 x 8 x 81 forward 63.8 and 67.1, backward 167 and 179.
+template <class T, bool FAST>
+constexpr bool kReadAhead = !FAST && sizeof(T) == 2;
+// All eight values one place down.
+template <class T>
+__device__ __forceinline__ void drop_first(Raw8<T>& r) {
+  uint32_t w[Raw8<T>::N * 4 + 1] = {};
+  __builtin_memcpy(w, &r, sizeof(r));
+#pragma unroll
+  for (int k = 0; k < Raw8<T>::N * 4; ++k) w[k] = sizeof(T) == 4 ? w[k + 1] : w[k] >> 16 | w[k + 1] << 16;
+  __builtin_memcpy(&r, w, sizeof(r));
+}
+// Of global memory: loads whose address space is open are waited for with the LDS reads.
+typedef const __attribute__((address_space(1))) char* GlobalBytes;
+template <bool AHEAD>
+struct TileUnderWay {};
+template <>
+struct TileUnderWay<true> {
+  int from, till;
+  bool near;  // its rows are read ahead
+};
 template <class T, int DP, bool FAST>
-struct TileLoader {
+struct TileLoader : TileUnderWay<kReadAhead<T, FAST>> {
+  static constexpr bool AHEAD = kReadAhead<T, FAST>;
   static constexpr int CPR = DP / 8;                    // chunks of eight values a row
   static constexpr int PER = kTileRows * CPR / 256;     // chunks a thread brings
+  static constexpr bool EVEN = 256 % CPR == 0;          // all of the same columns
   const T* base;
   int64_t stride;
   int dim, rows;  // rows: of the tensor
@@ -263,6 +292,14 @@ struct TileLoader {
         const int c = threadIdx.x + i * 256, row = c / CPR, col = (c % CPR) * 8;
         offset[i] = col < dim ? (uint32_t)(row * (int)stride + col) * (uint32_t)sizeof(T) : 0x80000000u;
       }
+    } else if constexpr (AHEAD) {
+      this->near = stride >= 8 && stride < ((int64_t)1 << 31) / ((int)sizeof(T) * kTileRows) &&
+             (int64_t)(rows - 1) * stride + dim >= 8;
+#pragma unroll
+      for (int i = 0; i < (EVEN ? 1 : PER); ++i) {
+        const int c = threadIdx.x + i * 256, row = c / CPR, col = (c % CPR) * 8;
+        offset[i] = this->near ? (uint32_t)(row * (int)stride + (col < dim ? col : 0)) * (uint32_t)sizeof(T) : 0u;
+      }
     }
   }
   // row0 and end are the same in all lanes
@@ -277,6 +314,25 @@ struct TileLoader {
 #pragma unroll
         for (int j = 0; j < Raw8<T>::N; ++j)
           r[i].q[j] = __builtin_amdgcn_raw_buffer_load_b128(rs, (int)offset[i] + 16 * j, 0, 0);
+    } else if constexpr (AHEAD) {
+      this->from = row0;
+      this->till = end;
+      uintptr_t tile = (uintptr_t)__builtin_amdgcn_kernarg_segment_ptr();
+      int64_t last = 0;
+      if (this->near) {
+        tile = (uintptr_t)(base + (int64_t)row0 * stride);
+        last = ((int64_t)(rows - 1 - row0) * stride + dim - 8) * (int)sizeof(T);
+        if (last < 0) tile += last;
+      }
+      const uint32_t next = this->near ? 256 / CPR * (uint32_t)stride * (uint32_t)sizeof(T) : 0;  // EVEN
+      const uint32_t most = (uint32_t)(last < 0 ? 0 : last < 0x7fffffff ? last : 0x7fffffff);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const uint32_t at = EVEN ? offset[0] + i * next : offset[i];
+        const GlobalBytes p = (GlobalBytes)tile + (at < most ? at : most);
+#pragma unroll
+        for (int j = 0; j < Raw8<T>::N; ++j) r[i].q[j] = ((const __attribute__((address_space(1))) u32x4_any*)p)[j];
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
@@ -288,13 +344,41 @@ struct TileLoader {
   }
   // into a tile of kPlanes planes of kTileRows rows
   template <class Layout>
-  __device__ __forceinline__ void put(Elem<T>* lds) const {
+  __device__ __forceinline__ void put(Elem<T>* lds) {
+    int thread = threadIdx.x;
+    if constexpr (AHEAD) {
+      asm volatile("" : "+v"(thread));  // what follows from it is not held from tile to tile: registers are short
+      if (!this->near) {
+#pragma unroll 1
+        for (int c = thread; c < PER * 256; c += 256) {
+          const int row = this->from + c / CPR, col = (c % CPR) * 8;
+          Raw8<T> values;
+          load_raw8(values, base + (int64_t)row * stride + col, row < this->till ? dim - col : 0);
+          *reinterpret_cast<Frag<T>*>(lds + Layout::at(c / CPR, (c % CPR) * 8)) = operand_of<T>(values);
+        }
+        return;
+      }
+      if (this->from + kTileRows >= rows) {  // the last row's last values were read as the last of eight
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const int c = thread + i * 256, col = (c % CPR) * 8;
+          if (this->from + c / CPR == rows - 1 && col < dim)
+            for (int n = dim - col; n < 8; ++n) drop_first(r[i]);
+        }
+      }
+      if (this->from + kTileRows > this->till) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+          if (this->from + (thread + i * 256) / CPR >= this->till) keep8(r[i], 0);
+      }
+    }
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int c = threadIdx.x + i * 256;
       Elem<T>* p = lds + Layout::at(c / CPR, (c % CPR) * 8);
       Raw8<T> kept = r[i];
-      if constexpr (!FAST) keep8(kept, dim - (c % CPR) * 8);
+      if constexpr (AHEAD) keep8(kept, dim - (thread + (EVEN ? 0 : i * 256)) % CPR * 8);
+      else if constexpr (!FAST) keep8(kept, dim - (c % CPR) * 8);
       const Opd<T> v = operand_of<T>(kept);
       if constexpr (sizeof(T) == 2) {
         *reinterpret_cast<Frag<T>*>(p) = v;
@@ -309,21 +393,59 @@ struct TileLoader {
 template <class T>
 constexpr int kBufs = sizeof(T) == 2 ? 2 : 1;
 
-// A row of a tensor as operands: lane l holds chunks of eight values, 8 (l / 32) + 16 kk (32-wide products).
-// WHOLE: the head size is a multiple of eight.
+// A row of a tensor in the order of operands: lane l holds chunks of eight values, 8 (l / 32) + 16 kk (32-wide products).
+// WHOLE: the head size is a multiple of eight.  Otherwise the last chunk is read as the row's last eight values, and
+// those that belong to the chunk before are dropped when all loads are under way.
 template <class T, bool WHOLE>
 __device__ __forceinline__ void load_chunk(Raw8<T>& r, const T* row, int kk, int dim, bool ok) {
   const int col = kk * 16 + ((threadIdx.x & 63) >> 5) * 8;
   if constexpr (WHOLE) load_whole8(r, row + col, ok && col < dim);
   else load_raw8(r, row + col, ok ? dim - col : 0);
 }
+template <class T, int N>
+__device__ __forceinline__ void load_chunks(Raw8<T> (&r)[N], const T* row, int dim, bool ok) {
+  const int col = ((threadIdx.x & 63) >> 5) * 8;
+  if (dim < 8) {
+#pragma unroll
+    for (int kk = 0; kk < N; ++kk) load_raw8(r[kk], row + col + kk * 16, ok ? dim - col - kk * 16 : 0);
+    return;
+  }
+#pragma unroll
+  for (int kk = 0; kk < N; ++kk) load_whole8(r[kk], row + (col + kk * 16 < dim - 8 ? col + kk * 16 : dim - 8), ok);
+#pragma unroll
+  for (int kk = 0; kk < N; ++kk) {
+    if (kk * 16 + 16 > dim)
+      for (int n = col + kk * 16 - (dim - 8) < 8 ? col + kk * 16 - (dim - 8) : 8; n > 0; --n) drop_first(r[kk]);
+  }
+}
 template <class T, int DP, bool WHOLE>
 __device__ __forceinline__ void load_operand(Opd<T> (&f)[DP / 16], const T* row, int dim, bool ok) {
+  if constexpr (!kReadAhead<T, WHOLE>) {
 #pragma unroll
-  for (int kk = 0; kk < DP / 16; ++kk) {
-    Raw8<T> r;
-    load_chunk<T, WHOLE>(r, row, kk, dim, ok);
-    f[kk] = operand_of<T>(r);
+    for (int kk = 0; kk < DP / 16; ++kk) {
+      Raw8<T> r;
+      load_chunk<T, WHOLE>(r, row, kk, dim, ok);
+      f[kk] = operand_of<T>(r);
+    }
+  } else {
+    Raw8<T> r[DP / 16];
+    load_chunks(r, row, dim, ok);
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk) f[kk] = operand_of<T>(r[kk]);
+  }
+}
+// Waits for operands.  Without WHOLE they come through branches, and a loop that uses them would wait at their first use
+// for all loads, its own next tile's too.
+template <class T, bool WHOLE, int N>
+__device__ __forceinline__ void wait_operands(Opd<T> (&f)[N]) {
+  if constexpr (kReadAhead<T, WHOLE>) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      u32x4_any w;
+      __builtin_memcpy(&w, &f[k], sizeof(w));
+      asm volatile("" : "+v"(w));
+      __builtin_memcpy(&f[k], &w, sizeof(w));
+    }
   }
 }
 // A result whose columns are rows of a tensor: the lane's row, values 8 r4 + 4 (l / 32) .. + 3 of each 32.

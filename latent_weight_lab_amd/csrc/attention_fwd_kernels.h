@@ -293,6 +293,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_rows(co
       vt.template put<VL>(lds_v[0]);
     }
   }
+  wait_operands<T, FAST>(qf);
   int buf = 0;
   for (; at.live(); at.step(), buf ^= kBufs<T> - 1) {
     const int j0 = at.j;
