@@ -347,7 +347,9 @@ struct TileLoader : TileUnderWay<kReadAhead<T, FAST>> {
   __device__ __forceinline__ void put(Elem<T>* lds) {
     int thread = threadIdx.x;
     if constexpr (AHEAD) {
-      asm volatile("" : "+v"(thread));  // what follows from it is not held from tile to tile: registers are short
+      // What follows from it is not held from tile to tile: 2 x 2048 x 8 x 115 would spill, 8 x 1024 x 12 x 50 run at two
+      // waves a SIMD, 31 and 34 us.  At 32 there are registers for it: a tree of size 18 237 and 217 us.
+      if constexpr (DP > 32) asm volatile("" : "+v"(thread));
       if (!this->near) {
 #pragma unroll 1
         for (int c = thread; c < PER * 256; c += 256) {
