@@ -35,6 +35,14 @@ constexpr float kLog2E = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
+// Workgroups along a grid's first axis; more go on along the second.  A launch holds an axis' threads in 32 bits and drops,
+// without an error, what is above.
+constexpr uint32_t kGridX = 1u << 21;
+inline dim3 grid_of(int64_t blocks) {
+  return dim3((unsigned)std::min<int64_t>(blocks, kGridX), (unsigned)((blocks + kGridX - 1) / kGridX));
+}
+__device__ __forceinline__ uint32_t block_number() { return blockIdx.y * kGridX + blockIdx.x; }
+
 template <class T>
 __device__ __forceinline__ const T* row_of(const LogProbArgs& a, int64_t r) {
   return (const T*)a.logits + r / a.inner * a.outer_stride + r % a.inner * a.inner_stride;
@@ -98,7 +106,8 @@ __global__ __launch_bounds__(THREADS) void log_probs_forward(const LogProbArgs a
   __shared__ float lds_sums[3][WAVES];
   __shared__ uint64_t lds_best[TOP ? THREADS : 1], lds_cand[TOP ? kCandidates : 1], lds_bound;
   __shared__ int lds_count, lds_hot[TOP ? THREADS : 1], lds_hot_count;
-  const int64_t row = blockIdx.x;
+  const int64_t row = block_number();
+  if (row >= a.outer * a.inner) return;
   const T* x = row_of<T>(a, row);
   const int vocab = (int)a.vocab, chunks = (vocab + 7) / 8;
   Raw8<T> raw[U];
@@ -299,8 +308,9 @@ template <class T, bool ENTROPY>
 __global__ __launch_bounds__(256) void log_probs_backward(const LogProbArgs a, uint32_t ranges) {
   __shared__ int lds_token[kListed];
   __shared__ float lds_grad[kListed];
-  const int64_t row = blockIdx.x / ranges;
-  const int begin = (int)(blockIdx.x % ranges) * kBwdRange;
+  const int64_t row = block_number() / ranges;
+  if (row >= a.outer * a.inner) return;
+  const int begin = (int)(block_number() % ranges) * kBwdRange;
   const T* x = row_of<T>(a, row);
   T* dz = (T*)a.grad_logits + row * a.vocab;
   const int vocab = (int)a.vocab, end = vocab - begin < kBwdRange ? vocab : begin + kBwdRange;
@@ -361,7 +371,7 @@ __global__ __launch_bounds__(256) void log_probs_backward(const LogProbArgs a, u
 
 template <class T, int THREADS, int U>
 void forward(const LogProbArgs& a, hipStream_t s) {
-  const dim3 grid((unsigned)(a.outer * a.inner)), block(THREADS);
+  const dim3 grid = grid_of(a.outer * a.inner), block(THREADS);
   if (a.top > 0) {
     if (a.entropy) hipLaunchKernelGGL((log_probs_forward<T, THREADS, U, true, true>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((log_probs_forward<T, THREADS, U, false, true>), grid, block, 0, s, a);
@@ -384,7 +394,7 @@ hipError_t run_forward(const LogProbArgs& a, hipStream_t s) {
 template <class T>
 hipError_t run_backward(const LogProbArgs& a, hipStream_t s) {
   const int64_t ranges = log_probs_bwd_ranges(a.vocab);
-  const dim3 grid((unsigned)(a.outer * a.inner * ranges));
+  const dim3 grid = grid_of(a.outer * a.inner * ranges);
   if (a.grad_entropy)
     hipLaunchKernelGGL((log_probs_backward<T, true>), grid, dim3(256), 0, s, a, (uint32_t)ranges);
   else

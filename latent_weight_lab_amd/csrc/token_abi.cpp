@@ -66,7 +66,7 @@ int check_log_probs(const lwl_log_probs_args* a) {
   if (a->each > LWL_LOG_PROBS_MAX_EACH || a->top > LWL_LOG_PROBS_MAX_TOP)
     return status_fail(LWL_ERR_UNSUPPORTED, "log probabilities support up to %d tokens a row and %d alternatives",
                        LWL_LOG_PROBS_MAX_EACH, LWL_LOG_PROBS_MAX_TOP);
-  // indexes in a row have 32 bits, workgroups are counted in 32
+  // indexes in a row have 32 bits, a grid's workgroups (of both axes together) are numbered in 32
   const int64_t kVocab = (int64_t)1 << 30, kCount = (int64_t)1 << 31;
   if (a->vocab > kVocab || a->outer >= kCount || a->inner >= kCount || a->outer * a->inner >= kCount ||
       a->outer * a->inner * lwl::log_probs_bwd_ranges(a->vocab) >= kCount)
