@@ -89,6 +89,8 @@ int lwl_gelu8_backward(const int8_t* codes, const float* scales, const void* gra
  * consecutive values along dim; any order, sharing (stride 0 of an input) and alignment of an element.
  * dim is 1 .. LWL_ATTENTION_MAX_DIM, heads a multiple of kv_heads, scale from 2^-100 to 2^100.  lse
  * (float32 [batch][heads][queries], contiguous) may be NULL in the forward.
+ * A call of 2^24 workgroups or more (a workgroup has up to 128 queries of a head, in the backward also 128 keys of a key
+ * head) is LWL_ERR_UNSUPPORTED.
  *
  * Not finite: a NaN in a key or value that some query may see reaches that query's results, and may reach
  * those of other queries whose `causal` limit hides it (its probability 0 is multiplied by it), as

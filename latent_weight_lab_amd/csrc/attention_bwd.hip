@@ -5,6 +5,8 @@ namespace lwl {
 
 int64_t attention_bwd_work(const AttnArgs& a) { return bwd_work<kAll>(a); }
 
+bool attention_bwd_fits(const AttnArgs& a) { return bwd_fits<kAll>(a); }
+
 hipError_t launch_attention_bwd(AttnArgs a, hipStream_t s) { return launch_bwd<kAll>(a, s); }
 
 }  // namespace lwl

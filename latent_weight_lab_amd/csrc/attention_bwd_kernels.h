@@ -712,12 +712,24 @@ void plan_query_splits(AttnArgs& a) {
   a.splits = splits > 1 ? (int)((keys + a.split_len - 1) / a.split_len) : 1;
 }
 
+// Workgroups of the key pass, planned, of the query pass with one range, and of the key pass's join.
+template <int MASK>
+int64_t key_workgroups(const AttnArgs& a) {
+  int64_t blocks = (a.keys + kBlock - 1) / kBlock * a.splits;
+  if (MASK == kWindow) blocks += sink_blocks(a) * (a.sink_splits - a.splits);
+  return blocks * a.batch * a.kv_heads;
+}
+inline int64_t query_workgroups(const AttnArgs& a) { return a.batch * a.heads * ((a.queries + kBlock - 1) / kBlock); }
+template <int MASK>
+int64_t join_workgroups(const AttnArgs& a) {
+  if (a.splits == 1 && !(MASK == kWindow && a.sink_splits > 1 && sink_blocks(a) > 0)) return 0;
+  const int64_t keys_wg = 128 / ((a.dim + 7) / 8);
+  return a.batch * a.kv_heads * ((join_keys<MASK>(a) + keys_wg - 1) / keys_wg);
+}
+
 template <class T, int DP, bool FAST, int MASK>
 hipError_t launch(const AttnArgs& a, hipStream_t s) {
-  int64_t kgrid = (a.keys + kBlock - 1) / kBlock * a.splits;
-  if (MASK == kWindow) kgrid += sink_blocks(a) * (a.sink_splits - a.splits);
-  kgrid *= a.batch * a.kv_heads;
-  const int64_t qgrid = a.batch * a.heads * ((a.queries + kBlock - 1) / kBlock);
+  const int64_t kgrid = key_workgroups<MASK>(a), qgrid = query_workgroups(a), jgrid = join_workgroups<MASK>(a);
   if (qgrid > 0) {
     AttnArgs by_keys = a;  // a's ranges are the key pass's
     plan_query_splits<MASK>(by_keys);
@@ -737,10 +749,7 @@ hipError_t launch(const AttnArgs& a, hipStream_t s) {
     hipLaunchKernelGGL((attention_bwd_keys<T, DP, FAST, MASK>), dim3((unsigned)kgrid), dim3(256), 0, s, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    if (a.splits > 1 || (MASK == kWindow && a.sink_splits > 1 && sink_blocks(a) > 0)) {
-      const int64_t keys_wg = 128 / ((a.dim + 7) / 8), blocks = (join_keys<MASK>(a) + keys_wg - 1) / keys_wg;
-      hipLaunchKernelGGL((attention_bwd_join<T, MASK>), dim3((unsigned)(a.batch * a.kv_heads * blocks)), dim3(256), 0, s, a);
-    }
+    if (jgrid > 0) hipLaunchKernelGGL((attention_bwd_join<T, MASK>), dim3((unsigned)jgrid), dim3(256), 0, s, a);
   }
   return hipGetLastError();
 }
@@ -820,6 +829,15 @@ void plan_bwd_splits(AttnArgs& a) {
       }
     }
   }
+}
+
+// (The query pass's ranges, and their join, are only where its workgroups are few.)
+template <int MASK>
+bool bwd_fits(AttnArgs a) {
+  // a block of keys has fewer than 512 ranges, sinks' and others, and 16 workgroups of the join
+  if (a.batch * a.heads * ((std::max(a.queries, a.keys) + kBlock - 1) / kBlock) <= kMostWorkgroups / 1024) return true;
+  plan_bwd_splits<MASK>(a);
+  return std::max({key_workgroups<MASK>(a), query_workgroups(a), join_workgroups<MASK>(a)}) <= kMostWorkgroups;
 }
 
 template <int MASK>

@@ -821,19 +821,29 @@ void plan(AttnArgs& a) {
   else plan_splits<MASK>(a);
 }
 
+// Workgroups of a planned call.  (The join has fewer: ranges are only where these are few.)
+template <int MASK>
+int64_t workgroups(const AttnArgs& a) {
+  if (by_token(a)) return a.kv_heads * (MASK == kTree ? (int64_t)a.slots : a.batch * a.splits);
+  if (MASK != kTree) return a.batch * a.heads * a.splits * ((a.queries + kRows - 1) / kRows);
+  const int64_t units = a.kv_heads * a.slots, blocks = tree_blocks(a);
+  return blocks == 1 ? units : (units + 7) / 8 * 8 * blocks;
+}
+template <int MASK>
+bool fwd_fits(AttnArgs a) {
+  // a block of queries has no more than kMaxSplits ranges
+  if (a.batch * a.heads * ((a.queries + kRows - 1) / kRows) <= kMostWorkgroups / 1024) return true;
+  plan<MASK>(a);
+  return workgroups<MASK>(a) <= kMostWorkgroups;
+}
+
 template <class T, int DP, int MASK>
 hipError_t run(const AttnArgs& a, hipStream_t s) {
+  const dim3 grid((unsigned)workgroups<MASK>(a));
   if (by_token(a)) {
-    const int64_t grid = a.kv_heads * (MASK == kTree ? (int64_t)a.slots : a.batch * a.splits);
-    if (a.dim % 8 == 0) hipLaunchKernelGGL((attention_token<T, DP, true, MASK>), dim3((unsigned)grid), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((attention_token<T, DP, false, MASK>), dim3((unsigned)grid), dim3(256), 0, s, a);
+    if (a.dim % 8 == 0) hipLaunchKernelGGL((attention_token<T, DP, true, MASK>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((attention_token<T, DP, false, MASK>), grid, dim3(256), 0, s, a);
   } else {
-    int64_t works = a.batch * a.heads * a.splits * ((a.queries + kRows - 1) / kRows);
-    if (MASK == kTree) {
-      const int64_t units = a.kv_heads * a.slots, blocks = tree_blocks(a);
-      works = blocks == 1 ? units : (units + 7) / 8 * 8 * blocks;
-    }
-    const dim3 grid((unsigned)works);
     const bool fast = a.dim % 8 == 0 && fast_rows(a.k, a.ks, sizeof(T)) && fast_rows(a.v, a.vs, sizeof(T));
     const auto launch = [&](auto halves) {
       constexpr int H = decltype(halves)::value;
@@ -851,19 +861,19 @@ hipError_t run(const AttnArgs& a, hipStream_t s) {
   if (e != hipSuccess || !(MASK == kTree ? a.slots > a.batch : a.splits > 1)) return e;
   const int64_t rows = a.batch * a.heads * a.queries;
   const int64_t per_row = (a.dim + 7) / 8, ranges = MASK == kTree ? a.slots / a.batch : a.splits;
-  const auto grid = [&](int64_t chunks) { return dim3((unsigned)((rows + chunks / per_row - 1) / (chunks / per_row))); };
+  const auto joins = [&](int64_t chunks) { return dim3((unsigned)((rows + chunks / per_row - 1) / (chunks / per_row))); };
   // Threads for a chunk of a row.  A tree's ranges of 4 for each, where 1024 workgroups hold them: 4096 rows of size 128 with
   // 8 ranges 7.1, 5.6 and 15 us with 1, 4 and 16, 976 rows with 64 ranges 29, 12 and 11, 8192 rows with 4 ranges 7.6, 9.2 and 37.
   if constexpr (MASK == kTree) {
-    if (ranges >= 4 && ranges <= 2 * kSplitsAlone && grid(64).x <= 1024) {
-      hipLaunchKernelGGL((attention_join<T, 4, MASK>), grid(64), dim3(256), 0, s, a);
+    if (ranges >= 4 && ranges <= 2 * kSplitsAlone && joins(64).x <= 1024) {
+      hipLaunchKernelGGL((attention_join<T, 4, MASK>), joins(64), dim3(256), 0, s, a);
       return hipGetLastError();
     }
   }
   if (ranges > kSplitsAlone)
-    hipLaunchKernelGGL((attention_join<T, 16, MASK>), grid(16), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((attention_join<T, 16, MASK>), joins(16), dim3(256), 0, s, a);
   else
-    hipLaunchKernelGGL((attention_join<T, 1, MASK>), grid(256), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((attention_join<T, 1, MASK>), joins(256), dim3(256), 0, s, a);
   return hipGetLastError();
 }
 

@@ -107,6 +107,10 @@ int check_attention(const lwl_attention_args* a) {
   return LWL_OK;
 }
 
+int fail_workgroups() {
+  return status_fail(LWL_ERR_UNSUPPORTED, "attention: more than %lld workgroups in one call", (long long)kMostWorkgroups);
+}
+
 AttnArgs attention_args(const lwl_attention_args* a) {
   AttnArgs t{};
   t.dtype = a->dtype;
@@ -144,6 +148,19 @@ AttnArgs attention_args(const lwl_attention_args* a) {
 }
 
 }  // namespace lwl
+
+namespace {
+
+int check_forward(const lwl_attention_args* a) {
+  const int rc = check_attention(a);
+  return rc || lwl::attention_fwd_fits(attention_args(a)) ? rc : lwl::fail_workgroups();
+}
+int check_backward(const lwl_attention_args* a) {
+  const int rc = check_attention(a);
+  return rc || lwl::attention_bwd_fits(attention_args(a)) ? rc : lwl::fail_workgroups();
+}
+
+}  // namespace
 
 extern "C" {
 
@@ -268,17 +285,17 @@ int lwl_gelu8_backward(const int8_t* codes, const float* scales, const void* gra
 }
 
 int lwl_attention_check(const lwl_attention_args* args) {
-  const int rc = check_attention(args);
+  const int rc = check_forward(args);
   return rc ? rc : status_ok();
 }
 
 size_t lwl_attention_forward_workspace_size(const lwl_attention_args* args) {
-  if (check_attention(args)) return 0;
+  if (check_forward(args)) return 0;
   return align_up((size_t)lwl::attention_fwd_work(attention_args(args)) * sizeof(float));
 }
 
 int lwl_attention_forward(const lwl_attention_args* args, void* workspace, size_t workspace_bytes, void* stream) {
-  int rc = check_attention(args);
+  int rc = check_forward(args);
   if (rc) return rc;
   if (args->batch == 0 || args->queries == 0) return status_ok();
   if (!args->q || !args->out || (args->keys > 0 && (!args->k || !args->v)))
@@ -291,12 +308,12 @@ int lwl_attention_forward(const lwl_attention_args* args, void* workspace, size_
 }
 
 size_t lwl_attention_backward_workspace_size(const lwl_attention_args* args) {
-  if (check_attention(args)) return 0;
+  if (check_backward(args)) return 0;
   return align_up((size_t)lwl::attention_bwd_work(attention_args(args)) * sizeof(float));
 }
 
 int lwl_attention_backward(const lwl_attention_args* args, void* workspace, size_t workspace_bytes, void* stream) {
-  int rc = check_attention(args);
+  int rc = check_backward(args);
   if (rc) return rc;
   if (args->batch == 0 || (args->queries == 0 && args->keys == 0)) return status_ok();
   if ((args->queries > 0 && (!args->q || !args->out || !args->lse || !args->grad_out || !args->grad_q)) ||

@@ -107,6 +107,15 @@ inline bool fast_rows(const void* p, const int64_t (&stride)[3], int64_t size) {
 // A caller's arguments (layer_abi.cpp): refused with a status, or taken.
 int check_attention(const lwl_attention_args* a);
 AttnArgs attention_args(const lwl_attention_args* a);
+// Workgroups of 256 threads in a launch, which holds an axis' threads in 32 bits and drops, without an error, what is above.
+constexpr int64_t kMostWorkgroups = (((int64_t)1 << 32) - 1) / 256;
+int fail_workgroups();  // the status of a call that would take more (layer_abi.cpp)
+// Whether a call's launches hold its workgroups.
+bool attention_fwd_fits(const AttnArgs& a);
+bool attention_bwd_fits(const AttnArgs& a);
+bool attention_window_fwd_fits(const AttnArgs& a);
+bool attention_window_bwd_fits(const AttnArgs& a);
+bool attention_tree_fits(const AttnArgs& a);
 // float32 values in the workspace
 int64_t attention_fwd_work(const AttnArgs& a);
 int64_t attention_bwd_work(const AttnArgs& a);

@@ -36,6 +36,15 @@ lwl::AttnArgs window_args(const lwl_attention_args* a, int64_t window, int64_t s
   return t;
 }
 
+int check_window_forward(const lwl_attention_args* a, int64_t window, int64_t sinks) {
+  const int rc = check_window(a, window, sinks);
+  return rc || lwl::attention_window_fwd_fits(window_args(a, window, sinks)) ? rc : lwl::fail_workgroups();
+}
+int check_window_backward(const lwl_attention_args* a, int64_t window, int64_t sinks) {
+  const int rc = check_window(a, window, sinks);
+  return rc || lwl::attention_window_bwd_fits(window_args(a, window, sinks)) ? rc : lwl::fail_workgroups();
+}
+
 int check_tree(const lwl_attention_args* a) {
   const int rc = check_attention(a);
   if (rc) return rc;
@@ -47,7 +56,7 @@ int check_tree(const lwl_attention_args* a) {
   // the rows on a key head are counted in 32 bits
   if (a->heads / a->kv_heads * a->queries > (int64_t)1 << 30)
     return status_fail(LWL_ERR_UNSUPPORTED, "attention of a tree: more than 2^30 rows on a key head");
-  return LWL_OK;
+  return lwl::attention_tree_fits(attention_args(a)) ? LWL_OK : lwl::fail_workgroups();
 }
 
 int check_log_probs(const lwl_log_probs_args* a) {
@@ -102,18 +111,18 @@ lwl::LogProbArgs log_prob_args(const lwl_log_probs_args* a) {
 extern "C" {
 
 int lwl_attention_window_check(const lwl_attention_args* args, int64_t window, int64_t sinks) {
-  const int rc = check_window(args, window, sinks);
+  const int rc = check_window_forward(args, window, sinks);
   return rc ? rc : status_ok();
 }
 
 size_t lwl_attention_window_forward_workspace_size(const lwl_attention_args* args, int64_t window, int64_t sinks) {
-  if (check_window(args, window, sinks)) return 0;
+  if (check_window_forward(args, window, sinks)) return 0;
   return align_up((size_t)lwl::attention_window_fwd_work(window_args(args, window, sinks)) * sizeof(float));
 }
 
 int lwl_attention_window_forward(const lwl_attention_args* args, int64_t window, int64_t sinks, void* workspace,
                                  size_t workspace_bytes, void* stream) {
-  int rc = check_window(args, window, sinks);
+  int rc = check_window_forward(args, window, sinks);
   if (rc) return rc;
   if (args->batch == 0 || args->queries == 0) return status_ok();
   if (!args->q || !args->out || (args->keys > 0 && (!args->k || !args->v)))
@@ -126,13 +135,13 @@ int lwl_attention_window_forward(const lwl_attention_args* args, int64_t window,
 }
 
 size_t lwl_attention_window_backward_workspace_size(const lwl_attention_args* args, int64_t window, int64_t sinks) {
-  if (check_window(args, window, sinks)) return 0;
+  if (check_window_backward(args, window, sinks)) return 0;
   return align_up((size_t)lwl::attention_window_bwd_work(window_args(args, window, sinks)) * sizeof(float));
 }
 
 int lwl_attention_window_backward(const lwl_attention_args* args, int64_t window, int64_t sinks, void* workspace,
                                   size_t workspace_bytes, void* stream) {
-  int rc = check_window(args, window, sinks);
+  int rc = check_window_backward(args, window, sinks);
   if (rc) return rc;
   if (args->batch == 0 || (args->queries == 0 && args->keys == 0)) return status_ok();
   if ((args->queries > 0 && (!args->q || !args->out || !args->lse || !args->grad_out || !args->grad_q)) ||
