@@ -3,11 +3,14 @@
 // Forward: one pass over a row with a running maximum m, S = sum exp(z - m) and A = sum exp(z - m) (z - m) a thread,
 // joined at the end in a fixed order:
 //
-//   log p_t = (z_t - m) - log S,  H = log S - A / S   (A <= 0: nothing cancels)
+//   log p_t = (z_t - m) - log S,  H = log S - A / S
 //
 // m starts at -FLT_MAX, so that a row of minus infinities sums zeros and nothing is NaN.
 //
-// m is raised lazily (kSlack), and to the largest value at the end.
+// Without the entropy m is raised lazily (kSlack), and to the largest value at the end.  With it, m is the largest value
+// so far: every term of A, and what a raise adds to it, is then 0 or below, and nothing cancels.  (Raised lazily, a
+// thread that met 0 after -8 held A = 8 e^8 and took 8 (1 + e^8) from it: entropies of some 5e-3 were off by up to 2.5e-4 of
+// themselves, where 2e-5 are left.)
 //
 // The alternatives need no second pass over the row.  Each thread also keeps the largest of its values and the chunk of
 // eight that it first met it in; groups of threads keep the largest of these pairs.  The top-th largest group's bounds the
@@ -17,7 +20,7 @@
 //
 // Bound by memory where rows are many: bfloat16 8192 x 50257 in rows of 50304 139 us (5.9 TB/s), float32 264 us (6.2);
 // 512 x 50304 with one alternative 14.0 us (3.7 TB/s, two rows for a compute unit at once).  Few rows are bound by one
-// compute unit: 16 x 50304 with the entropy and five alternatives 9.6 us, some 4 of them after the row has been read.
+// compute unit: 16 x 50304 with the entropy and five alternatives 9.8 us, some 4 of them after the row has been read.
 //
 // Backward: one pass that reads the logits and writes their gradient; tokens that are asked about are written once more
 // afterwards by the workgroup whose range they lie in, with all gradients given for them in the order given.  8192 x 50257
@@ -94,8 +97,8 @@ __device__ __forceinline__ void join_lanes(Sums& t) {
   if constexpr (ENTROPY) t.a = lanes_sum<LANES>(t.a);
 }
 
-// A thread's sums are taken relative to its largest value when that was last raised, which happens where one lies more
-// than this above it, and to the largest at the end.
+// Without the entropy a thread's sums are taken relative to its largest value when that was last raised, which happens where
+// one lies more than this above it, and to the largest at the end.
 constexpr float kSlack = 8.0f;
 constexpr int kCandidates = 1024;
 constexpr int kGroups = 128;  // of threads, whose largest values bound the alternatives: more than of these
@@ -128,30 +131,48 @@ __global__ __launch_bounds__(THREADS) void log_probs_forward(const LogProbArgs a
   Sums t = {-FLT_MAX, 0.0f, 0.0f};
   float best = -INFINITY;
   uint32_t best_chunk = threadIdx.x;
+  // A chunk's values, and the largest of them.
+  const auto look = [&](float (&v)[8], int u, int c) {
+    chunk_values(v, raw[u], vocab - c * 8);
+    const float most = max_nan(max_nan(max_nan(v[0], v[1]), max_nan(v[2], v[3])),
+                               max_nan(max_nan(v[4], v[5]), max_nan(v[6], v[7])));
+    if constexpr (TOP) {
+      if (!(most <= best) && best == best) {  // the first of equal ones; a NaN stays
+        best = most;
+        best_chunk = (uint32_t)c;
+      }
+    } else {
+      best = max_nan(best, most);
+    }
+    return most;
+  };
+  const auto add = [&](const float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float d = v[i] - t.m, e = exp2_hw(d * kLog2E);
+      t.s += e;
+      if constexpr (ENTROPY) t.a = fmaf(e, max_nan(d, -FLT_MAX), t.a);
+    }
+  };
   for (int base = 0; base < chunks; base += THREADS * U) {
     if (base > 0) load(base);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int c = base + u * THREADS + (int)threadIdx.x;
+    const int c = base + (int)threadIdx.x;
+    if constexpr (ENTROPY) {  // raised once for all chunks of a step: 16 x 50304 9.8 us, for each 10.2
       if (c >= chunks) break;
-      float v[8];
-      chunk_values(v, raw[u], vocab - c * 8);
-      const float most = max_nan(max_nan(max_nan(v[0], v[1]), max_nan(v[2], v[3])),
-                                 max_nan(max_nan(v[4], v[5]), max_nan(v[6], v[7])));
-      if constexpr (TOP) {
-        if (!(most <= best) && best == best) {  // the first of equal ones; a NaN stays
-          best = most;
-          best_chunk = (uint32_t)c;
-        }
-      } else {
-        best = max_nan(best, most);
-      }
-      if (__any(most > t.m + kSlack)) raise<ENTROPY>(t, fmaxf(t.m, most));
+      float v[U][8], most = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float d = v[i] - t.m, e = exp2_hw(d * kLog2E);
-        t.s += e;
-        if constexpr (ENTROPY) t.a = fmaf(e, max_nan(d, -FLT_MAX), t.a);
+      for (int u = 0; u < U; ++u) most = fmaxf(most, look(v[u], u, c + u * THREADS));
+      if (__any(most > t.m)) raise<true>(t, fmaxf(t.m, most));
+#pragma unroll
+      for (int u = 0; u < U; ++u) add(v[u]);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (c + u * THREADS >= chunks) break;
+        float v[8];
+        const float most = look(v, u, c + u * THREADS);
+        if (__any(most > t.m + kSlack)) raise<false>(t, fmaxf(t.m, most));
+        add(v);
       }
     }
   }
