@@ -8,6 +8,7 @@
 #include <dlfcn.h>
 
 #include <cmath>
+#include <limits>
 #include <optional>
 #include <stdexcept>
 #include <string>
@@ -119,6 +120,12 @@ Tensor scratch(size_t bytes, const Tensor& like) {
   return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)) : Tensor();
 }
 Tensor typed(const Tensor& t, at::ScalarType dtype) { return t.scalar_type() == dtype ? t : t.to(dtype); }
+// Integers as 64-bit ones, unsigned ones past these as the largest of them.
+Tensor longs(const Tensor& t) {
+  if (t.scalar_type() != at::kUInt64) return typed(t, at::kLong);
+  const Tensor same_bits = t.view(at::kLong);
+  return same_bits.masked_fill(same_bits.lt(0), std::numeric_limits<int64_t>::max());
+}
 
 MaybeTensor vector(const char* name, const MaybeTensor& t, int64_t n, at::ScalarType dtype) {
   if (!t) return t;
@@ -618,8 +625,10 @@ Tensor attention_tree(const Tensor& q0, const Tensor& k0, const Tensor& v0, cons
   const c10::DeviceGuard guard(q0.device());
   const MaybeTensor lengths = lengths_of(lengths0, a.batch);
   Tensor parents = parents0;
-  if (parents.scalar_type() != at::kInt)  // numbers that are no node's stay so in 32 bits
-    parents = parents.scalar_type() == at::kLong ? parents.clamp(-1, LWL_ATTENTION_MAX_NODES).to(at::kInt) : parents.to(at::kInt);
+  if (parents.scalar_type() != at::kInt) {  // numbers that are no node's stay so in 32 bits
+    if (parents.element_size() == 8) parents = longs(parents).clamp(-1, LWL_ATTENTION_MAX_NODES);
+    parents = parents.to(at::kInt);
+  }
   parents = parents.contiguous();
   const Tensor q = dense_dim(q0), k = dense_dim(k0), v = dense_dim(v0), out = empty_heads(a, a.queries, a.heads, q);
   a.q = q.data_ptr();
@@ -713,7 +722,7 @@ Judged log_probs_forward(const Tensor& logits0, const Tensor& tokens0, bool entr
            " alternatives, got ", each, " and ", top);
   const c10::DeviceGuard guard(logits0.device());
   const LogitRows r = logit_rows(logits0);
-  const Tensor tokens = typed(tokens0, at::kLong).contiguous();
+  const Tensor tokens = longs(tokens0).contiguous();
   lwl_log_probs_args a = log_probs_args(r, tokens, each, top);
   const auto floats = logits0.options().dtype(at::kFloat).requires_grad(false);
   const auto rows = logits0.sizes().slice(0, logits0.dim() - 1);
@@ -763,7 +772,7 @@ struct LogProbsFn : torch::autograd::Function<LogProbsFn> {
     const int64_t each = tokens_each(logits, s[1]), top = top_tokens.defined() ? top_tokens.size(-1) : 0;
     const c10::DeviceGuard guard(logits.device());
     const LogitRows r = logit_rows(logits);
-    const Tensor tokens = typed(s[1], at::kLong).contiguous();
+    const Tensor tokens = longs(s[1]).contiguous();
     const auto rows = logits.sizes().slice(0, logits.dim() - 1);
     std::vector<int64_t> tops(rows.begin(), rows.end());
     tops.push_back(top);
