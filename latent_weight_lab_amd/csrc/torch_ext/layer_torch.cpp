@@ -654,6 +654,11 @@ struct LogitRows {
 };
 LogitRows logit_rows(const Tensor& logits0) {
   LogitRows r;
+  if (logits0.numel() == 0) {  // no rows, whatever the axes' strides say
+    r.logits = logits0;
+    r.outer = 0;
+    return r;
+  }
   const auto two_axes = [&](const Tensor& t) {
     r = {t};
     if (t.size(-1) != 1 && t.stride(-1) != 1) return false;

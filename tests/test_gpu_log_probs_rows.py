@@ -1,4 +1,4 @@
-"""Rows of ``token_log_probs``: more than a grid's axis has workgroups."""
+"""Rows of ``token_log_probs``: none at all in any layout, and more than a grid's axis has workgroups."""
 from __future__ import annotations
 
 import pytest
@@ -9,6 +9,17 @@ from layer_oracle import U
 from latent_weight_lab_amd import token_log_probs
 
 pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not gpu_available(), reason="needs a GPU")]
+
+
+@pytest.mark.parametrize("empty", [0, 1, 2])
+def test_no_rows_of_axes_that_lie_apart(empty):
+    z = torch.randn(4, 6, 8, 20, device="cuda")[::2, :5, :7].narrow(empty, 0, 0).requires_grad_()
+    rows = z.shape[:-1]
+    tokens = torch.zeros(rows, dtype=torch.long, device="cuda")
+    out = token_log_probs(z, tokens, entropy=True, top=2)
+    assert [o.shape for o in out] == [rows, rows, (*rows, 2), (*rows, 2)]
+    (dz,) = torch.autograd.grad([out[0].sum(), out[1].sum()], z)
+    assert dz.shape == z.shape
 
 
 @pytest.mark.parametrize("rows", [(1 << 22) + 1, (1 << 24) + 3])
