@@ -120,10 +120,11 @@ class Stack(nn.Module):
         return F.linear(self.run(ids, torch.arange(ids.shape[1], device=ids.device), attend), self.tokens.weight)
 
     def step(self, ids, targets, optimizer):
-        """One training step through the weight cache; returns the loss."""
+        """One training step through the weight cache; returns the loss, the mean over the targets that are not padding
+        (negative ones)."""
         optimizer.zero_grad(set_to_none=True)
         lwl.prepare_block_fht_weight_cache(self)
-        loss = -lwl.token_log_probs(self(ids), targets).mean()
+        loss = -lwl.token_log_probs(self(ids), targets).sum() / (targets >= 0).sum()
         loss.backward()
         lwl.flush_block_fht_weight_cache(self)
         optimizer.step()

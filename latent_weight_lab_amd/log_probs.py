@@ -19,7 +19,8 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, entropy: bool = 
     ``logits`` is ``[..., vocabulary]`` in float32, float16 or bfloat16; rows may lie apart (slices of padded or shifted
     rows are read where they are).  ``tokens`` are integers of the leading shape, or with one more axis of up to 64
     tokens of each row; the result is float32 in their shape.  A negative token stands for none (padding): 0, without a
-    gradient.  One past the vocabulary gives NaN, without a gradient.
+    gradient.  One past the vocabulary gives NaN, without a gradient.  A loss over padded targets is their sum
+    divided by the number that is there, ``-token_log_probs(logits, targets).sum() / (targets >= 0).sum()``.
 
     With ``entropy`` or ``top`` the result is a tuple: the log probabilities; with ``entropy`` ``-sum p log p`` of every row;
     with ``top`` (up to 64) the largest log probabilities, ``[..., top]`` in descending order, and their tokens (int64).
