@@ -100,7 +100,7 @@ class Stack(nn.Module):
                  sinks=0) -> None:
         super().__init__()
         self.heads = heads
-        self.local = {"window": window, "sinks": sinks} if window else {}
+        self.local = {} if window is None and not sinks else {"window": window, "sinks": sinks}
         self.tokens, self.positions = nn.Embedding(vocabulary, width), nn.Embedding(context, width)
         nn.init.normal_(self.tokens.weight, std=0.02)
         nn.init.normal_(self.positions.weight, std=0.02)
@@ -276,7 +276,7 @@ def main() -> None:
         spent.append(clock() - t)
     print(f"decoding: prompts {1e3 * spent[0]:.2f} ms, then {1e3 * (spent[1] - spent[0]) / max(args.new_tokens - 1, 1):.2f}"
           f" ms a token for {args.batch} sequences", flush=True)
-    if not args.window:
+    if not model.local:
         t = clock()
         passes = model.decode_drafts(x, lengths, args.new_tokens, repeats)[2]
         print(f"with drafts from the sequences themselves: {passes} passes for {args.new_tokens} tokens, "
