@@ -687,6 +687,7 @@ __global__ __launch_bounds__(256) void attention_join(const AttnArgs a) {
   const float* lses = a.work + all * dim + first;
   const float* part = a.work + first * dim + col;
   float m = -FLT_MAX, total = 0.0f, v[8] = {};
+#pragma unroll 8  // one after the other, 130 ranges took 30 us, so 18
   for (int s = part_no; s < splits; s += SHARE) m = max_nan(m, lses[s * step]);
   if constexpr (SHARE > 1) {
     lds_m[part_no][chunk] = m;
@@ -785,8 +786,9 @@ void plan_splits(AttnArgs& a) {
 
 // A tree's ranges (tree_share): as many as make one workgroup for each compute unit, for a workgroup leaves up to 128 rows
 // of float32 outputs however short its range.  Two where one would leave sequences whole, for single tokens' kernel, and
-// where rows are short or at most 64 and ranges still long; no more than 256 of a sequence, for the join.  Where sequences
-// alone are as many, none is cut.  us with the join, one and two workgroups; bfloat16: 16 sequences of up to 8192 tokens, 32
+// where rows are short or at most 64 and ranges still long; no more than 256 of a sequence on average, for the join (one that
+// is longer than the others may have more: to hold that, too, took 0.3 us of every call).  Where sequences alone are as many,
+// none is cut.  us with the join, one and two workgroups; bfloat16: 16 sequences of up to 8192 tokens, 32
 // nodes, 16 heads on 4 of size 128 51 and 55 (uncut 161), of size 64 31 and 30; 8 of up to 8192 x 8 x 128, 32 nodes 42 and 38;
 // 2 of 8192 x 12 x 64, 60 nodes, ranges of 6 tiles 17.4 and 18.4; 64 x 12 sequences and heads of up to 1024 tokens of size 64, 20
 // nodes, uncut 27, cut 34.  Float16: 65536 tokens, 61 nodes, 16 heads on 2 of size 128 60 and 60; 2 x 64208, 67 nodes, 32 heads
@@ -814,6 +816,12 @@ inline void plan_tree(AttnArgs& a) {
     }
   }
   a.slots = (int)(a.spare > 0 ? batch + a.spare : batch * a.splits);
+}
+// The most ranges that one of a tree's sequences can have.
+inline int64_t tree_most(const AttnArgs& a) {
+  if (a.spare == 0) return a.splits;
+  const int64_t tiles = (a.keys + kKeys - 1) / kKeys;
+  return std::min<int64_t>(a.spare + 1, (tiles + kLeastTiles - 1) / kLeastTiles);
 }
 template <int MASK>
 void plan(AttnArgs& a) {
@@ -864,7 +872,14 @@ hipError_t run(const AttnArgs& a, hipStream_t s) {
   const auto joins = [&](int64_t chunks) { return dim3((unsigned)((rows + chunks / per_row - 1) / (chunks / per_row))); };
   // Threads for a chunk of a row.  A tree's ranges of 4 for each, where 1024 workgroups hold them: 4096 rows of size 128 with
   // 8 ranges 7.1, 5.6 and 15 us with 1, 4 and 16, 976 rows with 64 ranges 29, 12 and 11, 8192 rows with 4 ranges 7.6, 9.2 and 37.
+  // With lengths a sequence may have many more than the average: 16 where some may have more than 32 and as many
+  // workgroups hold them.  bfloat16, us by the average and by the most: 64 sequences of 32 rows, one of 65536 tokens, the others
+  // 60, 17.6 and 8.2; 4 of 256 rows, one of 131072, 15 and 10; all four of 131072 8.5 and 10.7; 16 of 32, all of 30000, 7.9 and 5.6.
   if constexpr (MASK == kTree) {
+    if (tree_most(a) > 2 * kSplitsAlone && joins(16).x <= 1024) {
+      hipLaunchKernelGGL((attention_join<T, 16, MASK>), joins(16), dim3(256), 0, s, a);
+      return hipGetLastError();
+    }
     if (ranges >= 4 && ranges <= 2 * kSplitsAlone && joins(64).x <= 1024) {
       hipLaunchKernelGGL((attention_join<T, 4, MASK>), joins(64), dim3(256), 0, s, a);
       return hipGetLastError();
