@@ -23,8 +23,9 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
     float32, float16 or bfloat16; any strides (a head's values are made dense if they are not).
     ``scale`` defaults to ``1 / sqrt(head size)`` and must be positive (from 2^-100 to 2^100).
 
-    ``key_lengths`` (integers on the device, ``[batch]``): keys of each sequence; what lies past them in k and
-    v is not read into any result (a cache's unused end).  ``causal``: query i sees keys up to
+    ``key_lengths`` (integers from 0 to ``keys`` on the device, ``[batch]``; int32 is read as it is, other types are
+    converted first): keys of each sequence; what lies past them in k and v is not read into any result (a cache's
+    unused end).  ``causal``: query i sees keys up to
     ``i + causal_offset``; by default the queries are the last tokens of their sequence (offset ``length -
     queries``), so the same call serves a prompt (as many queries as keys), new tokens over a cache and
     one token.  A batch padded at its end trains with ``causal_offset=0``.
@@ -66,7 +67,7 @@ def attention_tree(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, parents: t
     (``key_lengths`` counts them; without it the cache is full).  A node sees everything before the tree, its ancestors
     and itself; a chain (``parents[i] = i - 1``) gives what ``attention(..., causal=True)`` gives.
 
-    ``parents`` (integers on the device, ``[nodes]`` or ``[batch, nodes]``): the number of each node's parent, less than
+    ``parents`` (integers on the device, ``[nodes]`` or ``[batch, nodes]``; int32 is read as it is): the number of each node's parent, less than
     its own; any other number, -1 say, makes the node a root.  Nodes that no other refers to may stand for none.
     A sequence shorter than the tree lacks its first nodes; one that sees nothing gives zeros.
 

@@ -28,6 +28,9 @@
 // that a probability 2^-20 of the largest keeps its digits.  The first value is -FLT_MAX, not -infinity, so
 // that a row with no allowed key sums zeros: exp2(-inf + FLT_MAX) is 0 and nothing is NaN.
 //
+// 16-bit types: a probability is rounded to the type, half a step at most, as the operand of its product with the values;
+// the sum that the output is divided by takes it as it was.
+//
 // Measured on MI355X: prompts are bound by the matrix cores and by what stands between their instructions, the
 // exponentials (a quarter of the vector rate) and LDS reads: bfloat16 1 x 8192 x 16 on 4 x 128, causal, 297 us, 925
 // TFLOP/s of the pairs needed, where a library product of 8192^3 runs at 1030; 8 x 1024 x 12 x 64 23 us, 560 TFLOP/s,
@@ -195,6 +198,10 @@ __device__ __forceinline__ int64_t tree_partial(const AttnArgs& a, int slot, int
 // 32 rows and take 32 keys of every tile each; their sums meet in LDS at the end.  us with the join, 1 and 2: float32
 // 85810 tokens, 60 nodes, 12 heads of size 128 447 and 337, 16 sequences of up to 1024 x 12 x 64, 20 nodes 34.6 and 29.5; bfloat16,
 // which memory bounds, 8 sequences of up to 8192 x 8 x 128, 32 nodes 44.1 and 42.5, 64 of up to 1024 x 12 x 64 27 and 26.6.
+//
+// Size 128 of 16-bit types takes all 256 registers that two waves a SIMD leave.  A tree's then keeps 52 to 68 bytes a thread in
+// scratch, a window's 12 to 36, a call's without either 24 to 28 where rows are not FAST: what is set before the loop, of which
+// masked tiles read some back, behind the next tile's loads.
 template <class T, int DP, bool FAST, int MASK, int HALVES = 1>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_rows(const AttnArgs a) {
   using KL = KeyRows<DP>;
