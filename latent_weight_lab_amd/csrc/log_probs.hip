@@ -402,8 +402,8 @@ void forward(const LogProbArgs& a, hipStream_t s) {
   }
 }
 // Threads of a row: few lose less at the ends of short rows, many bring more of a long row at a time.  bfloat16, us with 256,
-// 512 and 1024: 2048 x 4000 with the entropy and five alternatives 12.5, 16, 27; 2048 x 16000 19.7, 23, 31; 8192 x 50257 in
-// rows of 50304, neither, 140, 142, 142; 16 x 50304 13.0, 9.6, 9.6; 1 x 200000 37, 22, 19.
+// 512 and 1024: 2048 x 4000 with the entropy and five alternatives 12.3, 18, 29; 2048 x 16000 19.2, 22, 31; 8192 x 50257 in
+// rows of 50304, neither, 141, 137, 139; 16 x 50304 12.7, 9.8, 9.8; 1 x 200000 33, 22.5, 20.
 template <class T>
 hipError_t run_forward(const LogProbArgs& a, hipStream_t s) {
   if (a.vocab > 65536 && a.outer * a.inner <= device_cus()) forward<T, 1024, 2>(a, s);
